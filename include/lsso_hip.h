@@ -38,6 +38,7 @@ extern "C" {
 /* Element types accepted by the projection entry point. */
 #define LSSO_HIP_F16 1
 #define LSSO_HIP_BF16 2
+#define LSSO_HIP_F32 3 /* lsso_hip_embedding*, lsso_hip_dropout_add and the feed-forward weights only */
 
 /* Position metadata layouts for the mixer (reference csrc/ball/common.cuh:245-257). */
 #define LSSO_HIP_POSITIONS_DEFAULT 0 /* p_t = t - (N - 1) / 2, computed on device */
@@ -525,6 +526,113 @@ int lsso_hip_linear_weight_grad(const void* g, int g_dtype, int64_t g_row_stride
                                 int64_t rows, int64_t in_features, int64_t out_features,
                                 const uint8_t* row_mask, float* grad_weight, float* grad_bias,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Token embedding: y[t] = cast(scale * weight[tokens[t]]).
+ * tokens: device int32 or int64 [count], by token_bytes (4 or 8).  weight:
+ * [vocabulary, dim] of weight_type with row stride weight_stride elements;
+ * y: contiguous [count, dim] of y_type; both one of LSSO_HIP_F16 / BF16 / F32.
+ * row_mask: optional device uint8 [count]; rows whose byte is 0 are written as
+ * zeros whatever their id.  The row of an id outside [0, vocabulary) is NaN.
+ * count may be 0; vocabulary and dim are positive, vocabulary < 2^31. */
+int lsso_hip_embedding(const void* tokens, int token_bytes, int64_t count,
+                       const void* weight, int weight_type, int64_t vocabulary, int64_t dim,
+                       int64_t weight_stride, float scale, const uint8_t* row_mask,
+                       void* y, int y_type, void* stream);
+
+/* Device scratch bytes needed by lsso_hip_embedding_grad. */
+int lsso_hip_embedding_grad_workspace_bytes(int64_t count, int64_t vocabulary, int64_t dim,
+                                            size_t* bytes);
+
+/* Gradient of lsso_hip_embedding's table:
+ *   grad_weight[v] = cast(scale * sum over t with tokens[t] = v of grad_y[t]),
+ * every row written (zeros where no token counts).  Tokens that row_mask
+ * excludes, that equal padding_index (-1: none) or lie outside the table count
+ * nowhere, whatever their grad_y holds.  grad_y: [count, dim] of grad_type
+ * with row stride grad_stride elements; grad_weight: contiguous
+ * [vocabulary, dim] of weight_type.  FP32 sums in an order that depends on
+ * the sizes alone: deterministic.  count < 2^31.  workspace: 256-byte aligned. */
+int lsso_hip_embedding_grad(const void* tokens, int token_bytes, int64_t count,
+                            const void* grad_y, int grad_type, int64_t grad_stride,
+                            int64_t vocabulary, int64_t dim, float scale,
+                            const uint8_t* row_mask, int64_t padding_index,
+                            void* grad_weight, int weight_type,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Residual dropout: y[i] = cast(residual[i] + keep[i] * x[i] * s) with
+ * s = 65536 / (65536 - threshold), and without a residual (NULL) the second
+ * term alone.  keep[i] is whether the 16-bit value i % 8 of the Philox-4x32-10
+ * block of counter (i / 8, offset) under the 64-bit key `seed` is at least
+ * threshold (0 .. 65535): a function of the index alone, so the same call on
+ * the upstream gradient gives the gradient of x.  state: optional device int64
+ * [2], read by the kernel: its first value replaces seed, its second is added
+ * to offset.  x, residual, y: contiguous [count] of dtype (LSSO_HIP_F16 / BF16
+ * / F32); count up to 2^34. */
+int lsso_hip_dropout_add(const void* x, const void* residual, int dtype, int64_t count,
+                         uint32_t threshold, uint64_t seed, uint64_t offset,
+                         const int64_t* state, void* y, void* stream);
+
+/* Activations of the gated feed-forward block. */
+#define LSSO_HIP_SILU 1 /* g * sigmoid(g) */
+#define LSSO_HIP_GELU 2 /* g * Phi(g), Phi the standard normal distribution function */
+
+/* Gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T of rows of x.
+ * dtype: LSSO_HIP_F16 or LSSO_HIP_BF16, of x, y and the kept values;
+ * weight_type: dtype, or LSSO_HIP_F32, whose values are rounded to dtype once
+ * per call.  x_stride: elements between rows of x (at least in_features). */
+typedef struct lsso_hip_feed_forward_shape {
+    int64_t rows;
+    int64_t in_features;
+    int64_t hidden;
+    int64_t out_features;
+    int64_t x_stride;
+    int dtype;
+    int weight_type;
+    int activation;
+} lsso_hip_feed_forward_shape;
+
+/* 16-bit values of the buffers a training forward keeps for its backward:
+ * gates [rows, 2, hidden rounded up to 8] and product [rows, hidden rounded up
+ * to 8]. */
+int lsso_hip_feed_forward_kept(const lsso_hip_feed_forward_shape* shape, size_t* gates,
+                               size_t* product);
+
+/* Device scratch bytes of lsso_hip_feed_forward: `training` is whether gates
+ * and product are given. */
+int lsso_hip_feed_forward_workspace_bytes(const lsso_hip_feed_forward_shape* shape, int training,
+                                          size_t* bytes);
+
+/* The block's forward.  x: [rows, in_features]; gate_weight, up_weight:
+ * contiguous [hidden, in_features]; down_weight: contiguous [out_features,
+ * hidden]; y: contiguous [rows, out_features].  x and the weights are 16-byte
+ * aligned.  Products accumulate in FP32 from 16-bit operands; act(g) * u is
+ * taken from the FP32 accumulators and rounded to dtype once for the second
+ * product.  row_mask: optional device uint8 [rows]; rows whose byte is 0 are
+ * written as zeros whatever their x holds.  gates, product: both NULL, or the
+ * buffers that the backward reads (lsso_hip_feed_forward_kept, 16-byte
+ * aligned).  workspace: 256-byte aligned.  rows may be 0. */
+int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* x,
+                          const void* gate_weight, const void* up_weight, const void* down_weight,
+                          const uint8_t* row_mask, void* gates, void* product, void* y,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Device scratch bytes of lsso_hip_feed_forward_backward.  grad_stride: elements
+ * between rows of grad_y; weights: which weight gradients are asked for, 1 (gate)
+ * + 2 (up) + 4 (down). */
+int lsso_hip_feed_forward_backward_workspace_bytes(const lsso_hip_feed_forward_shape* shape,
+                                                   int64_t grad_stride, int weights, size_t* bytes);
+
+/* First-order gradients of lsso_hip_feed_forward for grad_y [rows,
+ * out_features] of dtype (16-byte aligned).  grad_x: contiguous [rows,
+ * in_features] of dtype; grad_gate, grad_up, grad_down: contiguous, of
+ * weight_type; each may be NULL.  Excluded rows have zero grad_x and reach no
+ * weight gradient.  Deterministic: sums over rows are taken in an order that
+ * depends on the sizes alone. */
+int lsso_hip_feed_forward_backward(const lsso_hip_feed_forward_shape* shape, const void* grad_y,
+                                   int64_t grad_stride, const void* x, const void* gate_weight,
+                                   const void* up_weight, const void* down_weight,
+                                   const uint8_t* row_mask, const void* gates, const void* product,
+                                   void* grad_x, void* grad_gate, void* grad_up, void* grad_down,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

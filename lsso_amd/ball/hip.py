@@ -20,7 +20,8 @@ from threading import Lock
 
 import torch
 
-from . import ops
+from . import block, ops
+from .block import dropout_add, embedding, gated_feed_forward
 from .reference import rotary_inverse_frequency
 
 _LOAD_LOCK = Lock()
@@ -69,6 +70,7 @@ _SYMBOLS = (
     "lsso_hip_layer_backward",
     "lsso_hip_linear_weight_grad_workspace_bytes",
     "lsso_hip_linear_weight_grad",
+    *block.SYMBOLS,
 )
 
 
@@ -191,6 +193,7 @@ def _declare(library: ctypes.CDLL) -> None:
     ]  # shape, grad_y, dtype, stride, x, x_dtype, in_weight, row_mask, packed, mixed, base, drive, eta, inv_freq,
     #    positions, mode, counts, tape, out_weight, grads (x, in_weight, in_bias, base, drive, eta, out_weight,
     #    out_bias), workspace, workspace_bytes, stream
+    block.declare(library)
 
 
 def default_library_path() -> Path:
@@ -1623,9 +1626,12 @@ def linear(
 __all__ = [
     "backward",
     "center_positions",
+    "dropout_add",
+    "embedding",
     "fast_mix",
     "forward_inference",
     "forward_train",
+    "gated_feed_forward",
     "is_available",
     "layer_forward",
     "layer_train",

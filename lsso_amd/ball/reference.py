@@ -265,11 +265,91 @@ def compact_equilibrium_diagnostics(
         )
 
 
+def embedding(
+    tokens: torch.Tensor,
+    weight: torch.Tensor,
+    *,
+    scale: float = 1.0,
+    row_mask: torch.Tensor | None = None,
+    padding_index: int | None = None,
+    output_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """cast(scale * weight[tokens]) with zeros for the tokens that ``row_mask``
+    excludes and no gradient into the row ``padding_index``."""
+
+    output_dtype = weight.dtype if output_dtype is None else output_dtype
+    calc_dtype = _calculation_dtype(weight)
+    kept = torch.ones_like(tokens, dtype=torch.bool) if row_mask is None else row_mask
+    rows = functional.embedding(torch.where(kept, tokens, torch.zeros_like(tokens)), weight, padding_idx=padding_index)
+    value = rows.to(dtype=calc_dtype) * scale
+    return torch.where(kept[..., None], value, torch.zeros_like(value)).to(dtype=output_dtype)
+
+
+def gated_feed_forward(
+    x: torch.Tensor,
+    gate_weight: torch.Tensor,
+    up_weight: torch.Tensor,
+    down_weight: torch.Tensor,
+    *,
+    activation: str = "silu",
+    row_mask: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """(act(x Wg^T) * (x Wu^T)) Wd^T in FP32 (FP64 for FP64 x), one cast, zeros
+    for the rows that ``row_mask`` excludes."""
+
+    calc_dtype = _calculation_dtype(x)
+    value = x.to(dtype=calc_dtype)
+    if row_mask is not None:
+        value = torch.where(row_mask[..., None], value, torch.zeros_like(value))
+    with torch.autocast(device_type=x.device.type, enabled=False):
+        gate, up, down = (w.to(dtype=calc_dtype) for w in (gate_weight, up_weight, down_weight))
+        act = {"silu": functional.silu, "gelu": functional.gelu}[activation]
+        y = functional.linear(act(functional.linear(value, gate)) * functional.linear(value, up), down)
+    return y.to(dtype=x.dtype)
+
+
+def dropout_keep(shape: torch.Size, threshold: int, seed: int, offset: int, device: torch.device) -> torch.Tensor:
+    """The mask of dropout_add: element i is kept when the 16-bit value i % 8 of
+    the Philox-4x32-10 block (Salmon, Moraes, Dror and Shaw, SC 2011) of counter
+    (i // 8, offset) under the key ``seed`` is at least ``threshold``."""
+
+    low = 0xFFFFFFFF
+    count = math.prod(shape)
+    group = torch.arange((count + 7) // 8, dtype=torch.int64, device=device)
+    c = [group & low, group >> 32, torch.full_like(group, offset & low), torch.full_like(group, offset >> 32 & low)]
+    k = [seed & low, seed >> 32 & low]
+    for _ in range(10):
+        # The wrapped signed 64-bit product holds the bits of the unsigned one.
+        p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(q >> 32 & low) ^ c[1] ^ k[0], q & low, (p >> 32 & low) ^ c[3] ^ k[1], p & low]
+        k = [(k[0] + 0x9E3779B9) & low, (k[1] + 0xBB67AE85) & low]
+    bits = torch.stack([half for word in c for half in (word & 0xFFFF, word >> 16)], dim=-1)
+    return (bits.reshape(-1)[:count] >= threshold).reshape(shape)
+
+
+def dropout_add(
+    x: torch.Tensor, residual: torch.Tensor | None, threshold: int, seed: int, offset: int = 0
+) -> torch.Tensor:
+    """residual + keep * x * 65536 / (65536 - threshold)."""
+
+    calc_dtype = _calculation_dtype(x)
+    keep = dropout_keep(x.shape, threshold, seed, offset, x.device)
+    kept = x.to(dtype=calc_dtype) * (65536.0 / (65536 - threshold))
+    y = torch.where(keep, kept, torch.zeros_like(kept))
+    if residual is not None:
+        y = residual.to(dtype=calc_dtype) + y
+    return y.to(dtype=x.dtype)
+
+
 __all__ = [
     "accretive_equilibrium_mix",
     "accretive_generator",
     "bounded_complement",
     "compact_equilibrium_diagnostics",
+    "dropout_add",
+    "dropout_keep",
+    "embedding",
+    "gated_feed_forward",
     "linear",
     "qr_soft_frame",
     "rank_rotary",

@@ -34,6 +34,10 @@ SOURCES = (
     "lsso_backward.hip",
     "lsso_project_reduce.hip",
     "lsso_weight_grad.hip",
+    "lsso_block_capi.hip",
+    "lsso_dropout.hip",
+    "lsso_embedding.hip",
+    "lsso_feed_forward.hip",
 )
 PROBE_SOURCE = "lsso_probe.hip"
 PROBE_LIBRARY_NAME = f"liblsso_probe_{OFFLOAD_ARCH}.so"

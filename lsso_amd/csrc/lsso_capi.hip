@@ -36,6 +36,32 @@ int hip_failure(hipError_t error, const char* where) {
                 std::string(where) + " failed: " + hipGetErrorString(error));
 }
 
+}  // namespace
+
+namespace lsso_hip {
+
+int report(int code, const char* message) noexcept {
+    try {
+        g_last_error = message;
+    } catch (...) {   // no memory for the message: the code alone
+        g_last_error.clear();
+    }
+    return code;
+}
+
+int report_hip(hipError_t error, const char* where) noexcept {
+    try {
+        g_last_error = std::string(where) + " failed: " + hipGetErrorString(error);
+    } catch (...) {
+        g_last_error.clear();
+    }
+    return LSSO_HIP_ERUNTIME;
+}
+
+}  // namespace lsso_hip
+
+namespace {
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t value) { return (value + 255) & ~static_cast<size_t>(255); }
 

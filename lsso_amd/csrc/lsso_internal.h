@@ -279,6 +279,198 @@ struct WeightGradArgs {
     int large;                  // 256 x 256 output tiles, else 128 x 128 (set by the launcher)
 };
 
+// Residual dropout (lsso_dropout.hip).
+struct DropoutArgs {
+    const void* x;
+    const void* residual;       // or nullptr
+    void* y;
+    int64_t count;
+    uint32_t threshold;         // drop probability in units of 2^-16
+    float scale;                // 65536 / (65536 - threshold)
+    uint64_t seed;
+    uint64_t offset;
+    const int64_t* state;       // device (seed, offset): replaces seed, adds to offset; or nullptr
+};
+
+// Token embedding and its gradient (lsso_embedding.hip).
+struct EmbeddingArgs {
+    const void* tokens;         // int32 or int64 [count]
+    int wide_tokens;            // int64
+    int64_t count;
+    int64_t vocabulary;
+    int64_t dim;
+    const uint8_t* row_mask;    // [count] or nullptr; 0 rows are zeros and count nowhere
+    float scale;
+    // Lookup.
+    const void* weight;         // [vocabulary, dim], row stride weight_stride
+    int64_t weight_stride;
+    int weight_type;            // also of grad_weight
+    void* y;                    // [count, dim]
+    int64_t block_rows;
+    // Gradient.
+    const void* grad_y;         // [count, dim], row stride grad_stride
+    int64_t grad_stride;
+    int64_t padding_index;      // or -1
+    void* grad_weight;          // [vocabulary, dim]
+    uint32_t* histograms;       // [tiles, digits of the pass]
+    int64_t tile_tokens;
+    int64_t tiles;
+    int key_bits;
+    int passes;
+    const uint32_t* keys;       // sorted ids, then `vocabulary` for what counts nowhere
+    const uint32_t* index;      // token of each sorted position
+    float* partials;            // [chunks, 2, dim]
+    int64_t chunk_tokens;
+    int64_t chunks;
+    int64_t row_blocks;
+    size_t off_sorted[4];
+    size_t off_histograms;
+    size_t off_partials;
+};
+
+// One pass of the gradient's radix sort; without inputs the tokens themselves.
+struct SortPass {
+    const uint32_t* keys_in;
+    const uint32_t* index_in;
+    uint32_t* keys_out;
+    uint32_t* index_out;
+    int shift;
+    int bits;
+};
+
+// Gated feed-forward block (lsso_feed_forward.hip).  All matrices are 16-bit of
+// `type` unless they say otherwise; pitches are multiples of 8.
+struct FeedForwardArgs {
+    int type;
+    int activation;
+    int64_t rows;
+    int64_t hidden;
+    int64_t out_features;
+    int64_t in_pitch;           // columns of x, gate and up, zeros past in_features
+    int64_t pitch;              // columns of h: hidden rounded up
+    int64_t out_pitch;          // columns of dy
+    int64_t down_pitch;         // columns of down: pitch
+    const uint16_t* x;          // [rows, in_pitch], row stride x_stride
+    int64_t x_stride;
+    const uint16_t* gate;       // [hidden, in_pitch]
+    const uint16_t* up;         // [hidden, in_pitch]
+    const uint16_t* down;       // [out_features, down_pitch]
+    const uint8_t* row_mask;    // [rows] or nullptr
+    uint16_t* h;                // [rows, pitch]
+    uint16_t* gates;            // [rows, 2, pitch]: g, u; or nullptr
+    const uint16_t* dy;         // [rows, out_pitch], row stride dy_stride
+    int64_t dy_stride;
+    uint16_t* grads;            // [rows, 2, pitch]: dg, du
+    int stages;                 // set by the launcher, as the tiles
+    int64_t q_tiles;
+    int64_t tiles;
+};
+
+struct FeedForwardProduct {
+    int type;
+    const uint16_t* p;          // [rows, k], row stride p_stride
+    int64_t p_stride;
+    int64_t p_second;           // elements from p to the second segment's rows
+    int64_t rows;
+    int64_t k;                  // of a segment, a multiple of 8
+    const uint16_t* q;          // rows: [columns, k]; columns: [q_lines, q_pitch]
+    const uint16_t* q_second;
+    int64_t q_stride;
+    int64_t q_lines;
+    int64_t q_pitch;
+    const uint8_t* row_mask;
+    uint16_t* out;              // [rows, columns] contiguous
+    int64_t columns;
+    float* partials;            // [splits, rows, partial_pitch], unused with one split
+    int64_t partial_pitch;
+    int segment_stages;         // stages of the first segment
+    int stages;                 // of all segments; set by plan_product, as what follows
+    int split_stages;
+    int splits;
+    int mb, nb;
+    int64_t q_tiles;            // set by the launcher
+    int64_t tiles;
+};
+
+struct WeightProduct {
+    const uint16_t* p;          // [rows, p_columns], row stride p_stride
+    int64_t p_stride;
+    int64_t p_columns;
+    const uint16_t* q;          // [rows, q_columns], row stride q_stride
+    int64_t q_stride;
+    int64_t q_columns;
+    int64_t out_rows;
+    int64_t partial_pitch;      // columns of the product, a multiple of 8
+    int64_t partial_offset;     // set by plan_weights, as the tiles
+    int64_t q_tiles;
+    int64_t tiles;
+};
+constexpr int kWeightSplitRows = 8192;   // most rows of a split
+
+struct FeedForwardWeights {
+    int type;
+    int count;
+    WeightProduct products[3];
+    int64_t rows;
+    const uint8_t* row_mask;
+    float* partials;            // [splits, partial_floats]
+    int64_t partial_floats;
+    int64_t split_rows;
+    int64_t splits;
+    int64_t tiles;              // of one split
+    int mb;
+};
+
+struct JoinOutput {
+    int64_t offset;
+    int64_t pitch;
+    int64_t rows;
+    int64_t columns;
+    void* out;                  // [rows, columns] contiguous
+};
+
+struct FeedForwardJoin {
+    const float* partials;
+    int64_t splits;
+    int64_t split_floats;
+    const uint8_t* row_mask;    // of the outputs' rows, or nullptr
+    int type;                   // of the outputs
+    JoinOutput outputs[3];
+};
+
+struct PackMatrix {
+    const void* from;           // [rows, columns], row stride `stride`
+    int64_t stride;
+    int64_t columns;
+    int64_t pitch;
+    int wide;                   // FP32
+    uint16_t* to;               // [rows, pitch]
+    int64_t pieces;             // rows * pitch / 8
+};
+
+struct FeedForwardPack {
+    int count;
+    PackMatrix matrices[5];
+};
+
+void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProduct* a);
+void plan_weights(FeedForwardWeights* a);
+hipError_t launch_feed_forward_gate(const FeedForwardArgs& a, hipStream_t stream);
+hipError_t launch_feed_forward_product(const FeedForwardProduct& a, bool q_rows, hipStream_t stream);
+hipError_t launch_feed_forward_grad(const FeedForwardArgs& a, hipStream_t stream);
+hipError_t launch_feed_forward_weights(const FeedForwardWeights& a, hipStream_t stream);
+hipError_t launch_feed_forward_join(const FeedForwardJoin& a, int outputs, hipStream_t stream);
+hipError_t launch_feed_forward_pack(const FeedForwardPack& a, int type, hipStream_t stream);
+
+// Sets the calling thread's error message (lsso_hip_last_error) and returns code.
+int report(int code, const char* message) noexcept;
+int report_hip(hipError_t error, const char* where) noexcept;
+
+hipError_t launch_dropout(const DropoutArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_embedding(const EmbeddingArgs& a, int y_type, hipStream_t stream);
+void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes);
+hipError_t launch_embedding_grad(const EmbeddingArgs& a, void* workspace, int grad_type, hipStream_t stream);
+
 hipError_t launch_phase(const PhaseArgs& a, hipStream_t stream);
 hipError_t launch_geometry(const GeometryArgs& a, int position_type, hipStream_t stream);
 hipError_t launch_reduce(int rank, const ReduceArgs& a, int cpw, bool vec, hipStream_t stream);

@@ -1,0 +1,401 @@
+"""Gated feed-forward block: value and gradients against FP64 with bounds that
+follow each rounding, over tile edges, odd widths, masks and layouts; captured
+replays and refusals."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from lsso_amd.ball import GatedFeedForward, block, hip
+
+HALVES = (torch.float16, torch.bfloat16)
+
+
+def _act(g, kind):
+    if kind == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    cdf = torch.special.ndtr(g)
+    return g * cdf, cdf + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+
+
+def _expected(x, weights, dy, kind, dtype, grad_dtype, mask=None):
+    """{output: (value, bound)} in FP64.
+
+    The bounds follow the operator's roundings, each at most half a step `e` of
+    the type: of h = act(g) u, of the kept g and u, of dg and du, and of the
+    outputs; an FP32 sum of n products is off by at most n 2^-24 times the sum
+    of their magnitudes.  Through act and act' an error of g grows by at most
+    1.13 and 0.8 (the largest |act'| and |act''| of both activations); their own
+    evaluation in FP32 is off by |g| 2^-22 and (1 + |g|) 2^-21: a relative error
+    of |g| 2^-24 + 2^-23 in the exponential, which s (1 - s) <= 1 / 4 shrinks, and
+    roundings of FP32.  `tiny`: half a step of FP16 below its normal range.  5%
+    for the products of two errors."""
+
+    e = torch.finfo(dtype).eps / 2
+    out = torch.finfo(grad_dtype).eps / 2
+    tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-134
+    f = 2.0**-24
+    x, dy = (v.double().reshape(-1, v.shape[-1]) for v in (x, dy))
+    gate, up, down = (w.to(dtype).double() for w in weights)
+    if mask is not None:
+        x = torch.where(mask.reshape(-1, 1), x, 0.0)
+        dy = torch.where(mask.reshape(-1, 1), dy, 0.0)
+    k, hidden, n, rows = x.shape[1], gate.shape[0], down.shape[0], x.shape[0]
+    g, u = x @ gate.T, x @ up.T
+    eg, eu = k * f * (x.abs() @ gate.abs().T), k * f * (x.abs() @ up.abs().T)
+    act, slope = _act(g, kind)
+    ea = 1.13 * eg + g.abs() * 2.0**-22
+    h = act * u
+    eh = ea * u.abs() + act.abs() * eu + e * h.abs() + tiny
+    y = h @ down.T
+    found = {"y": (y, eh @ down.abs().T + hidden * f * (h.abs() @ down.abs().T) + e * y.abs() + tiny)}
+    dh = dy @ down
+    edh = n * f * (dy.abs() @ down.abs())
+    rg, ru = eg + e * g.abs() + tiny, eu + e * u.abs() + tiny
+    es = 0.8 * rg + (1 + g.abs()) * 2.0**-21
+    ea = 1.13 * rg + g.abs() * 2.0**-22
+    dg, du = dh * u * slope, dh * act
+    edg = edh * (u * slope).abs() + dh.abs() * (ru * slope.abs() + u.abs() * es) + e * dg.abs() + tiny
+    edu = edh * act.abs() + dh.abs() * ea + e * du.abs() + tiny
+    dx = dg @ gate + du @ up
+    found["x"] = (dx, edg @ gate.abs() + edu @ up.abs() + 2 * hidden * f * (dg.abs() @ gate.abs() + du.abs() @ up.abs())
+                  + e * dx.abs() + tiny)
+    for name, p, ep, q, eq in (("gate", dg, edg, x, None), ("up", du, edu, x, None), ("down", dy, None, h, eh)):
+        value = p.T @ q
+        bound = rows * f * (p.abs().T @ q.abs()) + out * value.abs() + tiny
+        bound = bound + (p.abs().T @ eq if ep is None else ep.T @ q.abs())
+        found[name] = (value, bound)
+    return {name: (value, 1.05 * bound) for name, (value, bound) in found.items()}
+
+
+def _inputs(rows, k, hidden, n, dtype, weight_dtype, seed=0):
+    generator = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, std=1.0, to=dtype):
+        return (torch.randn(shape, generator=generator, device="cuda") * std).to(to)
+
+    shape = rows if isinstance(rows, tuple) else (rows,)
+    x, dy = normal(*shape, k), normal(*shape, n)
+    weights = [normal(hidden, k, std=2 * k**-0.5, to=weight_dtype), normal(hidden, k, std=k**-0.5, to=weight_dtype),
+               normal(n, hidden, std=hidden**-0.5, to=weight_dtype)]
+    return x, weights, dy
+
+
+def _verify(got, expected, shape=None):
+    for name, value in got.items():
+        reference, bound = expected[name]
+        error = (value.double().reshape(reference.shape) - reference).abs()
+        assert torch.isfinite(value).all(), name
+        assert (error <= bound).all(), (name, float((error / bound).max()))
+
+
+def _run(native, x, weights, dy, kind, mask=None):
+    leaves = [v.detach().requires_grad_() for v in (x, *weights)]
+    y = native.gated_feed_forward(*leaves, activation=kind, row_mask=mask)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert y.is_contiguous() and y.dtype == x.dtype
+    for grad, leaf in zip(grads, leaves):
+        assert grad.shape == leaf.shape and grad.dtype == leaf.dtype
+    return dict(zip(("y", "x", "gate", "up", "down"), (y.detach(), *grads)))
+
+
+def _check(native, rows, k, hidden, n, dtype, kind="silu", weight_dtype=None, mask=None, seed=0):
+    weight_dtype = dtype if weight_dtype is None else weight_dtype
+    x, weights, dy = _inputs(rows, k, hidden, n, dtype, weight_dtype, seed)
+    got = _run(native, x, weights, dy, kind, mask)
+    _verify(got, _expected(x, weights, dy, kind, dtype, weight_dtype, mask))
+    with torch.no_grad():
+        assert torch.equal(native.gated_feed_forward(x, *weights, activation=kind, row_mask=mask), got["y"])
+    again = _run(native, x, weights, dy, kind, mask)
+    assert all(torch.equal(got[name], again[name]) for name in got)
+    return got
+
+
+def test_formula_against_differences() -> None:
+    """The bound's own formulas: gradients by central differences in FP64."""
+
+    torch.manual_seed(0)
+    x, dy = torch.randn(3, 4).double(), torch.randn(3, 2).double()
+    weights = [torch.randn(5, 4).double(), torch.randn(5, 4).double(), torch.randn(2, 5).double()]
+    for kind in ("silu", "gelu"):
+        value = lambda: _expected(x, weights, dy, kind, torch.float64, torch.float64)  # noqa: E731
+        found = value()
+        for name, leaf in zip(("x", "gate", "up", "down"), (x, *weights)):
+            flat = leaf.reshape(-1)
+            for i in range(flat.numel()):
+                at, step = float(flat[i]), 1e-5
+                ends = []
+                for to in (at + step, at - step):
+                    flat[i] = to
+                    ends.append(float((value()["y"][0] * dy).sum()))
+                flat[i] = at
+                assert abs((ends[0] - ends[1]) / (2 * step) - float(found[name][0].reshape(-1)[i])) < 1e-7
+
+
+def test_module_on_the_cpu() -> None:
+    layer = GatedFeedForward(6, 10, activation="gelu").double()
+    x = torch.randn(2, 3, 6, dtype=torch.float64, requires_grad=True)
+    mask = torch.tensor([[True, False, True], [False, False, False]])
+    y = layer(x, mask)
+    y.sum().backward()
+    expected = _expected(x.detach(), [layer.gate.weight.detach(), layer.up.weight.detach(), layer.down.weight.detach()],
+                         torch.ones(2, 3, 6, dtype=torch.float64), "gelu", torch.float64, torch.float64, mask)
+    for name, value in (("y", y), ("x", x.grad), ("gate", layer.gate.weight.grad), ("down", layer.down.weight.grad)):
+        torch.testing.assert_close(value.detach().reshape(expected[name][0].shape), expected[name][0])
+    assert not y[1].any() and not x.grad[1].any()
+    for wrong in ({"hidden": 0}, {"activation": "relu"}):
+        with pytest.raises(ValueError):
+            GatedFeedForward(**{"dim": 4, "hidden": 4, **wrong})
+    with pytest.raises(ValueError):
+        layer(x, implementation="other")
+
+
+def _shape(rows=4, k=16, hidden=24, n=16, stride=16, dtype=2, weight=2, activation=1):
+    return block.FeedForwardShape(rows, k, hidden, n, stride, dtype, weight, activation)
+
+
+def test_refusals_on_the_cpu() -> None:
+    library = hip.open_library()
+    size, other = ctypes.c_size_t(), ctypes.c_size_t()
+
+    def forward(shape=_shape(), x=16, gate=16, up=16, down=16, gates=None, product=None, y=16, workspace=256,
+                room=1 << 20):
+        return library.lsso_hip_feed_forward(ctypes.byref(shape), x, gate, up, down, None, gates, product, y, workspace,
+                                             room, None)
+
+    def backward(shape=_shape(), dy=16, stride=16, x=16, down=16, gates=16, product=16, grad_gate=16, workspace=256,
+                 room=1 << 20):
+        return library.lsso_hip_feed_forward_backward(ctypes.byref(shape), dy, stride, x, 16, 16, down, None, gates,
+                                                      product, None, grad_gate, None, None, workspace, room, None)
+
+    wrong_shapes = [_shape(rows=-1), _shape(k=0, stride=0), _shape(hidden=0), _shape(n=0), _shape(stride=15),
+                    _shape(dtype=3), _shape(weight=1), _shape(activation=0), _shape(activation=3),
+                    _shape(rows=2**31), _shape(hidden=2**20 + 1)]
+    for shape in wrong_shapes:
+        assert library.lsso_hip_feed_forward_workspace_bytes(ctypes.byref(shape), 0, ctypes.byref(size)) < 0
+        assert library.lsso_hip_feed_forward_kept(ctypes.byref(shape), ctypes.byref(size), ctypes.byref(other)) < 0
+        assert forward(shape=shape) < 0 and backward(shape=shape) < 0
+    assert forward(shape=_shape(rows=0), x=None, y=None, workspace=None, room=0) == 0
+    for wrong in ({"x": None}, {"gate": None}, {"down": None}, {"y": None}, {"x": 24}, {"up": 24}, {"gates": 16},
+                  {"product": 16}, {"gates": 24, "product": 16}, {"workspace": None}, {"workspace": 128}, {"room": 16}):
+        assert forward(**wrong) < 0, wrong
+    for wrong in ({"dy": None}, {"dy": 24}, {"stride": 15}, {"x": None}, {"down": 24}, {"gates": None},
+                  {"product": None}, {"workspace": None}, {"workspace": 128}, {"room": 16}):
+        assert backward(**wrong) < 0, wrong
+    shape = _shape(hidden=25)
+    assert library.lsso_hip_feed_forward_kept(ctypes.byref(shape), ctypes.byref(size), ctypes.byref(other)) == 0
+    assert (size.value, other.value) == (2 * 4 * 32, 4 * 32)
+    for mask in (-1, 8):
+        assert library.lsso_hip_feed_forward_backward_workspace_bytes(ctypes.byref(shape), 16, mask,
+                                                                      ctypes.byref(size)) < 0
+    assert library.lsso_hip_feed_forward_backward_workspace_bytes(ctypes.byref(shape), 15, 7, ctypes.byref(size)) < 0
+
+
+def test_workspaces_hold_every_size() -> None:
+    library = hip.open_library()
+    size = ctypes.c_size_t()
+    for rows in (0, 1, 63, 64, 513, 4104, 131072, 2**31 - 1):
+        for k, hidden, n in ((1, 1, 1), (8, 8, 8), (300, 801, 300), (768, 2048, 768), (4096, 16384, 4096)):
+            for weight in (2, 3):
+                shape = _shape(rows, k, hidden, n, k, weight=weight)
+                for training in (0, 1):
+                    assert library.lsso_hip_feed_forward_workspace_bytes(
+                        ctypes.byref(shape), training, ctypes.byref(size)) == 0
+                    copies = (k % 8 != 0) * 2 * rows * ((k + 7) // 8 * 8)
+                    assert size.value >= copies + (0 if training else 2 * rows * hidden)
+                assert library.lsso_hip_feed_forward_backward_workspace_bytes(
+                    ctypes.byref(shape), n, 7, ctypes.byref(size)) == 0
+                assert size.value >= 4 * rows * hidden
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("rows", (1, 2, 17, 33, 64, 65, 200))
+def test_rows(native, dtype, kind, rows) -> None:
+    _check(native, rows, 64, 136, 48, dtype, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("widths", [(8, 8, 8), (1, 1, 1), (7, 9, 3), (16, 24, 40), (33, 65, 31), (100, 266, 100),
+                                    (300, 801, 300), (64, 70, 521), (521, 64, 72), (256, 688, 256), (40, 1000, 24)])
+@pytest.mark.parametrize("dtype", HALVES)
+def test_widths(native, widths, dtype) -> None:
+    _check(native, 70, *widths, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("widths", [(64, 136, 48), (33, 65, 31)])
+@pytest.mark.parametrize("dtype", HALVES)
+def test_float32_weights(native, widths, dtype) -> None:
+    _check(native, 150, *widths, dtype, weight_dtype=torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,hidden,n", [(1576, 192, 512, 192), (4104, 300, 801, 300), (3000, 640, 256, 1040),
+                                             (20000, 64, 2112, 64), (40000, 72, 520, 264), (66000, 32, 64, 264)])
+def test_large_tiles_and_row_ranges(native, rows, k, hidden, n) -> None:
+    _check(native, rows, k, hidden, n, torch.bfloat16, "gelu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,hidden,n", [((3, 70), 64, 136, 48), ((2, 33), 33, 65, 31), ((8, 513), 128, 256, 128),
+                                             ((16, 2500), 64, 264, 136)])
+def test_masked_rows_may_hold_anything(native, rows, k, hidden, n) -> None:
+    dtype = torch.bfloat16
+    mask = torch.rand(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.7
+    mask[-1] = False
+    x, weights, dy = _inputs(rows, k, hidden, n, dtype, dtype)
+    expected = _expected(x, weights, dy, "silu", dtype, dtype, mask)
+    x[~mask], dy[~mask] = math.nan, math.inf
+    got = _run(native, x, weights, dy, "silu", mask)
+    _verify(got, expected)
+    assert not got["y"][~mask].any() and not got["x"][~mask].any()
+    nothing = _run(native, x, weights, dy, "silu", torch.zeros_like(mask))
+    assert not any(value.any() for value in nothing.values())
+
+
+@pytest.mark.gpu
+def test_masked_rows_equal_the_rows_alone(native) -> None:
+    x, weights, _ = _inputs((4, 100), 96, 264, 96, torch.float16, torch.float16)
+    mask = torch.zeros(4, 100, dtype=torch.bool, device="cuda")
+    mask[:, :37] = True
+    y = native.gated_feed_forward(x, *weights, row_mask=mask)
+    assert torch.equal(y[mask], native.gated_feed_forward(x, *weights)[mask])
+
+
+@pytest.mark.gpu
+def test_layouts(native) -> None:
+    x, weights, dy = _inputs((5, 30), 64, 72, 40, torch.bfloat16, torch.bfloat16)
+    plain = _run(native, x, weights, dy, "silu")
+    wide = torch.full((5, 30, 70), math.nan, device="cuda", dtype=torch.bfloat16)
+    for first, stop in ((0, 64), (3, 67)):   # rows of 140 bytes; an odd base
+        view = wide[..., first:stop]
+        view.copy_(x)
+        spread = torch.full((5, 30, 48), math.nan, device="cuda", dtype=torch.bfloat16)[..., 5:45]
+        spread.copy_(dy)
+        moved = [w.t().contiguous().t() for w in weights]
+        got = _run(native, view, moved, spread, "silu")
+        assert all(torch.equal(got[name], plain[name]) for name in plain)
+    padded = torch.full((5, 30, 80), math.nan, device="cuda", dtype=torch.bfloat16)
+    padded[..., :64] = x   # whole pieces, read in place; NaN behind each row
+    got = _run(native, padded[..., :64], weights, dy, "silu")
+    assert all(torch.equal(got[name], plain[name]) for name in plain)
+    got = _run(native, x.transpose(0, 1).contiguous().transpose(0, 1), weights, dy, "silu")
+    assert all(torch.equal(got[name], plain[name]) for name in plain)
+    leaves = [v.detach().requires_grad_() for v in (x, *weights)]
+    ones = torch.autograd.grad(native.gated_feed_forward(*leaves).sum(), leaves)   # stride-0 gradient
+    expected = torch.autograd.grad(native.gated_feed_forward(*leaves), leaves, torch.ones_like(dy))
+    assert all(torch.equal(a, b) for a, b in zip(ones, expected))
+
+
+@pytest.mark.gpu
+def test_gradients_asked_for_one_by_one(native) -> None:
+    x, weights, dy = _inputs(130, 64, 136, 48, torch.bfloat16, torch.bfloat16)
+    whole = _run(native, x, weights, dy, "gelu")
+    for name, wanted in (("x", 0), ("gate", 1), ("up", 2), ("down", 3)):
+        values = [v.detach() for v in (x, *weights)]
+        values[wanted].requires_grad_()
+        y = native.gated_feed_forward(*values, activation="gelu")
+        (grad,) = torch.autograd.grad(y, values[wanted], dy)
+        assert torch.equal(grad, whole[name]), name
+
+
+@pytest.mark.gpu
+def test_empty_batches_and_vectors(native) -> None:
+    x, weights, dy = _inputs((0, 5), 16, 24, 8, torch.float16, torch.float16)
+    got = _run(native, x, weights, dy, "silu")
+    assert got["y"].shape == (0, 5, 8) and not any(got[name].any() for name in ("gate", "up", "down"))
+    x, weights, dy = _inputs((), 16, 24, 8, torch.float16, torch.float16)
+    _verify(_run(native, x, weights, dy, "silu"), _expected(x[None], weights, dy[None], "silu", torch.float16, torch.float16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+def test_saturated_gates(native, kind) -> None:
+    """Gates of +-1 to +-3e4 in both types: no NaN from an exponential's range."""
+
+    for dtype in HALVES:
+        x = torch.eye(16, device="cuda", dtype=dtype)
+        gates = torch.logspace(0, 4.4, 16, device="cuda")
+        gate = torch.diag(torch.where(torch.arange(16, device="cuda") % 2 == 0, gates, -gates)).to(dtype)
+        up = torch.eye(16, device="cuda", dtype=dtype)
+        down = torch.eye(16, device="cuda", dtype=dtype)
+        dy = torch.ones(16, 16, device="cuda", dtype=dtype)
+        got = _run(native, x, [gate, up, down], dy, kind)
+        value, slope = _act(torch.diagonal(gate).double(), kind)
+        limit = torch.finfo(dtype).eps * value.abs() * 2 + gates.double() * 2.0**-22 + 2.0**-24
+        assert ((torch.diagonal(got["y"]).double() - value).abs() <= limit).all()
+        limit = torch.finfo(dtype).eps * slope.abs() * 2 + (1 + gates.double()) * 2.0**-21 + 2.0**-24
+        assert ((torch.diagonal(got["gate"]).double() - slope).abs() <= limit).all()
+
+
+@pytest.mark.gpu
+def test_captured_training_step(native) -> None:
+    x, weights, dy = _inputs((4, 65), 64, 136, 64, torch.bfloat16, torch.bfloat16)
+    x.requires_grad_()
+    for w in weights:
+        w.requires_grad_()
+    mask = torch.ones(4, 65, dtype=torch.bool, device="cuda")
+    mask[1, 40:] = False
+
+    def step():
+        y = native.gated_feed_forward(x, *weights, row_mask=mask)
+        return (y.detach(), *torch.autograd.grad(y, (x, *weights), dy))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.normal_()
+            dy.normal_()
+            mask[2, torch.randint(0, 65, (20,), device="cuda")] = False
+        graph.replay()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(native) -> None:
+    cases = [_inputs(300, 64, 520, 64, torch.bfloat16, torch.bfloat16, seed) for seed in (1, 2)]
+    expected = [_run(native, *case, "silu") for case in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    found = [None, None]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                found[i] = _run(native, *cases[i], "silu")
+    torch.cuda.synchronize()
+    for a, b in zip(found, expected):
+        assert all(torch.equal(a[name], b[name]) for name in b)
+
+
+@pytest.mark.gpu
+def test_refusals(native) -> None:
+    x, weights, _ = _inputs(4, 16, 24, 8, torch.float16, torch.float16)
+    gate, up, down = weights
+    for arguments, options, error in (
+        ((x.cpu(), gate, up, down), {}, RuntimeError), ((x, gate.cpu(), up, down), {}, RuntimeError),
+        ((x.float(), gate, up, down), {}, TypeError), ((x, gate.float(), up, down), {}, TypeError),
+        ((x, gate.bfloat16(), up.bfloat16(), down.bfloat16()), {}, TypeError),
+        ((x, gate, up[:8], down), {}, ValueError), ((x, gate, up, down[:, :8]), {}, ValueError),
+        ((x[:, :8], gate, up, down), {}, ValueError), ((x, gate[0], up, down), {}, ValueError),
+        ((x, gate, up, down), {"activation": "relu"}, ValueError),
+        ((x, gate, up, down), {"row_mask": torch.ones(3, dtype=torch.bool, device="cuda")}, ValueError),
+        ((x, gate, up, down), {"row_mask": torch.ones(4, dtype=torch.bool)}, RuntimeError),
+        ((x, gate, up, down[:0]), {}, ValueError),
+    ):
+        with pytest.raises(error):
+            native.gated_feed_forward(*arguments, **options)
