@@ -609,7 +609,7 @@ int lsso_hip_feed_forward_workspace_bytes(const lsso_hip_feed_forward_shape* sha
  * product.  row_mask: optional device uint8 [rows]; rows whose byte is 0 are
  * written as zeros whatever their x holds.  gates, product: both NULL, or the
  * buffers that the backward reads (lsso_hip_feed_forward_kept, 16-byte
- * aligned).  workspace: 256-byte aligned.  rows may be 0. */
+ * aligned): u act'(g) and act(g), and their forward product act(g) u.  workspace: 256-byte aligned.  rows may be 0. */
 int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* x,
                           const void* gate_weight, const void* up_weight, const void* down_weight,
                           const uint8_t* row_mask, void* gates, void* product, void* y,

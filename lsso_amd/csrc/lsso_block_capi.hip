@@ -114,14 +114,21 @@ const uint16_t* bind(FeedForwardPlan* plan, const Packed& p, const void* from, i
         return static_cast<const uint16_t*>(from);
     }
     uint16_t* to = reinterpret_cast<uint16_t*>(workspace + p.offset);
-    plan->pack.matrices[plan->pack.count++] = {from, stride, columns, p.stride, wide, to, rows * p.stride / 8};
+    plan->pack.matrices[plan->pack.count++] = {from, stride, rows, columns, wide, 0, to, p.stride, 0};
     return to;
+}
+
+// The transpose of `from` [rows, columns] as rows of `pitch` values at `to`.
+void transpose(FeedForwardPlan* plan, const void* from, int64_t rows, int64_t columns, bool wide, uint16_t* to,
+               int64_t pitch) {
+    plan->pack.matrices[plan->pack.count++] = {from, columns, rows, columns, wide, 1, to, pitch, 0};
 }
 
 struct FeedForwardLayout {
     FeedForwardPlan plan;
     Packed x, gate, up, down, dy;
     size_t h = 0, partials = 0, grads = 0, weight_partials = 0;
+    size_t in_columns = 0, down_columns = 0;   // [gate^T | up^T] [in, 2 pitch], down^T [hidden, out_pitch]
 };
 
 void common_args(const lsso_hip_feed_forward_shape& s, lsso_hip::FeedForwardArgs* a) {
@@ -133,10 +140,9 @@ void common_args(const lsso_hip_feed_forward_shape& s, lsso_hip::FeedForwardArgs
     a->in_pitch = round8(s.in_features);
     a->pitch = round8(s.hidden);
     a->out_pitch = round8(s.out_features);
-    a->down_pitch = a->pitch;
 }
 
-int64_t stages_of(int64_t k) { return (k + 31) / 32; }
+int64_t stages_of(int64_t k) { return (k + 63) / 64; }
 
 FeedForwardLayout forward_layout(const lsso_hip_feed_forward_shape& s, bool training) {
     FeedForwardLayout l;
@@ -192,15 +198,14 @@ void weight_products(const lsso_hip_feed_forward_shape& s, const bool (&wanted)[
 FeedForwardLayout backward_layout(const lsso_hip_feed_forward_shape& s, int64_t grad_stride, const bool (&wanted)[3]) {
     FeedForwardLayout l;
     common_args(s, &l.plan.args);
-    const bool wide = s.weight_type == LSSO_HIP_F32;
+    const lsso_hip::FeedForwardArgs& a = l.plan.args;
     l.x = place(&l.plan, s.rows, s.in_features, s.x_stride, false);
-    l.gate = place(&l.plan, s.hidden, s.in_features, s.in_features, wide);
-    l.up = place(&l.plan, s.hidden, s.in_features, s.in_features, wide);
-    l.down = place(&l.plan, s.out_features, s.hidden, s.hidden, wide);
     l.dy = place(&l.plan, s.rows, s.out_features, grad_stride, false);
-    l.grads = l.plan.take(4 * static_cast<size_t>(s.rows) * static_cast<size_t>(l.plan.args.pitch));
+    l.in_columns = l.plan.take(2 * static_cast<size_t>(s.in_features) * 2 * static_cast<size_t>(a.pitch));
+    l.down_columns = l.plan.take(2 * static_cast<size_t>(s.hidden) * static_cast<size_t>(a.out_pitch));
+    l.grads = l.plan.take(4 * static_cast<size_t>(s.rows) * static_cast<size_t>(a.pitch));
     lsso_hip::FeedForwardProduct& dx = l.plan.product;
-    lsso_hip::plan_product(s.rows, s.in_features, 2 * stages_of(l.plan.args.pitch), &dx);
+    lsso_hip::plan_product(s.rows, s.in_features, stages_of(2 * a.pitch), &dx);
     if (dx.splits > 1) {
         l.partials = l.plan.take(4 * static_cast<size_t>(dx.splits) * static_cast<size_t>(s.rows) *
                                  static_cast<size_t>(dx.partial_pitch));
@@ -286,11 +291,10 @@ int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* 
     p.rows = s.rows;
     p.k = a.pitch;
     p.q = a.down;
-    p.q_stride = a.down_pitch;
+    p.q_stride = a.pitch;
     p.row_mask = row_mask;
     p.out = static_cast<uint16_t*>(y);
     p.columns = s.out_features;
-    p.segment_stages = p.stages;
     p.partials = reinterpret_cast<float*>(ws + l.partials);
     const auto queue = static_cast<hipStream_t>(stream);
     hipError_t error = lsso_hip::launch_feed_forward_pack(l.plan.pack, s.dtype, queue);
@@ -298,7 +302,7 @@ int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* 
         error = lsso_hip::launch_feed_forward_gate(a, queue);
     }
     if (error == hipSuccess) {
-        error = lsso_hip::launch_feed_forward_product(p, true, queue);
+        error = lsso_hip::launch_feed_forward_product(p, queue);
     }
     return error == hipSuccess ? LSSO_HIP_OK : report_hip(error, "feed-forward launch");
 }
@@ -353,19 +357,27 @@ int lsso_hip_feed_forward_backward(const lsso_hip_feed_forward_shape* shape, con
     lsso_hip::FeedForwardArgs& a = l.plan.args;
     a.x = bind(&l.plan, l.x, x, s.rows, s.in_features, s.x_stride, false, ws);
     a.x_stride = l.x.stride;
-    a.gate = bind(&l.plan, l.gate, gate_weight, s.hidden, s.in_features, s.in_features, wide, ws);
-    a.up = bind(&l.plan, l.up, up_weight, s.hidden, s.in_features, s.in_features, wide, ws);
-    a.down = bind(&l.plan, l.down, down_weight, s.out_features, s.hidden, s.hidden, wide, ws);
     a.dy = bind(&l.plan, l.dy, grad_y, s.rows, s.out_features, grad_stride, false, ws);
     a.dy_stride = l.dy.stride;
     a.row_mask = row_mask;
     a.gates = static_cast<uint16_t*>(const_cast<void*>(gates));
     a.grads = reinterpret_cast<uint16_t*>(ws + l.grads);
+    uint16_t* const in_columns = reinterpret_cast<uint16_t*>(ws + l.in_columns);
+    uint16_t* const down_columns = reinterpret_cast<uint16_t*>(ws + l.down_columns);
+    a.down_columns = down_columns;
+    const bool through = grad_x != nullptr || wanted[0] || wanted[1];   // dg and du are needed
+    if (through) {
+        transpose(&l.plan, down_weight, s.out_features, s.hidden, wide, down_columns, a.out_pitch);
+    }
+    if (grad_x != nullptr) {
+        transpose(&l.plan, gate_weight, s.hidden, s.in_features, wide, in_columns, 2 * a.pitch);
+        transpose(&l.plan, up_weight, s.hidden, s.in_features, wide, in_columns + a.pitch, 2 * a.pitch);
+    }
     const auto queue = static_cast<hipStream_t>(stream);
     hipError_t error = hipSuccess;
     if (s.rows > 0) {
         error = lsso_hip::launch_feed_forward_pack(l.plan.pack, s.dtype, queue);
-        if (error == hipSuccess && (grad_x != nullptr || wanted[0] || wanted[1])) {
+        if (error == hipSuccess && through) {
             error = lsso_hip::launch_feed_forward_grad(a, queue);
         }
     }
@@ -374,20 +386,15 @@ int lsso_hip_feed_forward_backward(const lsso_hip_feed_forward_shape* shape, con
         p.type = s.dtype;
         p.p = a.grads;
         p.p_stride = 2 * a.pitch;
-        p.p_second = a.pitch;
         p.rows = s.rows;
-        p.k = a.pitch;
-        p.q = a.gate;
-        p.q_second = a.up;
-        p.q_stride = a.in_pitch;
-        p.q_lines = s.hidden;
-        p.q_pitch = a.in_pitch;
+        p.k = 2 * a.pitch;
+        p.q = in_columns;
+        p.q_stride = 2 * a.pitch;
         p.row_mask = row_mask;
         p.out = static_cast<uint16_t*>(grad_x);
         p.columns = s.in_features;
-        p.segment_stages = p.stages / 2;
         p.partials = reinterpret_cast<float*>(ws + l.partials);
-        error = lsso_hip::launch_feed_forward_product(p, false, queue);
+        error = lsso_hip::launch_feed_forward_product(p, queue);
     }
     lsso_hip::FeedForwardWeights& w = l.plan.weights;
     if (error == hipSuccess && w.count > 0) {

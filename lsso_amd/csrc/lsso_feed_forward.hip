@@ -1,18 +1,22 @@
 // Gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wd^T, and its
 // gradients.  All products are the tiled loop of lsso_product.h:
 //
-//   gate_kernel    g, u = x Wg^T, x Wu^T in one pass over x; h = act(g) * u
-//                  from the FP32 accumulators.  Training also keeps g and u.
+//   gate_kernel    g, u = x Wg^T, x Wu^T in one pass over x; h = act(g) u from
+//                  the FP32 accumulators.  Training also keeps the two factors
+//                  of the backward, u act'(g) and act(g): rounded once, where
+//                  kept g and u would be rounded before them (gradients off by
+//                  sqrt(3) instead of 1.85 output roundings), and the backward
+//                  evaluates no activation.
 //   product_kernel y = h Wd^T, and in the backward dx = dg Wg + du Wu
-//   grad_kernel    dh = dy Wd, and from it dg = dh u act'(g), du = dh act(g)
+//   grad_kernel    dh = dy Wd, and from it dg = dh (u act'(g)), du = dh act(g)
 //   weight_kernel  dWg = dg^T x, dWu = du^T x, dWd = dy^T h in one launch,
 //                  over row ranges whose FP32 partials join_kernel adds in order
 //
 // Operands are 16-bit values of x's type: x, the weights (FP32 weights are
-// rounded once per call, as the projections round theirs) and g, u, h, dg, du,
+// rounded once per call, as the projections round theirs) and h, dg and du,
 // which are rounded once when they are stored, because the products that take
-// them run on 16-bit matrix instructions.  g and u keep [rows, 2, Fp] and h
-// [rows, Fp], Fp the hidden width rounded up to 8 with zeros behind it, so
+// them run on 16-bit matrix instructions.  The kept factors lie as [rows, 2, Fp],
+// as do dg and du, and h as [rows, Fp], Fp the hidden width rounded up to 8 with zeros behind it, so
 // every row is whole 16-byte pieces.  Operands whose own rows are not (odd
 // widths or strides) are copied into such rows first: element loads in the
 // product's loop cost more than one more pass over x.
@@ -32,64 +36,138 @@ namespace lsso_hip {
 
 namespace {
 
-// act(g) and act'(g), FP32.
+// act(g), and with SLOPE act'(g), FP32.  SiLU: g / (1 + exp(-g)); an exponential
+// that overflows leaves a sigmoid of 0.  GELU: g Phi(g), with Phi's tail
+// Phi(-|g|) = t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| /
+// sqrt(2)), from Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi);
+// the exponential is also that of the derivative's normal density.  The error
+// function of the device library in its place took about twice the epilogue's
+// vector instructions.
+template <bool SLOPE>
 __device__ __forceinline__ void activation(int kind, float g, float& value, float& slope) {
     if (kind == LSSO_HIP_SILU) {
-        // g far below zero: exp overflows to infinity and the sigmoid is 0.
-        const float s = 1.0f / (1.0f + __expf(-g));
+        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
         value = g * s;
-        slope = s * (1.0f + g * (1.0f - s));
+        slope = SLOPE ? s * (1.0f + g * (1.0f - s)) : 0.0f;
     } else {
-        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        const float x = fabsf(g);
+        const float t = __builtin_amdgcn_rcpf(1.0f + (0.3275911f * 0.70710678f) * x);
+        const float e = __expf(-0.5f * g * g);
+        const float poly =
+            t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float tail = 0.5f * poly * e;
+        const float cdf = g < 0.0f ? tail : 1.0f - tail;
         value = g * cdf;
-        slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+        slope = SLOPE ? cdf + 0.39894228f * g * e : 0.0f;
     }
 }
 
-__device__ __forceinline__ void activation(int kind, float g, float& value) {
-    if (kind == LSSO_HIP_SILU) {
-        value = g * (1.0f / (1.0f + __expf(-g)));
-    } else {
-        value = g * (0.5f * (1.0f + erff(g * 0.70710678118654752f)));
-    }
-}
-
-// Tile of this workgroup: columns fastest, so that the tiles that share P's
-// rows follow each other on one XCD.
-struct Tile {
-    int64_t p0;
-    int64_t q0;
-};
-__device__ __forceinline__ Tile tile_of(int64_t q_tiles, int64_t tiles, int bp, int bq) {
-    const int64_t block = xcd_local_block(blockIdx.x, tiles);
-    const int64_t p = block / q_tiles;
-    return {p * bp, (block - p * q_tiles) * bq};
-}
-
-// Loads of one operand in rows: stage s of [k0, k1) of the rows from `base`.
-template <typename Layout>
-struct RowLoads {
-    BufferRsrc buffer;
+// Q's loads in rows: lines are the tile's columns.
+template <typename Stage>
+struct QRowLoads {
     uint32_t offset;       // this lane's line and element, bytes
     uint32_t step;         // bytes between the lines of consecutive loads
-    int64_t element;       // this lane's element of stage 0
-    int64_t elements;
+    int element;           // this lane's element of stage 0
+    int elements;
 
-    __device__ __forceinline__ RowLoads(const Operand& o, int wave, int lane, int64_t most_lines)
-        : buffer(lines(o, most_lines)),
-          offset(static_cast<uint32_t>(2 * (Layout::load_line(wave, lane, 0) * o.stride +
-                                            Layout::load_element(wave, lane)))),
-          step(static_cast<uint32_t>(2 * 64 * o.stride)),
-          element(Layout::load_element(wave, lane)),
-          elements(o.elements) {}
-    // The same lines of another matrix of this stride.
-    __device__ __forceinline__ static BufferRsrc lines(const Operand& o, int64_t most_lines) {
-        return make_buffer(o.base, 2 * (o.lines < most_lines ? o.lines : most_lines) * o.stride);
+    __device__ __forceinline__ QRowLoads(int64_t stride, int64_t k_elements, int wave, int lane)
+        : step(static_cast<uint32_t>(2 * 32 * stride)),
+          elements(static_cast<int>(k_elements)) {
+        element = Stage::load_element(wave, lane);
+        offset = static_cast<uint32_t>(2 * (Stage::load_row(wave, lane, 0) * stride + element));
     }
-    __device__ __forceinline__ void issue(char* lds, int wave, int64_t k, int j) const { issue(buffer, lds, wave, k, j); }
-    __device__ __forceinline__ void issue(BufferRsrc buffer, char* lds, int wave, int64_t k, int j) const {
-        const uint32_t at = k + element < elements ? offset + j * step + static_cast<uint32_t>(2 * k) : kOutOfRange;
-        load_to_lds(buffer, lds + 1024 * (4 * j + wave), at);
+    __device__ __forceinline__ static BufferRsrc lines(const uint16_t* base, int64_t stride, int64_t rows, int most) {
+        return make_buffer(base, 2 * (rows < most ? rows : most) * stride);
+    }
+    __device__ __forceinline__ void issue(BufferRsrc buffer, char* lds, int wave, int k, int j, int line_step) const {
+        load_to_lds(buffer, lds + 1024 * (4 * j + wave),
+                    k + element < elements ? offset + line_step * step + static_cast<uint32_t>(2 * k) : kOutOfRange);
+    }
+};
+
+// P's fragments: MB blocks of 16 rows, 8 k per lane.
+template <int MB>
+struct PRowLoads {
+    uint32_t offset;
+    uint32_t step;         // bytes between blocks
+    int element;
+    int elements;
+
+    __device__ __forceinline__ PRowLoads(int64_t stride, int64_t k_elements, int wave, int lane)
+        : offset(static_cast<uint32_t>(2 * ((16 * MB * wave + (lane & 15)) * stride + 8 * (lane >> 4)))),
+          step(static_cast<uint32_t>(2 * 16 * stride)),
+          element(8 * (lane >> 4)),
+          elements(static_cast<int>(k_elements)) {}
+    __device__ __forceinline__ static BufferRsrc lines(const uint16_t* base, int64_t stride, int64_t rows) {
+        return make_buffer(base, 2 * (rows < 64 * MB ? rows : 64 * MB) * stride);
+    }
+    __device__ __forceinline__ void load(BufferRsrc buffer, int k, u32x4 (&fragments)[MB]) const {
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            fragments[m] = buffer_load16(
+                buffer, k + element < elements ? offset + m * step + static_cast<uint32_t>(2 * k) : kOutOfRange);
+        }
+    }
+};
+
+// Both operands' loads of consecutive tiles, stages [first, last) of each: P
+// [rows, k] and Q [columns, k].
+template <typename S>
+struct RowStream {
+    using Q = typename S::QStage;
+    const uint16_t* p_base;
+    int64_t p_stride;
+    int64_t rows;
+    const uint16_t* q_base;
+    int64_t q_stride;
+    int64_t columns;
+    int first;
+    int last;
+    int wave;
+    PRowLoads<S::MB> p;
+    QRowLoads<Q> q;
+    TileWalk p_walk;
+    TileWalk q_walk;
+    int slot;
+    int stage;
+    BufferRsrc p_rows;
+    BufferRsrc q_rows;
+
+    __device__ __forceinline__ RowStream(const uint16_t* p_base_, int64_t p_stride_, int64_t rows_,
+                                         const uint16_t* q_base_, int64_t q_stride_, int64_t columns_, int64_t k,
+                                         int first_, int last_, const TileWalk& walk, int wave_, int lane)
+        : p_base(p_base_), p_stride(p_stride_), rows(rows_), q_base(q_base_), q_stride(q_stride_), columns(columns_),
+          first(first_), last(last_), wave(wave_), p(p_stride_, k, wave_, lane), q(q_stride_, k, wave_, lane),
+          p_walk(walk), q_walk(walk), slot(2 * first_), stage(first_) {
+        aim_p();
+        aim_q();
+    }
+    __device__ __forceinline__ void aim_p() {
+        const int64_t p0 = static_cast<int64_t>(p_walk.p) * S::BP;
+        p_rows = PRowLoads<S::MB>::lines(p_base + p0 * p_stride, p_stride, p_walk.left > 0 ? rows - p0 : 0);
+    }
+    __device__ __forceinline__ void aim_q() {
+        const int64_t q0 = static_cast<int64_t>(q_walk.q) * S::BQ;
+        q_rows = QRowLoads<Q>::lines(q_base + q0 * q_stride, q_stride, q_walk.left > 0 ? columns - q0 : 0, S::BQ);
+    }
+    __device__ __forceinline__ void load_p(u32x4 (&fragments)[S::MB]) {
+        p.load(p_rows, slot * kSlotK, fragments);
+        if (++slot == 2 * last) {
+            slot = 2 * first;
+            p_walk.next();
+            aim_p();
+        }
+    }
+    __device__ __forceinline__ void issue_q(char* lds) {
+#pragma unroll
+        for (int j = 0; j < Q::kLoads; ++j) {
+            q.issue(q_rows, lds, wave, stage * kRowsStageK, j, j);
+        }
+        if (++stage == last) {
+            stage = first;
+            q_walk.next();
+            aim_q();
+        }
     }
 };
 
@@ -119,251 +197,351 @@ struct ColumnLoads {
     }
 };
 
-// ---------------------------------------------------------------- h, g and u
-// Q is [gate rows | up rows] of the tile's 32 NB columns of h: wave column w
-// takes gate columns 32 w .. and the same up columns, so a lane holds both
-// factors of its products.
-template <int T, int MB, bool KEEP>
-__global__ __launch_bounds__(kProductThreads, 2) void gate_kernel(FeedForwardArgs a) {
-    using S = ProductShape<T, true, true, MB, 2>;
-    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-    const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
-    constexpr int kColumns = S::BQ / 2;
-    const Tile tile = tile_of(a.q_tiles, a.tiles, S::BP, kColumns);
-    const RowLoads<typename S::PLayout> x({a.x + tile.p0 * a.x_stride, a.x_stride, a.rows - tile.p0, a.in_pitch}, wave,
-                                          lane, S::BP);
-    // Load 0 of Q is rows 0 .. 63 of its stage, load 1 rows 64 .. 127.
-    const RowLoads<typename S::QLayout> gate({a.gate + tile.q0 * a.in_pitch, a.in_pitch, a.hidden - tile.q0,
-                                              a.in_pitch}, wave, lane, kColumns);
-    const RowLoads<typename S::QLayout> up({a.up + tile.q0 * a.in_pitch, a.in_pitch, a.hidden - tile.q0, a.in_pitch},
-                                           wave, lane, kColumns);
-    static_assert(S::QLayout::kLoads == 2 && kColumns == 64, "one load of each weight");
-    f32x16 acc[2][MB];
-    run_product<S>(
-        lds, a.stages, acc,
-        [&](char* stage, int s) {
-            const int64_t k = static_cast<int64_t>(s) * kStageK;
+// FP32 rows of a wave's blocks into partials [rows, pitch] from row p0 and
+// column q0 on.  Blocks: 32 x 32 (lane & 31 the row, entry 4 q + e column 8 q + 4
+// half + e).
+template <typename S>
+__device__ __forceinline__ void store_partials(char* mine, int lane, const f32x16 (&acc)[S::NB][S::MB],
+                                               float* partials, int64_t pitch, int64_t p0, int64_t rows, int64_t q0) {
+    using Exchange = RowExchange<32, 128>;
+    static_assert(Exchange::kSize <= S::kWaveBytes, "the exchange fits the wave's LDS");
 #pragma unroll
-            for (int j = 0; j < S::PLayout::kLoads; ++j) {
-                x.issue(stage, wave, k, j);
-            }
-            char* q = stage + S::PLayout::kBytes;
-            gate.issue(q, wave, k, 0);
-            up.issue(q + 4096, wave, k, 0);
-        },
-        [&](int n) { return kColumns * n + 32 * (wave >> 1); });
-
-    const int half = lane >> 5;
-    const int64_t column = tile.q0 + 32 * (wave >> 1) + 8 * half;
+    for (int m = 0; m < S::MB; ++m) {
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-        const int64_t row = tile.p0 + 32 * (MB * (wave & 1) + m) + (lane & 31);
-        float g[2][8];
-        float u[2][8];
-        row_pieces(acc[0][m], g);
-        row_pieces(acc[1][m], u);
-        const bool inside = row < a.rows;
-        const bool kept = inside && (a.row_mask == nullptr || a.row_mask[row] != 0);
+        for (int n = 0; n < S::NB; ++n) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (!inside || column + 16 * c >= a.pitch) {
-                continue;
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = {acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
+                Exchange::put(mine, lane, 32 * q + 16 * (lane >> 5), v);
             }
-            float h[8];
+            wave_lds_order();
+            const int64_t column = q0 + 32 * n + Exchange::byte(lane) / 4;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float act;
-                activation(a.activation, g[c][e], act);
-                h[e] = kept ? act * u[c][e] : 0.0f;
+            for (int i = 0; i < Exchange::kSteps; ++i) {
+                const u32x4 value = Exchange::get(mine, lane, i);
+                const int64_t row = p0 + 32 * m + Exchange::row(lane, i);
+                if (row < rows && column < pitch) {
+                    *reinterpret_cast<u32x4*>(partials + row * pitch + column) = value;
+                }
             }
-            store16_unaligned(a.h + row * a.pitch + column + 16 * c, Values<T>::pack8(h));
-            if (KEEP) {
-                uint16_t* at = a.gates + 2 * row * a.pitch + column + 16 * c;
-                store16_unaligned(at, Values<T>::pack8(g[c]));
-                store16_unaligned(at + a.pitch, Values<T>::pack8(u[c]));
-            }
+            wave_lds_order();
         }
     }
 }
 
-// ------------------------------------------------------------------ y and dx
-// out = P Q^T over one or two K segments: y = h Wd^T (Q in rows, one segment)
-// or dx = dg Wg + du Wu (Q in columns, two).  With `splits` > 1 the stages are
-// divided and FP32 partials left for join_kernel.
-template <int T, bool Q_ROWS, int MB, int NB>
-__global__ __launch_bounds__(kProductThreads, 2) void product_kernel(FeedForwardProduct a) {
-    using S = ProductShape<T, true, Q_ROWS, MB, NB>;
-    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-    const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
-    const Tile tile = tile_of(a.q_tiles, a.tiles, S::BP, S::BQ);
-    const int split = blockIdx.y;
-    const int first = split * a.split_stages;
-    const int last = first + a.split_stages < a.stages ? first + a.split_stages : a.stages;
-    const Operand rows{a.p + tile.p0 * a.p_stride, a.p_stride, a.rows - tile.p0, a.k};
-    const RowLoads<typename S::PLayout> p(rows, wave, lane, S::BP);
-    f32x16 acc[NB][MB];
-    const auto q_start = [&](int n) { return 32 * (NB * (wave >> 1) + n); };
-    if constexpr (Q_ROWS) {
-        const RowLoads<typename S::QLayout> q({a.q + tile.q0 * a.q_stride, a.q_stride, a.columns - tile.q0, a.k}, wave,
-                                              lane, S::BQ);
-        run_product<S>(
-            lds, last - first, acc,
-            [&](char* stage, int s) {
-                const int64_t k = first + s < last ? static_cast<int64_t>(first + s) * kStageK : a.k;
-#pragma unroll
-                for (int j = 0; j < S::PLayout::kLoads; ++j) {
-                    p.issue(stage, wave, k, j);
-                }
-#pragma unroll
-                for (int j = 0; j < S::QLayout::kLoads; ++j) {
-                    q.issue(stage + S::PLayout::kBytes, wave, k, j);
-                }
-            },
-            q_start);
-    } else {
-        ColumnLoads<typename S::QLayout> q({a.q + tile.q0, a.q_stride, a.k, a.q_pitch - tile.q0}, wave, lane);
-        const uint16_t* const second_q = a.q_second + tile.q0;
-        const uint16_t* const first_q = q.base;
-        run_product<S>(
-            lds, last - first, acc,
-            [&](char* stage, int s) {
-                const int at = first + s;
-                const bool second = at >= a.segment_stages;
-                const int64_t k = at < last ? static_cast<int64_t>(at - (second ? a.segment_stages : 0)) * kStageK : a.k;
-                Operand of = rows;
-                of.base += second ? a.p_second : 0;
-                const BufferRsrc pb = RowLoads<typename S::PLayout>::lines(of, S::BP);
-#pragma unroll
-                for (int j = 0; j < S::PLayout::kLoads; ++j) {
-                    p.issue(pb, stage, wave, k, j);
-                }
-                q.base = second ? second_q : first_q;
-                const BufferRsrc qb = q.stage(k, a.q_lines);
-#pragma unroll
-                for (int j = 0; j < S::QLayout::kLoads; ++j) {
-                    q.issue(qb, stage + S::PLayout::kBytes, wave, j);
-                }
-            },
-            q_start);
-    }
-
-    const int half = lane >> 5;
+// ------------------------------------------------------- h and its two factors
+// Q is [gate rows | up rows] of the tile's 64 columns of h, so a lane holds both
+// factors of its products: block n < 4 the gate's, n + 4 the up's.
+template <int T, int MB, bool KEEP>
+__device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
+                                              const f32x4 (&acc)[8][MB]) {
+    // 16 rows at a time: 16-bit rows of 64 columns through the exchange, h, then
+    // the factors.
+    using Exchange = RowExchange<16, 128>;
+    constexpr int kOutputs = KEEP ? 3 : 1;
+    const int64_t column = q0 + Exchange::byte(lane) / 2;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-        const int64_t row = tile.p0 + 32 * (MB * (wave & 1) + m) + (lane & 31);
-        const bool inside = row < a.rows;
-        const bool kept = inside && (a.row_mask == nullptr || a.row_mask[row] != 0);
+        const int64_t row0 = p0 + 16 * m;
+        const int64_t row = row0 + (lane & 15);
+        const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            float h[4];
+            float first[4];
+            float second[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float act, slope;
+                activation<KEEP>(a.activation, acc[n][m][e], act, slope);
+                const float u = acc[n + 4][m][e];
+                h[e] = kept ? act * u : 0.0f;
+                first[e] = slope * u;
+                second[e] = act;
+            }
+            const int byte = 32 * n + 8 * (lane >> 4);
+            Exchange::put(mine, lane, byte, (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])});
+            if (KEEP) {
+                Exchange::put(mine + Exchange::kSize, lane, byte,
+                              (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])});
+                Exchange::put(mine + 2 * Exchange::kSize, lane, byte,
+                              (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])});
+            }
+        }
+        wave_lds_order();
+#pragma unroll
+        for (int o = 0; o < kOutputs; ++o) {
+            uint16_t* const out = o == 0 ? a.h : a.gates + (o - 1) * a.pitch;
+            const int64_t pitch = o == 0 ? a.pitch : 2 * a.pitch;
+#pragma unroll
+            for (int i = 0; i < Exchange::kSteps; ++i) {
+                const u32x4 value = Exchange::get(mine + o * Exchange::kSize, lane, i);
+                const int64_t to = row0 + Exchange::row(lane, i);
+                if (to < a.rows && column < a.pitch) {
+                    store16_unaligned(out + to * pitch + column, value);
+                }
+            }
+        }
+        wave_lds_order();
+    }
+}
+
+template <int T, int MB, bool KEEP>
+using GateShape = RowsShape<T, MB, 8, (KEEP ? 3 : 1) * RowExchange<16, 128>::kSize>;
+
+template <int T, int MB, bool KEEP>
+__global__ __launch_bounds__(kProductThreads, 2) void gate_kernel(FeedForwardArgs a) {
+    using S = GateShape<T, MB, KEEP>;
+    using Q = typename S::QStage;
+    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    constexpr int kColumns = 64;
+    TileWalk walk(a.tiles, a.q_tiles);
+    if (walk.left == 0) {
+        return;
+    }
+    const PRowLoads<MB> p(a.x_stride, a.in_pitch, wave, lane);
+    const QRowLoads<Q> q(a.in_pitch, a.in_pitch, wave, lane);
+    static_assert(Q::kLoads == 4, "two loads of each weight");
+    TileWalk p_walk = walk;
+    int p_slot = 0;
+    const auto x_rows = [&] {
+        const int64_t p0 = static_cast<int64_t>(p_walk.p) * S::BP;
+        return PRowLoads<MB>::lines(a.x + p0 * a.x_stride, a.x_stride, p_walk.left > 0 ? a.rows - p0 : 0);
+    };
+    BufferRsrc x = x_rows();
+    TileWalk q_walk = walk;
+    int q_stage = 0;
+    const auto weight_rows = [&](const uint16_t* weight) {
+        const int64_t q0 = static_cast<int64_t>(q_walk.q) * kColumns;
+        return QRowLoads<Q>::lines(weight + q0 * a.in_pitch, a.in_pitch, q_walk.left > 0 ? a.hidden - q0 : 0, kColumns);
+    };
+    BufferRsrc gate = weight_rows(a.gate);
+    BufferRsrc up = weight_rows(a.up);
+    const auto load_p = [&](u32x4 (&fragments)[MB]) {
+        p.load(x, p_slot * kSlotK, fragments);
+        if (++p_slot == 2 * a.stages) {
+            p_slot = 0;
+            p_walk.next();
+            x = x_rows();
+        }
+    };
+    const auto issue_q = [&](char* stage) {
+        // Loads 0 and 1 of Q are rows 0 .. 63 of its stage, 2 and 3 the rest.
+        const int k = q_stage * kRowsStageK;
+        q.issue(gate, stage, wave, k, 0, 0);
+        q.issue(gate, stage, wave, k, 1, 1);
+        q.issue(up, stage, wave, k, 2, 0);
+        q.issue(up, stage, wave, k, 3, 1);
+        if (++q_stage == a.stages) {
+            q_stage = 0;
+            q_walk.next();
+            gate = weight_rows(a.gate);
+            up = weight_rows(a.up);
+        }
+    };
+    run_rows_tiles<S>(lds, walk.left, a.stages, load_p, issue_q, [&](const f32x4 (&acc)[8][MB]) {
+        gate_epilogue<T, MB, KEEP>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
+                                   static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
+                                   static_cast<int64_t>(walk.q) * kColumns, acc);
+        walk.next();
+    });
+}
+
+// ------------------------------------------------------------------ y and dx
+// out = P Q^T: y = h Wd^T, or dx = [dg | du] [Wg^T | Wu^T]^T with both weights
+// transposed side by side, as dg and du lie.  With `splits` > 1 the stages are
+// divided and FP32 partials left for join_kernel.
+template <int T, int MB, int NB>
+using ProductRows = RowsShape<T, MB, NB, RowExchange<16, 32 * NB>::kSize>;
+
+template <int T, int MB, int NB>
+__device__ __forceinline__ void product_epilogue(const FeedForwardProduct& a, char* mine, int lane, int split,
+                                                 int64_t p0, int64_t q0, const f32x4 (&acc)[NB][MB]) {
+    if (a.partials != nullptr) {   // uniform
+        using Exchange = RowExchange<16, 32 * NB>;   // half the columns at a time
+        float* const out = a.partials + split * a.rows * a.partial_pitch;
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int64_t row0 = p0 + 16 * m;
+#pragma unroll
+            for (int n0 = 0; n0 < NB; n0 += NB / 2) {
+#pragma unroll
+                for (int n = 0; n < NB / 2; ++n) {
+                    Exchange::put(mine, lane, 64 * n + 16 * (lane >> 4), acc[n0 + n][m]);
+                }
+                wave_lds_order();
+                const int64_t column = q0 + 16 * n0 + Exchange::byte(lane) / 4;
+#pragma unroll
+                for (int i = 0; i < Exchange::kSteps; ++i) {
+                    const u32x4 value = Exchange::get(mine, lane, i);
+                    const int64_t to = row0 + Exchange::row(lane, i);
+                    if (to < a.rows && column < a.partial_pitch) {
+                        *reinterpret_cast<u32x4*>(out + to * a.partial_pitch + column) = value;
+                    }
+                }
+                wave_lds_order();
+            }
+        }
+        return;
+    }
+    using Exchange = RowExchange<16, 32 * NB>;
+    const int64_t column = q0 + Exchange::byte(lane) / 2;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+        const int64_t row0 = p0 + 16 * m;
+        const int64_t row = row0 + (lane & 15);
+        const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            float v[2][8];
-            row_pieces(acc[n][m], v);
+            f32x4 v = acc[n][m];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int64_t column = tile.q0 + q_start(n) + 16 * c + 8 * half;
-                if (!inside || column >= a.columns) {
-                    continue;
-                }
-                if (a.partials != nullptr) {
-                    float* at = a.partials + (split * a.rows + row) * a.partial_pitch + column;
-                    Values<LSSO_HIP_F32>::store8(at, v[c]);
-                    continue;
-                }
+            for (int e = 0; e < 4; ++e) {
+                v[e] = kept ? v[e] : 0.0f;
+            }
+            Exchange::put(mine, lane, 32 * n + 8 * (lane >> 4),
+                          (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])});
+        }
+        wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < Exchange::kSteps; ++i) {
+            const u32x4 value = Exchange::get(mine, lane, i);
+            const int64_t to = row0 + Exchange::row(lane, i);
+            uint16_t* at = a.out + to * a.columns + column;
+            if (to < a.rows && column + 8 <= a.columns) {
+                store16_unaligned(at, value);
+            } else if (to < a.rows) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[c][e] = kept ? v[c][e] : 0.0f;
-                }
-                uint16_t* at = a.out + row * a.columns + column;
-                if (column + 8 <= a.columns) {
-                    Values<T>::store8(at, v[c]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (column + e < a.columns) {
-                            Values<T>::store(at + e, v[c][e]);
-                        }
+                    if (column + e < a.columns) {
+                        at[e] = static_cast<uint16_t>(value[e / 2] >> (16 * (e & 1)));
                     }
                 }
             }
         }
+        wave_lds_order();
     }
+}
+
+template <int T, int MB, int NB>
+__global__ __launch_bounds__(kProductThreads, 2) void product_kernel(FeedForwardProduct a) {
+    using S = ProductRows<T, MB, NB>;
+    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    TileWalk walk(a.tiles, a.q_tiles);
+    if (walk.left == 0) {
+        return;
+    }
+    const int split = blockIdx.y;
+    const int first = split * a.split_stages;
+    const int last = first + a.split_stages < a.stages ? first + a.split_stages : a.stages;
+    RowStream<S> stream(a.p, a.p_stride, a.rows, a.q, a.q_stride, a.columns, a.k, first, last, walk, wave, lane);
+    run_rows_tiles<S>(
+        lds, walk.left, last - first, [&](u32x4 (&fragments)[MB]) { stream.load_p(fragments); },
+        [&](char* stage) { stream.issue_q(stage); },
+        [&](const f32x4 (&acc)[NB][MB]) {
+            product_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane, split,
+                                        static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
+                                        static_cast<int64_t>(walk.q) * S::BQ, acc);
+            walk.next();
+        });
 }
 
 // ----------------------------------------------------------------- dg and du
 template <int T, int MB, int NB>
-__global__ __launch_bounds__(kProductThreads, 2) void grad_kernel(FeedForwardArgs a) {
-    using S = ProductShape<T, true, false, MB, NB>;
-    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-    const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
-    const Tile tile = tile_of(a.q_tiles, a.tiles, S::BP, S::BQ);
-    const RowLoads<typename S::PLayout> dy({a.dy + tile.p0 * a.dy_stride, a.dy_stride, a.rows - tile.p0, a.out_pitch},
-                                           wave, lane, S::BP);
-    const ColumnLoads<typename S::QLayout> down({a.down + tile.q0, a.down_pitch, a.out_features,
-                                                 a.down_pitch - tile.q0}, wave, lane);
-    f32x16 acc[NB][MB];
-    const auto q_start = [&](int n) { return 32 * (NB * (wave >> 1) + n); };
-    run_product<S>(
-        lds, a.stages, acc,
-        [&](char* stage, int s) {
-            const int64_t k = static_cast<int64_t>(s) * kStageK;
-#pragma unroll
-            for (int j = 0; j < S::PLayout::kLoads; ++j) {
-                dy.issue(stage, wave, k, j);
-            }
-            const BufferRsrc buffer = down.stage(k, a.out_features);
-#pragma unroll
-            for (int j = 0; j < S::QLayout::kLoads; ++j) {
-                down.issue(buffer, stage + S::PLayout::kBytes, wave, j);
-            }
-        },
-        q_start);
+using GradShape = RowsShape<T, MB, NB, RowExchange<16, 256>::kSize>;
 
-    const int half = lane >> 5;
+template <int T, int MB, int NB>
+__device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
+                                              const f32x4 (&acc)[NB][MB]) {
+    // dh goes through the exchange in FP32, 16 rows x 64 columns at a time: in
+    // its rows the factors are read and dg, du written whole pieces at a time.
+    using Exchange = RowExchange<16, 256>;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-        const int64_t row = tile.p0 + 32 * (MB * (wave & 1) + m) + (lane & 31);
-        const bool inside = row < a.rows;
-        const bool kept = inside && (a.row_mask == nullptr || a.row_mask[row] != 0);
+        const int64_t row0 = p0 + 16 * m;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float dh[2][8];
-            row_pieces(acc[n][m], dh);
+        for (int n0 = 0; n0 < NB; n0 += 4) {
+            const int64_t column = q0 + 16 * n0 + 8 * (lane & 7);
+            u32x4 raw[2][2];
+            bool kept[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int64_t column = tile.q0 + q_start(n) + 16 * c + 8 * half;
-                if (!inside || column >= a.pitch) {
-                    continue;
+            for (int i = 0; i < 2; ++i) {
+                const int64_t row = row0 + 8 * i + (lane >> 3);
+                if (row < a.rows && column < a.pitch) {
+                    const uint16_t* at = a.gates + 2 * row * a.pitch + column;
+                    raw[i][0] = load16_unaligned(at);
+                    raw[i][1] = load16_unaligned(at + a.pitch);
+                    kept[i] = a.row_mask == nullptr || a.row_mask[row] != 0;
                 }
-                const int64_t at = 2 * row * a.pitch + column;
-                float g[8];
-                float u[8];
-                Values<T>::load8(a.gates + at, g);
-                Values<T>::load8(a.gates + at + a.pitch, u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float act, slope;
-                    activation(a.activation, g[e], act, slope);
-                    g[e] = kept ? dh[c][e] * u[e] * slope : 0.0f;
-                    u[e] = kept ? dh[c][e] * act : 0.0f;
-                }
-                store16_unaligned(a.grads + at, Values<T>::pack8(g));
-                store16_unaligned(a.grads + at + a.pitch, Values<T>::pack8(u));
             }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                Exchange::put(mine, lane, 64 * n + 16 * (lane >> 4), acc[n0 + n][m]);
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 8 * i + (lane >> 3);
+                const int64_t row = row0 + r;
+                const char* from = mine + r * Exchange::kPitch + 32 * (lane & 7);
+                const f32x4 low = *reinterpret_cast<const f32x4*>(from);
+                const f32x4 high = *reinterpret_cast<const f32x4*>(from + 16);
+                if (row < a.rows && column < a.pitch) {
+                    float dg[8];
+                    float du[8];
+                    Values<T>::unpack8(raw[i][0], dg);
+                    Values<T>::unpack8(raw[i][1], du);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float dh = e < 4 ? low[e & 3] : high[e & 3];
+                        dg[e] = kept[i] ? dh * dg[e] : 0.0f;
+                        du[e] = kept[i] ? dh * du[e] : 0.0f;
+                    }
+                    uint16_t* at = a.grads + 2 * row * a.pitch + column;
+                    store16_unaligned(at, Values<T>::pack8(dg));
+                    store16_unaligned(at + a.pitch, Values<T>::pack8(du));
+                }
+            }
+            wave_lds_order();
         }
     }
 }
 
+template <int T, int MB, int NB>
+__global__ __launch_bounds__(kProductThreads, 2) void grad_kernel(FeedForwardArgs a) {
+    using S = GradShape<T, MB, NB>;
+    __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    TileWalk walk(a.tiles, a.q_tiles);
+    if (walk.left == 0) {
+        return;
+    }
+    RowStream<S> stream(a.dy, a.dy_stride, a.rows, a.down_columns, a.out_pitch, a.hidden, a.out_pitch, 0, a.stages, walk,
+                        wave, lane);
+    run_rows_tiles<S>(
+        lds, walk.left, a.stages, [&](u32x4 (&fragments)[MB]) { stream.load_p(fragments); },
+        [&](char* stage) { stream.issue_q(stage); },
+        [&](const f32x4 (&acc)[NB][MB]) {
+            grad_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
+                                     static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
+                                     static_cast<int64_t>(walk.q) * S::BQ, acc);
+            walk.next();
+        });
+}
+
 // ----------------------------------------------------------- weight gradients
 // One of up to three products P^T Q over a range of rows, P and Q in columns.
-template <int T, int MB, int NB, bool MASKED>
+template <int T, int MB, int NB, int WP, bool MASKED>
 __global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardWeights a) {
-    using S = ProductShape<T, false, false, MB, NB>;
+    using S = ProductShape<T, false, false, MB, NB, WP>;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
     __shared__ uint32_t kept[MASKED ? kWeightSplitRows / 32 + kRing : 1];   // rows of each stage
     const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
+    const int wave = wave_index();
     int64_t block = xcd_local_block(blockIdx.x, gridDim.x);
     const int64_t split = block / a.tiles;
     block -= split * a.tiles;
@@ -394,7 +572,7 @@ __global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardW
     const ColumnLoads<typename S::PLayout> p({w.p + p0, w.p_stride, 0, w.p_columns - p0}, wave, lane);
     const ColumnLoads<typename S::QLayout> q({w.q + q0, w.q_stride, 0, w.q_columns - q0}, wave, lane);
     f32x16 acc[NB][MB];
-    const auto q_start = [&](int n) { return 32 * (NB * (wave >> 1) + n); };
+    const auto q_start = [&](int n) { return S::wave_q(wave) + 32 * n; };
     run_product<S>(
         lds, static_cast<int>((r1 - r0 + kStageK - 1) / kStageK), acc,
         [&](char* stage, int s) {
@@ -414,24 +592,9 @@ __global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardW
         },
         q_start);
 
-    const int half = lane >> 5;
-#pragma unroll
-    for (int m = 0; m < MB; ++m) {
-        const int64_t row = p0 + 32 * (MB * (wave & 1) + m) + (lane & 31);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float v[2][8];
-            row_pieces(acc[n][m], v);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int64_t column = q0 + q_start(n) + 16 * c + 8 * half;
-                if (row < w.out_rows && column < w.partial_pitch) {
-                    float* at = a.partials + split * a.partial_floats + w.partial_offset + row * w.partial_pitch + column;
-                    Values<LSSO_HIP_F32>::store8(at, v[c]);
-                }
-            }
-        }
-    }
+    store_partials<S>(lds + S::kWaveBytes * wave, lane, acc,
+                      a.partials + split * a.partial_floats + w.partial_offset, w.partial_pitch,
+                      p0 + S::wave_p(wave), w.out_rows, q0 + q_start(0));
 }
 
 // Sum of `splits` partials [rows, pitch] in order, rounded once into out [rows,
@@ -474,41 +637,71 @@ __global__ __launch_bounds__(256) void join_kernel(FeedForwardJoin a) {
 }
 
 // Copies of up to five matrices as 16-bit rows of `pitch` columns with zeros
-// behind the last one: FP32 weights, and operands with odd rows.
+// behind the last one (FP32 weights, operands with odd rows), or of their
+// transposes.  A workgroup takes 64 x 64 of a matrix, a thread 2 pieces of 8.
+constexpr int kPackEdge = 64;
+
 template <int T>
 __global__ __launch_bounds__(256) void pack_kernel(FeedForwardPack a) {
-    int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    __shared__ uint16_t square[kPackEdge][kPackEdge + 8];
+    int block = static_cast<int>(blockIdx.x);
     int which = 0;
-    while (which < a.count && i >= a.matrices[which].pieces) {
-        i -= a.matrices[which].pieces;
+    while (block >= a.matrices[which].tiles) {   // the grid is the sum of all tiles
+        block -= a.matrices[which].tiles;
         ++which;
     }
-    if (which == a.count) {
+    const PackMatrix& m = a.matrices[which];
+    const int across = static_cast<int>((m.columns + kPackEdge - 1) / kPackEdge);
+    const int64_t r0 = static_cast<int64_t>(block / across) * kPackEdge;
+    const int64_t c0 = static_cast<int64_t>(block % across) * kPackEdge;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 32 * i + static_cast<int>(threadIdx.x >> 3);
+        const int c = 8 * static_cast<int>(threadIdx.x & 7);
+        float v[8] = {};
+        const auto get = [&](auto values) {
+            using V = decltype(values);
+            const auto* from = static_cast<const typename V::Element*>(m.from) + (r0 + r) * m.stride + c0 + c;
+            if (r0 + r < m.rows && c0 + c + 8 <= m.columns) {
+                V::load8(from, v);
+            } else if (r0 + r < m.rows) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = c0 + c + e < m.columns ? V::load(from + e) : 0.0f;
+                }
+            }
+        };
+        if (m.wide) {
+            get(Values<LSSO_HIP_F32>());
+        } else {
+            get(Values<T>());
+        }
+        const u32x4 packed = Values<T>::pack8(v);
+        if (!m.transposed) {
+            if (r0 + r < m.rows && c0 + c < m.pitch) {
+                store16_unaligned(m.to + (r0 + r) * m.pitch + c0 + c, packed);
+            }
+        } else {
+            *reinterpret_cast<u32x4*>(&square[r][c]) = packed;
+        }
+    }
+    if (!m.transposed) {   // the same for the whole workgroup
         return;
     }
-    const PackMatrix& m = a.matrices[which];
-    const int64_t per_row = m.pitch / 8;
-    const int64_t row = i / per_row;
-    const int64_t column = 8 * (i - row * per_row);
-    float v[8];
-    const auto get = [&](auto values) {
-        using V = decltype(values);
-        const auto* from = static_cast<const typename V::Element*>(m.from) + row * m.stride + column;
-        if (column + 8 <= m.columns) {
-            V::load8(from, v);
-        } else {
+    __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = column + e < m.columns ? V::load(from + e) : 0.0f;
+    for (int i = 0; i < 2; ++i) {
+        const int c = 32 * i + static_cast<int>(threadIdx.x >> 3);   // a row of the transpose
+        const int r = 8 * static_cast<int>(threadIdx.x & 7);
+        if (c0 + c < m.columns && r0 + r < m.rows) {
+            u32x4 out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                out[e] = static_cast<uint32_t>(square[r + 2 * e][c]) | static_cast<uint32_t>(square[r + 2 * e + 1][c]) << 16;
             }
+            store16_unaligned(m.to + (c0 + c) * m.pitch + r0 + r, out);
         }
-    };
-    if (m.wide) {
-        get(Values<LSSO_HIP_F32>());
-    } else {
-        get(Values<T>());
     }
-    store16_unaligned(m.to + row * m.pitch + column, Values<T>::pack8(v));
 }
 
 // Tile edges of a product, in 64s: P and Q.
@@ -537,43 +730,54 @@ int choose_gate(int64_t rows, int64_t pitch) {
     return tiles_of(rows, pitch, 128, 64) >= kSlots / 2 ? 2 : 1;
 }
 
+// A multiple of eight workgroups (one share per XCD), at most what is resident.
+dim3 tile_grid(int tiles, int slots, int splits = 1) {
+    const int per_xcd = (tiles + 7) / 8;
+    return dim3(static_cast<unsigned>(8 * (per_xcd < slots ? per_xcd : slots)), static_cast<unsigned>(splits));
+}
+
+template <int T, int MB, bool KEEP>
+hipError_t launch_gate(FeedForwardArgs a, hipStream_t stream) {
+    using S = GateShape<T, MB, KEEP>;
+    a.stages = static_cast<int>((a.in_pitch + kRowsStageK - 1) / kRowsStageK);
+    a.q_tiles = static_cast<int>((a.pitch + 63) / 64);
+    a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
+    gate_kernel<T, MB, KEEP><<<tile_grid(a.tiles, S::kSlots), kProductThreads, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
 template <int T, bool KEEP>
-void launch_gate(const FeedForwardArgs& a, int mb, dim3 grid, hipStream_t stream) {
-    switch (mb) {
-        case 4: gate_kernel<T, 4, KEEP><<<grid, kProductThreads, 0, stream>>>(a); break;
-        case 2: gate_kernel<T, 2, KEEP><<<grid, kProductThreads, 0, stream>>>(a); break;
-        default: gate_kernel<T, 1, KEEP><<<grid, kProductThreads, 0, stream>>>(a); break;
+hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
+    switch (choose_gate(a.rows, a.pitch)) {
+        case 4: return launch_gate<T, 4, KEEP>(a, stream);
+        case 2: return launch_gate<T, 2, KEEP>(a, stream);
+        default: return launch_gate<T, 1, KEEP>(a, stream);
     }
 }
 
 template <int T>
-hipError_t launch_gate(const FeedForwardArgs& args, hipStream_t stream) {
-    FeedForwardArgs a = args;
-    const int mb = choose_gate(a.rows, a.pitch);
-    a.stages = static_cast<int>((a.in_pitch + kStageK - 1) / kStageK);
-    a.q_tiles = (a.pitch + 63) / 64;
-    a.tiles = a.q_tiles * ((a.rows + 64 * mb - 1) / (64 * mb));
-    const dim3 grid(static_cast<unsigned>(a.tiles));
-    a.gates != nullptr ? launch_gate<T, true>(a, mb, grid, stream) : launch_gate<T, false>(a, mb, grid, stream);
+hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
+    return a.gates != nullptr ? launch_gate<T, true>(a, stream) : launch_gate<T, false>(a, stream);
+}
+
+template <int T, int MB, int NB>
+hipError_t launch_product(FeedForwardProduct a, hipStream_t stream) {
+    using S = ProductRows<T, MB, NB>;
+    a.q_tiles = static_cast<int>((a.columns + S::BQ - 1) / S::BQ);
+    a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
+    product_kernel<T, MB, NB><<<tile_grid(a.tiles, S::kSlots, a.splits), kProductThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
-template <int T, bool Q_ROWS>
+template <int T>
 hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     FeedForwardProduct a = args;
-    const Edges e{a.mb, a.nb};
-    a.q_tiles = (a.columns + 64 * e.nb - 1) / (64 * e.nb);
-    a.tiles = a.q_tiles * ((a.rows + 64 * e.mb - 1) / (64 * e.mb));
-    const dim3 grid(static_cast<unsigned>(a.tiles), static_cast<unsigned>(a.splits));
     if (a.splits == 1) {
         a.partials = nullptr;
     }
-    switch (e.mb) {
-        case 4: product_kernel<T, Q_ROWS, 4, 2><<<grid, kProductThreads, 0, stream>>>(a); break;
-        case 2: product_kernel<T, Q_ROWS, 2, 2><<<grid, kProductThreads, 0, stream>>>(a); break;
-        default: product_kernel<T, Q_ROWS, 1, 1><<<grid, kProductThreads, 0, stream>>>(a); break;
-    }
-    const hipError_t error = hipGetLastError();
+    const hipError_t error = a.mb == 4   ? launch_product<T, 4, 8>(a, stream)
+                             : a.mb == 2 ? launch_product<T, 2, 8>(a, stream)
+                                         : launch_product<T, 1, 4>(a, stream);
     if (a.splits == 1 || error != hipSuccess) {
         return error;
     }
@@ -588,28 +792,31 @@ hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int T>
-hipError_t launch_grad(const FeedForwardArgs& args, hipStream_t stream) {
-    FeedForwardArgs a = args;
-    const Edges e = choose_edges(a.rows, a.pitch);
-    a.stages = static_cast<int>((a.out_pitch + kStageK - 1) / kStageK);
-    a.q_tiles = (a.pitch + 64 * e.nb - 1) / (64 * e.nb);
-    a.tiles = a.q_tiles * ((a.rows + 64 * e.mb - 1) / (64 * e.mb));
-    const dim3 grid(static_cast<unsigned>(a.tiles));
-    switch (e.mb) {
-        case 4: grad_kernel<T, 4, 2><<<grid, kProductThreads, 0, stream>>>(a); break;
-        case 2: grad_kernel<T, 2, 2><<<grid, kProductThreads, 0, stream>>>(a); break;
-        default: grad_kernel<T, 1, 1><<<grid, kProductThreads, 0, stream>>>(a); break;
-    }
+template <int T, int MB, int NB>
+hipError_t launch_grad(FeedForwardArgs a, hipStream_t stream) {
+    using S = GradShape<T, MB, NB>;
+    a.stages = static_cast<int>((a.out_pitch + kRowsStageK - 1) / kRowsStageK);
+    a.q_tiles = static_cast<int>((a.pitch + S::BQ - 1) / S::BQ);
+    a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
+    grad_kernel<T, MB, NB><<<tile_grid(a.tiles, S::kSlots), kProductThreads, 0, stream>>>(a);
     return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_grad(const FeedForwardArgs& a, hipStream_t stream) {
+    switch (choose_edges(a.rows, a.pitch).mb) {
+        case 4: return launch_grad<T, 4, 8>(a, stream);
+        case 2: return launch_grad<T, 2, 8>(a, stream);
+        default: return launch_grad<T, 1, 4>(a, stream);
+    }
 }
 
 template <int T, bool MASKED>
 void launch_weights(const FeedForwardWeights& a, int mb, dim3 grid, hipStream_t stream) {
     if (mb == 4) {
-        weight_kernel<T, 4, 2, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
+        weight_kernel<T, 2, 4, 4, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
     } else {
-        weight_kernel<T, 2, 2, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
+        weight_kernel<T, 2, 2, 2, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
     }
 }
 
@@ -630,9 +837,9 @@ void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProd
     a->nb = e.nb;
     a->stages = static_cast<int>(stages);
     const int64_t tiles = tiles_of(rows, columns, 64 * e.mb, 64 * e.nb);
-    // A long K over few tiles: split so that the CUs fill, at least 8 stages each.
+    // A long K over few tiles: split so that the CUs fill, at least 4 stages each.
     int64_t splits = tiles > 0 ? kSlots / tiles : 1;
-    splits = splits < stages / 8 ? splits : stages / 8;
+    splits = splits < stages / 4 ? splits : stages / 4;
     splits = splits < 1 ? 1 : splits;
     a->split_stages = static_cast<int>((stages + splits - 1) / splits);
     a->splits = static_cast<int>((stages + a->split_stages - 1) / a->split_stages);
@@ -676,11 +883,8 @@ void plan_weights(FeedForwardWeights* a) {
 hipError_t launch_feed_forward_gate(const FeedForwardArgs& a, hipStream_t stream) {
     return a.type == LSSO_HIP_BF16 ? launch_gate<LSSO_HIP_BF16>(a, stream) : launch_gate<LSSO_HIP_F16>(a, stream);
 }
-hipError_t launch_feed_forward_product(const FeedForwardProduct& a, bool q_rows, hipStream_t stream) {
-    if (a.type == LSSO_HIP_BF16) {
-        return q_rows ? launch_product<LSSO_HIP_BF16, true>(a, stream) : launch_product<LSSO_HIP_BF16, false>(a, stream);
-    }
-    return q_rows ? launch_product<LSSO_HIP_F16, true>(a, stream) : launch_product<LSSO_HIP_F16, false>(a, stream);
+hipError_t launch_feed_forward_product(const FeedForwardProduct& a, hipStream_t stream) {
+    return a.type == LSSO_HIP_BF16 ? launch_product<LSSO_HIP_BF16>(a, stream) : launch_product<LSSO_HIP_F16>(a, stream);
 }
 hipError_t launch_feed_forward_grad(const FeedForwardArgs& a, hipStream_t stream) {
     return a.type == LSSO_HIP_BF16 ? launch_grad<LSSO_HIP_BF16>(a, stream) : launch_grad<LSSO_HIP_F16>(a, stream);
@@ -697,15 +901,19 @@ hipError_t launch_feed_forward_join(const FeedForwardJoin& a, int outputs, hipSt
     join_kernel<<<dim3(static_cast<unsigned>((most + 255) / 256), static_cast<unsigned>(outputs)), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
-hipError_t launch_feed_forward_pack(const FeedForwardPack& a, int type, hipStream_t stream) {
-    int64_t pieces = 0;
+hipError_t launch_feed_forward_pack(const FeedForwardPack& args, int type, hipStream_t stream) {
+    FeedForwardPack a = args;
+    int64_t tiles = 0;
     for (int i = 0; i < a.count; ++i) {
-        pieces += a.matrices[i].pieces;
+        PackMatrix& m = a.matrices[i];
+        const int64_t n = ((m.rows + kPackEdge - 1) / kPackEdge) * ((m.columns + kPackEdge - 1) / kPackEdge);
+        tiles += n;
+        m.tiles = static_cast<int>(n);
     }
-    if (pieces == 0) {
+    if (tiles == 0) {
         return hipSuccess;
     }
-    const dim3 grid(static_cast<unsigned>((pieces + 255) / 256));
+    const dim3 grid(static_cast<unsigned>(tiles));
     if (type == LSSO_HIP_BF16) {
         pack_kernel<LSSO_HIP_BF16><<<grid, 256, 0, stream>>>(a);
     } else {

@@ -349,47 +349,42 @@ struct FeedForwardArgs {
     int64_t in_pitch;           // columns of x, gate and up, zeros past in_features
     int64_t pitch;              // columns of h: hidden rounded up
     int64_t out_pitch;          // columns of dy
-    int64_t down_pitch;         // columns of down: pitch
     const uint16_t* x;          // [rows, in_pitch], row stride x_stride
     int64_t x_stride;
     const uint16_t* gate;       // [hidden, in_pitch]
     const uint16_t* up;         // [hidden, in_pitch]
-    const uint16_t* down;       // [out_features, down_pitch]
+    const uint16_t* down;       // [out_features, pitch]
+    const uint16_t* down_columns;   // its transpose [hidden, out_pitch], of the backward
     const uint8_t* row_mask;    // [rows] or nullptr
     uint16_t* h;                // [rows, pitch]
-    uint16_t* gates;            // [rows, 2, pitch]: g, u; or nullptr
+    uint16_t* gates;            // [rows, 2, pitch]: u act'(g), act(g); or nullptr
     const uint16_t* dy;         // [rows, out_pitch], row stride dy_stride
     int64_t dy_stride;
     uint16_t* grads;            // [rows, 2, pitch]: dg, du
     int stages;                 // set by the launcher, as the tiles
-    int64_t q_tiles;
-    int64_t tiles;
+    int q_tiles;
+    int tiles;
 };
 
 struct FeedForwardProduct {
     int type;
     const uint16_t* p;          // [rows, k], row stride p_stride
     int64_t p_stride;
-    int64_t p_second;           // elements from p to the second segment's rows
     int64_t rows;
-    int64_t k;                  // of a segment, a multiple of 8
-    const uint16_t* q;          // rows: [columns, k]; columns: [q_lines, q_pitch]
-    const uint16_t* q_second;
+    int64_t k;                  // a multiple of 8
+    const uint16_t* q;          // [columns, k], row stride q_stride
     int64_t q_stride;
-    int64_t q_lines;
-    int64_t q_pitch;
     const uint8_t* row_mask;
     uint16_t* out;              // [rows, columns] contiguous
     int64_t columns;
     float* partials;            // [splits, rows, partial_pitch], unused with one split
     int64_t partial_pitch;
-    int segment_stages;         // stages of the first segment
-    int stages;                 // of all segments; set by plan_product, as what follows
+    int stages;                 // set by plan_product, as what follows
     int split_stages;
     int splits;
     int mb, nb;
-    int64_t q_tiles;            // set by the launcher
-    int64_t tiles;
+    int q_tiles;                // set by the launcher
+    int tiles;
 };
 
 struct WeightProduct {
@@ -441,11 +436,13 @@ struct FeedForwardJoin {
 struct PackMatrix {
     const void* from;           // [rows, columns], row stride `stride`
     int64_t stride;
+    int64_t rows;
     int64_t columns;
-    int64_t pitch;
     int wide;                   // FP32
-    uint16_t* to;               // [rows, pitch]
-    int64_t pieces;             // rows * pitch / 8
+    int transposed;
+    uint16_t* to;               // [rows, pitch], or transposed [columns, pitch]
+    int64_t pitch;
+    int tiles;                  // set by the launcher
 };
 
 struct FeedForwardPack {
@@ -456,7 +453,7 @@ struct FeedForwardPack {
 void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProduct* a);
 void plan_weights(FeedForwardWeights* a);
 hipError_t launch_feed_forward_gate(const FeedForwardArgs& a, hipStream_t stream);
-hipError_t launch_feed_forward_product(const FeedForwardProduct& a, bool q_rows, hipStream_t stream);
+hipError_t launch_feed_forward_product(const FeedForwardProduct& a, hipStream_t stream);
 hipError_t launch_feed_forward_grad(const FeedForwardArgs& a, hipStream_t stream);
 hipError_t launch_feed_forward_weights(const FeedForwardWeights& a, hipStream_t stream);
 hipError_t launch_feed_forward_join(const FeedForwardJoin& a, int outputs, hipStream_t stream);

@@ -1,11 +1,12 @@
 // Tiled 16-bit matrix product of the feed-forward kernels:
 //   out[p][q] = sum over k of P[p, k] Q[q, k],  FP32 accumulation,
-// for operands that lie in memory either along k ([p][k], "rows") or across it
-// ([k][p], "columns"), so that x W^T, dy W and dy^T x are the same loop and no
-// operand is ever transposed in memory.
+// in two forms: for operands that lie in memory across k ([k][p], "columns": the
+// weight gradients dy^T x, whose k are the rows of long activations), and for
+// operands along k ([p][k], "rows": x W^T; dy W comes to it with W transposed
+// once per call), further down.
 //
-// A workgroup of 4 waves (2 x 2) owns a BP x BQ tile, a wave MB x NB blocks of
-// 32 x 32 on v_mfma_f32_32x32x16.  The operands' stages of 32 k go from memory
+// A workgroup of 4 waves owns a BP x BQ tile, a wave MB x NB blocks of 32 x 32
+// on v_mfma_f32_32x32x16.  The operands' stages of 32 k go from memory
 // to LDS without passing registers (buffer_load ... lds, 16 bytes per lane), in
 // a ring of three: two stages are in flight while one is multiplied.  The
 // largest tile, 256 x 128, keeps 128 accumulators and 72 KB of LDS, so two
@@ -81,24 +82,22 @@ struct StageLayout {
             return 16 * ((piece >> 1) ^ column_swizzle(line)) + 8 * (piece & 1);
         }
     }
-    // Byte of this lane's fragment of block b (32 p from p0) in a stage, first
-    // k step; the second one is second_step() further.
-    __device__ static __forceinline__ int fragment(int lane, int p0) {
+    // Byte of this lane's fragment of the block of 32 p from p0 (a multiple of
+    // 32) in a stage, of k step 0 or 1.
+    __device__ static __forceinline__ int fragment(int lane, int p0, int step) {
         if constexpr (IN_ROWS) {
-            const int p = p0 + (lane & 31);
-            return 64 * p + 16 * ((lane >> 5) ^ row_swizzle(p));
+            const int p = lane & 31;
+            return 64 * p0 + (64 * p + 16 * ((2 * step + (lane >> 5)) ^ row_swizzle(p)));
         } else {
             const int k = (lane & 15) / 4 + 8 * (lane >> 5);
             const int group = p0 / 16 + ((lane >> 4) & 1);
-            return 2 * WIDTH * k + 32 * (group ^ column_swizzle(k)) + 8 * (lane & 3);
+            return 2 * WIDTH * (k + 16 * step) + 32 * (group ^ column_swizzle(k)) + 8 * (lane & 3);
         }
     }
-    __device__ static __forceinline__ u32x4 read(const char* stage, int fragment_at, int step) {
+    __device__ static __forceinline__ u32x4 read(const char* at) {
         if constexpr (IN_ROWS) {
-            // Step 1 takes pieces 2 and 3: slot bit 1 flips.
-            return *reinterpret_cast<const u32x4*>(stage + (fragment_at ^ (32 * step)));
+            return *reinterpret_cast<const u32x4*>(at);
         } else {
-            const char* at = stage + fragment_at + 2 * WIDTH * 16 * step;
             const u32x2 low = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at)));
             const u32x2 high =
                 __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at + 2 * WIDTH * 4)));
@@ -132,40 +131,44 @@ struct Operand {
     int64_t elements;
 };
 
-template <int T_, bool P_ROWS_, bool Q_ROWS_, int MB_, int NB_>
+// T: type code; MB x NB blocks of 32 x 32 per wave; WP waves along P, 4 / WP
+// along Q.
+template <int T_, bool P_ROWS_, bool Q_ROWS_, int MB_, int NB_, int WP_>
 struct ProductShape {
     static constexpr int T = T_;
     static constexpr bool P_ROWS = P_ROWS_;
     static constexpr bool Q_ROWS = Q_ROWS_;
     static constexpr int MB = MB_;
     static constexpr int NB = NB_;
-    static constexpr int BP = 64 * MB;
-    static constexpr int BQ = 64 * NB;
+    static constexpr int WP = WP_;
+    static constexpr int WQ = 4 / WP;
+    static constexpr int BP = 32 * MB * WP;
+    static constexpr int BQ = 32 * NB * WQ;
     using PLayout = StageLayout<BP, P_ROWS>;
     using QLayout = StageLayout<BQ, Q_ROWS>;
     static constexpr int kStageBytes = PLayout::kBytes + QLayout::kBytes;
     static constexpr int kLdsBytes = kRing * kStageBytes;
+    static constexpr int kWaveBytes = kLdsBytes / 4;   // of the epilogue
     static constexpr int kLoads = PLayout::kLoads + QLayout::kLoads;
+    // First row and column of the tile that are this wave's.
+    __device__ static __forceinline__ int wave_p(int wave) { return 32 * MB * (wave % WP); }
+    __device__ static __forceinline__ int wave_q(int wave) { return 32 * NB * (wave / WP); }
 };
 
-// Runs `stages` stages: issue(buffer, s) starts the loads of stage s (which may
-// lie past the last) into the LDS stage `buffer`, exactly kLoads per wave.
-// q_start(nb) is the tile's first column of this wave's Q block nb.
+// This wave's index, as the scalar that it is.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// Runs `stages` stages (at least one): issue(buffer, s) starts the loads of
+// stage s (which may lie past the last) into the LDS stage `buffer`, exactly
+// kLoads per wave.  q_start(n) is the tile's first column of this wave's Q block
+// n.  The order is written down with scheduling barriers: left to itself the
+// compiler moves the fragments' reads down to their MFMAs, to save registers
+// that nothing else needs, and every MFMA then waits for LDS.
 template <typename S, typename Issue, typename QStart>
 __device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)[S::NB][S::MB], Issue issue,
                                             QStart q_start) {
     const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
-    int p_at[S::MB];
-    int q_at[S::NB];
-#pragma unroll
-    for (int m = 0; m < S::MB; ++m) {
-        p_at[m] = S::PLayout::fragment(lane, 32 * (S::MB * (wave & 1) + m));
-    }
-#pragma unroll
-    for (int n = 0; n < S::NB; ++n) {
-        q_at[n] = S::PLayout::kBytes + S::QLayout::fragment(lane, q_start(n));
-    }
+    const int wave = wave_index();
 #pragma unroll
     for (int n = 0; n < S::NB; ++n) {
 #pragma unroll
@@ -178,14 +181,16 @@ __device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)
     }
     u32x4 pf[2][S::MB];
     u32x4 qf[2][S::NB];
-    const auto read = [&](const char* stage, int step) {
+    const auto read = [&](int buffer, int step) {
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            qf[step][n] = S::QLayout::read(stage, q_at[n], step);
+            qf[step][n] = S::QLayout::read(lds + buffer * S::kStageBytes + S::PLayout::kBytes +
+                                           S::QLayout::fragment(lane, q_start(n), step));
         }
 #pragma unroll
         for (int m = 0; m < S::MB; ++m) {
-            pf[step][m] = S::PLayout::read(stage, p_at[m], step);
+            pf[step][m] = S::PLayout::read(lds + buffer * S::kStageBytes +
+                                           S::PLayout::fragment(lane, S::wave_p(wave) + 32 * m, step));
         }
     };
     const auto multiply = [&](int step) {
@@ -197,25 +202,33 @@ __device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)
             }
         }
     };
+    const auto stage = [&](int buffer, int s) {
+        issue(lds + (buffer + 2) % kRing * S::kStageBytes, s + 2);
+        read(buffer, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(0);
+        __builtin_amdgcn_sched_barrier(0);
+        stage_barrier<S::kLoads>();
+        read((buffer + 1) % kRing, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(1);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     issue(lds, 0);
     issue(lds + S::kStageBytes, 1);
     stage_barrier<S::kLoads>();
-    read(lds, 0);
-    int at = 0;   // this stage's buffer
-    for (int s = 0; s < stages; ++s) {
-        const int next = at == kRing - 1 ? 0 : at + 1;
-        const int after = next == kRing - 1 ? 0 : next + 1;
-        issue(lds + after * S::kStageBytes, s + 2);
-        read(lds + at * S::kStageBytes, 1);
-        multiply(0);
-        stage_barrier<S::kLoads>();
-        read(lds + next * S::kStageBytes, 0);
-        multiply(1);
-        at = next;
+    read(0, 0);
+    for (int s = 0;;) {
+        stage(0, s);
+        if (++s == stages) break;
+        stage(1, s);
+        if (++s == stages) break;
+        stage(2, s);
+        if (++s == stages) break;
     }
-    // The loads past the last stage still write their zeros: not into LDS that
-    // another workgroup may hold by then.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // The loads past the last stage still write their zeros: neither into LDS
+    // that the epilogue uses nor into what another workgroup may hold by then.
+    stage_barrier<0>();
 }
 
 // The accumulators of one block hold, in lane (half, j), row p = j and columns
@@ -234,5 +247,238 @@ __device__ __forceinline__ void row_pieces(const f32x16& acc, float (&piece)[2][
         }
     }
 }
+
+// ---------------------------------------------------------------------------
+// The product for both operands in rows (x W^T): P never passes LDS.  Each wave owns
+// 16 MB rows of P and all of the tile's columns, so no other wave needs its
+// rows, and on v_mfma_f32_16x16x32 a fragment of 16 rows x 32 k is one load of
+// 64 bytes from each row, straight into the lanes that multiply it.  With both
+// operands through LDS, their writes and the fragments' reads together exceed
+// the LDS's 128 bytes per clock at the matrix rate: the 256 x 128 tile ran at
+// 28% of the matrix peak, and at 70% with its loads left out.  Here only Q's
+// stage, half the width, is written to LDS and read by the four waves.
+//
+// A stage is 64 k: Q's in a ring of three (16 KB each at 128 columns, loaded by
+// buffer_load ... lds as above), P's as two slots of 32 k in a ring of four in
+// registers, loaded three slots ahead.  The stage's fragments of Q are read in
+// four groups, each under the MFMAs of the one before; the barrier that frees
+// the stage lies before the last group's MFMAs.
+constexpr int kSlotK = 32;
+constexpr int kRowsStageK = 64;
+constexpr int kRowsRing = 3;
+
+template <int T>
+__device__ __forceinline__ f32x4 mfma_small(const u32x4& a, const u32x4& b, const f32x4& c) {
+    if constexpr (T == LSSO_HIP_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+}
+
+// Q's stage of WIDTH rows.
+template <int WIDTH>
+struct RowsStage {
+    static constexpr int kBytes = WIDTH * kRowsStageK * 2;
+    static constexpr int kLoads = kBytes / 1024 / 4;   // per wave
+    // Piece c of row p lies at slot c ^ swizzle(p), so that any 8 or 16 rows of
+    // one piece fall on different banks.
+    __device__ static __forceinline__ int swizzle(int p) { return (p & 7) ^ ((p >> 3) & 1); }
+    // Row that this lane loads with load j, and its first element of that row,
+    // the same for every j.
+    __device__ static __forceinline__ int load_row(int wave, int lane, int j) { return 8 * (4 * j + wave) + (lane >> 3); }
+    __device__ static __forceinline__ int load_element(int wave, int lane) {
+        return 8 * ((lane & 7) ^ swizzle(load_row(wave, lane, 0)));
+    }
+    // This lane's fragment of rows 16 n .. of slot 0 or 1.
+    __device__ static __forceinline__ u32x4 read(const char* stage, int lane, int n, int slot) {
+        const int p = lane & 15;
+        return *reinterpret_cast<const u32x4*>(stage + 2048 * n + (128 * p + 16 * ((4 * slot + (lane >> 4)) ^ swizzle(p))));
+    }
+};
+
+// T: type code; MB x NB blocks of 16 x 16 per wave, the four waves along P;
+// EXCHANGE: bytes of LDS per wave for the epilogue.
+template <int T_, int MB_, int NB_, int EXCHANGE>
+struct RowsShape {
+    static constexpr int T = T_;
+    static constexpr int MB = MB_;
+    static constexpr int NB = NB_;
+    static constexpr int BP = 64 * MB;
+    static constexpr int BQ = 16 * NB;
+    using QStage = RowsStage<BQ>;
+    static constexpr int kRingBytes = kRowsRing * QStage::kBytes;
+    static constexpr int kWaveBytes = EXCHANGE;
+    static constexpr int kLdsBytes = kRingBytes + 4 * EXCHANGE;
+    // Workgroups of one XCD's 32 CUs that are resident at once: by LDS (160 KB)
+    // and by registers (accumulators, fragments and 32 more of 512 per SIMD
+    // lane, one wave of each workgroup per SIMD).
+    static constexpr int kByLds = 160 * 1024 / kLdsBytes;
+    static constexpr int kByRegisters = 512 / (4 * MB * NB + 16 * MB + 4 * NB + 32);
+    static constexpr int kSlots = 32 * (kByLds < kByRegisters ? kByLds : kByRegisters);
+};
+
+// The tiles of one workgroup: XCD x (workgroup index mod 8) takes the x-th eighth
+// of them, columns fastest, its workgroups in turn, so that the tiles that
+// share P's rows are multiplied at the same time beside one L2.
+struct TileWalk {
+    int p;            // tile of this step
+    int q;
+    int left;         // tiles to go, this one included
+    int step_p;
+    int step_q;
+    int q_tiles;
+
+    __device__ __forceinline__ TileWalk(int tiles, int q_tiles_) : q_tiles(q_tiles_) {
+        const int per_xcd = (tiles + 7) / 8;
+        const int begin = static_cast<int>(blockIdx.x % 8) * per_xcd;
+        const int end = begin + per_xcd < tiles ? begin + per_xcd : tiles;
+        const int first = begin + static_cast<int>(blockIdx.x / 8);
+        const int step = static_cast<int>(gridDim.x / 8);
+        left = first < end ? (end - first + step - 1) / step : 0;
+        p = first / q_tiles;
+        q = first - p * q_tiles;
+        step_p = step / q_tiles;
+        step_q = step - step_p * q_tiles;
+    }
+    __device__ __forceinline__ void next() {
+        --left;
+        p += step_p;
+        q += step_q;
+        if (q >= q_tiles) {
+            q -= q_tiles;
+            ++p;
+        }
+    }
+};
+
+// Runs `tiles` tiles of `stages` stages each.  load_p fills the fragments of the
+// next slot of P and issue_q starts the next stage of Q into an LDS stage, each
+// in order through all tiles and asked for a few past the last; epilogue(acc)
+// takes a tile's sums.  The loads run ahead across the tiles' borders, so a
+// tile's first stages arrive under the epilogue of the one before: a tile of
+// 256 k has four stages, and began with a wait for memory as long as all its
+// MFMAs.
+template <typename S, typename LoadP, typename IssueQ, typename Epilogue>
+__device__ __forceinline__ void run_rows_tiles(char* lds, int tiles, int stages, LoadP load_p, IssueQ issue_q,
+                                               Epilogue epilogue) {
+    constexpr int kHalf = S::NB / 2;
+    const int lane = threadIdx.x & 63;
+    f32x4 acc[S::NB][S::MB];
+    u32x4 pf[4][S::MB];
+    u32x4 qf[2][kHalf];
+    const auto read = [&](const char* stage, int group) {
+#pragma unroll
+        for (int n = 0; n < kHalf; ++n) {
+            qf[group & 1][n] = S::QStage::read(stage, lane, kHalf * (group & 1) + n, group >> 1);
+        }
+    };
+    const auto multiply = [&](int slot, int group) {
+#pragma unroll
+        for (int n = 0; n < kHalf; ++n) {
+#pragma unroll
+            for (int m = 0; m < S::MB; ++m) {
+                f32x4& c = acc[kHalf * (group & 1) + n][m];
+                c = mfma_small<S::T>(qf[group & 1][n], pf[slot][m], c);
+            }
+        }
+    };
+    int at = 0;   // LDS offset of this stage
+    // One stage; `slot`: the register slot of its first 32 k, 0 or 2.
+    const auto stage = [&](int slot) {
+        char* const here = lds + at;
+        const int next = at == (kRowsRing - 1) * S::QStage::kBytes ? 0 : at + S::QStage::kBytes;
+        read(here, 1);
+        load_p(pf[(slot + 3) & 3]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(slot, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        read(here, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(slot, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        read(here, 3);
+        load_p(pf[slot]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(slot + 1, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        // The next stage has landed when no more than what was issued behind it
+        // is outstanding: the stage after it and four slots.
+        stage_barrier<S::QStage::kLoads + 4 * S::MB>();
+        issue_q(here);
+        read(lds + next, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(slot + 1, 3);
+        __builtin_amdgcn_sched_barrier(0);
+        at = next;
+    };
+#pragma unroll
+    for (int i = 0; i < kRowsRing; ++i) {
+        issue_q(lds + i * S::QStage::kBytes);
+    }
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        load_p(pf[t]);
+    }
+    stage_barrier<2 * S::QStage::kLoads + 3 * S::MB>();
+    read(lds, 0);
+    for (int tile = 0; tile < tiles; ++tile) {
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) {
+#pragma unroll
+            for (int m = 0; m < S::MB; ++m) {
+                acc[n][m] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        for (int s = 0;;) {
+            stage(0);
+            if (++s == stages) break;
+            stage(2);
+            if (++s == stages) break;
+        }
+        epilogue(acc);
+        if ((stages & 1) != 0) {   // the next tile begins with register slot 0 again
+#pragma unroll
+            for (int m = 0; m < S::MB; ++m) {
+                const u32x4 first = pf[0][m];
+                const u32x4 second = pf[1][m];
+                pf[0][m] = pf[2][m];
+                pf[1][m] = pf[3][m];
+                pf[2][m] = first;
+                pf[3][m] = second;
+            }
+        }
+    }
+    // The loads past the last stage still write their zeros: not into LDS that
+    // another workgroup may hold by then.
+    stage_barrier<0>();
+}
+
+// A wave's exchange of ROWS rows of BYTES (64, 128 or 256) through its own part
+// of LDS, from a lane per row to BYTES / 16 consecutive lanes per row: stored
+// from the accumulators' layout, an instruction covers 32 bytes of each of 32
+// rows, and partly written lines cost the memory side twice (131,072 x 688 x 3
+// stores at 2.6 TB/s); exchanged, it covers whole rows' pieces of 128 bytes.
+// LDS serves a wave's accesses in order, so no barrier is needed, and the 16
+// bytes of padding keep both sides free of conflicts.
+template <int ROWS, int BYTES>
+struct RowExchange {
+    static constexpr int kPitch = BYTES + 16;
+    static constexpr int kSize = ROWS * kPitch;
+    static constexpr int kLanes = BYTES / 16;        // per row
+    static constexpr int kRows = 64 / kLanes;        // per access
+    static constexpr int kSteps = ROWS / kRows;
+    template <typename V>
+    __device__ static __forceinline__ void put(char* lds, int lane, int byte, const V& value) {
+        *reinterpret_cast<V*>(lds + (lane % ROWS) * kPitch + byte) = value;
+    }
+    __device__ static __forceinline__ int row(int lane, int step) { return kRows * step + lane / kLanes; }
+    __device__ static __forceinline__ int byte(int lane) { return 16 * (lane % kLanes); }
+    __device__ static __forceinline__ u32x4 get(const char* lds, int lane, int step) {
+        return *reinterpret_cast<const u32x4*>(lds + row(lane, step) * kPitch + byte(lane));
+    }
+};
 
 }  // namespace lsso_hip

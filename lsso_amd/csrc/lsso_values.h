@@ -59,7 +59,10 @@ struct Values<LSSO_HIP_F16> {
     using Element = uint16_t;
     __device__ static __forceinline__ float low(uint32_t pair) { return f16_lo(pair); }
     __device__ static __forceinline__ float high(uint32_t pair) { return f16_hi(pair); }
-    __device__ static __forceinline__ uint32_t pack(float a, float b) { return pack_f16(a, b); }
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+    }
     __device__ static __forceinline__ float load(const uint16_t* at) { return f16_bits_to_float(*at); }
     __device__ static __forceinline__ void store(uint16_t* at, float v) { *at = to_f16_bits(v); }
     __device__ static __forceinline__ void load8(const uint16_t* at, float (&v)[8]) { unpack8(load16_unaligned(at), v); }

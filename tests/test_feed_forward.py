@@ -27,8 +27,8 @@ def _expected(x, weights, dy, kind, dtype, grad_dtype, mask=None):
     """{output: (value, bound)} in FP64.
 
     The bounds follow the operator's roundings, each at most half a step `e` of
-    the type: of h = act(g) u, of the kept g and u, of dg and du, and of the
-    outputs; an FP32 sum of n products is off by at most n 2^-24 times the sum
+    the type: of h = act(g) u, of the kept u act'(g) and act(g), of dg and du,
+    and of the outputs; an FP32 sum of n products is off by at most n 2^-24 times the sum
     of their magnitudes.  Through act and act' an error of g grows by at most
     1.13 and 0.8 (the largest |act'| and |act''| of both activations); their own
     evaluation in FP32 is off by |g| 2^-22 and (1 + |g|) 2^-21: a relative error
@@ -56,12 +56,13 @@ def _expected(x, weights, dy, kind, dtype, grad_dtype, mask=None):
     found = {"y": (y, eh @ down.abs().T + hidden * f * (h.abs() @ down.abs().T) + e * y.abs() + tiny)}
     dh = dy @ down
     edh = n * f * (dy.abs() @ down.abs())
-    rg, ru = eg + e * g.abs() + tiny, eu + e * u.abs() + tiny
-    es = 0.8 * rg + (1 + g.abs()) * 2.0**-21
-    ea = 1.13 * rg + g.abs() * 2.0**-22
-    dg, du = dh * u * slope, dh * act
-    edg = edh * (u * slope).abs() + dh.abs() * (ru * slope.abs() + u.abs() * es) + e * dg.abs() + tiny
-    edu = edh * act.abs() + dh.abs() * ea + e * du.abs() + tiny
+    es = 0.8 * eg + (1 + g.abs()) * 2.0**-21
+    factor = u * slope
+    ef = eu * slope.abs() + u.abs() * es + e * factor.abs() + tiny
+    eb = ea + e * act.abs() + tiny
+    dg, du = dh * factor, dh * act
+    edg = edh * factor.abs() + dh.abs() * ef + e * dg.abs() + tiny
+    edu = edh * act.abs() + dh.abs() * eb + e * du.abs() + tiny
     dx = dg @ gate + du @ up
     found["x"] = (dx, edg @ gate.abs() + edu @ up.abs() + 2 * hidden * f * (dg.abs() @ gate.abs() + du.abs() @ up.abs())
                   + e * dx.abs() + tiny)
