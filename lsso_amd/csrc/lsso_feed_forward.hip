@@ -62,51 +62,29 @@ __device__ __forceinline__ void activation(int kind, float g, float& value, floa
     }
 }
 
-// Q's loads in rows: lines are the tile's columns.
+// One operand's loads: rows of a tile.
 template <typename Stage>
-struct QRowLoads {
-    uint32_t offset;       // this lane's line and element, bytes
-    uint32_t step;         // bytes between the lines of consecutive loads
+struct RowLoads {
+    uint32_t offset;       // this lane's row and element, bytes
+    uint32_t step;         // bytes between the rows of consecutive loads
     int element;           // this lane's element of stage 0
     int elements;
 
-    __device__ __forceinline__ QRowLoads(int64_t stride, int64_t k_elements, int wave, int lane)
-        : step(static_cast<uint32_t>(2 * 32 * stride)),
+    __device__ __forceinline__ RowLoads(int64_t stride, int64_t k_elements, int wave, int lane)
+        : step(static_cast<uint32_t>(2 * Stage::kRowsPerRound * stride)),
+          element(Stage::load_element(wave, lane)),
           elements(static_cast<int>(k_elements)) {
-        element = Stage::load_element(wave, lane);
-        offset = static_cast<uint32_t>(2 * (Stage::load_row(wave, lane, 0) * stride + element));
+        offset = static_cast<uint32_t>(2 * (Stage::load_row(wave, lane) * stride + element));
     }
-    __device__ __forceinline__ static BufferRsrc lines(const uint16_t* base, int64_t stride, int64_t rows, int most) {
+    // The `rows` rows from `base` on (none where that is negative), at most `most`.
+    __device__ __forceinline__ static BufferRsrc aim(const uint16_t* base, int64_t stride, int64_t rows, int most) {
         return make_buffer(base, 2 * (rows < most ? rows : most) * stride);
     }
-    __device__ __forceinline__ void issue(BufferRsrc buffer, char* lds, int wave, int k, int j, int line_step) const {
-        load_to_lds(buffer, lds + 1024 * (4 * j + wave),
-                    k + element < elements ? offset + line_step * step + static_cast<uint32_t>(2 * k) : kOutOfRange);
-    }
-};
-
-// P's fragments: MB blocks of 16 rows, 8 k per lane.
-template <int MB>
-struct PRowLoads {
-    uint32_t offset;
-    uint32_t step;         // bytes between blocks
-    int element;
-    int elements;
-
-    __device__ __forceinline__ PRowLoads(int64_t stride, int64_t k_elements, int wave, int lane)
-        : offset(static_cast<uint32_t>(2 * ((16 * MB * wave + (lane & 15)) * stride + 8 * (lane >> 4)))),
-          step(static_cast<uint32_t>(2 * 16 * stride)),
-          element(8 * (lane >> 4)),
-          elements(static_cast<int>(k_elements)) {}
-    __device__ __forceinline__ static BufferRsrc lines(const uint16_t* base, int64_t stride, int64_t rows) {
-        return make_buffer(base, 2 * (rows < 64 * MB ? rows : 64 * MB) * stride);
-    }
-    __device__ __forceinline__ void load(BufferRsrc buffer, int k, u32x4 (&fragments)[MB]) const {
-#pragma unroll
-        for (int m = 0; m < MB; ++m) {
-            fragments[m] = buffer_load16(
-                buffer, k + element < elements ? offset + m * step + static_cast<uint32_t>(2 * k) : kOutOfRange);
-        }
+    // Load j of a stage, of the rows of round `round` of the buffer.
+    __device__ __forceinline__ void issue(BufferRsrc buffer, char* lds, int waves, int wave, int k, int j,
+                                          int round) const {
+        load_to_lds(buffer, lds + 1024 * (waves * j + wave),
+                    k + element < elements ? offset + round * step + static_cast<uint32_t>(2 * k) : kOutOfRange);
     }
 };
 
@@ -114,6 +92,7 @@ struct PRowLoads {
 // [rows, k] and Q [columns, k].
 template <typename S>
 struct RowStream {
+    using P = typename S::PStage;
     using Q = typename S::QStage;
     const uint16_t* p_base;
     int64_t p_stride;
@@ -124,49 +103,41 @@ struct RowStream {
     int first;
     int last;
     int wave;
-    PRowLoads<S::MB> p;
-    QRowLoads<Q> q;
-    TileWalk p_walk;
-    TileWalk q_walk;
-    int slot;
+    RowLoads<P> p;
+    RowLoads<Q> q;
+    TileWalk walk;
     int stage;
     BufferRsrc p_rows;
     BufferRsrc q_rows;
 
     __device__ __forceinline__ RowStream(const uint16_t* p_base_, int64_t p_stride_, int64_t rows_,
                                          const uint16_t* q_base_, int64_t q_stride_, int64_t columns_, int64_t k,
-                                         int first_, int last_, const TileWalk& walk, int wave_, int lane)
+                                         int first_, int last_, const TileWalk& walk_, int wave_, int lane)
         : p_base(p_base_), p_stride(p_stride_), rows(rows_), q_base(q_base_), q_stride(q_stride_), columns(columns_),
           first(first_), last(last_), wave(wave_), p(p_stride_, k, wave_, lane), q(q_stride_, k, wave_, lane),
-          p_walk(walk), q_walk(walk), slot(2 * first_), stage(first_) {
-        aim_p();
-        aim_q();
+          walk(walk_), stage(first_) {
+        aim();
     }
-    __device__ __forceinline__ void aim_p() {
-        const int64_t p0 = static_cast<int64_t>(p_walk.p) * S::BP;
-        p_rows = PRowLoads<S::MB>::lines(p_base + p0 * p_stride, p_stride, p_walk.left > 0 ? rows - p0 : 0);
+    __device__ __forceinline__ void aim() {
+        const int64_t p0 = static_cast<int64_t>(walk.p) * S::BP;
+        const int64_t q0 = static_cast<int64_t>(walk.q) * S::BQ;
+        p_rows = RowLoads<P>::aim(p_base + p0 * p_stride, p_stride, walk.left > 0 ? rows - p0 : 0, S::BP);
+        q_rows = RowLoads<Q>::aim(q_base + q0 * q_stride, q_stride, walk.left > 0 ? columns - q0 : 0, S::BQ);
     }
-    __device__ __forceinline__ void aim_q() {
-        const int64_t q0 = static_cast<int64_t>(q_walk.q) * S::BQ;
-        q_rows = QRowLoads<Q>::lines(q_base + q0 * q_stride, q_stride, q_walk.left > 0 ? columns - q0 : 0, S::BQ);
-    }
-    __device__ __forceinline__ void load_p(u32x4 (&fragments)[S::MB]) {
-        p.load(p_rows, slot * kSlotK, fragments);
-        if (++slot == 2 * last) {
-            slot = 2 * first;
-            p_walk.next();
-            aim_p();
+    __device__ __forceinline__ void issue(char* lds) {
+        const int k = stage * kRowsStageK;
+#pragma unroll
+        for (int j = 0; j < P::kLoads; ++j) {
+            p.issue(p_rows, lds, S::kWaves, wave, k, j, j);
         }
-    }
-    __device__ __forceinline__ void issue_q(char* lds) {
 #pragma unroll
         for (int j = 0; j < Q::kLoads; ++j) {
-            q.issue(q_rows, lds, wave, stage * kRowsStageK, j, j);
+            q.issue(q_rows, lds + P::kBytes, S::kWaves, wave, k, j, j);
         }
         if (++stage == last) {
             stage = first;
-            q_walk.next();
-            aim_q();
+            walk.next();
+            aim();
         }
     }
 };
@@ -203,7 +174,7 @@ struct ColumnLoads {
 template <typename S>
 __device__ __forceinline__ void store_partials(char* mine, int lane, const f32x16 (&acc)[S::NB][S::MB],
                                                float* partials, int64_t pitch, int64_t p0, int64_t rows, int64_t q0) {
-    using Exchange = RowExchange<32, 128>;
+    using Exchange = RowExchange<128>;
     static_assert(Exchange::kSize <= S::kWaveBytes, "the exchange fits the wave's LDS");
 #pragma unroll
     for (int m = 0; m < S::MB; ++m) {
@@ -229,124 +200,168 @@ __device__ __forceinline__ void store_partials(char* mine, int lane, const f32x1
     }
 }
 
-// ------------------------------------------------------- h and its two factors
-// Q is [gate rows | up rows] of the tile's 64 columns of h, so a lane holds both
-// factors of its products: block n < 4 the gate's, n + 4 the up's.
-template <int T, int MB, bool KEEP>
-__device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
-                                              const f32x4 (&acc)[8][MB]) {
-    // 16 rows at a time: 16-bit rows of 64 columns through the exchange, h, then
-    // the factors.
-    using Exchange = RowExchange<16, 128>;
-    constexpr int kOutputs = KEEP ? 3 : 1;
-    const int64_t column = q0 + Exchange::byte(lane) / 2;
+// FP32 rows of a wave's blocks of 32 x 32 into partials [rows, pitch] from row
+// p0 and column q0 on.
+template <int MB, int NB>
+__device__ __forceinline__ void store_partials(char* mine, int lane, const f32x16 (&acc)[NB][MB], float* partials,
+                                               int64_t pitch, int64_t p0, int64_t rows, int64_t q0) {
+    using Exchange = RowExchange<128>;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-        const int64_t row0 = p0 + 16 * m;
-        const int64_t row = row0 + (lane & 15);
-        const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            float h[4];
-            float first[4];
-            float second[4];
+        for (int n = 0; n < NB; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float act, slope;
-                activation<KEEP>(a.activation, acc[n][m][e], act, slope);
-                const float u = acc[n + 4][m][e];
-                h[e] = kept ? act * u : 0.0f;
-                first[e] = slope * u;
-                second[e] = act;
+            for (int q = 0; q < 4; ++q) {
+                const f32x16& c = acc[n][m];
+                Exchange::put(mine, lane, 32 * q + 16 * (lane >> 5),
+                              (f32x4){c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]});
             }
-            const int byte = 32 * n + 8 * (lane >> 4);
-            Exchange::put(mine, lane, byte, (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])});
-            if (KEEP) {
-                Exchange::put(mine + Exchange::kSize, lane, byte,
-                              (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])});
-                Exchange::put(mine + 2 * Exchange::kSize, lane, byte,
-                              (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])});
+            wave_lds_order();
+            const int64_t column = q0 + 32 * n + Exchange::byte(lane) / 4;
+#pragma unroll
+            for (int i = 0; i < Exchange::kSteps; ++i) {
+                const u32x4 value = Exchange::get(mine, lane, i);
+                const int64_t row = p0 + 32 * m + Exchange::row(lane, i);
+                if (row < rows && column < pitch) {
+                    *reinterpret_cast<u32x4*>(partials + row * pitch + column) = value;
+                }
+            }
+            wave_lds_order();
+        }
+    }
+}
+
+// ------------------------------------------------------- h and its two factors
+// Q is [gate rows | up rows] of the tile's columns of h, and a wave takes the
+// same columns of both, so that a lane holds both factors of its products: block
+// n < NB / 2 the gate's, n + NB / 2 the up's.  A wave's 32 rows at a time go
+// through the exchange as 16-bit rows of its columns, h, then the factors.
+template <int T, int MB, int NB, bool KEEP>
+__device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
+                                              const f32x16 (&acc)[NB][MB]) {
+    using Exchange = RowExchange<32 * NB>;
+    const int64_t column = q0 + Exchange::byte(lane) / 2;
+    const int half = lane >> 5;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+        const int64_t row0 = p0 + 32 * m;
+        const int64_t row = row0 + (lane & 31);
+        const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
+        u32x2 factors[KEEP ? 2 : 1][NB / 2][4];
+#pragma unroll
+        for (int n = 0; n < NB / 2; ++n) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float h[4];
+                float first[4];
+                float second[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float act, slope;
+                    activation<KEEP>(a.activation, acc[n][m][4 * q + e], act, slope);
+                    const float u = acc[n + NB / 2][m][4 * q + e];
+                    h[e] = kept ? act * u : 0.0f;
+                    first[e] = slope * u;
+                    second[e] = act;
+                }
+                Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half,
+                              (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])});
+                if constexpr (KEEP) {
+                    factors[0][n][q] = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
+                    factors[1][n][q] =
+                        (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])};
+                }
             }
         }
-        wave_lds_order();
 #pragma unroll
-        for (int o = 0; o < kOutputs; ++o) {
+        for (int o = 0; o < (KEEP ? 3 : 1); ++o) {
+            if constexpr (KEEP) {
+                if (o > 0) {
+#pragma unroll
+                    for (int n = 0; n < NB / 2; ++n) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half, factors[o - 1][n][q]);
+                        }
+                    }
+                }
+            }
+            wave_lds_order();
             uint16_t* const out = o == 0 ? a.h : a.gates + (o - 1) * a.pitch;
             const int64_t pitch = o == 0 ? a.pitch : 2 * a.pitch;
 #pragma unroll
             for (int i = 0; i < Exchange::kSteps; ++i) {
-                const u32x4 value = Exchange::get(mine + o * Exchange::kSize, lane, i);
+                const u32x4 value = Exchange::get(mine, lane, i);
                 const int64_t to = row0 + Exchange::row(lane, i);
                 if (to < a.rows && column < a.pitch) {
                     store16_unaligned(out + to * pitch + column, value);
                 }
             }
+            wave_lds_order();
         }
-        wave_lds_order();
     }
 }
 
-template <int T, int MB, bool KEEP>
-using GateShape = RowsShape<T, MB, 8, (KEEP ? 3 : 1) * RowExchange<16, 128>::kSize>;
+template <int T, int MB, int NB, int WP, int WQ>
+using GateShape = RowsShape<T, MB, NB, WP, WQ, RowExchange<32 * NB>::kSize>;
 
-template <int T, int MB, bool KEEP>
-__global__ __launch_bounds__(kProductThreads, 2) void gate_kernel(FeedForwardArgs a) {
-    using S = GateShape<T, MB, KEEP>;
+template <int T, int MB, int NB, int WP, int WQ, bool KEEP>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void gate_kernel(FeedForwardArgs a) {
+    using S = GateShape<T, MB, NB, WP, WQ>;
+    using P = typename S::PStage;
     using Q = typename S::QStage;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
-    constexpr int kColumns = 64;
+    constexpr int kColumns = S::BQ / 2;
     TileWalk walk(a.tiles, a.q_tiles);
     if (walk.left == 0) {
         return;
     }
-    const PRowLoads<MB> p(a.x_stride, a.in_pitch, wave, lane);
-    const QRowLoads<Q> q(a.in_pitch, a.in_pitch, wave, lane);
-    static_assert(Q::kLoads == 4, "two loads of each weight");
-    TileWalk p_walk = walk;
-    int p_slot = 0;
-    const auto x_rows = [&] {
-        const int64_t p0 = static_cast<int64_t>(p_walk.p) * S::BP;
-        return PRowLoads<MB>::lines(a.x + p0 * a.x_stride, a.x_stride, p_walk.left > 0 ? a.rows - p0 : 0);
+    const RowLoads<P> p(a.x_stride, a.in_pitch, wave, lane);
+    const RowLoads<Q> q(a.in_pitch, a.in_pitch, wave, lane);
+    static_assert(Q::kLoads % 2 == 0, "whole loads of each weight");
+    TileWalk ahead = walk;
+    int stage = 0;
+    BufferRsrc x, gate, up;
+    const auto aim = [&] {
+        const int64_t p0 = static_cast<int64_t>(ahead.p) * S::BP;
+        const int64_t q0 = static_cast<int64_t>(ahead.q) * kColumns;
+        const int64_t rows = ahead.left > 0 ? a.rows - p0 : 0;
+        const int64_t columns = ahead.left > 0 ? a.hidden - q0 : 0;
+        x = RowLoads<P>::aim(a.x + p0 * a.x_stride, a.x_stride, rows, S::BP);
+        gate = RowLoads<Q>::aim(a.gate + q0 * a.in_pitch, a.in_pitch, columns, kColumns);
+        up = RowLoads<Q>::aim(a.up + q0 * a.in_pitch, a.in_pitch, columns, kColumns);
     };
-    BufferRsrc x = x_rows();
-    TileWalk q_walk = walk;
-    int q_stage = 0;
-    const auto weight_rows = [&](const uint16_t* weight) {
-        const int64_t q0 = static_cast<int64_t>(q_walk.q) * kColumns;
-        return QRowLoads<Q>::lines(weight + q0 * a.in_pitch, a.in_pitch, q_walk.left > 0 ? a.hidden - q0 : 0, kColumns);
-    };
-    BufferRsrc gate = weight_rows(a.gate);
-    BufferRsrc up = weight_rows(a.up);
-    const auto load_p = [&](u32x4 (&fragments)[MB]) {
-        p.load(x, p_slot * kSlotK, fragments);
-        if (++p_slot == 2 * a.stages) {
-            p_slot = 0;
-            p_walk.next();
-            x = x_rows();
-        }
-    };
-    const auto issue_q = [&](char* stage) {
-        // Loads 0 and 1 of Q are rows 0 .. 63 of its stage, 2 and 3 the rest.
-        const int k = q_stage * kRowsStageK;
-        q.issue(gate, stage, wave, k, 0, 0);
-        q.issue(gate, stage, wave, k, 1, 1);
-        q.issue(up, stage, wave, k, 2, 0);
-        q.issue(up, stage, wave, k, 3, 1);
-        if (++q_stage == a.stages) {
-            q_stage = 0;
-            q_walk.next();
-            gate = weight_rows(a.gate);
-            up = weight_rows(a.up);
-        }
-    };
-    run_rows_tiles<S>(lds, walk.left, a.stages, load_p, issue_q, [&](const f32x4 (&acc)[8][MB]) {
-        gate_epilogue<T, MB, KEEP>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
-                                   static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
-                                   static_cast<int64_t>(walk.q) * kColumns, acc);
-        walk.next();
-    });
+    aim();
+    const int wave_column = S::wave_q(wave) / 2;
+    run_rows_tiles<S>(
+        lds, walk.left, a.stages,
+        [&](char* to) {
+            const int k = stage * kRowsStageK;
+#pragma unroll
+            for (int j = 0; j < P::kLoads; ++j) {
+                p.issue(x, to, S::kWaves, wave, k, j, j);
+            }
+            // The first half of Q's loads are the gate's rows, the second the up's.
+#pragma unroll
+            for (int j = 0; j < Q::kLoads; ++j) {
+                constexpr int kEach = Q::kLoads / 2;
+                q.issue(j < kEach ? gate : up, to + P::kBytes, S::kWaves, wave, k, j, j % kEach);
+            }
+            if (++stage == a.stages) {
+                stage = 0;
+                ahead.next();
+                aim();
+            }
+        },
+        [&](int n) { return n < NB / 2 ? wave_column + 32 * n : kColumns + wave_column + 32 * (n - NB / 2); },
+        [&](const f32x16 (&acc)[NB][MB]) {
+            gate_epilogue<T, MB, NB, KEEP>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
+                                           static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
+                                           static_cast<int64_t>(walk.q) * kColumns + wave_column, acc);
+            walk.next();
+        });
 }
 
 // ------------------------------------------------------------------ y and dx
@@ -354,79 +369,65 @@ __global__ __launch_bounds__(kProductThreads, 2) void gate_kernel(FeedForwardArg
 // transposed side by side, as dg and du lie.  With `splits` > 1 the stages are
 // divided and FP32 partials left for join_kernel.
 template <int T, int MB, int NB>
-using ProductRows = RowsShape<T, MB, NB, RowExchange<16, 32 * NB>::kSize>;
-
-template <int T, int MB, int NB>
 __device__ __forceinline__ void product_epilogue(const FeedForwardProduct& a, char* mine, int lane, int split,
-                                                 int64_t p0, int64_t q0, const f32x4 (&acc)[NB][MB]) {
+                                                 int64_t p0, int64_t q0, const f32x16 (&acc)[NB][MB]) {
     if (a.partials != nullptr) {   // uniform
-        using Exchange = RowExchange<16, 32 * NB>;   // half the columns at a time
-        float* const out = a.partials + split * a.rows * a.partial_pitch;
-#pragma unroll
-        for (int m = 0; m < MB; ++m) {
-            const int64_t row0 = p0 + 16 * m;
-#pragma unroll
-            for (int n0 = 0; n0 < NB; n0 += NB / 2) {
-#pragma unroll
-                for (int n = 0; n < NB / 2; ++n) {
-                    Exchange::put(mine, lane, 64 * n + 16 * (lane >> 4), acc[n0 + n][m]);
-                }
-                wave_lds_order();
-                const int64_t column = q0 + 16 * n0 + Exchange::byte(lane) / 4;
-#pragma unroll
-                for (int i = 0; i < Exchange::kSteps; ++i) {
-                    const u32x4 value = Exchange::get(mine, lane, i);
-                    const int64_t to = row0 + Exchange::row(lane, i);
-                    if (to < a.rows && column < a.partial_pitch) {
-                        *reinterpret_cast<u32x4*>(out + to * a.partial_pitch + column) = value;
-                    }
-                }
-                wave_lds_order();
-            }
-        }
+        store_partials<MB, NB>(mine, lane, acc, a.partials + split * a.rows * a.partial_pitch, a.partial_pitch, p0,
+                               a.rows, q0);
         return;
     }
-    using Exchange = RowExchange<16, 32 * NB>;
-    const int64_t column = q0 + Exchange::byte(lane) / 2;
+    constexpr int kGroup = NB < 2 ? 1 : 2;   // blocks of 32 columns at a time
+    using Exchange = RowExchange<64 * kGroup>;
+    const int half = lane >> 5;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-        const int64_t row0 = p0 + 16 * m;
-        const int64_t row = row0 + (lane & 15);
+        const int64_t row0 = p0 + 32 * m;
+        const int64_t row = row0 + (lane & 31);
         const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            f32x4 v = acc[n][m];
+        for (int n0 = 0; n0 < NB; n0 += kGroup) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = kept ? v[e] : 0.0f;
+            for (int n = 0; n < kGroup; ++n) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = kept ? acc[n0 + n][m][4 * q + e] : 0.0f;
+                    }
+                    Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half,
+                                  (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])});
+                }
             }
-            Exchange::put(mine, lane, 32 * n + 8 * (lane >> 4),
-                          (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])});
-        }
-        wave_lds_order();
+            wave_lds_order();
+            const int64_t column = q0 + 32 * n0 + Exchange::byte(lane) / 2;
 #pragma unroll
-        for (int i = 0; i < Exchange::kSteps; ++i) {
-            const u32x4 value = Exchange::get(mine, lane, i);
-            const int64_t to = row0 + Exchange::row(lane, i);
-            uint16_t* at = a.out + to * a.columns + column;
-            if (to < a.rows && column + 8 <= a.columns) {
-                store16_unaligned(at, value);
-            } else if (to < a.rows) {
+            for (int i = 0; i < Exchange::kSteps; ++i) {
+                const u32x4 value = Exchange::get(mine, lane, i);
+                const int64_t to = row0 + Exchange::row(lane, i);
+                uint16_t* at = a.out + to * a.columns + column;
+                if (to < a.rows && column + 8 <= a.columns) {
+                    store16_unaligned(at, value);
+                } else if (to < a.rows) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (column + e < a.columns) {
-                        at[e] = static_cast<uint16_t>(value[e / 2] >> (16 * (e & 1)));
+                    for (int e = 0; e < 8; ++e) {
+                        if (column + e < a.columns) {
+                            at[e] = static_cast<uint16_t>(value[e / 2] >> (16 * (e & 1)));
+                        }
                     }
                 }
             }
+            wave_lds_order();
         }
-        wave_lds_order();
     }
 }
 
-template <int T, int MB, int NB>
-__global__ __launch_bounds__(kProductThreads, 2) void product_kernel(FeedForwardProduct a) {
-    using S = ProductRows<T, MB, NB>;
+template <int T, int MB, int NB, int WP, int WQ>
+using ProductRows = RowsShape<T, MB, NB, WP, WQ, RowExchange<128>::kSize>;
+
+template <int T, int MB, int NB, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardProduct a) {
+    using S = ProductRows<T, MB, NB, WP, WQ>;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
@@ -439,37 +440,38 @@ __global__ __launch_bounds__(kProductThreads, 2) void product_kernel(FeedForward
     const int last = first + a.split_stages < a.stages ? first + a.split_stages : a.stages;
     RowStream<S> stream(a.p, a.p_stride, a.rows, a.q, a.q_stride, a.columns, a.k, first, last, walk, wave, lane);
     run_rows_tiles<S>(
-        lds, walk.left, last - first, [&](u32x4 (&fragments)[MB]) { stream.load_p(fragments); },
-        [&](char* stage) { stream.issue_q(stage); },
-        [&](const f32x4 (&acc)[NB][MB]) {
+        lds, walk.left, last - first, [&](char* to) { stream.issue(to); },
+        [&](int n) { return S::wave_q(wave) + 32 * n; },
+        [&](const f32x16 (&acc)[NB][MB]) {
             product_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane, split,
-                                        static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
-                                        static_cast<int64_t>(walk.q) * S::BQ, acc);
+                                        static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
+                                        static_cast<int64_t>(walk.q) * S::BQ + S::wave_q(wave), acc);
             walk.next();
         });
 }
 
 // ----------------------------------------------------------------- dg and du
-template <int T, int MB, int NB>
-using GradShape = RowsShape<T, MB, NB, RowExchange<16, 256>::kSize>;
-
+// dh goes through the exchange in FP32, 32 rows x 32 columns at a time: in its
+// rows the factors are read and dg, du written as whole pieces.
 template <int T, int MB, int NB>
 __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
-                                              const f32x4 (&acc)[NB][MB]) {
-    // dh goes through the exchange in FP32, 16 rows x 64 columns at a time: in
-    // its rows the factors are read and dg, du written whole pieces at a time.
-    using Exchange = RowExchange<16, 256>;
+                                              const f32x16 (&acc)[NB][MB]) {
+    using Exchange = RowExchange<128>;
+    constexpr int kLanes = 4;   // of a row, 8 columns each
+    constexpr int kRows = 64 / kLanes;
+    constexpr int kSteps = 32 / kRows;
+    const int half = lane >> 5;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-        const int64_t row0 = p0 + 16 * m;
+        const int64_t row0 = p0 + 32 * m;
 #pragma unroll
-        for (int n0 = 0; n0 < NB; n0 += 4) {
-            const int64_t column = q0 + 16 * n0 + 8 * (lane & 7);
-            u32x4 raw[2][2];
-            bool kept[2];
+        for (int n = 0; n < NB; ++n) {
+            const int64_t column = q0 + 32 * n + 8 * (lane % kLanes);
+            u32x4 raw[kSteps][2];
+            bool kept[kSteps];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t row = row0 + 8 * i + (lane >> 3);
+            for (int i = 0; i < kSteps; ++i) {
+                const int64_t row = row0 + kRows * i + lane / kLanes;
                 if (row < a.rows && column < a.pitch) {
                     const uint16_t* at = a.gates + 2 * row * a.pitch + column;
                     raw[i][0] = load16_unaligned(at);
@@ -478,17 +480,18 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                Exchange::put(mine, lane, 64 * n + 16 * (lane >> 4), acc[n0 + n][m]);
+            for (int q = 0; q < 4; ++q) {
+                const f32x16& c = acc[n][m];
+                Exchange::put(mine, lane, 32 * q + 16 * half,
+                              (f32x4){c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]});
             }
             wave_lds_order();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = 8 * i + (lane >> 3);
+            for (int i = 0; i < kSteps; ++i) {
+                const int r = kRows * i + lane / kLanes;
                 const int64_t row = row0 + r;
-                const char* from = mine + r * Exchange::kPitch + 32 * (lane & 7);
-                const f32x4 low = *reinterpret_cast<const f32x4*>(from);
-                const f32x4 high = *reinterpret_cast<const f32x4*>(from + 16);
+                const f32x4 low = __builtin_bit_cast(f32x4, Exchange::piece(mine, r, 32 * (lane % kLanes)));
+                const f32x4 high = __builtin_bit_cast(f32x4, Exchange::piece(mine, r, 32 * (lane % kLanes) + 16));
                 if (row < a.rows && column < a.pitch) {
                     float dg[8];
                     float du[8];
@@ -510,9 +513,12 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
     }
 }
 
-template <int T, int MB, int NB>
-__global__ __launch_bounds__(kProductThreads, 2) void grad_kernel(FeedForwardArgs a) {
-    using S = GradShape<T, MB, NB>;
+template <int T, int MB, int NB, int WP, int WQ>
+using GradShape = RowsShape<T, MB, NB, WP, WQ, RowExchange<128>::kSize>;
+
+template <int T, int MB, int NB, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void grad_kernel(FeedForwardArgs a) {
+    using S = GradShape<T, MB, NB, WP, WQ>;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
@@ -523,12 +529,12 @@ __global__ __launch_bounds__(kProductThreads, 2) void grad_kernel(FeedForwardArg
     RowStream<S> stream(a.dy, a.dy_stride, a.rows, a.down_columns, a.out_pitch, a.hidden, a.out_pitch, 0, a.stages, walk,
                         wave, lane);
     run_rows_tiles<S>(
-        lds, walk.left, a.stages, [&](u32x4 (&fragments)[MB]) { stream.load_p(fragments); },
-        [&](char* stage) { stream.issue_q(stage); },
-        [&](const f32x4 (&acc)[NB][MB]) {
+        lds, walk.left, a.stages, [&](char* to) { stream.issue(to); },
+        [&](int n) { return S::wave_q(wave) + 32 * n; },
+        [&](const f32x16 (&acc)[NB][MB]) {
             grad_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
-                                     static_cast<int64_t>(walk.p) * S::BP + 16 * MB * wave,
-                                     static_cast<int64_t>(walk.q) * S::BQ, acc);
+                                     static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
+                                     static_cast<int64_t>(walk.q) * S::BQ + S::wave_q(wave), acc);
             walk.next();
         });
 }
@@ -592,9 +598,9 @@ __global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardW
         },
         q_start);
 
-    store_partials<S>(lds + S::kWaveBytes * wave, lane, acc,
-                      a.partials + split * a.partial_floats + w.partial_offset, w.partial_pitch,
-                      p0 + S::wave_p(wave), w.out_rows, q0 + q_start(0));
+    static_assert(RowExchange<128>::kSize <= S::kWaveBytes, "the exchange fits the wave's LDS");
+    store_partials<MB, NB>(lds + S::kWaveBytes * wave, lane, acc, a.partials + split * a.partial_floats + w.partial_offset,
+                           w.partial_pitch, p0 + S::wave_p(wave), w.out_rows, q0 + q_start(0));
 }
 
 // Sum of `splits` partials [rows, pitch] in order, rounded once into out [rows,
@@ -704,30 +710,20 @@ __global__ __launch_bounds__(256) void pack_kernel(FeedForwardPack a) {
     }
 }
 
-// Tile edges of a product, in 64s: P and Q.
-struct Edges {
-    int mb;
-    int nb;
-};
+// Tiles of the row products: 256 x 256 by 8 waves, 128 x 128 or 64 x 64 by 4.
+// The larger the tile, the fewer bytes a product moves between L2, LDS and
+// registers, so a size is taken once it gives nearly every CU a tile.
+enum class Edge { kLarge, kMiddle, kSmall };
 
 int64_t tiles_of(int64_t p, int64_t q, int64_t bp, int64_t bq) { return ((p + bp - 1) / bp) * ((q + bq - 1) / bq); }
 
-// The largest tile that still gives every CU its two workgroups; the larger
-// the tile, the fewer bytes a product moves between L2, LDS and registers.
-constexpr int64_t kSlots = 512;
+constexpr int64_t kCus = 256;
 
-Edges choose_edges(int64_t p, int64_t q) {
-    if (tiles_of(p, q, 256, 128) >= kSlots) {
-        return {4, 2};
+Edge choose_edge(int64_t p, int64_t q) {
+    if (tiles_of(p, q, 256, 256) >= kCus) {
+        return Edge::kLarge;
     }
-    return tiles_of(p, q, 128, 128) >= kSlots / 2 ? Edges{2, 2} : Edges{1, 1};
-}
-
-int choose_gate(int64_t rows, int64_t pitch) {
-    if (tiles_of(rows, pitch, 256, 64) >= kSlots) {
-        return 4;
-    }
-    return tiles_of(rows, pitch, 128, 64) >= kSlots / 2 ? 2 : 1;
+    return tiles_of(p, q, 128, 128) >= kCus ? Edge::kMiddle : Edge::kSmall;
 }
 
 // A multiple of eight workgroups (one share per XCD), at most what is resident.
@@ -736,22 +732,22 @@ dim3 tile_grid(int tiles, int slots, int splits = 1) {
     return dim3(static_cast<unsigned>(8 * (per_xcd < slots ? per_xcd : slots)), static_cast<unsigned>(splits));
 }
 
-template <int T, int MB, bool KEEP>
+template <int T, int MB, int NB, int WP, int WQ, bool KEEP>
 hipError_t launch_gate(FeedForwardArgs a, hipStream_t stream) {
-    using S = GateShape<T, MB, KEEP>;
+    using S = GateShape<T, MB, NB, WP, WQ>;
     a.stages = static_cast<int>((a.in_pitch + kRowsStageK - 1) / kRowsStageK);
-    a.q_tiles = static_cast<int>((a.pitch + 63) / 64);
+    a.q_tiles = static_cast<int>((a.pitch + S::BQ / 2 - 1) / (S::BQ / 2));
     a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
-    gate_kernel<T, MB, KEEP><<<tile_grid(a.tiles, S::kSlots), kProductThreads, 0, stream>>>(a);
+    gate_kernel<T, MB, NB, WP, WQ, KEEP><<<tile_grid(a.tiles, S::kSlots), S::kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 template <int T, bool KEEP>
 hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
-    switch (choose_gate(a.rows, a.pitch)) {
-        case 4: return launch_gate<T, 4, KEEP>(a, stream);
-        case 2: return launch_gate<T, 2, KEEP>(a, stream);
-        default: return launch_gate<T, 1, KEEP>(a, stream);
+    switch (choose_edge(a.rows, 2 * a.pitch)) {
+        case Edge::kLarge: return launch_gate<T, 2, 4, 4, 2, KEEP>(a, stream);
+        case Edge::kMiddle: return launch_gate<T, 2, 2, 2, 2, KEEP>(a, stream);
+        default: return launch_gate<T, 1, 2, 2, 2, KEEP>(a, stream);
     }
 }
 
@@ -760,12 +756,12 @@ hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
     return a.gates != nullptr ? launch_gate<T, true>(a, stream) : launch_gate<T, false>(a, stream);
 }
 
-template <int T, int MB, int NB>
+template <int T, int MB, int NB, int WP, int WQ>
 hipError_t launch_product(FeedForwardProduct a, hipStream_t stream) {
-    using S = ProductRows<T, MB, NB>;
+    using S = ProductRows<T, MB, NB, WP, WQ>;
     a.q_tiles = static_cast<int>((a.columns + S::BQ - 1) / S::BQ);
     a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
-    product_kernel<T, MB, NB><<<tile_grid(a.tiles, S::kSlots, a.splits), kProductThreads, 0, stream>>>(a);
+    product_kernel<T, MB, NB, WP, WQ><<<tile_grid(a.tiles, S::kSlots, a.splits), S::kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -775,9 +771,12 @@ hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     if (a.splits == 1) {
         a.partials = nullptr;
     }
-    const hipError_t error = a.mb == 4   ? launch_product<T, 4, 8>(a, stream)
-                             : a.mb == 2 ? launch_product<T, 2, 8>(a, stream)
-                                         : launch_product<T, 1, 4>(a, stream);
+    hipError_t error;
+    switch (choose_edge(a.rows, a.columns)) {
+        case Edge::kLarge: error = launch_product<T, 2, 4, 4, 2>(a, stream); break;
+        case Edge::kMiddle: error = launch_product<T, 2, 2, 2, 2>(a, stream); break;
+        default: error = launch_product<T, 1, 1, 2, 2>(a, stream); break;
+    }
     if (a.splits == 1 || error != hipSuccess) {
         return error;
     }
@@ -792,22 +791,22 @@ hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int T, int MB, int NB>
+template <int T, int MB, int NB, int WP, int WQ>
 hipError_t launch_grad(FeedForwardArgs a, hipStream_t stream) {
-    using S = GradShape<T, MB, NB>;
+    using S = GradShape<T, MB, NB, WP, WQ>;
     a.stages = static_cast<int>((a.out_pitch + kRowsStageK - 1) / kRowsStageK);
     a.q_tiles = static_cast<int>((a.pitch + S::BQ - 1) / S::BQ);
     a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
-    grad_kernel<T, MB, NB><<<tile_grid(a.tiles, S::kSlots), kProductThreads, 0, stream>>>(a);
+    grad_kernel<T, MB, NB, WP, WQ><<<tile_grid(a.tiles, S::kSlots), S::kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 template <int T>
 hipError_t launch_grad(const FeedForwardArgs& a, hipStream_t stream) {
-    switch (choose_edges(a.rows, a.pitch).mb) {
-        case 4: return launch_grad<T, 4, 8>(a, stream);
-        case 2: return launch_grad<T, 2, 8>(a, stream);
-        default: return launch_grad<T, 1, 4>(a, stream);
+    switch (choose_edge(a.rows, a.pitch)) {
+        case Edge::kLarge: return launch_grad<T, 2, 4, 4, 2>(a, stream);
+        case Edge::kMiddle: return launch_grad<T, 2, 2, 2, 2>(a, stream);
+        default: return launch_grad<T, 1, 1, 2, 2>(a, stream);
     }
 }
 
@@ -832,15 +831,16 @@ hipError_t launch_weights(const FeedForwardWeights& args, hipStream_t stream) {
 }  // namespace
 
 void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProduct* a) {
-    const Edges e = choose_edges(rows, columns);
-    a->mb = e.mb;
-    a->nb = e.nb;
     a->stages = static_cast<int>(stages);
-    const int64_t tiles = tiles_of(rows, columns, 64 * e.mb, 64 * e.nb);
-    // A long K over few tiles: split so that the CUs fill, at least 4 stages each.
-    int64_t splits = tiles > 0 ? kSlots / tiles : 1;
-    splits = splits < stages / 4 ? splits : stages / 4;
-    splits = splits < 1 ? 1 : splits;
+    int64_t splits = 1;
+    if (choose_edge(rows, columns) == Edge::kSmall) {
+        // A long K over few tiles: split so that each CU has two, at least 4
+        // stages each.
+        const int64_t tiles = tiles_of(rows, columns, 64, 64);
+        splits = tiles > 0 ? 2 * kCus / tiles : 1;
+        splits = splits < stages / 4 ? splits : stages / 4;
+        splits = splits < 1 ? 1 : splits;
+    }
     a->split_stages = static_cast<int>((stages + splits - 1) / splits);
     a->splits = static_cast<int>((stages + a->split_stages - 1) / a->split_stages);
     a->partial_pitch = (columns + 7) / 8 * 8;
@@ -856,7 +856,7 @@ void plan_weights(FeedForwardWeights* a) {
         return tiles;
     };
     // The large tile where its workgroups still have 512 rows each.
-    if (count(256, 128) * a->rows >= 512 * kSlots * 1) {
+    if (count(256, 128) * a->rows >= 1024 * kCus) {
         a->mb = 4;
     }
     const int64_t bp = 64 * a->mb;
@@ -869,7 +869,7 @@ void plan_weights(FeedForwardWeights* a) {
         w.partial_offset = a->partial_floats;
         a->partial_floats += w.out_rows * w.partial_pitch;
     }
-    int64_t splits = a->tiles > 0 ? kSlots / a->tiles : 1;
+    int64_t splits = a->tiles > 0 ? 2 * kCus / a->tiles : 1;
     const int64_t most = (a->rows + 127) / 128;
     splits = splits < most ? splits : most;
     const int64_t least = (a->rows + kWeightSplitRows - 1) / kWeightSplitRows;

@@ -382,7 +382,6 @@ struct FeedForwardProduct {
     int stages;                 // set by plan_product, as what follows
     int split_stages;
     int splits;
-    int mb, nb;
     int q_tiles;                // set by the launcher
     int tiles;
 };

@@ -249,75 +249,74 @@ __device__ __forceinline__ void row_pieces(const f32x16& acc, float (&piece)[2][
 }
 
 // ---------------------------------------------------------------------------
-// The product for both operands in rows (x W^T): P never passes LDS.  Each wave owns
-// 16 MB rows of P and all of the tile's columns, so no other wave needs its
-// rows, and on v_mfma_f32_16x16x32 a fragment of 16 rows x 32 k is one load of
-// 64 bytes from each row, straight into the lanes that multiply it.  With both
-// operands through LDS, their writes and the fragments' reads together exceed
-// the LDS's 128 bytes per clock at the matrix rate: the 256 x 128 tile ran at
-// 28% of the matrix peak, and at 70% with its loads left out.  Here only Q's
-// stage, half the width, is written to LDS and read by the four waves.
+// The product for both operands in rows (x W^T).  A stage is 64 k, so that every
+// load covers whole 128-byte lines: the L2 answers one request per channel and
+// clock whatever its size, half a request per CU, and with stages of 32 k (64
+// bytes of a row) the requests alone took longer than the MFMAs.  For the same
+// reason the largest tile is 256 x 256 (8 waves, 64 KB a stage): 32 bytes per CU
+// and clock at the matrix rate, where the L2 gives 54.  Fragments of P read
+// straight from memory into the lanes that multiply them save LDS bandwidth, but
+// 64 lanes on 16 rows are 64 separate accesses (16 bytes per clock).
 //
-// A stage is 64 k: Q's in a ring of three (16 KB each at 128 columns, loaded by
-// buffer_load ... lds as above), P's as two slots of 32 k in a ring of four in
-// registers, loaded three slots ahead.  The stage's fragments of Q are read in
-// four groups, each under the MFMAs of the one before; the barrier that frees
-// the stage lies before the last group's MFMAs.
-constexpr int kSlotK = 32;
+// Two stages alternate: one is multiplied while the next one's loads are in
+// flight.  Fragments of a step (16 k) are read under the MFMAs of the step
+// before; the barrier that frees a stage and admits the next lies before the
+// last step's MFMAs, whose fragments are in registers by then.
 constexpr int kRowsStageK = 64;
-constexpr int kRowsRing = 3;
+constexpr int kRowsSteps = 4;
 
-template <int T>
-__device__ __forceinline__ f32x4 mfma_small(const u32x4& a, const u32x4& b, const f32x4& c) {
-    if constexpr (T == LSSO_HIP_BF16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                       0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                      0, 0);
-    }
-}
-
-// Q's stage of WIDTH rows.
-template <int WIDTH>
+// Stage of WIDTH rows, loaded by WAVES waves.
+template <int WIDTH, int WAVES>
 struct RowsStage {
     static constexpr int kBytes = WIDTH * kRowsStageK * 2;
-    static constexpr int kLoads = kBytes / 1024 / 4;   // per wave
+    static constexpr int kLoads = kBytes / 1024 / WAVES;   // per wave
+    static constexpr int kRowsPerRound = 8 * WAVES;        // of one load of every wave
+    static_assert(kLoads >= 1, "every wave loads");
     // Piece c of row p lies at slot c ^ swizzle(p), so that any 8 or 16 rows of
     // one piece fall on different banks.
     __device__ static __forceinline__ int swizzle(int p) { return (p & 7) ^ ((p >> 3) & 1); }
-    // Row that this lane loads with load j, and its first element of that row,
-    // the same for every j.
-    __device__ static __forceinline__ int load_row(int wave, int lane, int j) { return 8 * (4 * j + wave) + (lane >> 3); }
+    // Row of this lane's first load (kRowsPerRound further for each one after
+    // it) and its first element of that row.
+    __device__ static __forceinline__ int load_row(int wave, int lane) { return 8 * wave + (lane >> 3); }
     __device__ static __forceinline__ int load_element(int wave, int lane) {
-        return 8 * ((lane & 7) ^ swizzle(load_row(wave, lane, 0)));
+        return 8 * ((lane & 7) ^ swizzle(load_row(wave, lane)));
     }
-    // This lane's fragment of rows 16 n .. of slot 0 or 1.
-    __device__ static __forceinline__ u32x4 read(const char* stage, int lane, int n, int slot) {
-        const int p = lane & 15;
-        return *reinterpret_cast<const u32x4*>(stage + 2048 * n + (128 * p + 16 * ((4 * slot + (lane >> 4)) ^ swizzle(p))));
+    // This lane's fragment of rows p0 .. p0 + 31 (p0 a multiple of 32) at a step.
+    __device__ static __forceinline__ u32x4 read(const char* stage, int lane, int p0, int step) {
+        const int p = lane & 31;
+        return *reinterpret_cast<const u32x4*>(stage + 128 * p0 +
+                                               (128 * p + 16 * ((2 * step + (lane >> 5)) ^ swizzle(p))));
     }
 };
 
-// T: type code; MB x NB blocks of 16 x 16 per wave, the four waves along P;
-// EXCHANGE: bytes of LDS per wave for the epilogue.
-template <int T_, int MB_, int NB_, int EXCHANGE>
+// T: type code; MB x NB blocks of 32 x 32 per wave, WP x WQ waves; EXCHANGE:
+// bytes of LDS per wave for the epilogue.
+template <int T_, int MB_, int NB_, int WP_, int WQ_, int EXCHANGE>
 struct RowsShape {
     static constexpr int T = T_;
     static constexpr int MB = MB_;
     static constexpr int NB = NB_;
-    static constexpr int BP = 64 * MB;
-    static constexpr int BQ = 16 * NB;
-    using QStage = RowsStage<BQ>;
-    static constexpr int kRingBytes = kRowsRing * QStage::kBytes;
+    static constexpr int WP = WP_;
+    static constexpr int WQ = WQ_;
+    static constexpr int kWaves = WP * WQ;
+    static constexpr int kThreads = 64 * kWaves;
+    static constexpr int BP = 32 * MB * WP;
+    static constexpr int BQ = 32 * NB * WQ;
+    using PStage = RowsStage<BP, kWaves>;
+    using QStage = RowsStage<BQ, kWaves>;
+    static constexpr int kStageBytes = PStage::kBytes + QStage::kBytes;
+    static constexpr int kRingBytes = 2 * kStageBytes;
     static constexpr int kWaveBytes = EXCHANGE;
-    static constexpr int kLdsBytes = kRingBytes + 4 * EXCHANGE;
-    // Workgroups of one XCD's 32 CUs that are resident at once: by LDS (160 KB)
-    // and by registers (accumulators, fragments and 32 more of 512 per SIMD
-    // lane, one wave of each workgroup per SIMD).
+    static constexpr int kLdsBytes = kRingBytes + kWaves * EXCHANGE;
+    static constexpr int kLoads = PStage::kLoads + QStage::kLoads;
+    // Workgroups that are resident on one XCD's 32 CUs: by LDS (160 KB) and by
+    // registers (accumulators, two steps' fragments and 48 more of 512 for the
+    // waves of a SIMD).
     static constexpr int kByLds = 160 * 1024 / kLdsBytes;
-    static constexpr int kByRegisters = 512 / (4 * MB * NB + 16 * MB + 4 * NB + 32);
+    static constexpr int kByRegisters = 512 / (16 * MB * NB + 8 * (MB + NB) + 48) * 4 / kWaves;
     static constexpr int kSlots = 32 * (kByLds < kByRegisters ? kByLds : kByRegisters);
+    __device__ static __forceinline__ int wave_p(int wave) { return 32 * MB * (wave % WP); }
+    __device__ static __forceinline__ int wave_q(int wave) { return 32 * NB * (wave / WP); }
 };
 
 // The tiles of one workgroup: XCD x (workgroup index mod 8) takes the x-th eighth
@@ -354,130 +353,111 @@ struct TileWalk {
     }
 };
 
-// Runs `tiles` tiles of `stages` stages each.  load_p fills the fragments of the
-// next slot of P and issue_q starts the next stage of Q into an LDS stage, each
-// in order through all tiles and asked for a few past the last; epilogue(acc)
-// takes a tile's sums.  The loads run ahead across the tiles' borders, so a
-// tile's first stages arrive under the epilogue of the one before: a tile of
-// 256 k has four stages, and began with a wait for memory as long as all its
-// MFMAs.
-template <typename S, typename LoadP, typename IssueQ, typename Epilogue>
-__device__ __forceinline__ void run_rows_tiles(char* lds, int tiles, int stages, LoadP load_p, IssueQ issue_q,
+// Runs `tiles` tiles of `stages` stages each.  issue(lds) starts the loads of the
+// next stage, kLoads per wave, in order through all tiles and asked for two past
+// the last; q_start(n) is the tile's first row of Q of this wave's block n;
+// epilogue(acc) takes a tile's sums.  The loads run ahead across the tiles'
+// borders, so a tile's first stages arrive under the epilogue of the one
+// before: a tile of 256 k has four stages, and began with a wait for memory as
+// long as all its MFMAs.
+template <typename S, typename Issue, typename QStart, typename Epilogue>
+__device__ __forceinline__ void run_rows_tiles(char* lds, int tiles, int stages, Issue issue, QStart q_start,
                                                Epilogue epilogue) {
-    constexpr int kHalf = S::NB / 2;
     const int lane = threadIdx.x & 63;
-    f32x4 acc[S::NB][S::MB];
-    u32x4 pf[4][S::MB];
-    u32x4 qf[2][kHalf];
-    const auto read = [&](const char* stage, int group) {
+    const int wave = wave_index();
+    f32x16 acc[S::NB][S::MB];
+    u32x4 pf[2][S::MB];
+    u32x4 qf[2][S::NB];
+    const auto read = [&](const char* stage, int step) {
 #pragma unroll
-        for (int n = 0; n < kHalf; ++n) {
-            qf[group & 1][n] = S::QStage::read(stage, lane, kHalf * (group & 1) + n, group >> 1);
+        for (int n = 0; n < S::NB; ++n) {
+            qf[step & 1][n] = S::QStage::read(stage + S::PStage::kBytes, lane, q_start(n), step);
+        }
+#pragma unroll
+        for (int m = 0; m < S::MB; ++m) {
+            pf[step & 1][m] = S::PStage::read(stage, lane, S::wave_p(wave) + 32 * m, step);
         }
     };
-    const auto multiply = [&](int slot, int group) {
+    const auto multiply = [&](int step) {
 #pragma unroll
-        for (int n = 0; n < kHalf; ++n) {
+        for (int m = 0; m < S::MB; ++m) {
 #pragma unroll
-            for (int m = 0; m < S::MB; ++m) {
-                f32x4& c = acc[kHalf * (group & 1) + n][m];
-                c = mfma_small<S::T>(qf[group & 1][n], pf[slot][m], c);
+            for (int n = 0; n < S::NB; ++n) {
+                acc[n][m] = mfma_block<S::T>(qf[step & 1][n], pf[step & 1][m], acc[n][m]);
             }
         }
     };
     int at = 0;   // LDS offset of this stage
-    // One stage; `slot`: the register slot of its first 32 k, 0 or 2.
-    const auto stage = [&](int slot) {
+    const auto stage = [&] {
         char* const here = lds + at;
-        const int next = at == (kRowsRing - 1) * S::QStage::kBytes ? 0 : at + S::QStage::kBytes;
-        read(here, 1);
-        load_p(pf[(slot + 3) & 3]);
+        at ^= S::kStageBytes;
+#pragma unroll
+        for (int step = 0; step < kRowsSteps - 1; ++step) {
+            read(here, step + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(step);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage_barrier<0>();   // the next stage has landed, and nobody reads this one any more
+        issue(here);
+        read(lds + at, 0);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(slot, 0);
+        multiply(kRowsSteps - 1);
         __builtin_amdgcn_sched_barrier(0);
-        read(here, 2);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(slot, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        read(here, 3);
-        load_p(pf[slot]);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(slot + 1, 2);
-        __builtin_amdgcn_sched_barrier(0);
-        // The next stage has landed when no more than what was issued behind it
-        // is outstanding: the stage after it and four slots.
-        stage_barrier<S::QStage::kLoads + 4 * S::MB>();
-        issue_q(here);
-        read(lds + next, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(slot + 1, 3);
-        __builtin_amdgcn_sched_barrier(0);
-        at = next;
     };
-#pragma unroll
-    for (int i = 0; i < kRowsRing; ++i) {
-        issue_q(lds + i * S::QStage::kBytes);
-    }
-#pragma unroll
-    for (int t = 0; t < 3; ++t) {
-        load_p(pf[t]);
-    }
-    stage_barrier<2 * S::QStage::kLoads + 3 * S::MB>();
+    issue(lds);
+    issue(lds + S::kStageBytes);
+    stage_barrier<S::kLoads>();
     read(lds, 0);
     for (int tile = 0; tile < tiles; ++tile) {
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
 #pragma unroll
             for (int m = 0; m < S::MB; ++m) {
-                acc[n][m] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    acc[n][m][e] = 0.0f;
+                }
             }
         }
-        for (int s = 0;;) {
-            stage(0);
-            if (++s == stages) break;
-            stage(2);
-            if (++s == stages) break;
+        for (int s = 0; s < stages; ++s) {
+            stage();
         }
         epilogue(acc);
-        if ((stages & 1) != 0) {   // the next tile begins with register slot 0 again
-#pragma unroll
-            for (int m = 0; m < S::MB; ++m) {
-                const u32x4 first = pf[0][m];
-                const u32x4 second = pf[1][m];
-                pf[0][m] = pf[2][m];
-                pf[1][m] = pf[3][m];
-                pf[2][m] = first;
-                pf[3][m] = second;
-            }
-        }
     }
     // The loads past the last stage still write their zeros: not into LDS that
     // another workgroup may hold by then.
     stage_barrier<0>();
 }
 
-// A wave's exchange of ROWS rows of BYTES (64, 128 or 256) through its own part
-// of LDS, from a lane per row to BYTES / 16 consecutive lanes per row: stored
-// from the accumulators' layout, an instruction covers 32 bytes of each of 32
-// rows, and partly written lines cost the memory side twice (131,072 x 688 x 3
-// stores at 2.6 TB/s); exchanged, it covers whole rows' pieces of 128 bytes.
-// LDS serves a wave's accesses in order, so no barrier is needed, and the 16
-// bytes of padding keep both sides free of conflicts.
-template <int ROWS, int BYTES>
+// A wave's exchange of 32 rows of BYTES (64 or 128) through its own part of LDS,
+// from a lane per row to BYTES / 16 consecutive lanes per row: stored from the
+// accumulators' layout, an instruction covers 32 bytes of each of 32 rows, and
+// partly written lines cost the memory side twice (131,072 x 688 x 3 stores at
+// 2.6 TB/s); exchanged, it covers whole lines.  LDS serves a wave's accesses in
+// order, so no barrier is needed; pieces are swizzled as in the stages.
+template <int BYTES>
 struct RowExchange {
-    static constexpr int kPitch = BYTES + 16;
-    static constexpr int kSize = ROWS * kPitch;
+    static constexpr int kSize = 32 * BYTES;
     static constexpr int kLanes = BYTES / 16;        // per row
     static constexpr int kRows = 64 / kLanes;        // per access
-    static constexpr int kSteps = ROWS / kRows;
+    static constexpr int kSteps = 32 / kRows;
+    __device__ static __forceinline__ int swizzle(int row) {
+        return BYTES == 128 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1);
+    }
+    // V: 8 or 16 bytes at `byte` of row lane % 32.
     template <typename V>
     __device__ static __forceinline__ void put(char* lds, int lane, int byte, const V& value) {
-        *reinterpret_cast<V*>(lds + (lane % ROWS) * kPitch + byte) = value;
+        const int r = lane & 31;
+        *reinterpret_cast<V*>(lds + r * BYTES + (byte ^ (16 * swizzle(r)))) = value;
     }
     __device__ static __forceinline__ int row(int lane, int step) { return kRows * step + lane / kLanes; }
     __device__ static __forceinline__ int byte(int lane) { return 16 * (lane % kLanes); }
+    __device__ static __forceinline__ u32x4 piece(const char* lds, int row, int byte) {
+        return *reinterpret_cast<const u32x4*>(lds + row * BYTES + (byte ^ (16 * swizzle(row))));
+    }
     __device__ static __forceinline__ u32x4 get(const char* lds, int lane, int step) {
-        return *reinterpret_cast<const u32x4*>(lds + row(lane, step) * kPitch + byte(lane));
+        return piece(lds, row(lane, step), byte(lane));
     }
 };
 
