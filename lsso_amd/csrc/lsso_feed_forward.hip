@@ -37,28 +37,28 @@ namespace lsso_hip {
 namespace {
 
 // act(g), and with SLOPE act'(g), FP32.  SiLU: g / (1 + exp(-g)); an exponential
-// that overflows leaves a sigmoid of 0.  GELU: g Phi(g), with Phi's tail
-// Phi(-|g|) = t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| /
-// sqrt(2)), from Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi);
-// the exponential is also that of the derivative's normal density.  The error
-// function of the device library in its place took about twice the epilogue's
-// vector instructions.
+// that overflows leaves a sigmoid of 0.  GELU: g Phi(g) = max(g, 0) - |g| tail,
+// tail = Phi(-|g|) = t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| /
+// sqrt(2)), from Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi); the
+// exponential is also that of the derivative's normal density.  With 256 input
+// features these instructions, not the MFMAs, are what the gate kernel's tile
+// costs: the error function of the device library in this place made it 577 us
+// instead of 495 at 262,144 rows of 1,024.
 template <bool SLOPE>
 __device__ __forceinline__ void activation(int kind, float g, float& value, float& slope) {
+    constexpr float kLog2e = 1.44269504f;
     if (kind == LSSO_HIP_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
         value = g * s;
-        slope = SLOPE ? s * (1.0f + g * (1.0f - s)) : 0.0f;
+        slope = SLOPE ? s + value * (1.0f - s) : 0.0f;
     } else {
         const float x = fabsf(g);
         const float t = __builtin_amdgcn_rcpf(1.0f + (0.3275911f * 0.70710678f) * x);
-        const float e = __expf(-0.5f * g * g);
-        const float poly =
-            t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-        const float tail = 0.5f * poly * e;
-        const float cdf = g < 0.0f ? tail : 1.0f - tail;
-        value = g * cdf;
-        slope = SLOPE ? cdf + 0.39894228f * g * e : 0.0f;
+        const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
+        const float tail =
+            e * (t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f)))));
+        value = fmaxf(g, 0.0f) - x * tail;
+        slope = SLOPE ? (g < 0.0f ? tail : 1.0f - tail) + 0.39894228f * g * e : 0.0f;
     }
 }
 
@@ -124,17 +124,14 @@ struct RowStream {
         p_rows = RowLoads<P>::aim(p_base + p0 * p_stride, p_stride, walk.left > 0 ? rows - p0 : 0, S::BP);
         q_rows = RowLoads<Q>::aim(q_base + q0 * q_stride, q_stride, walk.left > 0 ? columns - q0 : 0, S::BQ);
     }
-    __device__ __forceinline__ void issue(char* lds) {
+    __device__ __forceinline__ void issue(char* lds, int j) {
         const int k = stage * kRowsStageK;
-#pragma unroll
-        for (int j = 0; j < P::kLoads; ++j) {
+        if (j < P::kLoads) {
             p.issue(p_rows, lds, S::kWaves, wave, k, j, j);
+        } else {
+            q.issue(q_rows, lds + P::kBytes, S::kWaves, wave, k, j - P::kLoads, j - P::kLoads);
         }
-#pragma unroll
-        for (int j = 0; j < Q::kLoads; ++j) {
-            q.issue(q_rows, lds + P::kBytes, S::kWaves, wave, k, j, j);
-        }
-        if (++stage == last) {
+        if (j == S::kLoads - 1 && ++stage == last) {
             stage = first;
             walk.next();
             aim();
@@ -142,63 +139,31 @@ struct RowStream {
     }
 };
 
-// Loads of one operand in columns: lines are k.
-template <typename Layout>
+// One operand's loads in columns: lines are k.
+template <typename Stage>
 struct ColumnLoads {
     const uint16_t* base;
     int64_t stride;
+    int line;
     uint32_t offset;       // kOutOfRange for a lane past the columns
     uint32_t step;
 
-    __device__ __forceinline__ ColumnLoads(const Operand& o, int wave, int lane)
-        : base(o.base), stride(o.stride) {
-        const int element = Layout::load_element(wave, lane);
-        offset = element < o.elements
-                     ? static_cast<uint32_t>(2 * (Layout::load_line(wave, lane, 0) * o.stride + element))
-                     : kOutOfRange;
-        step = static_cast<uint32_t>(2 * 4 * Layout::kRowsPerLoad * o.stride);
+    // Of the columns from `base_` on, of which there are `columns`.
+    __device__ __forceinline__ ColumnLoads(const uint16_t* base_, int64_t stride_, int64_t columns, int wave, int lane)
+        : base(base_), stride(stride_), line(Stage::load_line(wave, lane)) {
+        const int element = Stage::load_element(wave, lane);
+        offset = element < columns ? static_cast<uint32_t>(2 * (line * stride + element)) : kOutOfRange;
+        step = static_cast<uint32_t>(2 * Stage::kLinesPerRound * stride);
     }
-    // Lines [k, min(k + kStageK, end)).
-    __device__ __forceinline__ BufferRsrc stage(int64_t k, int64_t end) const {
-        const int64_t lines = end - k < kStageK ? end - k : kStageK;
-        return make_buffer(base + (lines > 0 ? k : 0) * stride, 2 * lines * stride);
-    }
-    __device__ __forceinline__ void issue(BufferRsrc buffer, char* lds, int wave, int j, bool keep = true) const {
-        load_to_lds(buffer, lds + 1024 * (4 * j + wave), keep && offset != kOutOfRange ? offset + j * step : kOutOfRange);
+    // Load j of lines [k, min(k + kColumnsStageK, end)), of those whose bit in `kept` is set.
+    __device__ __forceinline__ void issue(char* lds, int waves, int wave, int64_t k, int64_t end, int j,
+                                          uint32_t kept) const {
+        const int64_t lines = end - k < kColumnsStageK ? end - k : kColumnsStageK;
+        const BufferRsrc buffer = make_buffer(base + (lines > 0 ? k : 0) * stride, 2 * lines * stride);
+        const bool load = offset != kOutOfRange && (kept >> (line + j * Stage::kLinesPerRound) & 1) != 0;
+        load_to_lds(buffer, lds + 1024 * (waves * j + wave), load ? offset + j * step : kOutOfRange);
     }
 };
-
-// FP32 rows of a wave's blocks into partials [rows, pitch] from row p0 and
-// column q0 on.  Blocks: 32 x 32 (lane & 31 the row, entry 4 q + e column 8 q + 4
-// half + e).
-template <typename S>
-__device__ __forceinline__ void store_partials(char* mine, int lane, const f32x16 (&acc)[S::NB][S::MB],
-                                               float* partials, int64_t pitch, int64_t p0, int64_t rows, int64_t q0) {
-    using Exchange = RowExchange<128>;
-    static_assert(Exchange::kSize <= S::kWaveBytes, "the exchange fits the wave's LDS");
-#pragma unroll
-    for (int m = 0; m < S::MB; ++m) {
-#pragma unroll
-        for (int n = 0; n < S::NB; ++n) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 v = {acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2], acc[n][m][4 * q + 3]};
-                Exchange::put(mine, lane, 32 * q + 16 * (lane >> 5), v);
-            }
-            wave_lds_order();
-            const int64_t column = q0 + 32 * n + Exchange::byte(lane) / 4;
-#pragma unroll
-            for (int i = 0; i < Exchange::kSteps; ++i) {
-                const u32x4 value = Exchange::get(mine, lane, i);
-                const int64_t row = p0 + 32 * m + Exchange::row(lane, i);
-                if (row < rows && column < pitch) {
-                    *reinterpret_cast<u32x4*>(partials + row * pitch + column) = value;
-                }
-            }
-            wave_lds_order();
-        }
-    }
-}
 
 // FP32 rows of a wave's blocks of 32 x 32 into partials [rows, pitch] from row
 // p0 and column q0 on.
@@ -260,12 +225,12 @@ __device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mi
                     float act, slope;
                     activation<KEEP>(a.activation, acc[n][m][4 * q + e], act, slope);
                     const float u = acc[n + NB / 2][m][4 * q + e];
-                    h[e] = kept ? act * u : 0.0f;
+                    h[e] = act * u;
                     first[e] = slope * u;
                     second[e] = act;
                 }
                 Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half,
-                              (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])});
+                              (u32x2){kept ? Values<T>::pack(h[0], h[1]) : 0u, kept ? Values<T>::pack(h[2], h[3]) : 0u});
                 if constexpr (KEEP) {
                     factors[0][n][q] = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
                     factors[1][n][q] =
@@ -337,19 +302,17 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gate_kernel(FeedForwardArgs a
     const int wave_column = S::wave_q(wave) / 2;
     run_rows_tiles<S>(
         lds, walk.left, a.stages,
-        [&](char* to) {
+        [&](char* to, int j) {
             const int k = stage * kRowsStageK;
-#pragma unroll
-            for (int j = 0; j < P::kLoads; ++j) {
+            if (j < P::kLoads) {
                 p.issue(x, to, S::kWaves, wave, k, j, j);
-            }
-            // The first half of Q's loads are the gate's rows, the second the up's.
-#pragma unroll
-            for (int j = 0; j < Q::kLoads; ++j) {
+            } else {
+                // The first half of Q's loads are the gate's rows, the second the up's.
                 constexpr int kEach = Q::kLoads / 2;
-                q.issue(j < kEach ? gate : up, to + P::kBytes, S::kWaves, wave, k, j, j % kEach);
+                const int i = j - P::kLoads;
+                q.issue(i < kEach ? gate : up, to + P::kBytes, S::kWaves, wave, k, i, i % kEach);
             }
-            if (++stage == a.stages) {
+            if (j == S::kLoads - 1 && ++stage == a.stages) {
                 stage = 0;
                 ahead.next();
                 aim();
@@ -390,13 +353,10 @@ __device__ __forceinline__ void product_epilogue(const FeedForwardProduct& a, ch
             for (int n = 0; n < kGroup; ++n) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = kept ? acc[n0 + n][m][4 * q + e] : 0.0f;
-                    }
+                    const f32x16& c = acc[n0 + n][m];
                     Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half,
-                                  (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])});
+                                  (u32x2){kept ? Values<T>::pack(c[4 * q], c[4 * q + 1]) : 0u,
+                                          kept ? Values<T>::pack(c[4 * q + 2], c[4 * q + 3]) : 0u});
                 }
             }
             wave_lds_order();
@@ -440,7 +400,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardPro
     const int last = first + a.split_stages < a.stages ? first + a.split_stages : a.stages;
     RowStream<S> stream(a.p, a.p_stride, a.rows, a.q, a.q_stride, a.columns, a.k, first, last, walk, wave, lane);
     run_rows_tiles<S>(
-        lds, walk.left, last - first, [&](char* to) { stream.issue(to); },
+        lds, walk.left, last - first, [&](char* to, int j) { stream.issue(to, j); },
         [&](int n) { return S::wave_q(wave) + 32 * n; },
         [&](const f32x16 (&acc)[NB][MB]) {
             product_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane, split,
@@ -529,7 +489,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grad_kernel(FeedForwardArgs a
     RowStream<S> stream(a.dy, a.dy_stride, a.rows, a.down_columns, a.out_pitch, a.hidden, a.out_pitch, 0, a.stages, walk,
                         wave, lane);
     run_rows_tiles<S>(
-        lds, walk.left, a.stages, [&](char* to) { stream.issue(to); },
+        lds, walk.left, a.stages, [&](char* to, int j) { stream.issue(to, j); },
         [&](int n) { return S::wave_q(wave) + 32 * n; },
         [&](const f32x16 (&acc)[NB][MB]) {
             grad_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
@@ -541,11 +501,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grad_kernel(FeedForwardArgs a
 
 // ----------------------------------------------------------- weight gradients
 // One of up to three products P^T Q over a range of rows, P and Q in columns.
-template <int T, int MB, int NB, int WP, bool MASKED>
-__global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardWeights a) {
-    using S = ProductShape<T, false, false, MB, NB, WP>;
+template <int T, int MB, int NB, int WP, int WQ, bool MASKED>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void weight_kernel(FeedForwardWeights a) {
+    using S = ColumnsShape<T, MB, NB, WP, WQ>;
+    using P = typename S::PStage;
+    using Q = typename S::QStage;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-    __shared__ uint32_t kept[MASKED ? kWeightSplitRows / 32 + kRing : 1];   // rows of each stage
+    __shared__ uint32_t kept[MASKED ? kWeightSplitRows / 32 + kColumnsRing : 1];   // rows of each stage
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
     int64_t block = xcd_local_block(blockIdx.x, gridDim.x);
@@ -563,44 +525,33 @@ __global__ __launch_bounds__(kProductThreads, 2) void weight_kernel(FeedForwardW
     const int64_t r0 = split * a.split_rows;
     const int64_t r1 = r0 + a.split_rows < a.rows ? r0 + a.split_rows : a.rows;
     if constexpr (MASKED) {
-        for (int64_t i = 64 * wave; i < a.split_rows + kRing * kStageK; i += kProductThreads) {
+        for (int64_t i = 64 * wave; i < a.split_rows + kColumnsRing * kColumnsStageK; i += S::kThreads) {
             const int64_t r = r0 + i + lane;
             const uint64_t rows = __ballot(r < r1 && a.row_mask[r < r1 ? r : r0] != 0);
-            if (lane < 2) {
-                const int word = static_cast<int>(i / 32) + lane;
-                if (word < kWeightSplitRows / 32 + kRing) {
-                    kept[word] = static_cast<uint32_t>(rows >> (32 * lane));
-                }
+            const int word = static_cast<int>(i / 32) + lane;
+            if (lane < 2 && word < kWeightSplitRows / 32 + kColumnsRing) {
+                kept[word] = static_cast<uint32_t>(rows >> (32 * lane));
             }
         }
         __syncthreads();
     }
-    const ColumnLoads<typename S::PLayout> p({w.p + p0, w.p_stride, 0, w.p_columns - p0}, wave, lane);
-    const ColumnLoads<typename S::QLayout> q({w.q + q0, w.q_stride, 0, w.q_columns - q0}, wave, lane);
+    const ColumnLoads<P> p(w.p + p0, w.p_stride, w.p_columns - p0, wave, lane);
+    const ColumnLoads<Q> q(w.q + q0, w.q_stride, w.q_columns - q0, wave, lane);
     f32x16 acc[NB][MB];
-    const auto q_start = [&](int n) { return S::wave_q(wave) + 32 * n; };
-    run_product<S>(
-        lds, static_cast<int>((r1 - r0 + kStageK - 1) / kStageK), acc,
-        [&](char* stage, int s) {
-            const int64_t k = r0 + static_cast<int64_t>(s) * kStageK;
-            const BufferRsrc pb = p.stage(k, r1);
-            const BufferRsrc qb = q.stage(k, r1);
-            const uint32_t rows = MASKED ? __builtin_amdgcn_readfirstlane(kept[s]) : ~0u;
-#pragma unroll
-            for (int j = 0; j < S::PLayout::kLoads; ++j) {
-                p.issue(pb, stage, wave, j, !MASKED || (rows >> S::PLayout::load_line(wave, lane, j)) & 1);
-            }
-#pragma unroll
-            for (int j = 0; j < S::QLayout::kLoads; ++j) {
-                q.issue(qb, stage + S::PLayout::kBytes, wave, j,
-                        !MASKED || (rows >> S::QLayout::load_line(wave, lane, j)) & 1);
-            }
-        },
-        q_start);
-
+    run_columns_product<S>(lds, static_cast<int>((r1 - r0 + kColumnsStageK - 1) / kColumnsStageK), acc,
+                           [&](char* to, int s, int j) {
+                               const int64_t k = r0 + static_cast<int64_t>(s) * kColumnsStageK;
+                               const uint32_t rows = MASKED ? __builtin_amdgcn_readfirstlane(kept[s]) : ~0u;
+                               if (j < P::kLoads) {
+                                   p.issue(to, S::kWaves, wave, k, r1, j, rows);
+                               } else {
+                                   q.issue(to + P::kBytes, S::kWaves, wave, k, r1, j - P::kLoads, rows);
+                               }
+                           });
     static_assert(RowExchange<128>::kSize <= S::kWaveBytes, "the exchange fits the wave's LDS");
-    store_partials<MB, NB>(lds + S::kWaveBytes * wave, lane, acc, a.partials + split * a.partial_floats + w.partial_offset,
-                           w.partial_pitch, p0 + S::wave_p(wave), w.out_rows, q0 + q_start(0));
+    store_partials<MB, NB>(lds + S::kWaveBytes * wave, lane, acc,
+                           a.partials + split * a.partial_floats + w.partial_offset, w.partial_pitch,
+                           p0 + S::wave_p(wave), w.out_rows, q0 + S::wave_q(wave));
 }
 
 // Sum of `splits` partials [rows, pitch] in order, rounded once into out [rows,
@@ -801,9 +752,17 @@ hipError_t launch_grad(FeedForwardArgs a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// With few stages a tile's time is its epilogue (the factors read, dg and du
+// written), which two workgroups of a CU overlap and one large one does not:
+// 131,072 x 256 -> 688 takes 224 us on middle tiles and 281 on large ones, 65,536 x
+// 384 -> 1,536 254 on both.
 template <int T>
 hipError_t launch_grad(const FeedForwardArgs& a, hipStream_t stream) {
-    switch (choose_edge(a.rows, a.pitch)) {
+    Edge edge = choose_edge(a.rows, a.pitch);
+    if (edge == Edge::kLarge && a.out_pitch <= 384) {
+        edge = Edge::kMiddle;
+    }
+    switch (edge) {
         case Edge::kLarge: return launch_grad<T, 2, 4, 4, 2>(a, stream);
         case Edge::kMiddle: return launch_grad<T, 2, 2, 2, 2>(a, stream);
         default: return launch_grad<T, 1, 1, 2, 2>(a, stream);
@@ -811,20 +770,18 @@ hipError_t launch_grad(const FeedForwardArgs& a, hipStream_t stream) {
 }
 
 template <int T, bool MASKED>
-void launch_weights(const FeedForwardWeights& a, int mb, dim3 grid, hipStream_t stream) {
-    if (mb == 4) {
-        weight_kernel<T, 2, 4, 4, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
+void launch_weights(const FeedForwardWeights& a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.tiles * a.splits));
+    if (a.large) {
+        weight_kernel<T, 2, 4, 4, 2, MASKED><<<grid, 512, 0, stream>>>(a);
     } else {
-        weight_kernel<T, 2, 2, 2, MASKED><<<grid, kProductThreads, 0, stream>>>(a);
+        weight_kernel<T, 2, 2, 2, 2, MASKED><<<grid, 256, 0, stream>>>(a);
     }
 }
 
 template <int T>
-hipError_t launch_weights(const FeedForwardWeights& args, hipStream_t stream) {
-    FeedForwardWeights a = args;
-    const dim3 grid(static_cast<unsigned>(a.tiles * a.splits));
-    a.row_mask != nullptr ? launch_weights<T, true>(a, a.mb, grid, stream)
-                          : launch_weights<T, false>(a, a.mb, grid, stream);
+hipError_t launch_weights(const FeedForwardWeights& a, hipStream_t stream) {
+    a.row_mask != nullptr ? launch_weights<T, true>(a, stream) : launch_weights<T, false>(a, stream);
     return hipGetLastError();
 }
 
@@ -846,37 +803,38 @@ void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProd
     a->partial_pitch = (columns + 7) / 8 * 8;
 }
 
+// Tiles of 256 x 256 (one workgroup per CU) where they are well filled and their
+// splits still have 512 rows, else of 128 x 128 (three).  The splits fill the
+// device's workgroups once: more of them would write and read more partials, a
+// second round of workgroups would be partly empty.
 void plan_weights(FeedForwardWeights* a) {
-    a->mb = 2;
-    const auto count = [&](int64_t bp, int64_t bq) {
+    const auto count = [&](int64_t edge) {
         int64_t tiles = 0;
         for (int i = 0; i < a->count; ++i) {
-            tiles += tiles_of(a->products[i].out_rows, a->products[i].partial_pitch, bp, bq);
+            tiles += tiles_of(a->products[i].out_rows, a->products[i].partial_pitch, edge, edge);
         }
         return tiles;
     };
-    // The large tile where its workgroups still have 512 rows each.
-    if (count(256, 128) * a->rows >= 1024 * kCus) {
-        a->mb = 4;
-    }
-    const int64_t bp = 64 * a->mb;
-    a->tiles = count(bp, 128);
+    const int64_t large = count(256);
+    a->large = 3 * large <= count(128) && large * a->rows >= 512 * kCus;
+    const int64_t edge = a->large ? 256 : 128;
+    a->tiles = count(edge);
     a->partial_floats = 0;
     for (int i = 0; i < a->count; ++i) {
         WeightProduct& w = a->products[i];
-        w.q_tiles = (w.partial_pitch + 127) / 128;
-        w.tiles = w.q_tiles * ((w.out_rows + bp - 1) / bp);
+        w.q_tiles = (w.partial_pitch + edge - 1) / edge;
+        w.tiles = w.q_tiles * ((w.out_rows + edge - 1) / edge);
         w.partial_offset = a->partial_floats;
         a->partial_floats += w.out_rows * w.partial_pitch;
     }
-    int64_t splits = a->tiles > 0 ? 2 * kCus / a->tiles : 1;
+    int64_t splits = a->tiles > 0 ? (a->large ? kCus : 3 * kCus) / a->tiles : 1;
     const int64_t most = (a->rows + 127) / 128;
     splits = splits < most ? splits : most;
     const int64_t least = (a->rows + kWeightSplitRows - 1) / kWeightSplitRows;
     splits = splits > least ? splits : least;
     splits = splits < 1 ? 1 : splits;
     const int64_t per = (a->rows + splits - 1) / splits;
-    a->split_rows = (per + kStageK - 1) / kStageK * kStageK;
+    a->split_rows = (per + kColumnsStageK - 1) / kColumnsStageK * kColumnsStageK;
     a->splits = a->rows > 0 ? (a->rows + a->split_rows - 1) / a->split_rows : 1;
 }
 

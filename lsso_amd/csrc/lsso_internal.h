@@ -412,7 +412,7 @@ struct FeedForwardWeights {
     int64_t split_rows;
     int64_t splits;
     int64_t tiles;              // of one split
-    int mb;
+    int large;                  // 256 x 256 tiles, else 128 x 128
 };
 
 struct JoinOutput {

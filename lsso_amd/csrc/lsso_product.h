@@ -1,31 +1,18 @@
-// Tiled 16-bit matrix product of the feed-forward kernels:
+// Tiled 16-bit matrix products of the feed-forward kernels:
 //   out[p][q] = sum over k of P[p, k] Q[q, k],  FP32 accumulation,
 // in two forms: for operands that lie in memory across k ([k][p], "columns": the
 // weight gradients dy^T x, whose k are the rows of long activations), and for
 // operands along k ([p][k], "rows": x W^T; dy W comes to it with W transposed
 // once per call), further down.
 //
-// A workgroup of 4 waves owns a BP x BQ tile, a wave MB x NB blocks of 32 x 32
-// on v_mfma_f32_32x32x16.  The operands' stages of 32 k go from memory
-// to LDS without passing registers (buffer_load ... lds, 16 bytes per lane), in
-// a ring of three: two stages are in flight while one is multiplied.  The
-// largest tile, 256 x 128, keeps 128 accumulators and 72 KB of LDS, so two
-// workgroups share a CU and one multiplies while the other waits, begins or
-// stores.  Per stage a wave reads 12 KB of fragments for 16 MFMAs; a stage's
-// second half is read under the first half's MFMAs and the next stage's first
-// half under the second's, so the one barrier per stage finds nothing to wait
-// for but the loads.
-//
-// LDS is written linearly by the loads (lane i at 16 i), so conflicts are
-// avoided by which global piece a lane asks for:
-//   rows:    64 bytes per p, piece c at slot c ^ f(p), f = ((p >> 1) & 3) ^
-//            ((p >> 3) & 1): any 8 or 16 consecutive rows of one piece fall on
-//            different banks;
-//   columns: 2 BP bytes per k, group of 16 columns g at g ^ {0, 3, 5, 6}[k % 4]
-//            (k % 4 for 4 groups): the 4 rows of a transposed read likewise.
-//
-// Rows past an operand's end, k past K and rows that a mask excludes are loads
-// past the buffer's end, which bring zeros and touch no memory.
+// A workgroup owns a BP x BQ tile, each of its waves MB x NB blocks of 32 x 32 on
+// v_mfma_f32_32x32x16.  The operands' stages go from memory to LDS without
+// passing registers (buffer_load ... lds, 16 bytes per lane), and a step's
+// fragments are read under the MFMAs of the step before.  LDS is written
+// linearly by the loads (lane i at 16 i), so bank conflicts are avoided by which
+// piece of memory a lane asks for (the swizzles below; the conflict counter reads
+// zero).  Rows past an operand's end, k past K and rows that a mask excludes are
+// loads past the buffer's end, which bring zeros and touch no memory.
 #pragma once
 
 #include "lsso_device.h"
@@ -35,10 +22,6 @@ namespace lsso_hip {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void LdsVoid;
-
-constexpr int kStageK = 32;
-constexpr int kRing = 3;
-constexpr int kProductThreads = 256;
 
 template <int T>
 __device__ __forceinline__ f32x16 mfma_block(const u32x4& a, const u32x4& b, const f32x16& c) {
@@ -50,61 +33,6 @@ __device__ __forceinline__ f32x16 mfma_block(const u32x4& a, const u32x4& b, con
                                                       0, 0);
     }
 }
-
-// Bytes of one operand's stage, and the per-lane side of its loads and reads.
-// WIDTH: rows (or columns) of the operand in the tile; IN_ROWS: [p][k] in memory.
-template <int WIDTH, bool IN_ROWS>
-struct StageLayout {
-    static constexpr int kBytes = WIDTH * kStageK * 2;
-    static constexpr int kLoads = kBytes / 1024 / 4;          // per wave
-    static constexpr int kRowsPerLoad = 1024 / (2 * WIDTH);   // of k, in columns
-    static_assert(kLoads >= 1, "a tile edge is at least 64");
-
-    __device__ static __forceinline__ int row_swizzle(int p) { return ((p >> 1) & 3) ^ ((p >> 3) & 1); }
-    __device__ static __forceinline__ int column_swizzle(int k) {
-        if constexpr (WIDTH == 64) {
-            return k & 3;
-        }
-        return ((k & 1) != 0 ? 3 : 0) ^ ((k & 2) != 0 ? 5 : 0);
-    }
-    // What lane `lane` of wave `wave` loads with load j: p (in rows) or k (in columns) ...
-    __device__ static __forceinline__ int load_line(int wave, int lane, int j) {
-        return IN_ROWS ? 16 * (4 * j + wave) + (lane >> 2)
-                       : kRowsPerLoad * (4 * j + wave) + lane / (WIDTH / 8);
-    }
-    // ... and its first element along the line; the same for every j.
-    __device__ static __forceinline__ int load_element(int wave, int lane) {
-        const int line = load_line(wave, lane, 0);
-        if constexpr (IN_ROWS) {
-            return 8 * ((lane & 3) ^ row_swizzle(line));
-        } else {
-            const int piece = lane % (WIDTH / 8);
-            return 16 * ((piece >> 1) ^ column_swizzle(line)) + 8 * (piece & 1);
-        }
-    }
-    // Byte of this lane's fragment of the block of 32 p from p0 (a multiple of
-    // 32) in a stage, of k step 0 or 1.
-    __device__ static __forceinline__ int fragment(int lane, int p0, int step) {
-        if constexpr (IN_ROWS) {
-            const int p = lane & 31;
-            return 64 * p0 + (64 * p + 16 * ((2 * step + (lane >> 5)) ^ row_swizzle(p)));
-        } else {
-            const int k = (lane & 15) / 4 + 8 * (lane >> 5);
-            const int group = p0 / 16 + ((lane >> 4) & 1);
-            return 2 * WIDTH * (k + 16 * step) + 32 * (group ^ column_swizzle(k)) + 8 * (lane & 3);
-        }
-    }
-    __device__ static __forceinline__ u32x4 read(const char* at) {
-        if constexpr (IN_ROWS) {
-            return *reinterpret_cast<const u32x4*>(at);
-        } else {
-            const u32x2 low = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at)));
-            const u32x2 high =
-                __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at + 2 * WIDTH * 4)));
-            return (u32x4){low[0], low[1], high[0], high[1]};
-        }
-    }
-};
 
 __device__ __forceinline__ void load_to_lds(BufferRsrc buffer, char* lds, uint32_t offset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsVoid*)lds, 16, offset, 0, 0, 0);
@@ -119,54 +47,81 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// An operand of the product.  In rows: `base` is the tile's first row, `lines`
-// the rows from there on, `elements` = K.  In columns: `base` is the tile's
-// first column of k = 0, `lines` = K, `elements` the columns from there on.
-// Both lines' strides and `elements` are multiples of 8 and base is 16-byte
-// aligned (or a tile offset of 16-byte pieces from such).
-struct Operand {
-    const uint16_t* base;
-    int64_t stride;
-    int64_t lines;
-    int64_t elements;
+// This wave's index, as the scalar that it is.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// ---------------------------------------------------------------------------
+// The product for both operands in columns.  A stage is 32 k of whole 128-byte
+// lines, in a ring of three: two are in flight while one is multiplied.
+// Fragments come from transposed LDS reads (4 k x 16 columns per 16 lanes).
+constexpr int kColumnsStageK = 32;
+constexpr int kColumnsRing = 3;
+
+// Stage of WIDTH columns, loaded by WAVES waves.
+template <int WIDTH, int WAVES>
+struct ColumnsStage {
+    static constexpr int kBytes = WIDTH * kColumnsStageK * 2;
+    static constexpr int kLoads = kBytes / 1024 / WAVES;       // per wave
+    static constexpr int kPieces = WIDTH / 8;                  // 16-byte pieces of a line
+    static constexpr int kLinesPerLoad = 64 / kPieces;
+    static constexpr int kLinesPerRound = kLinesPerLoad * WAVES;
+    static_assert(kLoads >= 1, "every wave loads");
+    // Group g of 16 columns of line k lies at g ^ swizzle(k), so that the four
+    // lines of a transposed read, and the two groups beside each other, fall on
+    // different banks.
+    __device__ static __forceinline__ int swizzle(int k) { return ((k & 1) != 0 ? 3 : 0) ^ ((k & 2) != 0 ? 5 : 0); }
+    // Line of this lane's first load (kLinesPerRound further for each one after
+    // it) and its first element of that line.
+    __device__ static __forceinline__ int load_line(int wave, int lane) {
+        return kLinesPerLoad * wave + lane / kPieces;
+    }
+    __device__ static __forceinline__ int load_element(int wave, int lane) {
+        const int piece = lane % kPieces;
+        return 16 * ((piece >> 1) ^ swizzle(load_line(wave, lane))) + 8 * (piece & 1);
+    }
+    // Byte in a stage of this lane's fragment of columns p0 .. p0 + 31 at a step.
+    __device__ static __forceinline__ int fragment(int lane, int p0, int step) {
+        const int k = (lane & 15) / 4 + 8 * (lane >> 5);
+        const int group = p0 / 16 + ((lane >> 4) & 1);
+        return 2 * WIDTH * (k + 16 * step) + 32 * (group ^ swizzle(k)) + 8 * (lane & 3);
+    }
+    __device__ static __forceinline__ u32x4 read(const char* at) {
+        const u32x2 low = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at)));
+        const u32x2 high =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(at + 2 * WIDTH * 4)));
+        return (u32x4){low[0], low[1], high[0], high[1]};
+    }
 };
 
-// T: type code; MB x NB blocks of 32 x 32 per wave; WP waves along P, 4 / WP
-// along Q.
-template <int T_, bool P_ROWS_, bool Q_ROWS_, int MB_, int NB_, int WP_>
-struct ProductShape {
+// T: type code; MB x NB blocks of 32 x 32 per wave, WP x WQ waves.
+template <int T_, int MB_, int NB_, int WP_, int WQ_>
+struct ColumnsShape {
     static constexpr int T = T_;
-    static constexpr bool P_ROWS = P_ROWS_;
-    static constexpr bool Q_ROWS = Q_ROWS_;
     static constexpr int MB = MB_;
     static constexpr int NB = NB_;
     static constexpr int WP = WP_;
-    static constexpr int WQ = 4 / WP;
+    static constexpr int WQ = WQ_;
+    static constexpr int kWaves = WP * WQ;
+    static constexpr int kThreads = 64 * kWaves;
     static constexpr int BP = 32 * MB * WP;
     static constexpr int BQ = 32 * NB * WQ;
-    using PLayout = StageLayout<BP, P_ROWS>;
-    using QLayout = StageLayout<BQ, Q_ROWS>;
-    static constexpr int kStageBytes = PLayout::kBytes + QLayout::kBytes;
-    static constexpr int kLdsBytes = kRing * kStageBytes;
-    static constexpr int kWaveBytes = kLdsBytes / 4;   // of the epilogue
-    static constexpr int kLoads = PLayout::kLoads + QLayout::kLoads;
-    // First row and column of the tile that are this wave's.
+    using PStage = ColumnsStage<BP, kWaves>;
+    using QStage = ColumnsStage<BQ, kWaves>;
+    static constexpr int kStageBytes = PStage::kBytes + QStage::kBytes;
+    static constexpr int kLdsBytes = kColumnsRing * kStageBytes;
+    static constexpr int kWaveBytes = kLdsBytes / kWaves;   // of the epilogue
+    static constexpr int kLoads = PStage::kLoads + QStage::kLoads;
     __device__ static __forceinline__ int wave_p(int wave) { return 32 * MB * (wave % WP); }
     __device__ static __forceinline__ int wave_q(int wave) { return 32 * NB * (wave / WP); }
 };
 
-// This wave's index, as the scalar that it is.
-__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-
-// Runs `stages` stages (at least one): issue(buffer, s) starts the loads of
-// stage s (which may lie past the last) into the LDS stage `buffer`, exactly
-// kLoads per wave.  q_start(n) is the tile's first column of this wave's Q block
-// n.  The order is written down with scheduling barriers: left to itself the
+// Runs `stages` stages (at least one): issue(stage, s, j) starts load j of the
+// kLoads per wave of stage s (which may lie past the last) into an LDS stage.
+// The order is written down with scheduling barriers: left to itself the
 // compiler moves the fragments' reads down to their MFMAs, to save registers
 // that nothing else needs, and every MFMA then waits for LDS.
-template <typename S, typename Issue, typename QStart>
-__device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)[S::NB][S::MB], Issue issue,
-                                            QStart q_start) {
+template <typename S, typename Issue>
+__device__ __forceinline__ void run_columns_product(char* lds, int stages, f32x16 (&acc)[S::NB][S::MB], Issue issue) {
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
 #pragma unroll
@@ -182,40 +137,54 @@ __device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)
     u32x4 pf[2][S::MB];
     u32x4 qf[2][S::NB];
     const auto read = [&](int buffer, int step) {
+        const char* const stage = lds + buffer * S::kStageBytes;
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            qf[step][n] = S::QLayout::read(lds + buffer * S::kStageBytes + S::PLayout::kBytes +
-                                           S::QLayout::fragment(lane, q_start(n), step));
+            qf[step][n] = S::QStage::read(stage + S::PStage::kBytes +
+                                          S::QStage::fragment(lane, S::wave_q(wave) + 32 * n, step));
         }
 #pragma unroll
         for (int m = 0; m < S::MB; ++m) {
-            pf[step][m] = S::PLayout::read(lds + buffer * S::kStageBytes +
-                                           S::PLayout::fragment(lane, S::wave_p(wave) + 32 * m, step));
+            pf[step][m] = S::PStage::read(stage + S::PStage::fragment(lane, S::wave_p(wave) + 32 * m, step));
         }
     };
-    const auto multiply = [&](int step) {
+    // The MFMAs of a step; with the first one's the loads of a stage, spread out.
+    const auto multiply = [&](int step, char* to, int s) {
+        constexpr int kBlocks = S::MB * S::NB;
 #pragma unroll
-        for (int m = 0; m < S::MB; ++m) {
+        for (int i = 0; i < kBlocks; ++i) {
+            if (step == 0) {
 #pragma unroll
-            for (int n = 0; n < S::NB; ++n) {
-                acc[n][m] = mfma_block<S::T>(qf[step][n], pf[step][m], acc[n][m]);
+                for (int j = 0; j < S::kLoads; ++j) {
+                    if (j * kBlocks / S::kLoads == i) {
+                        issue(to, s, j);
+                    }
+                }
+            }
+            f32x16& c = acc[i % S::NB][i / S::NB];
+            c = mfma_block<S::T>(qf[step][i % S::NB], pf[step][i / S::NB], c);
+            if (step == 0) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
     const auto stage = [&](int buffer, int s) {
-        issue(lds + (buffer + 2) % kRing * S::kStageBytes, s + 2);
         read(buffer, 1);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(0);
+        multiply(0, lds + (buffer + 2) % kColumnsRing * S::kStageBytes, s + 2);
+        stage_barrier<S::kLoads>();   // the next stage has landed, this one is in registers
+        read((buffer + 1) % kColumnsRing, 0);
         __builtin_amdgcn_sched_barrier(0);
-        stage_barrier<S::kLoads>();
-        read((buffer + 1) % kRing, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(1);
-        __builtin_amdgcn_sched_barrier(0);
+        multiply(1, nullptr, 0);
     };
-    issue(lds, 0);
-    issue(lds + S::kStageBytes, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::kLoads; ++j) {
+            issue(lds + i * S::kStageBytes, i, j);
+        }
+    }
     stage_barrier<S::kLoads>();
     read(0, 0);
     for (int s = 0;;) {
@@ -229,23 +198,6 @@ __device__ __forceinline__ void run_product(char* lds, int stages, f32x16 (&acc)
     // The loads past the last stage still write their zeros: neither into LDS
     // that the epilogue uses nor into what another workgroup may hold by then.
     stage_barrier<0>();
-}
-
-// The accumulators of one block hold, in lane (half, j), row p = j and columns
-// q = 8 i + 4 half + e of entry 4 i + e.  row_pieces() exchanges the halves so
-// that a lane holds two whole pieces of 8 columns: piece c (0, 1) the columns
-// 16 c + 8 half + 0 .. 7.
-__device__ __forceinline__ void row_pieces(const f32x16& acc, float (&piece)[2][8]) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const auto pair = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[8 * c + e]),
-                                                               __float_as_uint(acc[8 * c + 4 + e]), false, false);
-            piece[c][e] = __uint_as_float(pair[0]);
-            piece[c][4 + e] = __uint_as_float(pair[1]);
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -264,6 +216,11 @@ __device__ __forceinline__ void row_pieces(const f32x16& acc, float (&piece)[2][
 // last step's MFMAs, whose fragments are in registers by then.
 constexpr int kRowsStageK = 64;
 constexpr int kRowsSteps = 4;
+// Steps over which a wave spreads its loads of a stage.  It issues in order, and
+// all of them at once hold it until the address unit has taken them all.
+// Two steps measured best of one to three (8,192 x 4,096 -> 4,096: 1,105, 1,121 and
+// 1,110 TFLOP/s).
+constexpr int kSpreadSteps = 2;
 
 // Stage of WIDTH rows, loaded by WAVES waves.
 template <int WIDTH, int WAVES>
@@ -353,9 +310,9 @@ struct TileWalk {
     }
 };
 
-// Runs `tiles` tiles of `stages` stages each.  issue(lds) starts the loads of the
-// next stage, kLoads per wave, in order through all tiles and asked for two past
-// the last; q_start(n) is the tile's first row of Q of this wave's block n;
+// Runs `tiles` tiles of `stages` stages each.  issue(stage, j) starts load j of the
+// kLoads per wave of the next stage into an LDS stage, in order through all tiles
+// and asked for two stages past the last; q_start(n) is the tile's first row of Q of this wave's block n;
 // epilogue(acc) takes a tile's sums.  The loads run ahead across the tiles'
 // borders, so a tile's first stages arrive under the epilogue of the one
 // before: a tile of 256 k has four stages, and began with a wait for memory as
@@ -378,36 +335,55 @@ __device__ __forceinline__ void run_rows_tiles(char* lds, int tiles, int stages,
             pf[step & 1][m] = S::PStage::read(stage, lane, S::wave_p(wave) + 32 * m, step);
         }
     };
-    const auto multiply = [&](int step) {
+    // The MFMAs of a step, and between them the loads whose turn it is: load j of
+    // a stage goes before MFMA j * kSpread / kLoads, counted from the last step
+    // of the stage before last through the first steps of the last one.
+    constexpr int kBlocks = S::MB * S::NB;
+    constexpr int kSpread = kSpreadSteps * kBlocks;
+    const auto multiply = [&](int step, char* stage, int first) {
 #pragma unroll
-        for (int m = 0; m < S::MB; ++m) {
+        for (int i = 0; i < kBlocks; ++i) {
 #pragma unroll
-            for (int n = 0; n < S::NB; ++n) {
-                acc[n][m] = mfma_block<S::T>(qf[step & 1][n], pf[step & 1][m], acc[n][m]);
+            for (int j = 0; j < S::kLoads; ++j) {
+                if (j * kSpread / S::kLoads == first + i) {
+                    issue(stage, j);
+                }
+            }
+            f32x16& c = acc[i % S::NB][i / S::NB];
+            c = mfma_block<S::T>(qf[step & 1][i % S::NB], pf[step & 1][i / S::NB], c);
+            if (first < kSpread) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
     int at = 0;   // LDS offset of this stage
     const auto stage = [&] {
         char* const here = lds + at;
+        char* const other = lds + (at ^ S::kStageBytes);
         at ^= S::kStageBytes;
 #pragma unroll
         for (int step = 0; step < kRowsSteps - 1; ++step) {
             read(here, step + 1);
             __builtin_amdgcn_sched_barrier(0);
-            multiply(step);
-            __builtin_amdgcn_sched_barrier(0);
+            multiply(step, other, (step + 1) * kBlocks);
         }
         stage_barrier<0>();   // the next stage has landed, and nobody reads this one any more
-        issue(here);
-        read(lds + at, 0);
+        read(other, 0);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(kRowsSteps - 1);
-        __builtin_amdgcn_sched_barrier(0);
+        multiply(kRowsSteps - 1, here, 0);
     };
-    issue(lds);
-    issue(lds + S::kStageBytes);
-    stage_barrier<S::kLoads>();
+#pragma unroll
+    for (int j = 0; j < S::kLoads; ++j) {
+        issue(lds, j);
+    }
+    // What the last step of a stage before the first would have issued.
+    constexpr int kBegun = (S::kLoads + kSpreadSteps - 1) / kSpreadSteps;
+#pragma unroll
+    for (int j = 0; j < kBegun; ++j) {
+        issue(lds + S::kStageBytes, j);
+    }
+    stage_barrier<kBegun>();
     read(lds, 0);
     for (int tile = 0; tile < tiles; ++tile) {
 #pragma unroll
