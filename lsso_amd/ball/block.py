@@ -321,23 +321,28 @@ def dropout_add(
 
 # --------------------------------------------------------------- feed-forward
 @lru_cache(maxsize=1024)
-def _feed_forward_workspace(shape: tuple, training: bool) -> int:
+def _feed_forward_plan(shape: tuple, training: bool):
+    """(the native shape, its workspace's bytes) of a forward: they depend on
+    these integers alone, and a program asks for the same few on every call."""
+
     hip = _hip()
     library = hip._library()
+    native = FeedForwardShape(*shape)
     size = ctypes.c_size_t()
     hip._check(library.lsso_hip_feed_forward_workspace_bytes(
-        ctypes.byref(FeedForwardShape(*shape)), int(training), ctypes.byref(size)), library)
-    return size.value
+        ctypes.byref(native), int(training), ctypes.byref(size)), library)
+    return ctypes.byref(native), size.value
 
 
 @lru_cache(maxsize=1024)
-def _feed_forward_backward_workspace(shape: tuple, grad_stride: int, weights: int) -> int:
+def _feed_forward_backward_plan(shape: tuple, grad_stride: int, weights: int):
     hip = _hip()
     library = hip._library()
+    native = FeedForwardShape(*shape)
     size = ctypes.c_size_t()
     hip._check(library.lsso_hip_feed_forward_backward_workspace_bytes(
-        ctypes.byref(FeedForwardShape(*shape)), grad_stride, weights, ctypes.byref(size)), library)
-    return size.value
+        ctypes.byref(native), grad_stride, weights, ctypes.byref(size)), library)
+    return ctypes.byref(native), size.value
 
 
 def _aligned(value: torch.Tensor) -> torch.Tensor:
@@ -347,17 +352,26 @@ def _aligned(value: torch.Tensor) -> torch.Tensor:
 
 
 def _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation):
-    """(rows of x, contiguous weights, the shape's fields)."""
+    """(rows of x, weights, their addresses, the shape's fields)."""
 
     hidden, in_features = gate_weight.shape
-    flat = _aligned(_hip()._rows(x, in_features))
-    weights = tuple(_aligned(w.contiguous()) for w in (gate_weight, up_weight, down_weight))
+    flat = _hip()._rows(x, in_features)
+    if flat.data_ptr() % 16 != 0:
+        flat = flat.clone()
+    weights, pointers = (gate_weight, up_weight, down_weight), []
+    if not (gate_weight.is_contiguous() and up_weight.is_contiguous() and down_weight.is_contiguous()):
+        weights = tuple(w.contiguous() for w in weights)
+    for w in weights:
+        pointers.append(w.data_ptr())
+    if (pointers[0] | pointers[1] | pointers[2]) % 16 != 0:
+        weights = tuple(_aligned(w) for w in weights)
+        pointers = [w.data_ptr() for w in weights]
     rows = flat.shape[0]
     shape = (
         rows, in_features, hidden, down_weight.shape[0], flat.stride(0) if rows > 1 else in_features,
         _HALF_CODES[x.dtype], _VALUE_CODES[gate_weight.dtype], activation,
     )
-    return flat, weights, shape
+    return flat, weights, pointers, shape
 
 
 def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row_mask, training):
@@ -366,21 +380,22 @@ def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row
     hip = _hip()
     library = hip._library()
     device = x.device
-    _mask, mask_ptr = _mask_pointer(row_mask, x.shape[:-1], device)
-    flat, weights, shape = _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation)
+    mask_ptr = None
+    if row_mask is not None:
+        _mask, mask_ptr = _mask_pointer(row_mask, x.shape[:-1], device)
+    flat, _weights, pointers, shape = _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation)
     gates = product = None
     if training:
         pitch = (shape[2] + 7) // 8 * 8
         gates = torch.empty((shape[0], 2, pitch), dtype=x.dtype, device=device)
         product = torch.empty((shape[0], pitch), dtype=x.dtype, device=device)
     y = torch.empty((*x.shape[:-1], shape[3]), dtype=x.dtype, device=device)
-    size = _feed_forward_workspace(shape, training)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    native, size = _feed_forward_plan(shape, training)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     status = hip._launch(
         library.lsso_hip_feed_forward, device,
-        ctypes.byref(FeedForwardShape(*shape)), flat.data_ptr(), *[w.data_ptr() for w in weights], mask_ptr,
-        gates.data_ptr() if training else None, product.data_ptr() if training else None, y.data_ptr(),
-        workspace.data_ptr(), size,
+        native, flat.data_ptr(), *pointers, mask_ptr, gates.data_ptr() if training else None,
+        product.data_ptr() if training else None, y.data_ptr(), workspace.data_ptr() if size else None, size,
     )
     hip._check(status, library)
     return y, gates, product
@@ -407,7 +422,7 @@ class _FeedForward(torch.autograd.Function):
         for value, name, (shape, dtype) in zip((x, *weights), ("x", "gate_weight", "up_weight", "down_weight"), ctx.like):
             if value.device != device or value.dtype != dtype or tuple(value.shape) != shape:
                 _saved(value, name, dtype, shape, device)
-        flat, weights, shape = _feed_forward_inputs(x, *weights, ctx.activation)
+        flat, weights, pointers, shape = _feed_forward_inputs(x, *weights, ctx.activation)
         rows, in_features, hidden, out_features = shape[:4]
         pitch = (hidden + 7) // 8 * 8
         gates = _aligned(_saved(gates, "gates", x.dtype, (rows, 2, pitch), device))
@@ -425,14 +440,13 @@ class _FeedForward(torch.autograd.Function):
         ]
         if not any(needs):
             return (None,) * 6
-        size = _feed_forward_backward_workspace(
+        native, size = _feed_forward_backward_plan(
             shape, grad_stride, needs[1] + 2 * needs[2] + 4 * needs[3]
         )
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         status = hip._launch(
             library.lsso_hip_feed_forward_backward, device,
-            ctypes.byref(FeedForwardShape(*shape)), flat_grad.data_ptr(), grad_stride, flat.data_ptr(),
-            *[w.data_ptr() for w in weights], mask_ptr, gates.data_ptr(), product.data_ptr(),
+            native, flat_grad.data_ptr(), grad_stride, flat.data_ptr(), *pointers, mask_ptr, gates.data_ptr(), product.data_ptr(),
             *[None if grad is None else grad.data_ptr() for grad in grads], workspace.data_ptr(), size,
         )
         hip._check(status, library)

@@ -14,12 +14,14 @@
 //   1. radix sort of (id, index) in one or two passes of up to 10 bits: a
 //      histogram per tile of tokens, then a stable scatter that ranks equal
 //      digits of 64 lanes by ballots and takes its bases from the histograms;
-//   2. row sums: one wave per table row finds its run by a 64-ary search (three
-//      probes of the sorted ids for 262,144 tokens), and adds it up unless it is
-//      long; rows that no token names are written as zeros here;
-//   3. a long run is cut at fixed chunks of the sorted order: a wave per chunk
-//      leaves partial sums (beside step 2, in the same launch);
-//   4. a workgroup per long run adds its partials.
+//   2. a wave finds the runs of up to 8 table rows by a 64-ary search (three probes
+//      of the sorted ids for 262,144 tokens) and adds up those of at most 8 tokens;
+//      rows that no token names are written as zeros here;
+//   3. beside it, in the same launch, a wave per chunk of the sorted order adds up
+//      the longer runs, and leaves partial sums of those that cross its ends: the
+//      frequent words of a text lie side by side, and by rows a few waves had
+//      nearly all tokens (365 us instead of about 30 at 32,800 tokens of 768);
+//   4. the partials of each such run are added, by a wave or a workgroup.
 // Tokens that count nowhere (excluded, padding, out of range) get the id
 // `vocabulary` and sort behind every row.
 //
@@ -45,6 +47,8 @@ constexpr int kSumThreads = 256;
 constexpr int kSumWaves = kSumThreads / 64;
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinWaves = kJoinThreads / 64;
+constexpr int kFewTokens = 8;    // longest run that the wave of its row sums
+constexpr int kWaveChunks = 16;  // longest run, in chunks, that one wave joins
 
 __device__ __forceinline__ int64_t read_token(const EmbeddingArgs& a, int64_t t) {
     return a.wide_tokens ? static_cast<const int64_t*>(a.tokens)[t]
@@ -142,19 +146,31 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(EmbeddingArg
     for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) {
         at[i / kDigits][i % kDigits] = 0;
     }
-    // Digit d = this thread's: tokens of d in the tiles before this one, and in all.
+    // Tokens of each digit in the tiles before this one, and in all: every digit
+    // has 1024 / digits threads, which take the tiles in turn.
+    const int my_digit = static_cast<int>(threadIdx.x) & (digits - 1);
     uint32_t before = 0;
     uint32_t all = 0;
-    if (static_cast<int>(threadIdx.x) < digits) {
-        const uint32_t* column = a.histograms + threadIdx.x;
 #pragma unroll 8
-        for (int64_t tile = 0; tile < a.tiles; ++tile) {
-            const uint32_t n = column[tile * digits];
-            before += tile < static_cast<int64_t>(blockIdx.x) ? n : 0;
-            all += n;
-        }
+    for (int64_t tile = threadIdx.x >> p.bits; tile < a.tiles; tile += kSortThreads >> p.bits) {
+        const uint32_t n = a.histograms[tile * digits + my_digit];
+        before += tile < static_cast<int64_t>(blockIdx.x) ? n : 0;
+        all += n;
     }
     __syncthreads();
+    if (digits < kSortThreads) {
+        // Integers: the order of these additions changes nothing.
+        atomicAdd(&at[0][my_digit], before);
+        atomicAdd(&at[1][my_digit], all);
+        __syncthreads();
+        before = at[0][my_digit];
+        all = static_cast<int>(threadIdx.x) < digits ? at[1][my_digit] : 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * kDigits; i += kSortThreads) {
+            at[i / kDigits][i % kDigits] = 0;
+        }
+        __syncthreads();
+    }
     // The tile's tokens in order: each wave takes a contiguous part of them.
     const int64_t part = a.tile_tokens / kSortWaves;
     const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.tile_tokens + wave * part;
@@ -229,8 +245,8 @@ __device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t 
     return low;
 }
 
-// Sum of dy rows index[i0 .. i1) over 8 features of this lane, taken by
-// `groups` groups of lanes in turn and then joined, the same in every group.
+// Sum of dy rows index[i0 .. i1) over 8 features of this lane, taken by the
+// groups of `width` lanes in turn and then joined, the same in every group.
 template <int G>
 __device__ __forceinline__ void sum_rows(const EmbeddingArgs& a, int64_t i0, int64_t i1, int k, int lane, int width,
                                          float (&sum)[8]) {
@@ -241,25 +257,30 @@ __device__ __forceinline__ void sum_rows(const EmbeddingArgs& a, int64_t i0, int
     for (int e = 0; e < 8; ++e) {
         sum[e] = 0.0f;
     }
-    const auto add = [&](int64_t i) {
-        const auto* row = dy + static_cast<int64_t>(a.index[i]) * a.grad_stride;
-        float v[8];
-        if (dim >= 8) {
-            Values<G>::load8(row + k, v);
-        } else {
+    for (int64_t base = i0; base < i1; base += 64) {
+        // One load brings the next 64 indices, a shuffle hands them out.
+        const int mine = static_cast<int>(a.index[base + lane < i1 ? base + lane : base]);
+        const int here = static_cast<int>(i1 - base < 64 ? i1 - base : 64);
+#pragma unroll 8
+        for (int i = 0; i < here; i += groups) {
+            const int at = i + lane / width;
+            const int64_t token = __shfl(mine, at < 64 ? at : 0);
+            const auto* row = dy + token * a.grad_stride;
+            float v[8];
+            if (dim >= 8) {
+                Values<G>::load8(row + k, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = e < dim ? Values<G>::load(row + e) : 0.0f;
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = e < dim ? Values<G>::load(row + e) : 0.0f;
+                // Not 0 * v: what a lane reads past the run may be anything.
+                sum[e] += at < here ? v[e] : 0.0f;
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            sum[e] += v[e];
-        }
-    };
-#pragma unroll 4
-    for (int64_t i = i0 + lane / width; i < i1; i += groups) {
-        add(i);
     }
     for (int s = width; s < 64; s <<= 1) {
 #pragma unroll
@@ -321,116 +342,201 @@ __global__ __launch_bounds__(kSumThreads) void row_sum_kernel(EmbeddingArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
     const int width = row_lanes(a.dim);
-    bool inside;
-    const int k = lane_feature(a, blockIdx.y, lane, width, inside);
+    const int blocks = static_cast<int>((a.dim + 511) / 512);
     float sum[8];
     if (blockIdx.x < a.row_blocks) {
-        const int64_t row = static_cast<int64_t>(blockIdx.x) * kSumWaves + wave;
-        if (row >= a.vocabulary) {
+        // wave_rows consecutive rows: one search for the first one's run, then the
+        // others' borders from the next 64 ids, where those reach far enough.
+        const int64_t first = (static_cast<int64_t>(blockIdx.x) * kSumWaves + wave) * a.wave_rows;
+        const int64_t end = first + a.wave_rows < a.vocabulary ? first + a.wave_rows : a.vocabulary;
+        if (first >= end) {
             return;
         }
-        const int64_t i0 = first_at_least(a.keys, a.count, static_cast<uint32_t>(row), lane);
-        const int64_t i1 = i0 + first_at_least(a.keys + i0, a.count - i0, static_cast<uint32_t>(row) + 1, lane);
-        if (i1 - i0 > 2 * a.chunk_tokens) {
-            return;   // by chunks
-        }
-        sum_rows<G>(a, i0, i1, k, lane, width, sum);
-        if (inside && lane < width) {
-            store_row(a, row, k, sum);
+        int64_t i0 = first_at_least(a.keys, a.count, static_cast<uint32_t>(first), lane);
+        int64_t window = i0;   // position of the ids in `ahead`
+        uint32_t ahead = window + lane < a.count ? a.keys[window + lane] : ~0u;
+        for (int64_t row = first; row < end; ++row) {
+            const int inside = __popcll(__ballot(ahead <= static_cast<uint32_t>(row)));
+            int64_t i1 = window + inside;
+            if (inside == 64) {   // the run may go on behind the window
+                i1 = i0 + first_at_least(a.keys + i0, a.count - i0, static_cast<uint32_t>(row) + 1, lane);
+                window = i1;
+                ahead = window + lane < a.count ? a.keys[window + lane] : ~0u;
+            }
+            if (i1 - i0 <= kFewTokens) {   // a longer one goes by chunks
+                for (int block = 0; block < blocks; ++block) {
+                    bool inside_row;
+                    const int k = lane_feature(a, block, lane, width, inside_row);
+                    sum_rows<G>(a, i0, i1, k, lane, width, sum);
+                    if (inside_row && lane < width) {
+                        store_row(a, row, k, sum);
+                    }
+                }
+            }
+            i0 = i1;
         }
         return;
     }
-    // Chunk c meets at most two long runs, since each spans more than two
-    // chunks: the one that holds its first position (slot 0) and the one that
-    // begins inside it (slot 1), which then holds its last.
+    // The runs of more than kFewTokens that chunk c meets: one that lies inside it
+    // is summed here, one that begins before it or goes on behind it leaves a
+    // partial sum, in slot 0 if it holds the chunk's first position, else in 1.
     const int64_t c = static_cast<int64_t>(blockIdx.x - a.row_blocks) * kSumWaves + wave;
     if (c >= a.chunks) {
         return;
     }
     const int64_t c0 = c * a.chunk_tokens;
     const int64_t c1 = c0 + a.chunk_tokens < a.count ? c0 + a.chunk_tokens : a.count;
-    for (int slot = 0; slot < 2; ++slot) {
-        const uint32_t key = a.keys[slot == 0 ? c0 : c1 - 1];
-        if (key >= a.vocabulary || (slot == 1 && key == a.keys[c0])) {
-            continue;
+    const uint32_t before = c0 > 0 ? a.keys[c0 - 1] : ~0u;
+    const uint32_t behind = c1 < a.count ? a.keys[c1] : ~0u;
+    for (int64_t base = c0; base < c1;) {
+        // One run a turn: its end among the next 64 ids, or the chunk's.
+        const uint32_t ahead = base + lane < c1 ? a.keys[base + lane] : ~0u;
+        const uint32_t key = __shfl(ahead, 0);
+        int64_t end = base + __popcll(__ballot(ahead == key));
+        while (end < c1 && a.keys[end] == key) {   // a chunk may be longer than a wave
+            end = base + first_at_least(a.keys + base, c1 - base, key + 1, lane);
         }
-        const int64_t i0 = first_at_least(a.keys, a.count, key, lane);
-        const int64_t i1 = i0 + first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
-        if (i1 - i0 <= 2 * a.chunk_tokens) {
-            continue;
+        if (key >= a.vocabulary) {
+            break;
         }
-        sum_rows<G>(a, i0 > c0 ? i0 : c0, i1 < c1 ? i1 : c1, k, lane, width, sum);
-        if (inside && lane < width) {
-            float* at = a.partials + (2 * c + slot) * a.dim;
+        const bool crosses = (base == c0 && before == key) || (end == c1 && behind == key);
+        int64_t length = end - base;
+        if (crosses && length <= kFewTokens) {
+            const int64_t i0 = base == c0 ? first_at_least(a.keys, a.count, key, lane) : base;
+            length = first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
+        }
+        if (length > kFewTokens) {
+            for (int block = 0; block < blocks; ++block) {
+                bool inside;
+                const int k = lane_feature(a, block, lane, width, inside);
+                sum_rows<G>(a, base, end, k, lane, width, sum);
+                if (inside && lane < width) {
+                    if (!crosses) {
+                        store_row(a, key, k, sum);
+                    } else {
+                        float* at = a.partials + (2 * c + (base == c0 ? 0 : 1)) * a.dim;
+                        if (a.dim >= 8) {
+                            Values<LSSO_HIP_F32>::store8(at + k, sum);
+                        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (a.dim >= 8 || e < a.dim) {
-                    at[k + e] = sum[e];
+                            for (int e = 0; e < 8; ++e) {
+                                if (e < a.dim) {
+                                    at[e] = sum[e];
+                                }
+                            }
+                        }
+                    }
                 }
             }
+        }
+        base = end;
+    }
+}
+
+// Adds the partials of chunks [from, to) of a run that begins in chunk c at
+// position i0.
+__device__ __forceinline__ void add_partials(const EmbeddingArgs& a, int64_t from, int64_t to, int64_t c, int64_t i0,
+                                             int k, float (&sum)[8]) {
+#pragma unroll 4
+    for (int64_t p = from; p < to; ++p) {
+        const float* at = a.partials + (2 * p + (p == c && i0 > c * a.chunk_tokens ? 1 : 0)) * a.dim + k;
+        float v[8];
+        if (a.dim >= 8) {
+            Values<LSSO_HIP_F32>::load8(at, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = e < a.dim ? at[e] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum[e] += v[e];
         }
     }
 }
 
-// Workgroup c: the long run that begins in chunk c, if there is one (no two
-// do); it then holds the chunk's last position.
+// The runs that begin in a chunk and go on behind it (at most one per chunk; it
+// holds the chunk's last position).  A wave takes one chunk; a run of few chunks
+// is joined by it, a longer one afterwards by the whole workgroup.
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(EmbeddingArgs a) {
     __shared__ float parts[kJoinWaves][64][8];
+    __shared__ int64_t begins[kJoinWaves];   // position of a wave's run, or -1
+    __shared__ int64_t ends[kJoinWaves];
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
-    const int64_t c = blockIdx.x;
-    const int64_t c0 = c * a.chunk_tokens;
-    const int64_t c1 = c0 + a.chunk_tokens < a.count ? c0 + a.chunk_tokens : a.count;
-    const uint32_t key = a.keys[c1 - 1];
-    if (key >= a.vocabulary || (c > 0 && a.keys[c0 - 1] == key)) {
-        return;   // the same for the whole workgroup, as every condition here
-    }
-    const int64_t i0 = c0 + first_at_least(a.keys + c0, c1 - c0, key, lane);
-    const int64_t i1 = i0 + first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
-    if (i1 - i0 <= 2 * a.chunk_tokens) {
-        return;
-    }
     const int width = row_lanes(a.dim);
-    const int groups = 64 / width * kJoinWaves;
-    const int group = wave * (64 / width) + lane / width;
-    const int64_t last = (i1 - 1) / a.chunk_tokens;
+    const int lane_groups = 64 / width;
     bool inside;
     const int k = lane_feature(a, blockIdx.y, lane, width, inside);
-    float sum[8] = {};
-    // Consecutive chunks to each group of lanes, in order.
-    const int64_t share = (last - c + groups) / groups;
-    const int64_t from = c + group * share;
-    const int64_t to = from + share < last + 1 ? from + share : last + 1;
-    if (inside) {
-#pragma unroll 4
-        for (int64_t p = from; p < to; ++p) {
-            const float* at = a.partials + (2 * p + (p == c && i0 > c0 ? 1 : 0)) * a.dim + k;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sum[e] += a.dim >= 8 || e < a.dim ? at[e] : 0.0f;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * kJoinWaves + wave;
+    const int64_t c0 = c * a.chunk_tokens;
+    const int64_t c1 = c0 + a.chunk_tokens;
+    int64_t found = -1;
+    int64_t found_end = 0;
+    if (c1 < a.count) {   // all conditions are the same for the whole wave
+        const uint32_t key = a.keys[c1 - 1];
+        const bool here = c0 == 0 || a.keys[c0 - 1] != key;
+        if (key < a.vocabulary && here && a.keys[c1] == key) {
+            const int64_t i0 = c0 + first_at_least(a.keys + c0, a.chunk_tokens, key, lane);
+            const int64_t i1 = i0 + first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
+            const int64_t last = (i1 - 1) / a.chunk_tokens;
+            if (i1 - i0 > kFewTokens && last - c < kWaveChunks) {
+                if (inside && lane < width) {
+                    float sum[8] = {};
+                    add_partials(a, c, last + 1, c, i0, k, sum);
+                    store_row(a, key, k, sum);
+                }
+            } else if (i1 - i0 > kFewTokens) {
+                found = i0;
+                found_end = i1;
             }
         }
     }
-    for (int s = width; s < 64; s <<= 1) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            sum[e] += __shfl_xor(sum[e], s);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        parts[wave][lane][e] = sum[e];
+    if (lane == 0) {
+        begins[wave] = found;
+        ends[wave] = found_end;
     }
     __syncthreads();
-    if (wave == 0 && inside && lane < width) {
+    const int groups = lane_groups * kJoinWaves;
+    const int group = wave * lane_groups + lane / width;
+    for (int w = 0; w < kJoinWaves; ++w) {
+        const int64_t i0 = begins[w];
+        if (i0 < 0) {   // the same for the whole workgroup
+            continue;
+        }
+        const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinWaves + w;
+        const int64_t last = (ends[w] - 1) / a.chunk_tokens;
+        float sum[8] = {};
+        // Consecutive chunks to each group of lanes, in order.
+        const int64_t share = (last - first + groups) / groups;
+        const int64_t from = first + group * share;
+        const int64_t to = from + share < last + 1 ? from + share : last + 1;
+        if (inside) {
+            add_partials(a, from, to, first, i0, k, sum);
+        }
+        for (int s = width; s < 64; s <<= 1) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            sum[e] = 0.0f;
-            for (int w = 0; w < kJoinWaves; ++w) {
-                sum[e] += parts[w][lane][e];
+            for (int e = 0; e < 8; ++e) {
+                sum[e] += __shfl_xor(sum[e], s);
             }
         }
-        store_row(a, key, k, sum);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            parts[wave][lane][e] = sum[e];
+        }
+        __syncthreads();
+        if (wave == 0 && inside && lane < width) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum[e] = 0.0f;
+                for (int v = 0; v < kJoinWaves; ++v) {
+                    sum[e] += parts[v][lane][e];
+                }
+            }
+            store_row(a, a.keys[i0], k, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -467,15 +573,17 @@ hipError_t launch_embedding(const EmbeddingArgs& args, int y_type, hipStream_t s
     }
 }
 
-// Sizes of the gradient's steps.  Tiles of 4,096 tokens (64 per lane-row of a
-// wave's part), more where that would make over 256 tiles, whose histograms
-// every tile reads.  Chunks of 32 to 128 tokens: short ones keep a wave's
-// chain of gathers short, long ones keep the partials few.
+// Sizes of the gradient's steps.  Tiles of 1,024 tokens (64 per wave), more where
+// that would make over 128 tiles, whose histograms every tile reads.  Chunks of
+// 32 to 128 tokens: short ones keep a wave's chain of gathers short, long ones
+// keep the partials few.  Rows per wave: up to 8, so that a large table's empty
+// rows share a search, while a small table still has 2,048 waves.
 void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes) {
-    int64_t tile = 4096;
-    while ((a->count + tile - 1) / tile > 256) {
+    int64_t tile = 1024;
+    while ((a->count + tile - 1) / tile > 128) {
         tile *= 2;
     }
+    a->wave_rows = a->vocabulary >= 8 * 2048 ? 8 : a->vocabulary / 2048 > 1 ? a->vocabulary / 2048 : 1;
     a->tile_tokens = tile;
     a->tiles = (a->count + tile - 1) / tile;
     a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (1 << 17) ? 64 : 32;
@@ -532,18 +640,17 @@ hipError_t launch_embedding_grad(const EmbeddingArgs& args, void* workspace, int
     a.keys = sorted[2 * copy];
     a.index = sorted[2 * copy + 1];
     const unsigned feature_blocks = static_cast<unsigned>((a.dim + 511) / 512);
-    a.row_blocks = (a.vocabulary + kSumWaves - 1) / kSumWaves;
-    // Runs longer than two chunks exist only where there are more tokens.
-    const bool long_runs = a.count > 2 * a.chunk_tokens;
-    const int64_t chunk_blocks = long_runs ? (a.chunks + kSumWaves - 1) / kSumWaves : 0;
-    const dim3 sums(static_cast<unsigned>(a.row_blocks + chunk_blocks), feature_blocks);
+    a.row_blocks = (a.vocabulary + kSumWaves * a.wave_rows - 1) / (kSumWaves * a.wave_rows);
+    const int64_t chunk_blocks = a.count > kFewTokens ? (a.chunks + kSumWaves - 1) / kSumWaves : 0;
+    const dim3 sums(static_cast<unsigned>(a.row_blocks + chunk_blocks));
     switch (grad_type) {
         case LSSO_HIP_F16: row_sum_kernel<LSSO_HIP_F16><<<sums, kSumThreads, 0, stream>>>(a); break;
         case LSSO_HIP_BF16: row_sum_kernel<LSSO_HIP_BF16><<<sums, kSumThreads, 0, stream>>>(a); break;
         default: row_sum_kernel<LSSO_HIP_F32><<<sums, kSumThreads, 0, stream>>>(a); break;
     }
-    if (long_runs) {
-        join_kernel<<<dim3(static_cast<unsigned>(a.chunks), feature_blocks), kJoinThreads, 0, stream>>>(a);
+    if (a.chunks > 1) {   // else no run goes on behind its chunk
+        join_kernel<<<dim3(static_cast<unsigned>((a.chunks + kJoinWaves - 1) / kJoinWaves), feature_blocks), kJoinThreads,
+                      0, stream>>>(a);
     }
     return hipGetLastError();
 }

@@ -410,6 +410,155 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardPro
         });
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 32 rows (a decoding step): the time is the weights' bytes and the
+// launches, not the MFMAs.  A workgroup takes 16 columns of h (16 rows of both
+// weights) or of y, its eight waves share K, and a wave multiplies fragments on
+// v_mfma_f32_16x16x32 as its loads bring them, four steps ahead and nothing
+// staged; the waves' sums meet in LDS, in order.  With the large tiles' kernels
+// instead a token of 256 -> 1,024 -> 256 ran 40 workgroups through up to 16
+// stages and needed a third launch to join K's splits.
+constexpr int kFewRows = 32;
+constexpr int kFewWaves = 8;
+
+// Rows of 8 k per lane: lane & 15 the row, lane >> 4 the piece.
+struct FewLoads {
+    BufferRsrc buffer;
+    uint32_t offset;
+    int element;
+    int elements;
+    __device__ __forceinline__ FewLoads(const uint16_t* base, int64_t stride, int64_t rows, int64_t k, int lane)
+        : buffer(make_buffer(base, 2 * (rows < 16 ? rows : 16) * stride)),
+          offset(static_cast<uint32_t>(2 * ((lane & 15) * stride + 8 * (lane >> 4)))),
+          element(8 * (lane >> 4)),
+          elements(static_cast<int>(k)) {}
+    __device__ __forceinline__ u32x4 load(int k) const {
+        return buffer_load16(buffer, k + element < elements ? offset + static_cast<uint32_t>(2 * k) : kOutOfRange);
+    }
+};
+
+// sums[n][t]: of Q's operand n and P's row tile t, complete in the waves t < RT:
+// lane & 15 the row, 4 (lane >> 4) + e the column.
+template <int T, int NQ, int RT>
+__device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const FewLoads (&p)[RT], int k_end,
+                                                 f32x4 (&total)[NQ]) {
+    __shared__ f32x4 parts[kFewWaves][NQ][RT][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    f32x4 acc[NQ][RT] = {};
+#pragma unroll 4
+    for (int k = 32 * wave; k < k_end; k += 32 * kFewWaves) {
+        u32x4 qf[NQ];
+        u32x4 pf[RT];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            qf[n] = q[n].load(k);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            pf[t] = p[t].load(k);
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                acc[n][t] = mfma_small<T>(qf[n], pf[t], acc[n][t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            parts[wave][n][t][lane] = acc[n][t];
+        }
+    }
+    __syncthreads();
+    if (wave < RT) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            f32x4 sum = parts[0][n][wave][lane];
+#pragma unroll
+            for (int w = 1; w < kFewWaves; ++w) {
+                sum += parts[w][n][wave][lane];
+            }
+            total[n] = sum;
+        }
+    }
+}
+
+template <int T, int RT, bool KEEP>
+__global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    const int64_t q0 = 16 * static_cast<int64_t>(blockIdx.x);
+    const FewLoads q[2] = {FewLoads(a.gate + q0 * a.in_pitch, a.in_pitch, a.hidden - q0, a.in_pitch, lane),
+                           FewLoads(a.up + q0 * a.in_pitch, a.in_pitch, a.hidden - q0, a.in_pitch, lane)};
+    f32x4 total[2];
+    if constexpr (RT == 1) {
+        const FewLoads p[1] = {FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane)};
+        few_rows_product<T, 2, 1>(q, p, static_cast<int>(a.in_pitch), total);
+    } else {
+        const FewLoads p[2] = {FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane),
+                               FewLoads(a.x + 16 * a.x_stride, a.x_stride, a.rows - 16, a.in_pitch, lane)};
+        few_rows_product<T, 2, 2>(q, p, static_cast<int>(a.in_pitch), total);
+    }
+    const int64_t row = 16 * wave + (lane & 15);
+    const int64_t column = q0 + 4 * (lane >> 4);
+    if (wave >= RT || row >= a.rows || column >= a.pitch) {
+        return;
+    }
+    const bool kept = a.row_mask == nullptr || a.row_mask[row] != 0;
+    float h[4];
+    float first[4];
+    float second[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float act, slope;
+        activation<KEEP>(a.activation, total[0][e], act, slope);
+        h[e] = kept ? act * total[1][e] : 0.0f;
+        first[e] = slope * total[1][e];
+        second[e] = act;
+    }
+    *reinterpret_cast<u32x2*>(a.h + row * a.pitch + column) =
+        (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])};
+    if (KEEP) {
+        uint16_t* at = a.gates + 2 * row * a.pitch + column;
+        *reinterpret_cast<u32x2*>(at) = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
+        *reinterpret_cast<u32x2*>(at + a.pitch) =
+            (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])};
+    }
+}
+
+template <int T, int RT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_product_kernel(FeedForwardProduct a) {
+    const int lane = threadIdx.x & 63;
+    const int wave = wave_index();
+    const int64_t q0 = 16 * static_cast<int64_t>(blockIdx.x);
+    const FewLoads q[1] = {FewLoads(a.q + q0 * a.q_stride, a.q_stride, a.columns - q0, a.k, lane)};
+    f32x4 total[1];
+    if constexpr (RT == 1) {
+        const FewLoads p[1] = {FewLoads(a.p, a.p_stride, a.rows, a.k, lane)};
+        few_rows_product<T, 1, 1>(q, p, static_cast<int>(a.k), total);
+    } else {
+        const FewLoads p[2] = {FewLoads(a.p, a.p_stride, a.rows, a.k, lane),
+                               FewLoads(a.p + 16 * a.p_stride, a.p_stride, a.rows - 16, a.k, lane)};
+        few_rows_product<T, 1, 2>(q, p, static_cast<int>(a.k), total);
+    }
+    const int64_t row = 16 * wave + (lane & 15);
+    const int64_t column = q0 + 4 * (lane >> 4);
+    if (wave >= RT || row >= a.rows) {
+        return;
+    }
+    const bool kept = a.row_mask == nullptr || a.row_mask[row] != 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (column + e < a.columns) {
+            Values<T>::store(a.out + row * a.columns + column + e, kept ? total[0][e] : 0.0f);
+        }
+    }
+}
+
 // ----------------------------------------------------------------- dg and du
 // dh goes through the exchange in FP32, 32 rows x 32 columns at a time: in its
 // rows the factors are read and dg, du written as whole pieces.
@@ -702,8 +851,22 @@ hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
     }
 }
 
+template <int T, bool KEEP>
+hipError_t launch_few_gate(const FeedForwardArgs& a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((a.pitch + 15) / 16));
+    if (a.rows <= 16) {
+        few_gate_kernel<T, 1, KEEP><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+    } else {
+        few_gate_kernel<T, 2, KEEP><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+
 template <int T>
 hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
+    if (a.rows <= kFewRows) {
+        return a.gates != nullptr ? launch_few_gate<T, true>(a, stream) : launch_few_gate<T, false>(a, stream);
+    }
     return a.gates != nullptr ? launch_gate<T, true>(a, stream) : launch_gate<T, false>(a, stream);
 }
 
@@ -719,6 +882,15 @@ hipError_t launch_product(FeedForwardProduct a, hipStream_t stream) {
 template <int T>
 hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     FeedForwardProduct a = args;
+    if (a.rows <= kFewRows) {
+        const dim3 grid(static_cast<unsigned>((a.columns + 15) / 16));
+        if (a.rows <= 16) {
+            few_product_kernel<T, 1><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+        } else {
+            few_product_kernel<T, 2><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+        }
+        return hipGetLastError();
+    }
     if (a.splits == 1) {
         a.partials = nullptr;
     }
@@ -790,7 +962,7 @@ hipError_t launch_weights(const FeedForwardWeights& a, hipStream_t stream) {
 void plan_product(int64_t rows, int64_t columns, int64_t stages, FeedForwardProduct* a) {
     a->stages = static_cast<int>(stages);
     int64_t splits = 1;
-    if (choose_edge(rows, columns) == Edge::kSmall) {
+    if (rows > kFewRows && choose_edge(rows, columns) == Edge::kSmall) {
         // A long K over few tiles: split so that each CU has two, at least 4
         // stages each.
         const int64_t tiles = tiles_of(rows, columns, 64, 64);
@@ -830,9 +1002,11 @@ void plan_weights(FeedForwardWeights* a) {
     int64_t splits = a->tiles > 0 ? (a->large ? kCus : 3 * kCus) / a->tiles : 1;
     const int64_t most = (a->rows + 127) / 128;
     splits = splits < most ? splits : most;
+    splits = splits < 1 ? 1 : splits;
+    // The kernel keeps a split's mask in LDS; as many splits with a mask as
+    // without one, so that it only changes what is added.
     const int64_t least = (a->rows + kWeightSplitRows - 1) / kWeightSplitRows;
     splits = splits > least ? splits : least;
-    splits = splits < 1 ? 1 : splits;
     const int64_t per = (a->rows + splits - 1) / splits;
     a->split_rows = (per + kColumnsStageK - 1) / kColumnsStageK * kColumnsStageK;
     a->splits = a->rows > 0 ? (a->rows + a->split_rows - 1) / a->split_rows : 1;

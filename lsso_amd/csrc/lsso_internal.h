@@ -322,6 +322,7 @@ struct EmbeddingArgs {
     float* partials;            // [chunks, 2, dim]
     int64_t chunk_tokens;
     int64_t chunks;
+    int64_t wave_rows;          // table rows per wave
     int64_t row_blocks;
     size_t off_sorted[4];
     size_t off_histograms;
@@ -399,7 +400,7 @@ struct WeightProduct {
     int64_t q_tiles;
     int64_t tiles;
 };
-constexpr int kWeightSplitRows = 8192;   // most rows of a split
+constexpr int kWeightSplitRows = 32768;   // most rows of a split
 
 struct FeedForwardWeights {
     int type;

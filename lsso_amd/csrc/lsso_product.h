@@ -34,6 +34,17 @@ __device__ __forceinline__ f32x16 mfma_block(const u32x4& a, const u32x4& b, con
     }
 }
 
+template <int T>
+__device__ __forceinline__ f32x4 mfma_small(const u32x4& a, const u32x4& b, const f32x4& c) {
+    if constexpr (T == LSSO_HIP_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+}
+
 __device__ __forceinline__ void load_to_lds(BufferRsrc buffer, char* lds, uint32_t offset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (LdsVoid*)lds, 16, offset, 0, 0, 0);
 }
