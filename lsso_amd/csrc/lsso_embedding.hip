@@ -336,6 +336,10 @@ __device__ __forceinline__ int lane_feature(const EmbeddingArgs& a, int block, i
     return dim < 8 || !inside ? 0 : piece_at(piece, dim);
 }
 
+// Bound by the latency of ids -> index -> gathered rows of dy; a wave keeps up to 8
+// of the rows in flight.  32,800 tokens of 768 features, a third of them excluded,
+// and 32,000 table rows: 50 us; 262,144 tokens of 192 features and 6 rows: 29 us,
+// 3.5 TB/s of dy.
 // Workgroups past row_blocks take the chunks of long runs.
 template <int G>
 __global__ __launch_bounds__(kSumThreads) void row_sum_kernel(EmbeddingArgs a) {
@@ -577,13 +581,17 @@ hipError_t launch_embedding(const EmbeddingArgs& args, int y_type, hipStream_t s
 // that would make over 128 tiles, whose histograms every tile reads.  Chunks of
 // 32 to 128 tokens: short ones keep a wave's chain of gathers short, long ones
 // keep the partials few.  Rows per wave: up to 8, so that a large table's empty
-// rows share a search, while a small table still has 2,048 waves.
+// rows share a search (2, 4, 8: 24, 22, 20 us for 8,192 tokens of a table of 32,000
+// x 256; 53, 48, 55 for 32,800 of 768), while a small table still has 2,048 waves;
+// more where a launch would otherwise pass 2^32 threads.
 void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes) {
     int64_t tile = 1024;
     while ((a->count + tile - 1) / tile > 128) {
         tile *= 2;
     }
+    const int64_t least = (a->vocabulary + (1 << 24) - 1) >> 24;
     a->wave_rows = a->vocabulary >= 8 * 2048 ? 8 : a->vocabulary / 2048 > 1 ? a->vocabulary / 2048 : 1;
+    a->wave_rows = a->wave_rows > least ? a->wave_rows : least;
     a->tile_tokens = tile;
     a->tiles = (a->count + tile - 1) / tile;
     a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (1 << 17) ? 64 : 32;

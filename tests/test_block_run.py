@@ -1,0 +1,187 @@
+"""The operators around the mixer as a program uses them: tokens -> embedding ->
+blocks of (mixer, residual dropout, feed-forward, residual dropout), trained,
+decoded and captured."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn as nn
+
+from lsso_amd.ball import LSSO, GatedFeedForward, LSSOConfig, ResidualDropout, TokenEmbedding
+
+VOCABULARY, DIM, HIDDEN, PROBABILITY = 37, 64, 136, 0.1
+
+
+class Stack(nn.Module):
+    def __init__(self, layers: int, dim: int = DIM, hidden: int = HIDDEN, heads: int = 2, rank: int = 16) -> None:
+        super().__init__()
+        # A table of variance 1 / dim times sqrt(dim): a stream of variance 1.
+        self.embed = TokenEmbedding(VOCABULARY, dim, scale=dim**0.5, padding_index=0)
+        self.mixers = nn.ModuleList(LSSO(LSSOConfig(dim=dim, num_heads=heads, rank=rank)) for _ in range(layers))
+        self.blocks = nn.ModuleList(GatedFeedForward(dim, hidden) for _ in range(layers))
+        self.join = ResidualDropout(PROBABILITY)
+
+    def forward(self, tokens, mask, seed, *, dtype, implementation, keep=None):
+        x = self.embed(tokens, mask, dtype=dtype, implementation=implementation)
+        for layer, (mixer, block) in enumerate(zip(self.mixers, self.blocks)):
+            for part, step in enumerate((mixer, block)):
+                y = step(x, mask, implementation=implementation)
+                if keep is not None:
+                    keep.append((x, y))
+                x = self.join(y, x, seed=seed, offset=2 * layer + part, implementation=implementation)
+        return x
+
+
+def _stack(layers, device, **sizes):
+    torch.manual_seed(5)
+    stack = Stack(layers, **sizes)
+    with torch.no_grad():
+        for mixer in stack.mixers:   # zero as constructed
+            mixer.core_base_raw.normal_(0, 0.2)
+            mixer.core_drive_weight.normal_(0, 0.2)
+    return stack.to(device)
+
+
+def _batch(device, batch=3, length=70):
+    generator = torch.Generator().manual_seed(11)
+    tokens = torch.randint(0, VOCABULARY, (batch, length), generator=generator)
+    mask = torch.ones(batch, length, dtype=torch.bool)
+    mask[1, length // 2:] = False
+    mask[2, :] = False   # a sequence of padding alone
+    tokens[~mask] = 10**6
+    dy = torch.randn(batch, length, DIM, generator=generator)
+    return tokens.to(device), mask.to(device), dy.to(device)
+
+
+def test_reference_run_against_differences() -> None:
+    stack = _stack(1, "cpu", dim=8, hidden=8, heads=1, rank=4).double()
+    tokens = torch.tensor([[1, 2, 0, 1, 5]])
+    mask = torch.tensor([[True, True, True, True, False]])
+    names, values = zip(*((name, value.detach()) for name, value in stack.named_parameters()))
+
+    def run(*parameters):
+        return torch.func.functional_call(
+            stack, dict(zip(names, parameters)), (tokens, mask, 3), {"dtype": torch.float64, "implementation": "reference"}
+        )
+
+    # The padding row feeds the output and has no gradient: differences of the
+    # table are taken of its other rows.
+    table = values[names.index("embed.weight")]
+    free = table[1:].clone().requires_grad_()
+    others = [value.clone().requires_grad_() for name, value in zip(names, values) if name != "embed.weight"]
+
+    def whole(rows, *rest):
+        at = names.index("embed.weight")
+        return run(*rest[:at], torch.cat((table[:1], rows)), *rest[at:])
+
+    assert torch.autograd.gradcheck(whole, (free, *others), eps=1e-6, atol=1e-6, rtol=1e-5, fast_mode=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("masked", (True, False))
+def test_training_run_against_the_formulas(native, dtype, masked) -> None:
+    """Against the reference path in FP64.
+
+    Every rounding moves the stream, or its gradient, by at most half a step of
+    bfloat16 (the mixer computes in it for both types), 2^-8, of what is
+    rounded, and the branches' gains are below 1.  A path from a token to a
+    gradient meets, per block and direction, up to 8 of them in the mixer
+    (projection, weights, content, output and their gradients), 2 in the sums
+    and 6 in the feed-forward block (weights, h, factors, dg, du, y): 16 x 2
+    blocks x 2 directions x 2^-8 = 0.25 of each output's norm if all of them
+    agreed."""
+
+    stack = _stack(2, "cuda")
+    tokens, mask, dy = _batch("cuda")
+    if not masked:
+        tokens, mask = tokens.clamp(max=VOCABULARY - 1), None
+    dy = dy.to(dtype)
+    y = stack(tokens, mask, 17, dtype=dtype, implementation="hip")
+    parameters = dict(stack.named_parameters())
+    grads = torch.autograd.grad(y, list(parameters.values()), dy)
+    exact = _stack(2, "cuda").double()
+    z = exact(tokens, mask, 17, dtype=torch.float64, implementation="reference")
+    expected = torch.autograd.grad(z, list(exact.parameters()), dy.double())
+    for name, a, b in zip(("y", *parameters), (y, *grads), (z, *expected)):
+        assert torch.isfinite(a).all(), name
+        assert (a.double() - b).norm() <= 0.25 * b.norm(), name
+    if masked:
+        assert not y[~mask].any()
+    assert not grads[0][0].any()   # the padding row
+
+
+@pytest.mark.gpu
+def test_run_is_its_steps(native) -> None:
+    """One backward through the run equals the operators' own gradients, step by
+    step, bit for bit."""
+
+    stack = _stack(2, "cuda")
+    tokens, mask, dy = _batch("cuda")
+    dy = dy.bfloat16()
+    steps = []
+    y = stack(tokens, mask, 17, dtype=torch.bfloat16, implementation="hip", keep=steps)
+    grads = dict(zip(dict(stack.named_parameters()), torch.autograd.grad(y, list(stack.parameters()), dy)))
+    flow = dy
+    for layer in reversed(range(2)):
+        for part, (name, module) in reversed(list(enumerate((("mixers", stack.mixers), ("blocks", stack.blocks))))):
+            x, _ = steps[2 * layer + part]
+            x = x.detach().requires_grad_()
+            out = module[layer](x, mask, implementation="hip")
+            branch = native.dropout_add(flow, None, PROBABILITY, 17, 2 * layer + part)
+            parameters = dict(module[layer].named_parameters())
+            d, *found = torch.autograd.grad(out, [x, *parameters.values()], branch)
+            for key, value in zip(parameters, found):
+                assert torch.equal(value, grads[f"{name}.{layer}.{key}"]), (name, layer, key)
+            flow = flow + d
+    table = stack.embed.weight.detach().requires_grad_()
+    x = native.embedding(tokens, table, scale=stack.embed.scale, row_mask=mask, padding_index=0,
+                         output_dtype=torch.bfloat16)
+    assert torch.equal(torch.autograd.grad(x, table, flow)[0], grads["embed.weight"])
+
+
+@pytest.mark.gpu
+def test_captured_training_run(native) -> None:
+    stack = _stack(2, "cuda")
+    tokens, mask, dy = _batch("cuda")
+    dy = dy.bfloat16()
+    state = torch.tensor([17, 0], dtype=torch.int64, device="cuda")
+    parameters = list(stack.parameters())
+
+    def step():
+        y = stack(tokens, mask, state, dtype=torch.bfloat16, implementation="hip")
+        return (y.detach(), *torch.autograd.grad(y, parameters, dy))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    before = None
+    for replay in range(3):
+        tokens.copy_(torch.randint(0, VOCABULARY, tokens.shape, device="cuda"))
+        mask[0, 60 - replay:] = False
+        state[1] += 4   # four joins a step
+        graph.replay()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
+        assert before is None or not torch.equal(before, captured[0])
+        before = captured[0].clone()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", (1, 31, 33))
+def test_evaluation_of_one_sequence(native, length) -> None:
+    """A request: a single sequence, down to one token, without dropout; the
+    bound of the training run, one direction."""
+
+    stack = _stack(2, "cuda").eval()
+    tokens = torch.randint(1, VOCABULARY, (1, length), device="cuda")
+    with torch.no_grad():
+        y = stack(tokens, None, 0, dtype=torch.bfloat16, implementation="hip")
+        z = _stack(2, "cuda").double().eval()(tokens, None, 0, dtype=torch.float64, implementation="reference")
+    assert (y.double() - z).norm() <= 0.125 * z.norm()

@@ -130,6 +130,18 @@ def test_first_elements_are_the_integers_generator(native) -> None:
 
 
 @pytest.mark.gpu
+def test_elements_past_32_bits(native) -> None:
+    count = (1 << 31) + 29
+    y = native.dropout_add(torch.ones(count, dtype=torch.float16, device="cuda"), None, 0.5, 9, 4)
+    first = (1 << 31) - 24   # the first element of a block of 8
+    values = []
+    for group in range(first // 8, (count + 7) // 8):
+        words = _philox((group & 0xFFFFFFFF, group >> 32, 4, 0), (9, 0))
+        values += [half >= 32768 for word in words for half in (word & 0xFFFF, word >> 16)]
+    assert torch.equal(y[first:].cpu(), 2.0 * torch.tensor(values[:count - first]).half())
+
+
+@pytest.mark.gpu
 def test_layouts_do_not_change_the_mask(native) -> None:
     base = torch.randn(40, 24, device="cuda")
     plain = native.dropout_add(base, None, 0.4, 5)

@@ -151,6 +151,47 @@ def test_runs_at_chunk_borders(native) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", (5, 16, 520))
+def test_runs_by_rows_by_chunks_and_joined(native, dim) -> None:
+    # Runs of up to 8 tokens are summed by their row's wave, longer ones by
+    # chunks of 32, those of more than 16 chunks joined by a whole workgroup.
+    for lengths in ((8, 9, 7, 8, 10, 8), (30, 8, 30, 9, 30, 4), (31, 1, 8, 24, 9, 9), (16 * 32, 1, 16 * 32 + 1),
+                    (20, 15 * 32 + 12, 5), (20, 15 * 32 + 13, 5), (3, 17 * 32, 40, 70 * 32 + 5, 1)):
+        tokens = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
+        shuffle = torch.randperm(tokens.numel(), generator=torch.Generator().manual_seed(2))
+        _check(native, tokens[shuffle], len(lengths) + 1, dim, torch.float32, torch.float32)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(native) -> None:
+    count, dim = 262200, 8200
+    weight = torch.randn(5, dim, device="cuda").bfloat16().requires_grad_()
+    tokens = torch.arange(count, device="cuda") % 5
+    y = native.embedding(tokens, weight)
+    assert torch.equal(y[-7:], weight.detach()[tokens[-7:]])
+    dy = torch.zeros_like(y)
+    dy[-7:] = torch.randint(-8, 9, (7, dim), device="cuda")   # sums of small integers are exact
+    (grad,) = torch.autograd.grad(y, weight, dy)
+    expected = torch.zeros(5, dim, device="cuda").index_add_(0, tokens[-7:], dy[-7:].float())
+    assert torch.equal(grad.float(), expected)
+
+
+@pytest.mark.gpu
+def test_tables_past_one_launch_of_eight_rows_a_wave(native) -> None:
+    vocabulary = (1 << 29) + 77
+    weight = torch.zeros(vocabulary, 1, dtype=torch.bfloat16, device="cuda")
+    tokens = torch.tensor([3, vocabulary - 1, 1 << 28, vocabulary - 1, vocabulary, 0], device="cuda")
+    weight[tokens[1]] = 5.0
+    weight.requires_grad_()
+    y = native.embedding(tokens, weight)
+    assert y[1].item() == y[3].item() == 5.0 and y[0].item() == 0.0 and y[4].isnan().all()
+    (grad,) = torch.autograd.grad(y, weight, torch.full_like(y, 1.5))
+    named = grad.nonzero()[:, 0]
+    assert named.tolist() == [0, 3, 1 << 28, vocabulary - 1]
+    assert grad[named, 0].tolist() == [1.5, 1.5, 1.5, 3.0]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", (torch.int32, torch.int64))
 def test_masks_padding_and_ids_outside(native, dtype) -> None:
     generator = torch.Generator().manual_seed(4)

@@ -262,6 +262,31 @@ def test_masked_rows_may_hold_anything(native, rows, k, hidden, n) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", (1, 15, 16, 18, 31, 32, 33))
+@pytest.mark.parametrize("widths", [(64, 136, 48), (33, 65, 31), (768, 520, 1000)])
+@pytest.mark.parametrize("weight_dtype", (torch.bfloat16, torch.float32))
+def test_few_masked_rows(native, rows, widths, weight_dtype) -> None:
+    mask = torch.ones(rows, dtype=torch.bool, device="cuda")
+    mask[rows // 2::3] = False   # of a single row, that row
+    _check(native, (rows,), *widths, torch.bfloat16, "gelu", weight_dtype=weight_dtype, mask=mask, seed=rows)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(native) -> None:
+    """The last rows of h and its factors lie past 2^31 elements: they meet the
+    bounds of those rows alone."""
+
+    rows, k, hidden, n, tail = (1 << 20) + 300, 16, 2048, 8, 300
+    x, weights, dy = _inputs(rows, k, hidden, n, torch.bfloat16, torch.bfloat16)
+    mask = torch.ones(rows, dtype=torch.bool, device="cuda")
+    mask[:-tail] = False   # the weights' gradients come from the tail alone
+    whole = _run(native, x, weights, dy, "silu", mask)
+    expected = _expected(x[-tail:], weights, dy[-tail:], "silu", torch.bfloat16, torch.bfloat16)
+    _verify({name: value[-tail:] if name in ("y", "x") else value for name, value in whole.items()}, expected)
+    assert not whole["y"][:-tail].any() and not whole["x"][:-tail].any()
+
+
+@pytest.mark.gpu
 def test_masked_rows_equal_the_rows_alone(native) -> None:
     x, weights, _ = _inputs((4, 100), 96, 264, 96, torch.float16, torch.float16)
     mask = torch.zeros(4, 100, dtype=torch.bool, device="cuda")

@@ -66,3 +66,26 @@ def test_projection_kernels_do_not_spill() -> None:
                 found[kernel[".name"]] = kernel[".vgpr_spill_count"]
     assert all(any(part in name for name in found) for part in KERNELS)
     assert {name: count for name, count in found.items() if count} == {}
+
+
+BLOCK_KERNELS = ("11gate_kernel", "14product_kernel", "11grad_kernel", "13weight_kernel", "15few_gate_kernel",
+                 "18few_product_kernel", "14row_sum_kernel", "13lookup_kernel", "14dropout_kernel")
+
+
+def test_block_kernels_do_not_spill() -> None:
+    """The same of the kernels around the mixer; the tile loops hold 128 of a
+    lane's registers as accumulators, and one of the forms tried (branches
+    inside a stage) spilled 60 and more."""
+
+    path = build.library_path()
+    if not path.is_file():
+        import __graft_entry__
+
+        __graft_entry__.build()
+    found = {}
+    for image in _code_objects(path.read_bytes()):
+        for kernel in _kernels(image):
+            if any(part in kernel[".name"] for part in BLOCK_KERNELS):
+                found[kernel[".name"]] = kernel[".vgpr_spill_count"]
+    assert all(any(part in name for name in found) for part in BLOCK_KERNELS)
+    assert {name: count for name, count in found.items() if count} == {}
