@@ -80,7 +80,10 @@ def declare(library: ctypes.CDLL) -> None:
         entry.argtypes = arguments
 
 
+@lru_cache(maxsize=1)
 def _hip():
+    """The boundary module, which imports this one."""
+
     from . import hip
 
     return hip
@@ -114,7 +117,7 @@ def _saved(value: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, dev
             f"the saved {name} must be {dtype} {list(shape)} on {device}, "
             f"got {value.dtype} {list(value.shape)} on {value.device}"
         )
-    return value.contiguous()
+    return value if value.is_contiguous() else value.contiguous()
 
 
 # ------------------------------------------------------------------ embedding
@@ -133,7 +136,8 @@ def _embedding_forward(tokens, weight, scale, row_mask, output_dtype):
     device = weight.device
     vocabulary, dim = weight.shape
     mask, mask_ptr = _mask_pointer(row_mask, tokens.shape, device)
-    tokens = tokens.contiguous()
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     if weight.stride(1) != 1 or weight.stride(0) < dim:
         weight = weight.contiguous()
     y = torch.empty((*tokens.shape, dim), dtype=output_dtype, device=device)
@@ -238,9 +242,11 @@ def dropout_threshold(probability: float) -> int:
 def _dropout_launch(x, residual, threshold, seed, offset, state):
     hip = _hip()
     library = hip._library()
-    x = x.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if residual is not None and not residual.is_contiguous():
+        residual = residual.contiguous()
+    y = torch.empty_like(x)
     status = hip._launch(
         library.lsso_hip_dropout_add, x.device,
         x.data_ptr(), None if residual is None else residual.data_ptr(), _VALUE_CODES[x.dtype], x.numel(), threshold,
@@ -253,20 +259,20 @@ def _dropout_launch(x, residual, threshold, seed, offset, state):
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, threshold, seed, offset, state):
-        ctx.save_for_backward(state)
-        ctx.draw = (threshold, seed, offset)
+        if state is not None:
+            ctx.save_for_backward(state)
+        ctx.draw = (threshold, seed, offset, state is not None)
         ctx.device = x.device
         return _dropout_launch(x, residual, threshold, seed, offset, state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
-        (state,) = ctx.saved_tensors
-        threshold, seed, offset = ctx.draw
-        if state is not None:
-            state = _saved(state, "seed", torch.int64, (2,), ctx.device)
-        grad_x = _dropout_launch(grad_y, None, threshold, seed, offset, state) if ctx.needs_input_grad[0] else None
-        return grad_x, grad_y if ctx.needs_input_grad[1] else None, None, None, None, None
+        threshold, seed, offset, by_state = ctx.draw
+        state = _saved(ctx.saved_tensors[0], "seed", torch.int64, (2,), ctx.device) if by_state else None
+        needs_x, needs_residual = ctx.needs_input_grad[:2]
+        grad_x = _dropout_launch(grad_y, None, threshold, seed, offset, state) if needs_x else None
+        return grad_x, grad_y if needs_residual else None, None, None, None, None
 
 
 def dropout_add(
