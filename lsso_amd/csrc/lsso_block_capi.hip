@@ -20,14 +20,14 @@ bool aligned(const void* pointer, uintptr_t bytes) { return reinterpret_cast<uin
 uintptr_t type_bytes(int type) { return type == LSSO_HIP_F32 ? 4 : 2; }
 
 constexpr int64_t kMostIds = 0x7fffffff;
-constexpr int64_t kMostFeatures = 1 << 24;
+constexpr int64_t kMostFeatures = 1 << 22;
 
 int check_embedding(const void* tokens, int token_bytes, int64_t count, int64_t vocabulary, int64_t dim) {
     if (count < 0 || vocabulary <= 0 || dim <= 0) {
         return report(LSSO_HIP_EINVAL, "count must not be negative, vocabulary and dim must be positive");
     }
     if (count > kMostIds || vocabulary > kMostIds - 1 || dim > kMostFeatures) {
-        return report(LSSO_HIP_EUNSUPPORTED, "the embedding takes fewer than 2^31 tokens and rows of up to 2^24 features");
+        return report(LSSO_HIP_EUNSUPPORTED, "the embedding takes fewer than 2^31 tokens and rows of up to 2^22 features");
     }
     if (token_bytes != 4 && token_bytes != 8) {
         return report(LSSO_HIP_EINVAL, "tokens must be int32 or int64");

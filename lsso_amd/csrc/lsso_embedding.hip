@@ -14,14 +14,15 @@
 //   1. radix sort of (id, index) in one or two passes of up to 10 bits: a
 //      histogram per tile of tokens, then a stable scatter that ranks equal
 //      digits of 64 lanes by ballots and takes its bases from the histograms;
-//   2. a wave finds the runs of up to 8 table rows by a 64-ary search (three probes
-//      of the sorted ids for 262,144 tokens) and adds up those of at most 8 tokens;
-//      rows that no token names are written as zeros here;
-//   3. beside it, in the same launch, a wave per chunk of the sorted order adds up
-//      the longer runs, and leaves partial sums of those that cross its ends: the
-//      frequent words of a text lie side by side, and by rows a few waves had
-//      nearly all tokens (365 us instead of about 30 at 32,800 tokens of 768);
-//   4. the partials of each such run are added, by a wave or a workgroup.
+//      Workgroups beside the sort's few write zeros over dW, which most rows of a
+//      large table keep;
+//   2. the sorted order is cut into chunks, and lanes that cover a row (whole
+//      waves from 512 features on) go through one chunk each: the rows of dy are
+//      gathered 8 ahead whatever the runs' lengths, a run that ends is stored, and
+//      one that crosses the chunk's ends leaves a partial sum.  A wave per table
+//      row instead had to search its run, gathered a row at a time, and left
+//      the frequent words of a text to few waves;
+//   3. the partials of each run that crosses are added, by a wave or a workgroup.
 // Tokens that count nowhere (excluded, padding, out of range) get the id
 // `vocabulary` and sort behind every row.
 //
@@ -47,7 +48,6 @@ constexpr int kSumThreads = 256;
 constexpr int kSumWaves = kSumThreads / 64;
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinWaves = kJoinThreads / 64;
-constexpr int kFewTokens = 8;    // longest run that the wave of its row sums
 constexpr int kWaveChunks = 16;  // longest run, in chunks, that one wave joins
 
 __device__ __forceinline__ int64_t read_token(const EmbeddingArgs& a, int64_t t) {
@@ -109,8 +109,30 @@ __device__ __forceinline__ uint32_t sort_key(const EmbeddingArgs& a, const SortP
     return p.keys_in == nullptr ? token_key(a, i) : p.keys_in[i];
 }
 
+// Zeros over the pass' part of the gradient by the workgroups behind the tiles';
+// the sums that follow write the rows that tokens name.
+__device__ __forceinline__ void clear_part(const EmbeddingArgs& a, const SortPass& p, int64_t part) {
+    char* to = static_cast<char*>(a.grad_weight);
+    const int64_t bytes = a.vocabulary * a.dim * (a.weight_type == LSSO_HIP_F32 ? 4 : 2);
+    const int64_t begin = bytes / 16 * part / p.parts;
+    const int64_t end = bytes / 16 * (part + 1) / p.parts;
+    const int64_t step = static_cast<int64_t>(gridDim.x - a.tiles) * kSortThreads;
+#pragma unroll 4
+    for (int64_t i = begin + (blockIdx.x - a.tiles) * kSortThreads + threadIdx.x; i < end; i += step) {
+        store16_unaligned(to + 16 * i, (u32x4){0, 0, 0, 0});
+    }
+    const int64_t rest = bytes / 16 * 16 + 2 * static_cast<int64_t>(threadIdx.x);
+    if (part == 0 && blockIdx.x == a.tiles && rest < bytes) {
+        *reinterpret_cast<uint16_t*>(to + rest) = 0;
+    }
+}
+
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(EmbeddingArgs a, SortPass p) {
     __shared__ uint32_t histogram[kDigits];
+    if (blockIdx.x >= a.tiles) {
+        clear_part(a, p, p.part);
+        return;
+    }
     const int digits = 1 << p.bits;
     for (int d = threadIdx.x; d < digits; d += kSortThreads) {
         histogram[d] = 0;
@@ -140,6 +162,10 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool ac
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(EmbeddingArgs a, SortPass p) {
     __shared__ uint32_t at[kSortWaves][kDigits];   // per wave: counts, then the next place of each digit
     __shared__ uint32_t wave_total[kSortWaves];
+    if (blockIdx.x >= a.tiles) {
+        clear_part(a, p, p.part + 1);
+        return;
+    }
     const int digits = 1 << p.bits;
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
@@ -245,195 +271,202 @@ __device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t 
     return low;
 }
 
-// Sum of dy rows index[i0 .. i1) over 8 features of this lane, taken by the
-// groups of `width` lanes in turn and then joined, the same in every group.
-template <int G>
-__device__ __forceinline__ void sum_rows(const EmbeddingArgs& a, int64_t i0, int64_t i1, int k, int lane, int width,
-                                         float (&sum)[8]) {
-    const auto* dy = static_cast<const typename Values<G>::Element*>(a.grad_y);
-    const int groups = 64 / width;
-    const int dim = static_cast<int>(a.dim);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        sum[e] = 0.0f;
-    }
-    for (int64_t base = i0; base < i1; base += 64) {
-        // One load brings the next 64 indices, a shuffle hands them out.
-        const int mine = static_cast<int>(a.index[base + lane < i1 ? base + lane : base]);
-        const int here = static_cast<int>(i1 - base < 64 ? i1 - base : 64);
-#pragma unroll 8
-        for (int i = 0; i < here; i += groups) {
-            const int at = i + lane / width;
-            const int64_t token = __shfl(mine, at < 64 ? at : 0);
-            const auto* row = dy + token * a.grad_stride;
-            float v[8];
-            if (dim >= 8) {
-                Values<G>::load8(row + k, v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[e] = e < dim ? Values<G>::load(row + e) : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // Not 0 * v: what a lane reads past the run may be anything.
-                sum[e] += at < here ? v[e] : 0.0f;
-            }
-        }
-    }
-    for (int s = width; s < 64; s <<= 1) {
+template <int W>
+__device__ __forceinline__ void store_row(const EmbeddingArgs& a, int64_t row, int k, const float (&sum)[8]) {
+    auto* at = static_cast<typename Values<W>::Element*>(a.grad_weight) + row * a.dim;
+    if (a.dim >= 8) {
+        float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            sum[e] += __shfl_xor(sum[e], s);
+            v[e] = a.scale * sum[e];
+        }
+        Values<W>::store8(at + k, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e < a.dim) {
+                Values<W>::store(at + e, a.scale * sum[e]);
+            }
         }
     }
 }
 
 __device__ __forceinline__ void store_row(const EmbeddingArgs& a, int64_t row, int k, const float (&sum)[8]) {
-    const auto put = [&](auto values) {
-        using V = decltype(values);
-        auto* at = static_cast<typename V::Element*>(a.grad_weight) + row * a.dim;
-        if (a.dim >= 8) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = a.scale * sum[e];
-            }
-            V::store8(at + k, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (e < a.dim) {
-                    V::store(at + e, a.scale * sum[e]);
-                }
-            }
-        }
-    };
     if (a.weight_type == LSSO_HIP_F32) {
-        put(Values<LSSO_HIP_F32>());
+        store_row<LSSO_HIP_F32>(a, row, k, sum);
     } else if (a.weight_type == LSSO_HIP_BF16) {
-        put(Values<LSSO_HIP_BF16>());
+        store_row<LSSO_HIP_BF16>(a, row, k, sum);
     } else {
-        put(Values<LSSO_HIP_F16>());
+        store_row<LSSO_HIP_F16>(a, row, k, sum);
     }
 }
 
-// Lanes that share a row: the power of two that covers its pieces, at most 64.
-__device__ __forceinline__ int row_lanes(int64_t dim) {
+// Lanes that share a row: the power of two that covers its pieces, at most `most`.
+__device__ __forceinline__ int row_lanes(int64_t dim, int most) {
     int width = 1;
-    while (width < 64 && 8 * width < dim) {
+    while (width < most && 8 * width < dim) {
         width *= 2;
     }
     return width;
 }
 
-// Features of this lane in feature block `block` (64 lanes x 8 features).
-__device__ __forceinline__ int lane_feature(const EmbeddingArgs& a, int block, int lane, int width, bool& inside) {
-    const int piece = 64 * block + (lane & (width - 1));
+// Lanes of a row in the join: 128 features a workgroup, more where that would cut a
+// row into more than four.  A long run's partials come as fast as the CUs that read
+// them (262,144 tokens of 256 features, a table of 6: 22 us on one, 15 on two),
+// but short ones cost each of them a search.
+__host__ __device__ inline int join_lanes(int64_t dim) { return dim <= 512 ? 16 : dim <= 1024 ? 32 : 64; }
+
+// Features of this lane: piece `piece` of its row.
+__device__ __forceinline__ int lane_feature(const EmbeddingArgs& a, int piece, bool& inside) {
     const int dim = static_cast<int>(a.dim);
     inside = 8 * piece < dim;
     return dim < 8 || !inside ? 0 : piece_at(piece, dim);
 }
 
-// Bound by the latency of ids -> index -> gathered rows of dy; a wave keeps up to 8
-// of the rows in flight.  32,800 tokens of 768 features, a third of them excluded,
-// and 32,000 table rows: 50 us; 262,144 tokens of 256 features and 6 rows: 29 us,
-// 4.6 TB/s of dy.
-// Workgroups past row_blocks take the chunks of long runs.
-template <int G>
-__global__ __launch_bounds__(kSumThreads) void row_sum_kernel(EmbeddingArgs a) {
+// N sorted positions from a multiple of N on: their ids and tokens.
+template <int N>
+struct Positions {
+    uint32_t key[N];
+    uint32_t index[N];
+    __device__ __forceinline__ Positions(const EmbeddingArgs& a, int64_t at) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {   // the arrays end at a multiple of 64
+            const u32x4 keys = *reinterpret_cast<const u32x4*>(a.keys + at + i);
+            const u32x4 tokens = *reinterpret_cast<const u32x4*>(a.index + at + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                key[i + e] = keys[e];
+                index[i + e] = tokens[e];
+            }
+        }
+    }
+};
+
+// Their rows of dy, 8 features each, as they were loaded.
+template <int G, int N>
+struct Gathered {
+    static constexpr int kPieces = G == LSSO_HIP_F32 ? 2 : 1;
+    u32x4 raw[N][kPieces];
+    // Of the first `here` positions; behind them any row that is there.
+    __device__ __forceinline__ Gathered(const EmbeddingArgs& a, const Positions<N>& p, int here, int k) {
+        const auto* dy = static_cast<const typename Values<G>::Element*>(a.grad_y);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const auto* row = dy + static_cast<int64_t>(p.index[j < here ? j : 0]) * a.grad_stride;
+            if (a.dim >= 8) {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    raw[j][i] = load16_unaligned(row + k + 4 * i);
+                }
+            } else {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = e < a.dim ? Values<G>::load(row + e) : 0.0f;
+                }
+                put(raw[j], v);
+            }
+        }
+    }
+    __device__ __forceinline__ static void put(u32x4 (&to)[kPieces], const float (&v)[8]) {
+        if constexpr (G == LSSO_HIP_F32) {
+            to[0] = __builtin_bit_cast(u32x4, (f32x4){v[0], v[1], v[2], v[3]});
+            to[1] = __builtin_bit_cast(u32x4, (f32x4){v[4], v[5], v[6], v[7]});
+        } else {
+            to[0] = Values<G>::pack8(v);
+        }
+    }
+    __device__ __forceinline__ void add(int j, float (&sum)[8]) const {
+        float v[8];
+        if constexpr (G == LSSO_HIP_F32) {
+            const f32x4 low = __builtin_bit_cast(f32x4, raw[j][0]);
+            const f32x4 high = __builtin_bit_cast(f32x4, raw[j][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = low[e];
+                v[4 + e] = high[e];
+            }
+        } else {
+            Values<G>::unpack8(raw[j][0], v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum[e] += v[e];
+        }
+    }
+};
+
+// The runs of one chunk, by the lanes of a row.  A run that lies inside the chunk
+// is stored, one that begins before it or goes on behind it leaves a partial sum,
+// in slot 0 if it holds the chunk's first position, else in 1.  Bound by the latency
+// of ids -> tokens -> rows of dy, so the next batch of each is in flight while one
+// is added: 32,800 tokens of 768 features and 32,000 table rows 18 us (23 without
+// the second batch, 50 by table rows), 262,144 of 256 and 6 rows 25 us, 5.3 TB/s
+// of dy (47; 29).
+template <int G, int W>
+__global__ __launch_bounds__(kSumThreads) void sum_kernel(EmbeddingArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
-    const int width = row_lanes(a.dim);
-    const int blocks = static_cast<int>((a.dim + 511) / 512);
-    float sum[8];
-    if (blockIdx.x < a.row_blocks) {
-        // wave_rows consecutive rows: one search for the first one's run, then the
-        // others' borders from the next 64 ids, where those reach far enough.
-        const int64_t first = (static_cast<int64_t>(blockIdx.x) * kSumWaves + wave) * a.wave_rows;
-        const int64_t end = first + a.wave_rows < a.vocabulary ? first + a.wave_rows : a.vocabulary;
-        if (first >= end) {
-            return;
-        }
-        int64_t i0 = first_at_least(a.keys, a.count, static_cast<uint32_t>(first), lane);
-        int64_t window = i0;   // position of the ids in `ahead`
-        uint32_t ahead = window + lane < a.count ? a.keys[window + lane] : ~0u;
-        for (int64_t row = first; row < end; ++row) {
-            const int inside = __popcll(__ballot(ahead <= static_cast<uint32_t>(row)));
-            int64_t i1 = window + inside;
-            if (inside == 64) {   // the run may go on behind the window
-                i1 = i0 + first_at_least(a.keys + i0, a.count - i0, static_cast<uint32_t>(row) + 1, lane);
-                window = i1;
-                ahead = window + lane < a.count ? a.keys[window + lane] : ~0u;
-            }
-            if (i1 - i0 <= kFewTokens) {   // a longer one goes by chunks
-                for (int block = 0; block < blocks; ++block) {
-                    bool inside_row;
-                    const int k = lane_feature(a, block, lane, width, inside_row);
-                    sum_rows<G>(a, i0, i1, k, lane, width, sum);
-                    if (inside_row && lane < width) {
-                        store_row(a, row, k, sum);
-                    }
-                }
-            }
-            i0 = i1;
-        }
-        return;
-    }
-    // The runs of more than kFewTokens that chunk c meets: one that lies inside it
-    // is summed here, one that begins before it or goes on behind it leaves a
-    // partial sum, in slot 0 if it holds the chunk's first position, else in 1.
-    const int64_t c = static_cast<int64_t>(blockIdx.x - a.row_blocks) * kSumWaves + wave;
+    const int width = row_lanes(a.dim, 64);
+    bool inside;
+    const int k = lane_feature(a, 64 * blockIdx.y + (lane & (width - 1)), inside);
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * kSumWaves + wave) * (64 / width) + lane / width;
     if (c >= a.chunks) {
         return;
     }
     const int64_t c0 = c * a.chunk_tokens;
     const int64_t c1 = c0 + a.chunk_tokens < a.count ? c0 + a.chunk_tokens : a.count;
-    const uint32_t before = c0 > 0 ? a.keys[c0 - 1] : ~0u;
+    const uint32_t before = c0 > 0 ? a.keys[c0 - 1] : ~0u;   // no id
     const uint32_t behind = c1 < a.count ? a.keys[c1] : ~0u;
-    for (int64_t base = c0; base < c1;) {
-        // One run a turn: its end among the next 64 ids, or the chunk's.
-        const uint32_t ahead = base + lane < c1 ? a.keys[base + lane] : ~0u;
-        const uint32_t key = __shfl(ahead, 0);
-        int64_t end = base + __popcll(__ballot(ahead == key));
-        while (end < c1 && a.keys[end] == key) {   // a chunk may be longer than a wave
-            end = base + first_at_least(a.keys + base, c1 - base, key + 1, lane);
-        }
-        if (key >= a.vocabulary) {
-            break;
-        }
-        const bool crosses = (base == c0 && before == key) || (end == c1 && behind == key);
-        int64_t length = end - base;
-        if (crosses && length <= kFewTokens) {
-            const int64_t i0 = base == c0 ? first_at_least(a.keys, a.count, key, lane) : base;
-            length = first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
-        }
-        if (length > kFewTokens) {
-            for (int block = 0; block < blocks; ++block) {
-                bool inside;
-                const int k = lane_feature(a, block, lane, width, inside);
-                sum_rows<G>(a, base, end, k, lane, width, sum);
-                if (inside && lane < width) {
-                    if (!crosses) {
-                        store_row(a, key, k, sum);
-                    } else {
-                        float* at = a.partials + (2 * c + (base == c0 ? 0 : 1)) * a.dim;
-                        if (a.dim >= 8) {
-                            Values<LSSO_HIP_F32>::store8(at + k, sum);
-                        } else {
+    const uint32_t vocabulary = static_cast<uint32_t>(a.vocabulary);
+    constexpr int N = G == LSSO_HIP_F32 ? 4 : 8;   // rows of a batch; a second one is in flight
+    const auto at_most = [&](int64_t base) { return static_cast<int>(c1 - base < N ? c1 - base : N); };
+    const auto within = [&](int64_t base) { return base < c1 ? base : c0; };
+    float sum[8] = {};
+    bool first_run = true;
+    Positions<N> now(a, c0);
+    Positions<N> next(a, within(c0 + N));
+    Gathered<G, N> rows(a, now, at_most(c0), k);
+    for (int64_t base = c0; base < c1 && now.key[0] < vocabulary; base += N) {
+        const Positions<N> later(a, within(base + 2 * N));
+        const Gathered<G, N> following(a, next, at_most(within(base + N)), k);
+        const int here = at_most(base);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                if (e < a.dim) {
-                                    at[e] = sum[e];
-                                }
-                            }
+        for (int j = 0; j < N; ++j) {
+            const uint32_t key = now.key[j];
+            if (j >= here || key >= vocabulary) {
+                continue;
+            }
+            rows.add(j, sum);
+            const bool last = base + j + 1 == c1;
+            const uint32_t after = last ? behind : j + 1 < N ? now.key[(j + 1) % N] : next.key[0];
+            if (after == key && !last) {
+                continue;
+            }
+            if (inside && (first_run && before == key || after == key)) {
+                float* at = a.partials + (2 * c + (first_run ? 0 : 1)) * a.dim;
+                if (a.dim >= 8) {
+                    Values<LSSO_HIP_F32>::store8(at + k, sum);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (e < a.dim) {
+                            at[e] = sum[e];
                         }
                     }
                 }
+            } else if (inside) {
+                store_row<W>(a, key, k, sum);
+            }
+            first_run = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum[e] = 0.0f;
             }
         }
-        base = end;
+        now = next;
+        next = later;
+        rows = following;
     }
 }
 
@@ -469,10 +502,10 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(EmbeddingArgs a) {
     __shared__ int64_t ends[kJoinWaves];
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
-    const int width = row_lanes(a.dim);
+    const int width = row_lanes(a.dim, join_lanes(a.dim));
     const int lane_groups = 64 / width;
     bool inside;
-    const int k = lane_feature(a, blockIdx.y, lane, width, inside);
+    const int k = lane_feature(a, join_lanes(a.dim) * blockIdx.y + (lane & (width - 1)), inside);
     const int64_t c = static_cast<int64_t>(blockIdx.x) * kJoinWaves + wave;
     const int64_t c0 = c * a.chunk_tokens;
     const int64_t c1 = c0 + a.chunk_tokens;
@@ -485,13 +518,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(EmbeddingArgs a) {
             const int64_t i0 = c0 + first_at_least(a.keys + c0, a.chunk_tokens, key, lane);
             const int64_t i1 = i0 + first_at_least(a.keys + i0, a.count - i0, key + 1, lane);
             const int64_t last = (i1 - 1) / a.chunk_tokens;
-            if (i1 - i0 > kFewTokens && last - c < kWaveChunks) {
+            if (last - c < kWaveChunks) {
                 if (inside && lane < width) {
                     float sum[8] = {};
                     add_partials(a, c, last + 1, c, i0, k, sum);
                     store_row(a, key, k, sum);
                 }
-            } else if (i1 - i0 > kFewTokens) {
+            } else {
                 found = i0;
                 found_end = i1;
             }
@@ -554,6 +587,15 @@ hipError_t launch_lookup(const EmbeddingArgs& a, int y_type, dim3 grid, hipStrea
     return hipGetLastError();
 }
 
+template <int G>
+void launch_sum(const EmbeddingArgs& a, dim3 grid, hipStream_t stream) {
+    switch (a.weight_type) {
+        case LSSO_HIP_F16: sum_kernel<G, LSSO_HIP_F16><<<grid, kSumThreads, 0, stream>>>(a); break;
+        case LSSO_HIP_BF16: sum_kernel<G, LSSO_HIP_BF16><<<grid, kSumThreads, 0, stream>>>(a); break;
+        default: sum_kernel<G, LSSO_HIP_F32><<<grid, kSumThreads, 0, stream>>>(a); break;
+    }
+}
+
 }  // namespace
 
 hipError_t launch_embedding(const EmbeddingArgs& args, int y_type, hipStream_t stream) {
@@ -579,22 +621,18 @@ hipError_t launch_embedding(const EmbeddingArgs& args, int y_type, hipStream_t s
 
 // Sizes of the gradient's steps.  Tiles of 1,024 tokens (64 per wave), more where
 // that would make over 128 tiles, whose histograms every tile reads.  Chunks of
-// 32 to 128 tokens: short ones keep a wave's chain of gathers short, long ones
-// keep the partials few.  Rows per wave: up to 8, so that a large table's empty
-// rows share a search (2, 4, 8: 24, 22, 20 us for 8,192 tokens of a table of 32,000
-// x 256; 53, 48, 55 for 32,800 of 768), while a small table still has 2,048 waves;
-// more where a launch would otherwise pass 2^32 threads.
+// 16 to 128 tokens: short ones keep a wave's chain of gathers short, long ones
+// keep the partials few (chunks of 16, 32, 64: sums of 7, 12, 20 us and joins of 7,
+// 6, 6 for 8,192 tokens of 256 features; 19, 18, 24 and 9, 7, 7 for 32,800 of 768;
+// 33, 32, 26 and 70, 38, 22 for 262,144 of 256 with a table of 6).
 void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes) {
     int64_t tile = 1024;
     while ((a->count + tile - 1) / tile > 128) {
         tile *= 2;
     }
-    const int64_t least = (a->vocabulary + (1 << 24) - 1) >> 24;
-    a->wave_rows = a->vocabulary >= 8 * 2048 ? 8 : a->vocabulary / 2048 > 1 ? a->vocabulary / 2048 : 1;
-    a->wave_rows = a->wave_rows > least ? a->wave_rows : least;
     a->tile_tokens = tile;
     a->tiles = (a->count + tile - 1) / tile;
-    a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (1 << 17) ? 64 : 32;
+    a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (1 << 17) ? 64 : a->count >= (1 << 14) ? 32 : 16;
     a->chunks = (a->count + a->chunk_tokens - 1) / a->chunk_tokens;
     a->key_bits = 1;
     while ((a->vocabulary >> a->key_bits) != 0) {
@@ -626,39 +664,51 @@ hipError_t launch_embedding_grad(const EmbeddingArgs& args, void* workspace, int
     for (int i = 0; i < 4; ++i) {
         sorted[i] = reinterpret_cast<uint32_t*>(base + a.off_sorted[i]);
     }
-    const dim3 tiles(static_cast<unsigned>(a.tiles));
-    const int each = (a.key_bits + a.passes - 1) / (a.passes > 0 ? a.passes : 1);
+    // Workgroups that write zeros: 64 KiB each and launch, at most two rounds.
+    const int64_t bytes_out = a.vocabulary * a.dim * (a.weight_type == LSSO_HIP_F32 ? 4 : 2);
+    const int launches = a.count > 0 ? 2 * a.passes : 1;
+    const int64_t clear = (bytes_out / launches + 65535) / 65536;
+    const dim3 blocks(static_cast<unsigned>(a.tiles + (clear < 512 ? clear : 512)));
+    const int each = (a.key_bits + a.passes - 1) / a.passes;
     int copy = 0;
-    if (a.count > 0) {
-        for (int pass = 0; pass < a.passes; ++pass) {
-            SortPass p{};
-            p.shift = pass * each;
-            p.bits = a.key_bits - p.shift < each ? a.key_bits - p.shift : each;
-            if (pass > 0) {
-                p.keys_in = sorted[2 * copy];
-                p.index_in = sorted[2 * copy + 1];
-                copy ^= 1;
-            }
-            p.keys_out = sorted[2 * copy];
-            p.index_out = sorted[2 * copy + 1];
-            sort_count_kernel<<<tiles, kSortThreads, 0, stream>>>(a, p);
-            sort_scatter_kernel<<<tiles, kSortThreads, 0, stream>>>(a, p);
+    for (int pass = 0; pass < (a.count > 0 ? a.passes : 1); ++pass) {
+        SortPass p{};
+        p.shift = pass * each;
+        p.bits = a.key_bits - p.shift < each ? a.key_bits - p.shift : each;
+        p.part = 2 * pass;
+        p.parts = launches;
+        if (pass > 0) {
+            p.keys_in = sorted[2 * copy];
+            p.index_in = sorted[2 * copy + 1];
+            copy ^= 1;
+        }
+        p.keys_out = sorted[2 * copy];
+        p.index_out = sorted[2 * copy + 1];
+        sort_count_kernel<<<blocks, kSortThreads, 0, stream>>>(a, p);
+        if (a.count > 0) {
+            sort_scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(a, p);
         }
     }
     a.keys = sorted[2 * copy];
     a.index = sorted[2 * copy + 1];
     const unsigned feature_blocks = static_cast<unsigned>((a.dim + 511) / 512);
-    a.row_blocks = (a.vocabulary + kSumWaves * a.wave_rows - 1) / (kSumWaves * a.wave_rows);
-    const int64_t chunk_blocks = a.count > kFewTokens ? (a.chunks + kSumWaves - 1) / kSumWaves : 0;
-    const dim3 sums(static_cast<unsigned>(a.row_blocks + chunk_blocks));
-    switch (grad_type) {
-        case LSSO_HIP_F16: row_sum_kernel<LSSO_HIP_F16><<<sums, kSumThreads, 0, stream>>>(a); break;
-        case LSSO_HIP_BF16: row_sum_kernel<LSSO_HIP_BF16><<<sums, kSumThreads, 0, stream>>>(a); break;
-        default: row_sum_kernel<LSSO_HIP_F32><<<sums, kSumThreads, 0, stream>>>(a); break;
+    int64_t lanes = 8;   // of a row, eight features each, to the power of two
+    while (lanes < 512 && lanes < a.dim) {
+        lanes *= 2;
+    }
+    const int64_t per_block = kSumWaves * (512 / lanes);
+    if (a.count > 0) {
+        const dim3 sums(static_cast<unsigned>((a.chunks + per_block - 1) / per_block), feature_blocks);
+        switch (grad_type) {
+            case LSSO_HIP_F16: launch_sum<LSSO_HIP_F16>(a, sums, stream); break;
+            case LSSO_HIP_BF16: launch_sum<LSSO_HIP_BF16>(a, sums, stream); break;
+            default: launch_sum<LSSO_HIP_F32>(a, sums, stream); break;
+        }
     }
     if (a.chunks > 1) {   // else no run goes on behind its chunk
-        join_kernel<<<dim3(static_cast<unsigned>((a.chunks + kJoinWaves - 1) / kJoinWaves), feature_blocks), kJoinThreads,
-                      0, stream>>>(a);
+        const dim3 joins(static_cast<unsigned>((a.chunks + kJoinWaves - 1) / kJoinWaves),
+                         static_cast<unsigned>((a.dim + 8 * join_lanes(a.dim) - 1) / (8 * join_lanes(a.dim))));
+        join_kernel<<<joins, kJoinThreads, 0, stream>>>(a);
     }
     return hipGetLastError();
 }

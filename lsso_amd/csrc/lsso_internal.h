@@ -322,8 +322,6 @@ struct EmbeddingArgs {
     float* partials;            // [chunks, 2, dim]
     int64_t chunk_tokens;
     int64_t chunks;
-    int64_t wave_rows;          // table rows per wave
-    int64_t row_blocks;
     size_t off_sorted[4];
     size_t off_histograms;
     size_t off_partials;
@@ -337,6 +335,8 @@ struct SortPass {
     uint32_t* index_out;
     int shift;
     int bits;
+    int part;    // of the gradient that the first of the pass' two launches clears
+    int parts;
 };
 
 // Gated feed-forward block (lsso_feed_forward.hip).  All matrices are 16-bit of

@@ -152,10 +152,11 @@ def test_runs_at_chunk_borders(native) -> None:
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", (5, 16, 520))
-def test_runs_by_rows_by_chunks_and_joined(native, dim) -> None:
-    # Runs of up to 8 tokens are summed by their row's wave, longer ones by
-    # chunks of 32, those of more than 16 chunks joined by a whole workgroup.
-    for lengths in ((8, 9, 7, 8, 10, 8), (30, 8, 30, 9, 30, 4), (31, 1, 8, 24, 9, 9), (16 * 32, 1, 16 * 32 + 1),
+def test_runs_inside_chunks_across_them_and_joined(native, dim) -> None:
+    # Runs that end inside a chunk of 16, cross its ends, and are joined by a wave
+    # (up to 16 chunks) or a workgroup.
+    for lengths in ((8, 9, 7, 8, 10, 8), (30, 8, 30, 9, 30, 4), (31, 1, 8, 24, 9, 9), (16 * 16, 1, 16 * 16 + 1),
+                    (10, 15 * 16 + 6, 5), (10, 15 * 16 + 7, 5), (16 * 32, 1, 16 * 32 + 1),
                     (20, 15 * 32 + 12, 5), (20, 15 * 32 + 13, 5), (3, 17 * 32, 40, 70 * 32 + 5, 1)):
         tokens = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
         shuffle = torch.randperm(tokens.numel(), generator=torch.Generator().manual_seed(2))

@@ -69,7 +69,7 @@ def test_projection_kernels_do_not_spill() -> None:
 
 
 BLOCK_KERNELS = ("11gate_kernel", "14product_kernel", "11grad_kernel", "13weight_kernel", "15few_gate_kernel",
-                 "18few_product_kernel", "14row_sum_kernel", "13lookup_kernel", "14dropout_kernel")
+                 "18few_product_kernel", "10sum_kernel", "13lookup_kernel", "14dropout_kernel")
 
 
 def test_block_kernels_do_not_spill() -> None:
