@@ -127,7 +127,7 @@ void transpose(FeedForwardPlan* plan, const void* from, int64_t rows, int64_t co
 struct FeedForwardLayout {
     FeedForwardPlan plan;
     Packed x, gate, up, down, dy;
-    size_t h = 0, partials = 0, grads = 0, weight_partials = 0;
+    size_t h = 0, h_low = 0, partials = 0, grads = 0, weight_partials = 0;
     size_t in_columns = 0, down_columns = 0;   // [gate^T | up^T] [in, 2 pitch], down^T [hidden, out_pitch]
 };
 
@@ -155,6 +155,9 @@ FeedForwardLayout forward_layout(const lsso_hip_feed_forward_shape& s, bool trai
     const size_t pitch = static_cast<size_t>(l.plan.args.pitch);
     if (!training) {
         l.h = l.plan.take(2 * static_cast<size_t>(s.rows) * pitch);
+    }
+    if (s.rows <= lsso_hip::kFewRows) {
+        l.h_low = l.plan.take(2 * static_cast<size_t>(s.rows) * pitch);
     }
     lsso_hip::FeedForwardProduct& y = l.plan.product;
     lsso_hip::plan_product(s.rows, s.out_features, stages_of(l.plan.args.pitch), &y);
@@ -284,9 +287,12 @@ int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* 
     a.row_mask = row_mask;
     a.gates = static_cast<uint16_t*>(gates);
     a.h = product != nullptr ? static_cast<uint16_t*>(product) : reinterpret_cast<uint16_t*>(ws + l.h);
+    const bool few = s.rows <= lsso_hip::kFewRows;
+    a.h_low = few ? reinterpret_cast<uint16_t*>(ws + l.h_low) : nullptr;
     lsso_hip::FeedForwardProduct& p = l.plan.product;
     p.type = s.dtype;
     p.p = a.h;
+    p.p_low = a.h_low;
     p.p_stride = a.pitch;
     p.rows = s.rows;
     p.k = a.pitch;

@@ -415,10 +415,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardPro
 // launches, not the MFMAs.  A workgroup takes 16 columns of h (16 rows of both
 // weights) or of y, its eight waves share K, and a wave multiplies fragments on
 // v_mfma_f32_16x16x32 as its loads bring them, four steps ahead and nothing
-// staged; the waves' sums meet in LDS, in order.  With the large tiles' kernels
-// instead a token of 256 -> 1,024 -> 256 ran 40 workgroups through up to 16
-// stages and needed a third launch to join K's splits.
-constexpr int kFewRows = 32;
+// staged; the waves' sums meet in LDS, in order.  h is carried as two 16-bit values
+// (rounded, and what rounding left): its bytes are few here, and y is then rounded
+// once, not after h.  A token of 256 -> 1,024 -> 256 takes 3.8 + 3.7 us; with the
+// tiles' kernels 40 workgroups went through up to 16 stages and a third launch
+// joined K's splits, 11 us.
 constexpr int kFewWaves = 8;
 
 // Rows of 8 k per lane: lane & 15 the row, lane >> 4 the piece.
@@ -439,8 +440,9 @@ struct FewLoads {
 
 // sums[n][t]: of Q's operand n and P's row tile t, complete in the waves t < RT:
 // lane & 15 the row, 4 (lane >> 4) + e the column.
-template <int T, int NQ, int RT>
-__device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const FewLoads (&p)[RT], int k_end,
+// PARTS: 16-bit parts of P, which are added up.
+template <int T, int NQ, int RT, int PARTS>
+__device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const FewLoads (&p)[PARTS][RT], int k_end,
                                                  f32x4 (&total)[NQ]) {
     __shared__ f32x4 parts[kFewWaves][NQ][RT][64];
     const int lane = threadIdx.x & 63;
@@ -449,20 +451,20 @@ __device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const 
 #pragma unroll 4
     for (int k = 32 * wave; k < k_end; k += 32 * kFewWaves) {
         u32x4 qf[NQ];
-        u32x4 pf[RT];
+        u32x4 pf[PARTS][RT];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             qf[n] = q[n].load(k);
         }
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            pf[t] = p[t].load(k);
+        for (int i = 0; i < PARTS * RT; ++i) {
+            pf[i / RT][i % RT] = p[i / RT][i % RT].load(k);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                acc[n][t] = mfma_small<T>(qf[n], pf[t], acc[n][t]);
+            for (int i = 0; i < PARTS * RT; ++i) {
+                acc[n][i % RT] = mfma_small<T>(qf[n], pf[i / RT][i % RT], acc[n][i % RT]);
             }
         }
     }
@@ -496,12 +498,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
                            FewLoads(a.up + q0 * a.in_pitch, a.in_pitch, a.hidden - q0, a.in_pitch, lane)};
     f32x4 total[2];
     if constexpr (RT == 1) {
-        const FewLoads p[1] = {FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane)};
-        few_rows_product<T, 2, 1>(q, p, static_cast<int>(a.in_pitch), total);
+        const FewLoads p[1][1] = {{FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane)}};
+        few_rows_product<T, 2, 1, 1>(q, p, static_cast<int>(a.in_pitch), total);
     } else {
-        const FewLoads p[2] = {FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane),
-                               FewLoads(a.x + 16 * a.x_stride, a.x_stride, a.rows - 16, a.in_pitch, lane)};
-        few_rows_product<T, 2, 2>(q, p, static_cast<int>(a.in_pitch), total);
+        const FewLoads p[1][2] = {{FewLoads(a.x, a.x_stride, a.rows, a.in_pitch, lane),
+                                   FewLoads(a.x + 16 * a.x_stride, a.x_stride, a.rows - 16, a.in_pitch, lane)}};
+        few_rows_product<T, 2, 2, 1>(q, p, static_cast<int>(a.in_pitch), total);
     }
     const int64_t row = 16 * wave + (lane & 15);
     const int64_t column = q0 + 4 * (lane >> 4);
@@ -520,8 +522,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
         first[e] = slope * total[1][e];
         second[e] = act;
     }
-    *reinterpret_cast<u32x2*>(a.h + row * a.pitch + column) =
-        (u32x2){Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])};
+    const u32x2 rounded = {Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])};
+    *reinterpret_cast<u32x2*>(a.h + row * a.pitch + column) = rounded;
+    *reinterpret_cast<u32x2*>(a.h_low + row * a.pitch + column) =
+        (u32x2){Values<T>::pack(h[0] - Values<T>::low(rounded[0]), h[1] - Values<T>::high(rounded[0])),
+                Values<T>::pack(h[2] - Values<T>::low(rounded[1]), h[3] - Values<T>::high(rounded[1]))};
     if (KEEP) {
         uint16_t* at = a.gates + 2 * row * a.pitch + column;
         *reinterpret_cast<u32x2*>(at) = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
@@ -530,20 +535,26 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
     }
 }
 
-template <int T, int RT>
+template <int T, int RT, int PARTS>
 __global__ __launch_bounds__(64 * kFewWaves) void few_product_kernel(FeedForwardProduct a) {
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
     const int64_t q0 = 16 * static_cast<int64_t>(blockIdx.x);
     const FewLoads q[1] = {FewLoads(a.q + q0 * a.q_stride, a.q_stride, a.columns - q0, a.k, lane)};
+    const auto rows = [&](const uint16_t* base, int from) {
+        return FewLoads(base + from * a.p_stride, a.p_stride, a.rows - from, a.k, lane);
+    };
+    const uint16_t* const low = PARTS == 2 ? a.p_low : a.p;
     f32x4 total[1];
-    if constexpr (RT == 1) {
-        const FewLoads p[1] = {FewLoads(a.p, a.p_stride, a.rows, a.k, lane)};
-        few_rows_product<T, 1, 1>(q, p, static_cast<int>(a.k), total);
+    if constexpr (RT == 1 && PARTS == 1) {
+        few_rows_product<T, 1, 1, 1>(q, {{rows(a.p, 0)}}, static_cast<int>(a.k), total);
+    } else if constexpr (RT == 1) {
+        few_rows_product<T, 1, 1, 2>(q, {{rows(a.p, 0)}, {rows(low, 0)}}, static_cast<int>(a.k), total);
+    } else if constexpr (PARTS == 1) {
+        few_rows_product<T, 1, 2, 1>(q, {{rows(a.p, 0), rows(a.p, 16)}}, static_cast<int>(a.k), total);
     } else {
-        const FewLoads p[2] = {FewLoads(a.p, a.p_stride, a.rows, a.k, lane),
-                               FewLoads(a.p + 16 * a.p_stride, a.p_stride, a.rows - 16, a.k, lane)};
-        few_rows_product<T, 1, 2>(q, p, static_cast<int>(a.k), total);
+        few_rows_product<T, 1, 2, 2>(q, {{rows(a.p, 0), rows(a.p, 16)}, {rows(low, 0), rows(low, 16)}},
+                                     static_cast<int>(a.k), total);
     }
     const int64_t row = 16 * wave + (lane & 15);
     const int64_t column = q0 + 4 * (lane >> 4);
@@ -879,17 +890,22 @@ hipError_t launch_product(FeedForwardProduct a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int T, int PARTS>
+hipError_t launch_few_product(const FeedForwardProduct& a, dim3 grid, hipStream_t stream) {
+    if (a.rows <= 16) {
+        few_product_kernel<T, 1, PARTS><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+    } else {
+        few_product_kernel<T, 2, PARTS><<<grid, 64 * kFewWaves, 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+
 template <int T>
 hipError_t launch_product(const FeedForwardProduct& args, hipStream_t stream) {
     FeedForwardProduct a = args;
     if (a.rows <= kFewRows) {
         const dim3 grid(static_cast<unsigned>((a.columns + 15) / 16));
-        if (a.rows <= 16) {
-            few_product_kernel<T, 1><<<grid, 64 * kFewWaves, 0, stream>>>(a);
-        } else {
-            few_product_kernel<T, 2><<<grid, 64 * kFewWaves, 0, stream>>>(a);
-        }
-        return hipGetLastError();
+        return a.p_low != nullptr ? launch_few_product<T, 2>(a, grid, stream) : launch_few_product<T, 1>(a, grid, stream);
     }
     if (a.splits == 1) {
         a.partials = nullptr;

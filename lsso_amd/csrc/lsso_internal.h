@@ -341,6 +341,8 @@ struct SortPass {
 
 // Gated feed-forward block (lsso_feed_forward.hip).  All matrices are 16-bit of
 // `type` unless they say otherwise; pitches are multiples of 8.
+constexpr int kFewRows = 32;   // up to here without tiles
+
 struct FeedForwardArgs {
     int type;
     int activation;
@@ -358,6 +360,7 @@ struct FeedForwardArgs {
     const uint16_t* down_columns;   // its transpose [hidden, out_pitch], of the backward
     const uint8_t* row_mask;    // [rows] or nullptr
     uint16_t* h;                // [rows, pitch]
+    uint16_t* h_low;            // what rounding h left, of up to kFewRows rows
     uint16_t* gates;            // [rows, 2, pitch]: u act'(g), act(g); or nullptr
     const uint16_t* dy;         // [rows, out_pitch], row stride dy_stride
     int64_t dy_stride;
@@ -370,6 +373,7 @@ struct FeedForwardArgs {
 struct FeedForwardProduct {
     int type;
     const uint16_t* p;          // [rows, k], row stride p_stride
+    const uint16_t* p_low;      // a second part of p, added to it, of up to kFewRows rows; or nullptr
     int64_t p_stride;
     int64_t rows;
     int64_t k;                  // a multiple of 8

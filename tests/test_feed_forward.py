@@ -272,6 +272,30 @@ def test_few_masked_rows(native, rows, widths, weight_dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows", (1, 17, 32))
+def test_few_rows_are_rounded_once(native, dtype, rows) -> None:
+    """Up to 32 rows carry h as two 16-bit values: half a step of what the first
+    rounding left, e^2 of h (FP16: or half a step below the normal range), stands
+    in the place of e."""
+
+    x, weights, _ = _inputs(rows, 96, 264, 80, dtype, dtype)
+    y = native.gated_feed_forward(x, *weights)
+    e, f = torch.finfo(dtype).eps / 2, 2.0**-24
+    tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-134
+    xs, (gate, up, down) = x.double(), (w.double() for w in weights)
+    g, u = xs @ gate.T, xs @ up.T
+    h = _act(g, "silu")[0] * u
+    eg, eu = 96 * f * (xs.abs() @ gate.abs().T), 96 * f * (xs.abs() @ up.abs().T)
+    act = _act(g, "silu")[0].abs()
+    eh = (1.13 * eg + g.abs() * 2.0**-22) * u.abs() + act * eu + (e * e + f) * h.abs() + tiny
+    exact = h @ down.T
+    # Twice the products: each part's are summed.
+    bound = eh @ down.abs().T + 2 * 264 * f * (h.abs() @ down.abs().T) + e * exact.abs() + tiny
+    assert ((y.double() - exact).abs() <= 1.05 * bound).all()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(native) -> None:
     """The last rows of h and its factors lie past 2^31 elements: they meet the
     bounds of those rows alone."""
