@@ -417,10 +417,12 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardPro
 // v_mfma_f32_16x16x32 as its loads bring them, four steps ahead and nothing
 // staged; the waves' sums meet in LDS, in order.  h is carried as two 16-bit values
 // (rounded, and what rounding left): its bytes are few here, and y is then rounded
-// once, not after h.  A token of 256 -> 1,024 -> 256 takes 3.8 + 3.7 us; with the
+// once, not after h.  A token of 256 -> 1,024 -> 256 takes 4.1 + 3.8 us; with the
 // tiles' kernels 40 workgroups went through up to 16 stages and a third launch
-// joined K's splits, 11 us.
+// joined K's splits, 11 us.  A token of 4,096 -> 11,008 -> 4,096 with weights from
+// HBM: 37 + 24 us, 4.9 and 3.8 TB/s (loads as the compiler places them: 36 + 40).
 constexpr int kFewWaves = 8;
+constexpr int kFewSteps = 4;   // of 32 k per wave, in flight together
 
 // Rows of 8 k per lane: lane & 15 the row, lane >> 4 the piece.
 struct FewLoads {
@@ -448,23 +450,29 @@ __device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const 
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
     f32x4 acc[NQ][RT] = {};
-#pragma unroll 4
-    for (int k = 32 * wave; k < k_end; k += 32 * kFewWaves) {
-        u32x4 qf[NQ];
-        u32x4 pf[PARTS][RT];
+    for (int k = 32 * wave; k < k_end; k += 32 * kFewWaves * kFewSteps) {
+        u32x4 qf[kFewSteps][NQ];
+        u32x4 pf[kFewSteps][PARTS * RT];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            qf[n] = q[n].load(k);
-        }
+        for (int s = 0; s < kFewSteps; ++s) {   // zeros behind k_end
 #pragma unroll
-        for (int i = 0; i < PARTS * RT; ++i) {
-            pf[i / RT][i % RT] = p[i / RT][i % RT].load(k);
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
+            for (int n = 0; n < NQ; ++n) {
+                qf[s][n] = q[n].load(k + 32 * kFewWaves * s);
+            }
 #pragma unroll
             for (int i = 0; i < PARTS * RT; ++i) {
-                acc[n][i % RT] = mfma_small<T>(qf[n], pf[i / RT][i % RT], acc[n][i % RT]);
+                pf[s][i] = p[i / RT][i % RT].load(k + 32 * kFewWaves * s);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);   // else the compiler moves each load down to its use
+#pragma unroll
+        for (int s = 0; s < kFewSteps; ++s) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+                for (int i = 0; i < PARTS * RT; ++i) {
+                    acc[n][i % RT] = mfma_small<T>(qf[s][n], pf[s][i], acc[n][i % RT]);
+                }
             }
         }
     }
