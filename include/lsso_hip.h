@@ -533,7 +533,8 @@ int lsso_hip_linear_weight_grad(const void* g, int g_dtype, int64_t g_row_stride
  * y: contiguous [count, dim] of y_type; both one of LSSO_HIP_F16 / BF16 / F32.
  * row_mask: optional device uint8 [count]; rows whose byte is 0 are written as
  * zeros whatever their id.  The row of an id outside [0, vocabulary) is NaN.
- * count may be 0; vocabulary and dim are positive, vocabulary < 2^31. */
+ * count may be 0; vocabulary and dim are positive, vocabulary < 2^31, dim up to
+ * 2^22. */
 int lsso_hip_embedding(const void* tokens, int token_bytes, int64_t count,
                        const void* weight, int weight_type, int64_t vocabulary, int64_t dim,
                        int64_t weight_stride, float scale, const uint8_t* row_mask,
@@ -606,10 +607,12 @@ int lsso_hip_feed_forward_workspace_bytes(const lsso_hip_feed_forward_shape* sha
  * hidden]; y: contiguous [rows, out_features].  x and the weights are 16-byte
  * aligned.  Products accumulate in FP32 from 16-bit operands; act(g) * u is
  * taken from the FP32 accumulators and rounded to dtype once for the second
- * product.  row_mask: optional device uint8 [rows]; rows whose byte is 0 are
- * written as zeros whatever their x holds.  gates, product: both NULL, or the
- * buffers that the backward reads (lsso_hip_feed_forward_kept, 16-byte
- * aligned): u act'(g) and act(g), and their forward product act(g) u.  workspace: 256-byte aligned.  rows may be 0. */
+ * product (of up to 32 rows, carried in two values of dtype).  row_mask:
+ * optional device uint8 [rows]; rows whose byte is 0 are written as zeros
+ * whatever their x holds.  gates, product: both NULL, or the buffers that the
+ * backward reads (lsso_hip_feed_forward_kept, 16-byte aligned): u act'(g) and
+ * act(g), and their forward product act(g) u.  workspace: 256-byte aligned.
+ * rows may be 0. */
 int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* x,
                           const void* gate_weight, const void* up_weight, const void* down_weight,
                           const uint8_t* row_mask, void* gates, void* product, void* y,

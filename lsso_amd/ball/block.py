@@ -479,9 +479,9 @@ def gated_feed_forward(
 
     Products accumulate in FP32 from 16-bit operands; the product act(g) * u
     and, for the backward, u * act'(g) and act(g) are rounded to x's type once
-    (so in float16 they must stay below 65,504).  Differentiable (first order)
-    in x and the weights, deterministically; the backward keeps 3 F values per
-    row."""
+    (so in float16 they must stay below 65,504); of up to 32 rows y's product
+    takes act(g) * u in two 16-bit parts.  Differentiable (first order) in x and
+    the weights, deterministically; the backward keeps 3 F values per row."""
 
     hip = _hip()
     hip.require_available()
