@@ -16,8 +16,8 @@
 // rounded once per call, as the projections round theirs) and h, dg and du,
 // which are rounded once when they are stored, because the products that take
 // them run on 16-bit matrix instructions.  The kept factors lie as [rows, 2, Fp],
-// as do dg and du, and h as [rows, Fp], Fp the hidden width rounded up to 8 with zeros behind it, so
-// every row is whole 16-byte pieces.  Operands whose own rows are not (odd
+// as do dg and du, and h as [rows, Fp], Fp the hidden width rounded up to 8 with
+// zeros behind it, so every row is whole 16-byte pieces.  Operands whose own rows are not (odd
 // widths or strides) are copied into such rows first: element loads in the
 // product's loop cost more than one more pass over x.
 //
