@@ -421,8 +421,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product_kernel(FeedForwardPro
 // weights) or of y, its eight waves share K, and a wave multiplies fragments on
 // v_mfma_f32_16x16x32 as its loads bring them, four steps ahead and nothing
 // staged; the waves' sums meet in LDS, in order.  h is carried as two 16-bit values
-// (rounded, and what rounding left): its bytes are few here, and y is then rounded
-// once, not after h.  A token of 256 -> 1,024 -> 256 takes 4.1 + 3.8 us; with the
+// (rounded, and what rounding left, nothing of a value past the type's range): its
+// bytes are few here, and y is then rounded once, not after h.  A token of 256 -> 1,024 -> 256 takes 4.1 + 3.8 us; with the
 // tiles' kernels 40 workgroups went through up to 16 stages and a third launch
 // joined K's splits, 11 us.  A token of 4,096 -> 11,008 -> 4,096 with weights from
 // HBM: 37 + 24 us, 4.9 and 3.8 TB/s (loads as the compiler places them: 36 + 40).
@@ -537,9 +537,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
     }
     const u32x2 rounded = {Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])};
     *reinterpret_cast<u32x2*>(a.h + row * a.pitch + column) = rounded;
+    // Of an infinity the difference would be the other one, or NaN, and y NaN.
+    const auto left = [](float value, float part) { return __builtin_isfinite(part) ? value - part : 0.0f; };
     *reinterpret_cast<u32x2*>(a.h_low + row * a.pitch + column) =
-        (u32x2){Values<T>::pack(h[0] - Values<T>::low(rounded[0]), h[1] - Values<T>::high(rounded[0])),
-                Values<T>::pack(h[2] - Values<T>::low(rounded[1]), h[3] - Values<T>::high(rounded[1]))};
+        (u32x2){Values<T>::pack(left(h[0], Values<T>::low(rounded[0])), left(h[1], Values<T>::high(rounded[0]))),
+                Values<T>::pack(left(h[2], Values<T>::low(rounded[1])), left(h[3], Values<T>::high(rounded[1])))};
     if (KEEP) {
         uint16_t* at = a.gates + 2 * row * a.pitch + column;
         *reinterpret_cast<u32x2*>(at) = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};

@@ -386,6 +386,20 @@ def test_saturated_gates(native, kind) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("rows", (16, 32, 48))
+def test_products_past_the_range_are_infinite(native, kind, rows) -> None:
+    """h of 200 times +-400, past FP16's 65,504: an infinite y with h's sign, of a
+    few rows as of many.  (Its row's other columns are infinity times 0: NaN.)"""
+
+    x = torch.eye(16, device="cuda", dtype=torch.float16).repeat(rows // 16, 1)
+    sign = torch.where(torch.arange(16, device="cuda") % 2 == 0, 1.0, -1.0)
+    gate, up = torch.eye(16, device="cuda") * 200, torch.diag(400 * sign)
+    y = native.gated_feed_forward(x, gate.half(), up.half(), torch.eye(16, device="cuda").half(), activation=kind)
+    assert torch.equal(torch.diagonal(y[-16:]), (sign * math.inf).half())
+
+
+@pytest.mark.gpu
 def test_captured_training_step(native) -> None:
     x, weights, dy = _inputs((4, 65), 64, 136, 64, torch.bfloat16, torch.bfloat16)
     x.requires_grad_()
