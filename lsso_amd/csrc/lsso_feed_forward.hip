@@ -37,10 +37,12 @@ namespace lsso_hip {
 namespace {
 
 // act(g), and with SLOPE act'(g), FP32.  SiLU: g / (1 + exp(-g)); an exponential
-// that overflows leaves a sigmoid of 0.  GELU: g Phi(g) = max(g, 0) - |g| tail,
-// tail = Phi(-|g|) = t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| /
-// sqrt(2)), from Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi); the
-// exponential is also that of the derivative's normal density.  With 256 input
+// that overflows leaves a sigmoid of 0.  GELU: g Phi(g), Phi(-|g|) = tail =
+// t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| / sqrt(2)), from
+// Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi); the exponential is
+// also that of the derivative's normal density.  Of an infinite g both activations
+// are what their formulas are: inf at inf, NaN at -inf.  (max(g, 0) - |g| tail saves
+// an instruction, but is NaN at both.)  With 256 input
 // features these instructions, not the MFMAs, are what the gate kernel's tile
 // costs: the error function of the device library in this place made it 577 us
 // instead of 495 at 262,144 rows of 1,024.
@@ -57,8 +59,9 @@ __device__ __forceinline__ void activation(int kind, float g, float& value, floa
         const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
         const float tail =
             e * (t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f)))));
-        value = fmaxf(g, 0.0f) - x * tail;
-        slope = SLOPE ? (g < 0.0f ? tail : 1.0f - tail) + 0.39894228f * g * e : 0.0f;
+        const float phi = g < 0.0f ? tail : 1.0f - tail;
+        value = g * phi;
+        slope = SLOPE ? phi + 0.39894228f * g * e : 0.0f;
     }
 }
 

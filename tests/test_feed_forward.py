@@ -400,6 +400,22 @@ def test_products_past_the_range_are_infinite(native, kind, rows) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("rows", (16, 48))
+def test_infinite_gates(native, kind, rows) -> None:
+    """Gates whose FP32 sums overflow: act(inf) u is infinite, and act(-inf) =
+    -inf * 0 is NaN, as the formulas are in FP64."""
+
+    x = torch.eye(16, device="cuda", dtype=torch.bfloat16).repeat(rows // 16, 1) * 1e38
+    sign = torch.where(torch.arange(16, device="cuda") % 2 == 0, 1.0, -1.0)
+    gate, up = torch.diag(16 * sign).bfloat16(), (torch.eye(16, device="cuda") * 1e-37).bfloat16()
+    y = native.gated_feed_forward(x, gate, up, torch.eye(16, device="cuda").bfloat16(), activation=kind)
+    found, expected = torch.diagonal(y[-16:]), _act(sign.double() * math.inf, kind)[0].bfloat16()
+    assert torch.equal(found.isnan(), expected.isnan())
+    assert torch.equal(found[::2], expected[::2]) and expected[0] == math.inf
+
+
+@pytest.mark.gpu
 def test_captured_training_step(native) -> None:
     x, weights, dy = _inputs((4, 65), 64, 136, 64, torch.bfloat16, torch.bfloat16)
     x.requires_grad_()
