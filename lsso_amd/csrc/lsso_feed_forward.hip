@@ -38,14 +38,17 @@ namespace {
 
 // act(g), and with SLOPE act'(g), FP32.  SiLU: g / (1 + exp(-g)); an exponential
 // that overflows leaves a sigmoid of 0.  GELU: g Phi(g), Phi(-|g|) = tail =
-// t (a1 + t (a2 + ...)) exp(-g^2 / 2) / 2, t = 1 / (1 + p |g| / sqrt(2)), from
-// Abramowitz and Stegun 7.1.26 (off by at most 7.5e-8 of Phi); the exponential is
-// also that of the derivative's normal density.  Of an infinite g both activations
-// are what their formulas are: inf at inf, NaN at -inf.  (max(g, 0) - |g| tail saves
-// an instruction, but is NaN at both.)  With 256 input
-// features these instructions, not the MFMAs, are what the gate kernel's tile
-// costs: the error function of the device library in this place made it 577 us
-// instead of 495 at 262,144 rows of 1,024.
+// exp(-g^2 / 2) P(|g|) / Q(|g|); the exponential is also that of the derivative's
+// normal density.  P / Q is a fit to Mills' ratio over sqrt(2 pi), of degrees 3 and 4,
+// from linear programs that minimize the largest weighted error over [0, 13.4]: off
+// by at most 1.6e-8 of Phi and 1.3e-6 of the tail, in FP32 with the exponential's
+// rounded argument by 1.5e-7 and, down to g = -13, 8e-6 of the tail.  (Abramowitz and
+// Stegun 7.1.26, five terms bounded in Phi alone, leaves 3% of the tail at -12, more
+// than a 16-bit rounding from -6 on; with it the gate kernel takes 467 us instead of
+// 491 at 262,144 rows of 256 -> 1,024, whose tiles cost these instructions more than
+// MFMAs, and with the device library's error function about 80 more.)  Behind 13.2 the
+// exponential is below FP32's range and the tail 0.  Of an infinite g both activations
+// are what their formulas are: inf at inf, NaN at -inf.
 template <bool SLOPE>
 __device__ __forceinline__ void activation(int kind, float g, float& value, float& slope) {
     constexpr float kLog2e = 1.44269504f;
@@ -54,11 +57,11 @@ __device__ __forceinline__ void activation(int kind, float g, float& value, floa
         value = g * s;
         slope = SLOPE ? s + value * (1.0f - s) : 0.0f;
     } else {
-        const float x = fabsf(g);
-        const float t = __builtin_amdgcn_rcpf(1.0f + (0.3275911f * 0.70710678f) * x);
+        const float x = fminf(fabsf(g), 14.0f);   // the powers stay finite
+        const float p = 0.49999997f + x * (0.344746023f + x * (0.109477423f + x * 0.0146328295f));
+        const float q = 1.0f + x * (1.48737419f + x * (0.905736148f + x * (0.274088085f + x * 0.0366882086f)));
         const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
-        const float tail =
-            e * (t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f)))));
+        const float tail = e * (p * __builtin_amdgcn_rcpf(q));
         const float phi = g < 0.0f ? tail : 1.0f - tail;
         value = g * phi;
         slope = SLOPE ? phi + 0.39894228f * g * e : 0.0f;
@@ -271,7 +274,7 @@ __device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mi
 }
 
 //
-// 262,144 x 256 -> 2 x 1,024 FP16 GELU: 482 us, 570 TFLOP/s, with 4 stages a tile
+// 262,144 x 256 -> 2 x 1,024 FP16 GELU: 491 us, 560 TFLOP/s, with 4 stages a tile
 // bound by the epilogue's VALU work between the tiles' MFMAs (the eight waves of the
 // one workgroup run in step); 8,192 x 768 -> 2 x 2,048: 52 us, 990 TFLOP/s, by LDS and
 // L2 requests (a plain 8,192^3 product of the vendor's library reaches 1,436).

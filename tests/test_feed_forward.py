@@ -416,6 +416,36 @@ def test_infinite_gates(native, kind, rows) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("rows", (32, 96))
+@pytest.mark.parametrize("dtype,lowest,scale", [(torch.float16, -6.0, 6e4), (torch.bfloat16, -12.0, 1.0)])
+def test_negative_gates_to_a_relative_error(native, kind, rows, dtype, lowest, scale) -> None:
+    """y = act(g) u of single gates down to where a 16-bit h is still normal, to
+    one rounding of the value itself: act's own FP32 steps are off by the rounded
+    argument of the exponential (three roundings of at most 104 in powers of two:
+    2^-15.9 of it), the fit (2^-19) and a few roundings of 2^-23: less than 2^-15.
+    In bfloat16 the kept factors round once more, and the sum of equal rows once."""
+
+    x = torch.eye(32, device="cuda", dtype=dtype).repeat(rows // 32, 1)
+    g = torch.linspace(-3.0, lowest, 32, device="cuda").to(dtype)
+    weights = [torch.diag(g), torch.eye(32, device="cuda", dtype=dtype) * scale, torch.eye(32, device="cuda", dtype=dtype)]
+    got = _run(native, x, weights, torch.ones_like(x), kind)
+    act, slope = _act(g.double(), kind)
+    if kind == "gelu":   # ndtr takes the tail from 1 - erf, which is 0 from -8.3 on
+        cdf = torch.special.erfc(-g.double() * math.sqrt(0.5)) / 2
+        act, slope = g.double() * cdf, cdf + g.double() * torch.exp(-0.5 * g.double() ** 2) / math.sqrt(2 * math.pi)
+    e, fine = torch.finfo(dtype).eps / 2, 2.0**-15
+    u = torch.diagonal(weights[1]).double()
+    found = torch.diagonal(got["y"][-32:]).double()
+    # h, and of more than a few rows nothing else: the second product is by 1.
+    assert ((found - act * u).abs() <= (e + fine) * 1.01 * (act * u).abs()).all()
+    if dtype == torch.bfloat16:
+        for name, value in (("up", act), ("gate", slope)):
+            found = torch.diagonal(got[name]).double() / (rows // 32)
+            assert ((found - value).abs() <= (2 * e + 2 * fine) * 1.01 * value.abs()).all(), name
+
+
+@pytest.mark.gpu
 def test_captured_training_step(native) -> None:
     x, weights, dy = _inputs((4, 65), 64, 136, 64, torch.bfloat16, torch.bfloat16)
     x.requires_grad_()
