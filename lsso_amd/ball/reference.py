@@ -295,7 +295,8 @@ def gated_feed_forward(
     row_mask: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """(act(x Wg^T) * (x Wu^T)) Wd^T in FP32 (FP64 for FP64 x), one cast, zeros
-    for the rows that ``row_mask`` excludes."""
+    for the rows that ``row_mask`` excludes.  They reach no gradient, whatever x
+    or the upstream gradient holds there."""
 
     calc_dtype = _calculation_dtype(x)
     value = x.to(dtype=calc_dtype)
@@ -305,6 +306,8 @@ def gated_feed_forward(
         gate, up, down = (w.to(dtype=calc_dtype) for w in (gate_weight, up_weight, down_weight))
         act = {"silu": functional.silu, "gelu": functional.gelu}[activation]
         y = functional.linear(act(functional.linear(value, gate)) * functional.linear(value, up), down)
+    if row_mask is not None:
+        y = torch.where(row_mask[..., None], y, torch.zeros_like(y))
     return y.to(dtype=x.dtype)
 
 

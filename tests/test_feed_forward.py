@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from lsso_amd.ball import GatedFeedForward, block, hip
+from lsso_amd.ball import reference as canonical
 
 HALVES = (torch.float16, torch.bfloat16)
 
@@ -154,6 +155,25 @@ def test_module_on_the_cpu() -> None:
             GatedFeedForward(**{"dim": 4, "hidden": 4, **wrong})
     with pytest.raises(ValueError):
         layer(x, implementation="other")
+
+
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+def test_reference_masked_rows_may_hold_anything(kind) -> None:
+    torch.manual_seed(1)
+    leaves = [torch.randn(shape).double().requires_grad_() for shape in ((2, 3, 4), (5, 4), (5, 4), (6, 5))]
+    mask = torch.tensor([[True, False, True], [False, False, True]])
+    dy = torch.randn(2, 3, 6).double()
+
+    def run():
+        y = canonical.gated_feed_forward(*leaves, activation=kind, row_mask=mask)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    plain = run()
+    with torch.no_grad():
+        leaves[0][~mask], dy[~mask] = math.nan, math.inf
+    for a, b in zip(run(), plain):
+        assert torch.equal(a, b)
+    assert not plain[0][~mask].any() and not plain[1][~mask].any()
 
 
 def _shape(rows=4, k=16, hidden=24, n=16, stride=16, dtype=2, weight=2, activation=1):
