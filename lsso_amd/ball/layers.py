@@ -103,7 +103,8 @@ class GatedFeedForward(nn.Module):
 
 class ResidualDropout(nn.Module):
     """residual + dropout(x), with a mask that is a function of ``seed`` and
-    ``offset`` alone; in evaluation the plain sum."""
+    ``offset`` alone; in evaluation the plain sum (on the native path the same
+    kernel, with nothing dropped, and the same arguments refused)."""
 
     def __init__(self, probability: float) -> None:
         super().__init__()
@@ -121,13 +122,12 @@ class ResidualDropout(nn.Module):
         offset: int = 0,
         implementation: str = "reference",
     ) -> torch.Tensor:
-        native = _native(implementation)
-        if not self.training:
-            return x if residual is None else residual + x
-        if native:
+        if _native(implementation):
             from . import hip
 
-            return hip.dropout_add(x, residual, self.probability, seed, offset)
+            return hip.dropout_add(x, residual, self.probability if self.training else 0.0, seed, offset)
+        if not self.training:
+            return x if residual is None else residual + x
         if isinstance(seed, torch.Tensor):
             key, step = (int(value) for value in seed.tolist())
             seed, offset = key, offset + step

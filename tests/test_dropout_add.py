@@ -71,6 +71,17 @@ def test_module_on_the_cpu() -> None:
         layer(x, r, seed=9, implementation="other")
 
 
+def test_native_evaluation_calls_the_kernel(monkeypatch) -> None:
+    """With probability 0, so that it refuses what training refuses."""
+
+    monkeypatch.setattr(hip, "dropout_add", lambda *arguments: arguments)
+    x, r = torch.randn(2, 3), torch.randn(2, 3)
+    layer = ResidualDropout(0.25)
+    for implementation in ("hip", "cuda"):
+        assert layer.train()(x, r, seed=9, offset=2, implementation=implementation) == (x, r, 0.25, 9, 2)
+        assert layer.eval()(x, r, seed=9, offset=2, implementation=implementation) == (x, r, 0.0, 9, 2)
+
+
 def test_refusals_on_the_cpu() -> None:
     library = hip.open_library()
 
@@ -212,3 +223,18 @@ def test_refusals(native) -> None:
     ):
         with pytest.raises(error):
             native.dropout_add(*arguments)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_native_evaluation(native, dtype) -> None:
+    layer = ResidualDropout(0.25).eval()
+    x, r = (torch.randn(5, 37, device="cuda").to(dtype) for _ in range(2))
+    assert torch.equal(layer(x, r, seed=1, implementation="hip"), r + x)
+    assert torch.equal(layer(x, seed=1, implementation="hip"), x)
+    other = torch.float16 if dtype == torch.float32 else torch.float32
+    for arguments, error in (((x.cpu(), r.cpu()), RuntimeError), ((x, r.cpu()), RuntimeError), ((x, r[:1]), ValueError),
+                             ((x, r.to(other)), ValueError), ((x.double(), r.double()), TypeError)):
+        for mode in (True, False):
+            with pytest.raises(error):
+                layer.train(mode)(*arguments, seed=1, implementation="hip")
