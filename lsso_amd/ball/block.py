@@ -12,6 +12,7 @@ import ctypes
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 _F32 = 3
 _VALUE_CODES = {torch.float16: 1, torch.bfloat16: 2, torch.float32: _F32}
@@ -94,6 +95,17 @@ def _on_device(value: torch.Tensor, name: str, device: torch.device) -> None:
         raise RuntimeError(f"{name} must be a CUDA (ROCm device) tensor")
     if value.device != device:
         raise RuntimeError(f"{name} must be on {device}, got {value.device}")
+
+
+def _without_tangents(*values: torch.Tensor | None) -> None:
+    """Refuse forward-mode derivatives: a launch outside autograd would drop
+    them without a word."""
+
+    if forward_ad._current_level < 0:   # no forward-mode level is open
+        return
+    for value in values:
+        if value is not None and forward_ad.unpack_dual(value).tangent is not None:
+            raise NotImplementedError("the native operators have no forward-mode derivatives")
 
 
 def _mask_pointer(row_mask: torch.Tensor | None, shape: tuple, device: torch.device):
@@ -210,6 +222,7 @@ def embedding(
     summed in FP32 per table row over the sorted tokens, deterministically."""
 
     _hip().require_available()
+    _without_tangents(weight)
     if not weight.is_cuda:
         raise RuntimeError("weight must be a CUDA (ROCm device) tensor")
     if weight.dim() != 2 or weight.dtype not in _VALUE_CODES:
@@ -300,6 +313,7 @@ def dropout_add(
     again."""
 
     _hip().require_available()
+    _without_tangents(x, residual)
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA (ROCm device) tensor")
     if x.dtype not in _VALUE_CODES:
@@ -485,6 +499,7 @@ def gated_feed_forward(
 
     hip = _hip()
     hip.require_available()
+    _without_tangents(x, gate_weight, up_weight, down_weight)
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA (ROCm device) tensor")
     if x.dtype not in _HALF_CODES:

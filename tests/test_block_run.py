@@ -7,8 +7,9 @@ from __future__ import annotations
 import pytest
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
-from lsso_amd.ball import LSSO, GatedFeedForward, LSSOConfig, ResidualDropout, TokenEmbedding
+from lsso_amd.ball import LSSO, GatedFeedForward, LSSOConfig, ResidualDropout, TokenEmbedding, hip
 
 VOCABULARY, DIM, HIDDEN, PROBABILITY = 37, 64, 136, 0.1
 
@@ -76,6 +77,46 @@ def test_reference_run_against_differences() -> None:
         return run(*rest[:at], torch.cat((table[:1], rows)), *rest[at:])
 
     assert torch.autograd.gradcheck(whole, (free, *others), eps=1e-6, atol=1e-6, rtol=1e-5, fast_mode=True)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch) -> None:
+    """With and without a reverse-mode graph; the check comes before the device's."""
+
+    monkeypatch.setattr(hip, "require_available", lambda: None)
+    x, weight = torch.randn(3, 4), torch.randn(4, 4)
+    tokens = torch.tensor([0, 1])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(weight, torch.ones(4, 4))
+        rows = forward_ad.make_dual(x, torch.ones(3, 4))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: hip.embedding(tokens, dual), lambda: hip.dropout_add(rows, None, 0.1, 1),
+                             lambda: hip.dropout_add(x, rows, 0.1, 1),
+                             lambda: hip.gated_feed_forward(rows, weight, weight, weight),
+                             lambda: hip.gated_feed_forward(x, weight, dual, weight),
+                             lambda: hip.gated_feed_forward(x, weight, weight, dual)):
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call()
+        with pytest.raises(RuntimeError, match="CUDA"):   # without a tangent
+            hip.dropout_add(x, None, 0.1, 1)
+
+
+@pytest.mark.gpu
+def test_forward_mode_leaves_plain_calls_alone(native) -> None:
+    x = torch.randn(5, 8, device="cuda")
+    weights = [torch.randn(8, 8, device="cuda") for _ in range(3)]
+    calls = (lambda: native.embedding(torch.tensor([0, 4, 2], device="cuda"), x),
+             lambda: native.dropout_add(x, x, 0.3, 5),
+             lambda: native.gated_feed_forward(x.bfloat16(), *weights))
+    expected = [call() for call in calls]
+    with forward_ad.dual_level():
+        forward_ad.make_dual(torch.randn(2, device="cuda"), torch.ones(2, device="cuda"))
+        for call, value in zip(calls, expected):
+            assert torch.equal(call(), value)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            native.dropout_add(forward_ad.make_dual(x, torch.ones_like(x)), None, 0.1, 1)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: native.dropout_add(v, None, 0.1, 1), (x,), (torch.ones_like(x),))
 
 
 @pytest.mark.gpu
