@@ -219,6 +219,12 @@ def open_library(path: str | os.PathLike[str] | None = None) -> ctypes.CDLL:
             "`python -m lsso_amd.build` or pass its path to load()"
         )
     library = ctypes.CDLL(str(library_path.resolve()))
+    missing = [name for name in _SYMBOLS if not hasattr(library, name)]
+    if missing:   # built from earlier sources of the same contract version, or another library
+        raise RuntimeError(
+            f"the library at {library_path} lacks {', '.join(missing[:3])}{' ...' if missing[3:] else ''}; "
+            "rebuild it with `python -m lsso_amd.build` and restart the process"
+        )
     _declare(library)
     return library
 

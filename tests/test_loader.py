@@ -20,7 +20,7 @@ import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from lsso_amd.ball import hip, ops
+from lsso_amd.ball import block, hip, ops
 
 # The reference's schemas as binding.cpp:80-95 writes them.
 REFERENCE_SCHEMAS = {
@@ -110,6 +110,20 @@ def test_loader_rejects_a_stale_same_name_artifact(unloaded, tmp_path: Path) -> 
         hip.load(path=library)
     assert opened == [library]
     assert hip._LIBRARY is None and hip._LOADED_ARCHITECTURE is None
+
+
+def test_a_library_without_the_newest_entries_asks_for_a_rebuild(monkeypatch: pytest.MonkeyPatch, tmp_path: Path) -> None:
+    """One built before the operators around the mixer, at the same version."""
+
+    class Older:
+        def __init__(self, path: str) -> None:
+            for name in hip._SYMBOLS:
+                if name not in block.SYMBOLS:
+                    setattr(self, name, lambda: 1)
+
+    monkeypatch.setattr(hip.ctypes, "CDLL", Older)
+    with pytest.raises(RuntimeError, match="lacks lsso_hip_embedding, .*rebuild it"):
+        hip.open_library(_artifact(tmp_path))
 
 
 def test_loader_rejects_a_library_for_another_target(unloaded, tmp_path: Path) -> None:
