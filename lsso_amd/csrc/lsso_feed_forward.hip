@@ -778,15 +778,19 @@ __global__ __launch_bounds__(256) void join_kernel(FeedForwardJoin a) {
 // behind the last one (FP32 weights, operands with odd rows), or of their
 // transposes.  A workgroup takes 64 x 64 of a matrix, a thread 2 pieces of 8.
 constexpr int kPackEdge = 64;
+constexpr int kPackBlocks = 1 << 22;   // in x: a launch's x holds fewer than 2^32 threads
 
 template <int T>
 __global__ __launch_bounds__(256) void pack_kernel(FeedForwardPack a) {
     __shared__ uint16_t square[kPackEdge][kPackEdge + 8];
-    int block = static_cast<int>(blockIdx.x);
+    int block = static_cast<int>(blockIdx.y) * kPackBlocks + static_cast<int>(blockIdx.x);
     int which = 0;
-    while (block >= a.matrices[which].tiles) {   // the grid is the sum of all tiles
+    while (which < a.count && block >= a.matrices[which].tiles) {
         block -= a.matrices[which].tiles;
         ++which;
+    }
+    if (which == a.count) {   // the grid is at least the sum of all tiles
+        return;
     }
     const PackMatrix& m = a.matrices[which];
     const int across = static_cast<int>((m.columns + kPackEdge - 1) / kPackEdge);
@@ -1086,7 +1090,8 @@ hipError_t launch_feed_forward_pack(const FeedForwardPack& args, int type, hipSt
     if (tiles == 0) {
         return hipSuccess;
     }
-    const dim3 grid(static_cast<unsigned>(tiles));
+    const dim3 grid(static_cast<unsigned>(tiles < kPackBlocks ? tiles : kPackBlocks),
+                    static_cast<unsigned>((tiles + kPackBlocks - 1) / kPackBlocks));
     if (type == LSSO_HIP_BF16) {
         pack_kernel<LSSO_HIP_BF16><<<grid, 256, 0, stream>>>(a);
     } else {

@@ -331,6 +331,21 @@ def test_offsets_past_32_bits(native) -> None:
 
 
 @pytest.mark.gpu
+def test_rows_past_one_grid_of_copies(native) -> None:
+    """2^30 rows of one feature, copied into whole pieces by more workgroups than
+    fit a launch's x; all but the last rows are zeros."""
+
+    rows, tail = (1 << 30) + 77, 300
+    x, weights, dy = _inputs(tail, 1, 1, 1, torch.bfloat16, torch.bfloat16)
+    long_x, long_dy = (torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    long_x[-tail:], long_dy[-tail:] = x, dy
+    got = _run(native, long_x, weights, long_dy, "silu")
+    _verify({name: value[-tail:] if name in ("y", "x") else value for name, value in got.items()},
+            _expected(x, weights, dy, "silu", torch.bfloat16, torch.bfloat16))
+    assert not got["y"][:-tail].any() and not got["x"][:-tail].any()
+
+
+@pytest.mark.gpu
 def test_masked_rows_equal_the_rows_alone(native) -> None:
     x, weights, _ = _inputs((4, 100), 96, 264, 96, torch.float16, torch.float16)
     mask = torch.zeros(4, 100, dtype=torch.bool, device="cuda")
