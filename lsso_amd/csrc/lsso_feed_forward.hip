@@ -846,24 +846,37 @@ __global__ __launch_bounds__(256) void pack_kernel(FeedForwardPack a) {
     }
 }
 
-// Tiles of the row products: 256 x 256 by 8 waves, 128 x 128 or 64 x 64 by 4.
-// The larger the tile, the fewer bytes a product moves between L2, LDS and
-// registers, so a size is taken once it gives enough CUs a tile.  Measured on
-// both sides: 150 large tiles instead of 594 middle ones (12,608 x 2,048 -> 768) 51
-// against 56 us, 192 instead of 768 (16,384 x 1,024 -> 768) 30 and 31, but 128 instead of 512
-// (4,096 x 768 -> 2 x 1,024) 23 against 18; 384 middle tiles instead of 1,536 small ones
-// (8,192 x 2,048 -> 768) 32 against 44, 192 instead of 768 14 against 13.
+// Tiles of the row products: 256 x 256 by 8 waves, one workgroup per CU; 128 x 128
+// by 4, two per CU; or small ones (64 x 64, three; the gate's 64 x 128, two) by 4.  The
+// larger the tile, the fewer bytes a product moves between L2, LDS and registers, but
+// what counts first is how often the workgroups that are resident go round: small
+// tiles while they go round once, then the fewer of 5 per round of large tiles and 3
+// per round of middle ones.  Measured with kernel and K the same on both sides:
+//   small and middle, y of K = 2,048 and 768 columns: 768 and 192 tiles (one round and
+//   one) 22.8 and 25.0 us, 864 and 216 (two and one) 37.0 and 26.0; gate of K = 768: 512
+//   and 256 13.4 and 14.0, 544 and 272 18.6 and 14.8; dg and du of K = 768: 736 and 184 16.0
+//   and 18.3, 800 and 200 23.6 and 18.5;
+//   middle and large, the same y: 480 and 120 tiles (one and one) 39.9 and 47.6, 516 and
+//   129 (two and one) 56.3 and 50.8, 1,020 and 255 69.7 and 60.5, 1,032 and 258 (three
+//   and two) 82.0 and 93.0, 1,536 and 384 102 and 100, 1,548 and 387 (four and two) 133 and
+//   130, 3,072 and 768 (six and three) 224 and 187; the gate of K = 768: 512 and 128 18.1
+//   and 22.4, 544 and 136 23.8 and 22.6, 1,056 and 264 36.2 and 42.8, 1,568 and 392 53.7 and
+//   44.3.  (The gate of K = 256, whose epilogue is most of it, keeps 12.4 against 15.3
+//   on middle tiles up to 224 large ones, and loses 16.4 to 15.1 from 240 on.)
 enum class Edge { kLarge, kMiddle, kSmall };
 
 int64_t tiles_of(int64_t p, int64_t q, int64_t bp, int64_t bq) { return ((p + bp - 1) / bp) * ((q + bq - 1) / bq); }
 
 constexpr int64_t kCus = 256;
 
-Edge choose_edge(int64_t p, int64_t q) {
-    if (tiles_of(p, q, 256, 256) >= 9 * kCus / 16) {
-        return Edge::kLarge;
+// small_q: columns of a small tile, of which small_slots are resident at a time.
+Edge choose_edge(int64_t p, int64_t q, int64_t small_q = 64, int64_t small_slots = 3 * kCus) {
+    if (tiles_of(p, q, 64, small_q) <= small_slots) {
+        return Edge::kSmall;
     }
-    return tiles_of(p, q, 128, 128) >= kCus ? Edge::kMiddle : Edge::kSmall;
+    const int64_t large = (tiles_of(p, q, 256, 256) + kCus - 1) / kCus;
+    const int64_t middle = (tiles_of(p, q, 128, 128) + 2 * kCus - 1) / (2 * kCus);
+    return 5 * large <= 3 * middle ? Edge::kLarge : Edge::kMiddle;
 }
 
 // A multiple of eight workgroups (one share per XCD), at most what is resident.
@@ -884,7 +897,7 @@ hipError_t launch_gate(FeedForwardArgs a, hipStream_t stream) {
 
 template <int T, bool KEEP>
 hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
-    switch (choose_edge(a.rows, 2 * a.pitch)) {
+    switch (choose_edge(a.rows, 2 * a.pitch, 128, 2 * kCus)) {
         case Edge::kLarge: return launch_gate<T, 2, 4, 4, 2, KEEP>(a, stream);
         case Edge::kMiddle: return launch_gate<T, 2, 2, 2, 2, KEEP>(a, stream);
         default: return launch_gate<T, 1, 2, 2, 2, KEEP>(a, stream);
@@ -970,13 +983,14 @@ hipError_t launch_grad(FeedForwardArgs a, hipStream_t stream) {
 }
 
 // With few stages a tile's time is its epilogue (the factors read, dg and du
-// written), which two workgroups of a CU overlap and one large one does not:
-// 131,072 x 256 -> 688 takes 224 us on middle tiles and 281 on large ones, 65,536 x
-// 384 -> 1,536 254 on both.
+// written), which two workgroups of a CU overlap and one large one does not: 65,536
+// rows of 1,024 take 142 us on middle tiles and 181 on large ones with K = 256, 163 and
+// 190 with 384, 179 and 202 with 512; 32,768 of 2,048 with 768 225 and 218, 16,384 of 2,048
+// with 1,024 129 and 123.
 template <int T>
 hipError_t launch_grad(const FeedForwardArgs& a, hipStream_t stream) {
     Edge edge = choose_edge(a.rows, a.pitch);
-    if (edge == Edge::kLarge && a.out_pitch <= 384) {
+    if (edge == Edge::kLarge && a.out_pitch <= 512) {
         edge = Edge::kMiddle;
     }
     switch (edge) {

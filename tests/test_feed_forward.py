@@ -265,6 +265,17 @@ def test_large_tiles_and_row_ranges(native, rows, k, hidden, n) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows,k,hidden,n", [(8000, 72, 2048, 520), (8000, 520, 2041, 72), (22000, 512, 72, 520),
+                                             (4200, 200, 1032, 776), (2100, 200, 1032, 776)])
+def test_tiles_of_every_size(native, rows, k, hidden, n, dtype) -> None:
+    """Products of each kernel whose tiles go round the device once and twice, in
+    each of the three sizes, the last ones partly outside."""
+
+    _check(native, rows, k, hidden, n, dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,k,hidden,n", [((3, 70), 64, 136, 48), ((2, 33), 33, 65, 31), ((8, 513), 128, 256, 128),
                                              ((16, 2500), 64, 264, 136)])
 def test_masked_rows_may_hold_anything(native, rows, k, hidden, n) -> None:
