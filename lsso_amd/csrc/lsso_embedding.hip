@@ -11,7 +11,8 @@
 // symbols in 262,144 tokens) would queue at one address.  Instead the tokens
 // are sorted by id (stable, so a row's tokens keep their order), and each row
 // is summed once, in FP32, in an order that depends on the sizes alone:
-//   1. radix sort of (id, index) in one or two passes of up to 10 bits: a
+//   1. radix sort of (id, index) in passes of up to 10 bits of the id (one for
+//      tables of up to 1,023 rows, two up to 2^20 - 1, three up to 2^30 - 1): a
 //      histogram per tile of tokens, then a stable scatter that ranks equal
 //      digits of 64 lanes by ballots and takes its bases from the histograms;
 //      Workgroups beside the sort's few write zeros over dW, which most rows of a
@@ -26,8 +27,8 @@
 // Tokens that count nowhere (excluded, padding, out of range) get the id
 // `vocabulary` and sort behind every row.
 //
-// Bound: reading dy (gathered whole rows) and writing dW, plus the latency of
-// four or six launches.
+// Bound: reading dy (gathered whole rows) and writing dW, plus the latency of two
+// launches per pass, the sums' and, with more than one chunk, the join's.
 
 #include "lsso_device.h"
 #include "lsso_internal.h"
@@ -312,7 +313,7 @@ __device__ __forceinline__ int row_lanes(int64_t dim, int most) {
 
 // Lanes of a row in the join: 128 features a workgroup, more where that would cut a
 // row into more than four.  A long run's partials come as fast as the CUs that read
-// them (262,144 tokens of 256 features, a table of 6: 22 us on one, 15 on two),
+// them (262,144 tokens of 256 features, a table of 6: 22 us on one, 13 on two),
 // but short ones cost each of them a search.
 __host__ __device__ inline int join_lanes(int64_t dim) { return dim <= 512 ? 16 : dim <= 1024 ? 32 : 64; }
 
@@ -622,9 +623,14 @@ hipError_t launch_embedding(const EmbeddingArgs& args, int y_type, hipStream_t s
 // Sizes of the gradient's steps.  Tiles of 1,024 tokens (64 per wave), more where
 // that would make over 128 tiles, whose histograms every tile reads.  Chunks of
 // 16 to 128 tokens: short ones keep a wave's chain of gathers short, long ones
-// keep the partials few (chunks of 16, 32, 64: sums of 7, 12, 20 us and joins of 7,
-// 6, 6 for 8,192 tokens of 256 features; 19, 18, 24 and 9, 7, 7 for 32,800 of 768;
-// 33, 32, 26 and 70, 38, 22 for 262,144 of 256 with a table of 6).
+// keep the partials few.  Sums and join together, us, 256 features (a table of 6, and
+// one of 32,000) and 768:
+//   16,384 tokens: chunks of 16 13.7, 15.2, 19.7; of 32 15.3, 19.4, 20.6
+//   32,768: of 16 14.6, 15.8, 29.6; of 32 15.8, 19.7, 23.8
+//   65,536: of 16 22.3, 25.3, 49.5; of 32 17.4, 21.9, 42.3; of 64 21.7, 29.3, 35.8
+//   98,304: of 32 27.8, 28.2, 67.0; of 64 22.3, 29.0, 63.5
+//   262,144: of 32 49.5, 62.6, 171; of 64 36.9, 51.6, 159; of 128 34.4, 53.1, 160
+//   524,288: of 64 103, 116; of 128 93, 105
 void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes) {
     int64_t tile = 1024;
     while ((a->count + tile - 1) / tile > 128) {
@@ -632,7 +638,7 @@ void plan_embedding_grad(EmbeddingArgs* a, size_t* bytes) {
     }
     a->tile_tokens = tile;
     a->tiles = (a->count + tile - 1) / tile;
-    a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (1 << 17) ? 64 : a->count >= (1 << 14) ? 32 : 16;
+    a->chunk_tokens = a->count >= (1 << 19) ? 128 : a->count >= (3 << 15) ? 64 : a->count >= (1 << 15) ? 32 : 16;
     a->chunks = (a->count + a->chunk_tokens - 1) / a->chunk_tokens;
     a->key_bits = 1;
     while ((a->vocabulary >> a->key_bits) != 0) {

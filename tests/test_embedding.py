@@ -151,6 +151,20 @@ def test_runs_at_chunk_borders(native) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,chunk", [(32767, 16), (32768, 32), (98303, 32), (98304, 64), (524287, 64), (524288, 128)])
+def test_runs_at_the_borders_of_every_chunk_length(native, count, chunk) -> None:
+    """Runs that end before, at and behind a chunk's border, from a chunk's length
+    to more than a wave joins (16 chunks), each then a run of the rest."""
+
+    lengths = [chunk - 1, 1, chunk, chunk + 1, chunk - 1, 2 * chunk, 1, 15 * chunk - 2, chunk + 2, 16 * chunk,
+               16 * chunk + 1, chunk - 1, 33 * chunk, 3]
+    lengths.append(count - sum(lengths))
+    tokens = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
+    shuffle = torch.randperm(count, generator=torch.Generator().manual_seed(3))
+    _check(native, tokens[shuffle], len(lengths), 8, torch.float32, torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", (5, 16, 520))
 def test_runs_inside_chunks_across_them_and_joined(native, dim) -> None:
     # Runs that end inside a chunk of 16, cross its ends, and are joined by a wave
