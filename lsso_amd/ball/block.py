@@ -20,7 +20,6 @@ _HALF_CODES = {torch.float16: 1, torch.bfloat16: 2}
 _TOKEN_BYTES = {torch.int32: 4, torch.int64: 8}
 _ACTIVATIONS = {"silu": 1, "gelu": 2}
 _MOST_ELEMENTS = 1 << 34
-_MOST_IDS = (1 << 31) - 1
 
 SYMBOLS = (
     "lsso_hip_embedding",

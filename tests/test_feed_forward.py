@@ -234,6 +234,43 @@ def test_workspaces_hold_every_size() -> None:
                 assert size.value >= 4 * rows * hidden
 
 
+def test_workspaces_hold_every_buffer() -> None:
+    """The sum of all that a call keeps beside each other: copies of operands with
+    odd rows or of float32, h (its second part of few rows), dg and du, both
+    transposes, the weight gradients' partials, and at least two splits' partials
+    of a small product with a long K."""
+
+    library = hip.open_library()
+    size = ctypes.c_size_t()
+
+    def whole(n):
+        return (n + 7) // 8 * 8
+
+    def split(rows, columns, k):   # 64 x 64 tiles for half the 256 CUs or fewer, 8 stages of 64 k or more
+        tiles = -(-rows // 64) * -(-columns // 64)
+        return 4 * 2 * rows * whole(columns) if rows > 32 and tiles <= 128 and k >= 512 else 0
+
+    for rows in (1, 32, 33, 64, 513, 4104, 131072):
+        for k, hidden, n in ((1, 1, 1), (8, 8, 8), (300, 801, 300), (64, 4096, 72), (4096, 64, 4096), (768, 2048, 768)):
+            for weight in (2, 3):
+                shape = _shape(rows, k, hidden, n, k, weight=weight)
+                x = 2 * rows * whole(k) * (k % 8 != 0)
+                weights = 2 * (2 * hidden * whole(k) * (weight == 3 or k % 8 != 0)
+                               + n * whole(hidden) * (weight == 3 or hidden % 8 != 0))
+                h = 2 * rows * whole(hidden)
+                for training in (0, 1):
+                    assert library.lsso_hip_feed_forward_workspace_bytes(
+                        ctypes.byref(shape), training, ctypes.byref(size)) == 0
+                    assert size.value >= (x + weights + (0 if training else h) + (h if rows <= 32 else 0)
+                                          + split(rows, n, hidden)), (rows, k, hidden, n, weight, training)
+                partials = 4 * (2 * hidden * whole(k) + n * whole(hidden))
+                transposes = 2 * (2 * k * whole(hidden) + hidden * whole(n))
+                assert library.lsso_hip_feed_forward_backward_workspace_bytes(
+                    ctypes.byref(shape), n, 7, ctypes.byref(size)) == 0
+                assert size.value >= (x + 2 * rows * whole(n) * (n % 8 != 0) + 2 * h + partials + transposes
+                                      + split(rows, k, 2 * hidden)), (rows, k, hidden, n, weight)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("kind", ("silu", "gelu"))
