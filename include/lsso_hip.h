@@ -579,7 +579,10 @@ int lsso_hip_dropout_add(const void* x, const void* residual, int dtype, int64_t
 /* Gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T of rows of x.
  * dtype: LSSO_HIP_F16 or LSSO_HIP_BF16, of x, y and the kept values;
  * weight_type: dtype, or LSSO_HIP_F32, whose values are rounded to dtype once
- * per call.  x_stride: elements between rows of x (at least in_features). */
+ * per call.  x_stride: elements between rows of x (at least in_features).
+ * fine_factors: the two factors that a training forward keeps for its backward are
+ * rounded to dtype (0), or (1) FP32 values rounded to their upper 20 bits for BF16, 24
+ * for FP16. */
 typedef struct lsso_hip_feed_forward_shape {
     int64_t rows;
     int64_t in_features;
@@ -589,11 +592,13 @@ typedef struct lsso_hip_feed_forward_shape {
     int dtype;
     int weight_type;
     int activation;
+    int fine_factors;
 } lsso_hip_feed_forward_shape;
 
 /* 16-bit values of the buffers a training forward keeps for its backward:
- * gates [rows, 2, hidden rounded up to 8] and product [rows, hidden rounded up
- * to 8]. */
+ * gates [rows, 2, hidden rounded up to 8], with fine_factors and behind it [rows,
+ * hidden rounded up to 32] times one byte for BF16, two for FP16, and product [rows,
+ * hidden rounded up to 8]. */
 int lsso_hip_feed_forward_kept(const lsso_hip_feed_forward_shape* shape, size_t* gates,
                                size_t* product);
 

@@ -46,6 +46,7 @@ class FeedForwardShape(ctypes.Structure):
         ("dtype", ctypes.c_int),
         ("weight_type", ctypes.c_int),
         ("activation", ctypes.c_int),
+        ("fine_factors", ctypes.c_int),
     ]
 
 
@@ -370,7 +371,16 @@ def _aligned(value: torch.Tensor) -> torch.Tensor:
     return value if value.data_ptr() % 16 == 0 else value.clone()
 
 
-def _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation):
+def _feed_forward_kept(rows: int, hidden: int, dtype: torch.dtype, fine: bool) -> tuple[int, int]:
+    """Values of the kept gates, and a row of the kept product
+    (``lsso_hip_feed_forward_kept``)."""
+
+    pitch = (hidden + 7) // 8 * 8
+    lower = (hidden + 31) // 32 * (16 if dtype == torch.bfloat16 else 32) if fine else 0
+    return rows * (2 * pitch + lower), pitch
+
+
+def _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation, fine):
     """(rows of x, weights, their addresses, the shape's fields)."""
 
     hidden, in_features = gate_weight.shape
@@ -388,12 +398,12 @@ def _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation):
     rows = flat.shape[0]
     shape = (
         rows, in_features, hidden, down_weight.shape[0], flat.stride(0) if rows > 1 else in_features,
-        _HALF_CODES[x.dtype], _VALUE_CODES[gate_weight.dtype], activation,
+        _HALF_CODES[x.dtype], _VALUE_CODES[gate_weight.dtype], activation, int(fine),
     )
     return flat, weights, pointers, shape
 
 
-def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row_mask, training):
+def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row_mask, training, fine=False):
     """y, and with ``training`` the kept gates and product."""
 
     hip = _hip()
@@ -402,11 +412,13 @@ def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row
     mask_ptr = None
     if row_mask is not None:
         _mask, mask_ptr = _mask_pointer(row_mask, x.shape[:-1], device)
-    flat, _weights, pointers, shape = _feed_forward_inputs(x, gate_weight, up_weight, down_weight, activation)
+    flat, _weights, pointers, shape = _feed_forward_inputs(
+        x, gate_weight, up_weight, down_weight, activation, fine
+    )
     gates = product = None
     if training:
-        pitch = (shape[2] + 7) // 8 * 8
-        gates = torch.empty((shape[0], 2, pitch), dtype=x.dtype, device=device)
+        kept, pitch = _feed_forward_kept(shape[0], shape[2], x.dtype, fine)
+        gates = torch.empty(kept, dtype=x.dtype, device=device)
         product = torch.empty((shape[0], pitch), dtype=x.dtype, device=device)
     y = torch.empty((*x.shape[:-1], shape[3]), dtype=x.dtype, device=device)
     native, size = _feed_forward_plan(shape, training)
@@ -422,12 +434,13 @@ def _feed_forward_launch(x, gate_weight, up_weight, down_weight, activation, row
 
 class _FeedForward(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_weight, up_weight, down_weight, activation, row_mask):
+    def forward(ctx, x, gate_weight, up_weight, down_weight, activation, row_mask, fine):
         y, gates, product = _feed_forward_launch(
-            x, gate_weight, up_weight, down_weight, activation, row_mask, True
+            x, gate_weight, up_weight, down_weight, activation, row_mask, True, fine
         )
         ctx.save_for_backward(x, gate_weight, up_weight, down_weight, row_mask, gates, product)
         ctx.activation = activation
+        ctx.fine = fine
         ctx.like = tuple((tuple(v.shape), v.dtype) for v in (x, gate_weight, up_weight, down_weight))
         return y
 
@@ -441,10 +454,10 @@ class _FeedForward(torch.autograd.Function):
         for value, name, (shape, dtype) in zip((x, *weights), ("x", "gate_weight", "up_weight", "down_weight"), ctx.like):
             if value.device != device or value.dtype != dtype or tuple(value.shape) != shape:
                 _saved(value, name, dtype, shape, device)
-        flat, weights, pointers, shape = _feed_forward_inputs(x, *weights, ctx.activation)
+        flat, weights, pointers, shape = _feed_forward_inputs(x, *weights, ctx.activation, ctx.fine)
         rows, in_features, hidden, out_features = shape[:4]
-        pitch = (hidden + 7) // 8 * 8
-        gates = _aligned(_saved(gates, "gates", x.dtype, (rows, 2, pitch), device))
+        kept, pitch = _feed_forward_kept(rows, hidden, x.dtype, ctx.fine)
+        gates = _aligned(_saved(gates, "gates", x.dtype, (kept,), device))
         product = _aligned(_saved(product, "product", x.dtype, (rows, pitch), device))
         mask_ptr = None
         if row_mask is not None:
@@ -458,7 +471,7 @@ class _FeedForward(torch.autograd.Function):
             for need, (like, dtype) in zip(needs, ctx.like)
         ]
         if not any(needs):
-            return (None,) * 6
+            return (None,) * 7
         native, size = _feed_forward_backward_plan(
             shape, grad_stride, needs[1] + 2 * needs[2] + 4 * needs[3]
         )
@@ -469,7 +482,7 @@ class _FeedForward(torch.autograd.Function):
             *[None if grad is None else grad.data_ptr() for grad in grads], workspace.data_ptr(), size,
         )
         hip._check(status, library)
-        return (*grads, None, None)
+        return (*grads, None, None, None)
 
 
 def gated_feed_forward(
@@ -480,6 +493,7 @@ def gated_feed_forward(
     *,
     activation: str = "silu",
     row_mask: torch.Tensor | None = None,
+    fine_factors: bool = True,
 ) -> torch.Tensor:
     """Gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T.
 
@@ -491,10 +505,14 @@ def gated_feed_forward(
     whatever they hold.
 
     Products accumulate in FP32 from 16-bit operands; the product act(g) * u
-    and, for the backward, u * act'(g) and act(g) are rounded to x's type once
-    (so in float16 they must stay below 65,504); of up to 32 rows y's product
-    takes act(g) * u in two 16-bit parts.  Differentiable (first order) in x and
-    the weights, deterministically; the backward keeps 3 F values per row."""
+    is rounded to x's type once (so in float16 it must stay below 65,504); of up
+    to 32 rows y's product takes it in two 16-bit parts.  Differentiable (first
+    order) in x and the weights, deterministically.  For the backward u * act'(g)
+    and act(g) are kept: with ``fine_factors`` as FP32 values rounded to their
+    upper 20 bits for bfloat16 and 24 for float16 (7 F and 8 F bytes per row with
+    the product), else rounded to x's type (6 F bytes; in float16 they must then
+    stay below 65,504 too, and gradients of both types are off by sqrt(3) instead
+    of sqrt(2) roundings of their own)."""
 
     hip = _hip()
     hip.require_available()
@@ -524,7 +542,7 @@ def gated_feed_forward(
     for name, value in zip(("gate_weight", "up_weight", "down_weight"), weights):
         _on_device(value, name, x.device)
     if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights)):
-        return _FeedForward.apply(x, *weights, kind, row_mask)
+        return _FeedForward.apply(x, *weights, kind, row_mask, bool(fine_factors))
     return _feed_forward_launch(x, *weights, kind, row_mask, False)[0]
 
 

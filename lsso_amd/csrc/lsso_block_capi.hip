@@ -40,6 +40,10 @@ int check_embedding(const void* tokens, int token_bytes, int64_t count, int64_t 
 
 size_t round256(size_t bytes) { return (bytes + 255) & ~static_cast<size_t>(255); }
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+// Bytes per row of what fine factors keep beside their upper 16 bits.
+int64_t lower_pitch(const lsso_hip_feed_forward_shape& s) {
+    return (s.hidden + 31) / 32 * (s.dtype == LSSO_HIP_BF16 ? 32 : 64);
+}
 
 // Rows whose pieces the product's loads can address: 16-byte pieces, and 256
 // rows within a buffer's 2^31 bytes.
@@ -67,6 +71,9 @@ int check_feed_forward(const lsso_hip_feed_forward_shape* s) {
     }
     if (s->activation != LSSO_HIP_SILU && s->activation != LSSO_HIP_GELU) {
         return report(LSSO_HIP_EUNSUPPORTED, "activation must be LSSO_HIP_SILU or LSSO_HIP_GELU");
+    }
+    if (s->fine_factors != 0 && s->fine_factors != 1) {
+        return report(LSSO_HIP_EINVAL, "fine_factors must be 0 or 1");
     }
     if (s->x_stride < s->in_features) {
         return report(LSSO_HIP_EINVAL, "x_stride must be at least in_features");
@@ -140,6 +147,15 @@ void common_args(const lsso_hip_feed_forward_shape& s, lsso_hip::FeedForwardArgs
     a->in_pitch = round8(s.in_features);
     a->pitch = round8(s.hidden);
     a->out_pitch = round8(s.out_features);
+    a->lower_pitch = lower_pitch(s);
+}
+
+// The kept factors: 16 bits of each, and behind all of them the rest of fine ones.
+void bind_gates(const lsso_hip_feed_forward_shape& s, void* gates, lsso_hip::FeedForwardArgs* a) {
+    a->gates = static_cast<uint16_t*>(gates);
+    if (gates != nullptr && s.fine_factors != 0) {
+        a->gates_lower = reinterpret_cast<char*>(a->gates + 2 * s.rows * a->pitch);
+    }
 }
 
 int64_t stages_of(int64_t k) { return (k + 63) / 64; }
@@ -235,6 +251,9 @@ int lsso_hip_feed_forward_kept(const lsso_hip_feed_forward_shape* shape, size_t*
     }
     *product = static_cast<size_t>(shape->rows) * static_cast<size_t>(round8(shape->hidden));
     *gates = 2 * *product;
+    if (shape->fine_factors != 0) {
+        *gates += static_cast<size_t>(shape->rows) * static_cast<size_t>(lower_pitch(*shape) / 2);
+    }
     return LSSO_HIP_OK;
 }
 
@@ -285,7 +304,7 @@ int lsso_hip_feed_forward(const lsso_hip_feed_forward_shape* shape, const void* 
     a.up = bind(&l.plan, l.up, up_weight, s.hidden, s.in_features, s.in_features, wide, ws);
     a.down = bind(&l.plan, l.down, down_weight, s.out_features, s.hidden, s.hidden, wide, ws);
     a.row_mask = row_mask;
-    a.gates = static_cast<uint16_t*>(gates);
+    bind_gates(s, gates, &a);
     a.h = product != nullptr ? static_cast<uint16_t*>(product) : reinterpret_cast<uint16_t*>(ws + l.h);
     const bool few = s.rows <= lsso_hip::kFewRows;
     a.h_low = few ? reinterpret_cast<uint16_t*>(ws + l.h_low) : nullptr;
@@ -366,7 +385,7 @@ int lsso_hip_feed_forward_backward(const lsso_hip_feed_forward_shape* shape, con
     a.dy = bind(&l.plan, l.dy, grad_y, s.rows, s.out_features, grad_stride, false, ws);
     a.dy_stride = l.dy.stride;
     a.row_mask = row_mask;
-    a.gates = static_cast<uint16_t*>(const_cast<void*>(gates));
+    bind_gates(s, const_cast<void*>(gates), &a);
     a.grads = reinterpret_cast<uint16_t*>(ws + l.grads);
     uint16_t* const in_columns = reinterpret_cast<uint16_t*>(ws + l.in_columns);
     uint16_t* const down_columns = reinterpret_cast<uint16_t*>(ws + l.down_columns);

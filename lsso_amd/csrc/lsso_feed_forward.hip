@@ -3,10 +3,11 @@
 //
 //   gate_kernel    g, u = x Wg^T, x Wu^T in one pass over x; h = act(g) u from
 //                  the FP32 accumulators.  Training also keeps the two factors
-//                  of the backward, u act'(g) and act(g): rounded once, where
-//                  kept g and u would be rounded before them (gradients off by
-//                  sqrt(3) instead of 1.85 output roundings), and the backward
-//                  evaluates no activation.
+//                  of the backward, u act'(g) and act(g), fine or rounded to
+//                  16 bits, so that the backward evaluates no activation.  From
+//                  fine ones gradients are off by sqrt(2) output roundings (dg
+//                  or du, and the output), from 16-bit ones by sqrt(3), and
+//                  from kept 16-bit g and u they would be by 1.85.
 //   product_kernel y = h Wd^T, and in the backward dx = dg Wg + du Wu
 //   grad_kernel    dh = dy Wd, and from it dg = dh (u act'(g)), du = dh act(g)
 //   weight_kernel  dWg = dg^T x, dWu = du^T x, dWd = dy^T h in one launch,
@@ -17,7 +18,13 @@
 // which are rounded once when they are stored, because the products that take
 // them run on 16-bit matrix instructions.  The kept factors lie as [rows, 2, Fp],
 // as do dg and du, and h as [rows, Fp], Fp the hidden width rounded up to 8 with
-// zeros behind it, so every row is whole 16-byte pieces.  Operands whose own rows are not (odd
+// zeros behind it, so every row is whole 16-byte pieces.  Fine factors are the
+// upper bits of the FP32 value, so with its range: 20 beside BF16, 24 beside FP16, whose
+// roundings are then at most a sixteenth of the type's.  Their first 16 bits lie where
+// 16-bit factors do, the rest behind all of them: per column a byte of four bits of
+// either, or by 8 columns 8 bytes of either.  131,072 x 256 -> 688: gate kernel 234 us
+// instead of 199, gradient kernel 265 instead of 226; 8,192 x 768 -> 2,048: 71 instead of
+// 64, 64 instead of 57.  Operands whose own rows are not (odd
 // widths or strides) are copied into such rows first: element loads in the
 // product's loop cost more than one more pass over x.
 //
@@ -35,6 +42,66 @@
 namespace lsso_hip {
 
 namespace {
+
+// Fine factors: FP32 values rounded to their upper bits (round), of which the first 16 of
+// two are `upper`, and the rest of four columns' first and second factors `lower`.
+template <int T>
+struct Fine {
+    static constexpr int kLowerBytes = T == LSSO_HIP_BF16 ? 1 : 2;   // per column, of both factors
+    __device__ static __forceinline__ float round(float v) {
+        return __uint_as_float(__float_as_uint(v) + (T == LSSO_HIP_BF16 ? 0x800u : 0x80u));
+    }
+    __device__ static __forceinline__ uint32_t upper(float a, float b) {
+        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    // The third bytes of four values.
+    __device__ static __forceinline__ uint32_t third(const float (&v)[4]) {
+        return __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501u) |
+               __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x05010c0cu);
+    }
+    // BF16: of both factors of four columns in one word.
+    __device__ static __forceinline__ uint32_t lower(const float (&first)[4], const float (&second)[4]) {
+        return (third(first) >> 4 & 0x0f0f0f0fu) | (third(second) & 0xf0f0f0f0u);
+    }
+    // Eight columns of one factor from their upper and third bytes.
+    __device__ static __forceinline__ void join(const u32x4& upper, uint32_t third0, uint32_t third1, float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t select = ((e & 1) != 0 ? 0x0706000cu : 0x0504000cu) | static_cast<uint32_t>(e & 3) << 8;
+            v[e] = __uint_as_float(__builtin_amdgcn_perm(upper[e / 2], e < 4 ? third0 : third1, select));
+        }
+    }
+    // Of eight columns: both factors from their upper bits and what `lower` points to.
+    struct Lower {
+        uint32_t word[T == LSSO_HIP_BF16 ? 2 : 4];
+        __device__ __forceinline__ void load(const char* at) {
+            if constexpr (T == LSSO_HIP_BF16) {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(at);
+                word[0] = v[0];
+                word[1] = v[1];
+            } else {
+                const u32x4 v = load16_unaligned(at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    word[i] = v[i];
+                }
+            }
+        }
+        __device__ __forceinline__ void join(const u32x4& upper0, const u32x4& upper1, float (&first)[8],
+                                             float (&second)[8]) const {
+            if constexpr (T == LSSO_HIP_BF16) {
+                Fine::join(upper0, word[0] << 4 & 0xf0f0f0f0u, word[1] << 4 & 0xf0f0f0f0u, first);
+                Fine::join(upper1, word[0] & 0xf0f0f0f0u, word[1] & 0xf0f0f0f0u, second);
+            } else {
+                Fine::join(upper0, word[0], word[1], first);
+                Fine::join(upper1, word[2], word[3], second);
+            }
+        }
+    };
+};
+
+// What is kept for the backward.
+enum class Keep { kNothing, kRounded, kFine };
 
 // act(g), and with SLOPE act'(g), FP32.  SiLU: g / (1 + exp(-g)); an exponential
 // that overflows leaves a sigmoid of 0.  GELU: g Phi(g), Phi(-|g|) = tail =
@@ -206,69 +273,108 @@ __device__ __forceinline__ void store_partials(char* mine, int lane, const f32x1
 // Q is [gate rows | up rows] of the tile's columns of h, and a wave takes the
 // same columns of both, so that a lane holds both factors of its products: block
 // n < NB / 2 the gate's, n + NB / 2 the up's.  A wave's 32 rows at a time go
-// through the exchange as 16-bit rows of its columns, h, then the factors.
-template <int T, int MB, int NB, bool KEEP>
+// through the exchange as rows of its columns: h, the factors' 16 bits one after the
+// other, then what more of both is kept.  The factors wait for their turn in the
+// accumulators that they come from.
+
+// A pass of the exchange to memory: rows of BYTES from byte `first` of `to`'s on,
+// `pitch` bytes apart, up to byte `end`.
+template <int BYTES>
+__device__ __forceinline__ void store_exchange(const char* mine, int lane, char* to, int64_t pitch, int64_t row0,
+                                               int64_t rows, int64_t first, int64_t end) {
+    using Exchange = RowExchange<BYTES>;
+    wave_lds_order();
+    const int64_t piece = first + Exchange::byte(lane);
+#pragma unroll
+    for (int i = 0; i < Exchange::kSteps; ++i) {
+        const u32x4 value = Exchange::get(mine, lane, i);
+        const int64_t row = row0 + Exchange::row(lane, i);
+        if (row < rows && piece < end) {
+            store16_unaligned(to + row * pitch + piece, value);
+        }
+    }
+    wave_lds_order();
+}
+
+template <int T, int MB, int NB, Keep KEEP>
 __device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
-                                              const f32x16 (&acc)[NB][MB]) {
+                                              f32x16 (&acc)[NB][MB]) {
     using Exchange = RowExchange<32 * NB>;
-    const int64_t column = q0 + Exchange::byte(lane) / 2;
-    const int half = lane >> 5;
+    constexpr bool kFine = KEEP == Keep::kFine;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
         const int64_t row0 = p0 + 32 * m;
         const int64_t row = row0 + (lane & 31);
         const bool kept = row < a.rows && (a.row_mask == nullptr || a.row_mask[row] != 0);
-        u32x2 factors[KEEP ? 2 : 1][NB / 2][4];
+        // Opaque where there are more passes: else the addresses of all are held at once.
+        int here = KEEP == Keep::kNothing ? lane : opaque_int(lane);
 #pragma unroll
         for (int n = 0; n < NB / 2; ++n) {
+            f32x16& gate = acc[n][m];
+            f32x16& up = acc[n + NB / 2][m];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float h[4];
-                float first[4];
-                float second[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float act, slope;
-                    activation<KEEP>(a.activation, acc[n][m][4 * q + e], act, slope);
-                    const float u = acc[n + NB / 2][m][4 * q + e];
-                    h[e] = act * u;
-                    first[e] = slope * u;
-                    second[e] = act;
+                    activation<KEEP != Keep::kNothing>(a.activation, gate[4 * q + e], act, slope);
+                    h[e] = act * up[4 * q + e];
+                    if (KEEP != Keep::kNothing) {
+                        slope *= up[4 * q + e];
+                        gate[4 * q + e] = kFine ? Fine<T>::round(slope) : slope;
+                        up[4 * q + e] = kFine ? Fine<T>::round(act) : act;
+                    }
                 }
-                Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half,
+                Exchange::put(mine, here, 64 * n + 16 * q + 8 * (here >> 5),
                               (u32x2){kept ? Values<T>::pack(h[0], h[1]) : 0u, kept ? Values<T>::pack(h[2], h[3]) : 0u});
-                if constexpr (KEEP) {
-                    factors[0][n][q] = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
-                    factors[1][n][q] =
-                        (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])};
-                }
             }
         }
+        store_exchange<32 * NB>(mine, here, reinterpret_cast<char*>(a.h), 2 * a.pitch, row0, a.rows, 2 * q0, 2 * a.pitch);
 #pragma unroll
-        for (int o = 0; o < (KEEP ? 3 : 1); ++o) {
-            if constexpr (KEEP) {
-                if (o > 0) {
+        for (int o = 0; o < (KEEP != Keep::kNothing ? 2 : 0); ++o) {
+            here = opaque_int(lane);
 #pragma unroll
-                    for (int n = 0; n < NB / 2; ++n) {
+            for (int n = 0; n < NB / 2; ++n) {
+                const f32x16& v = acc[n + o * (NB / 2)][m];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            Exchange::put(mine, lane, 64 * n + 16 * q + 8 * half, factors[o - 1][n][q]);
-                        }
+                for (int q = 0; q < 4; ++q) {
+                    Exchange::put(mine, here, 64 * n + 16 * q + 8 * (here >> 5),
+                                  kFine ? (u32x2){Fine<T>::upper(v[4 * q], v[4 * q + 1]),
+                                                  Fine<T>::upper(v[4 * q + 2], v[4 * q + 3])}
+                                        : (u32x2){Values<T>::pack(v[4 * q], v[4 * q + 1]),
+                                                  Values<T>::pack(v[4 * q + 2], v[4 * q + 3])});
+                }
+            }
+            store_exchange<32 * NB>(mine, here, reinterpret_cast<char*>(a.gates + o * a.pitch), 4 * a.pitch, row0,
+                                    a.rows, 2 * q0, 2 * a.pitch);
+        }
+        if constexpr (kFine) {
+            constexpr int kBytes = Fine<T>::kLowerBytes;
+            using LowerExchange = RowExchange<16 * NB * kBytes>;
+            here = opaque_int(lane);
+#pragma unroll
+            for (int n = 0; n < NB / 2; ++n) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float first[4];
+                    float second[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        first[e] = acc[n][m][4 * q + e];
+                        second[e] = acc[n + NB / 2][m][4 * q + e];
+                    }
+                    const int byte = kBytes * (32 * n + 8 * q) + 4 * (here >> 5);
+                    if constexpr (T == LSSO_HIP_BF16) {
+                        LowerExchange::put(mine, here, byte, Fine<T>::lower(first, second));
+                    } else {
+                        LowerExchange::put(mine, here, byte, Fine<T>::third(first));
+                        LowerExchange::put(mine, here, byte + 8, Fine<T>::third(second));
                     }
                 }
             }
-            wave_lds_order();
-            uint16_t* const out = o == 0 ? a.h : a.gates + (o - 1) * a.pitch;
-            const int64_t pitch = o == 0 ? a.pitch : 2 * a.pitch;
-#pragma unroll
-            for (int i = 0; i < Exchange::kSteps; ++i) {
-                const u32x4 value = Exchange::get(mine, lane, i);
-                const int64_t to = row0 + Exchange::row(lane, i);
-                if (to < a.rows && column < a.pitch) {
-                    store16_unaligned(out + to * pitch + column, value);
-                }
-            }
-            wave_lds_order();
+            store_exchange<16 * NB * kBytes>(mine, here, a.gates_lower, a.lower_pitch, row0, a.rows, kBytes * q0,
+                                             a.lower_pitch);
         }
     }
 }
@@ -281,7 +387,7 @@ __device__ __forceinline__ void gate_epilogue(const FeedForwardArgs& a, char* mi
 template <int T, int MB, int NB, int WP, int WQ>
 using GateShape = RowsShape<T, MB, NB, WP, WQ, RowExchange<32 * NB>::kSize>;
 
-template <int T, int MB, int NB, int WP, int WQ, bool KEEP>
+template <int T, int MB, int NB, int WP, int WQ, Keep KEEP>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void gate_kernel(FeedForwardArgs a) {
     using S = GateShape<T, MB, NB, WP, WQ>;
     using P = typename S::PStage;
@@ -330,7 +436,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gate_kernel(FeedForwardArgs a
             }
         },
         [&](int n) { return n < NB / 2 ? wave_column + 32 * n : kColumns + wave_column + 32 * (n - NB / 2); },
-        [&](const f32x16 (&acc)[NB][MB]) {
+        [&](f32x16 (&acc)[NB][MB]) {
             gate_epilogue<T, MB, NB, KEEP>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
                                            static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
                                            static_cast<int64_t>(walk.q) * kColumns + wave_column, acc);
@@ -508,7 +614,7 @@ __device__ __forceinline__ void few_rows_product(const FewLoads (&q)[NQ], const 
     }
 }
 
-template <int T, int RT, bool KEEP>
+template <int T, int RT, Keep KEEP>
 __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArgs a) {
     const int lane = threadIdx.x & 63;
     const int wave = wave_index();
@@ -536,10 +642,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float act, slope;
-        activation<KEEP>(a.activation, total[0][e], act, slope);
+        activation<KEEP != Keep::kNothing>(a.activation, total[0][e], act, slope);
         h[e] = kept ? act * total[1][e] : 0.0f;
-        first[e] = slope * total[1][e];
-        second[e] = act;
+        first[e] = KEEP == Keep::kFine ? Fine<T>::round(slope * total[1][e]) : slope * total[1][e];
+        second[e] = KEEP == Keep::kFine ? Fine<T>::round(act) : act;
     }
     const u32x2 rounded = {Values<T>::pack(h[0], h[1]), Values<T>::pack(h[2], h[3])};
     *reinterpret_cast<u32x2*>(a.h + row * a.pitch + column) = rounded;
@@ -548,11 +654,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_kernel(FeedForwardArg
     *reinterpret_cast<u32x2*>(a.h_low + row * a.pitch + column) =
         (u32x2){Values<T>::pack(left(h[0], Values<T>::low(rounded[0])), left(h[1], Values<T>::high(rounded[0]))),
                 Values<T>::pack(left(h[2], Values<T>::low(rounded[1])), left(h[3], Values<T>::high(rounded[1])))};
-    if (KEEP) {
+    if constexpr (KEEP == Keep::kRounded) {
         uint16_t* at = a.gates + 2 * row * a.pitch + column;
         *reinterpret_cast<u32x2*>(at) = (u32x2){Values<T>::pack(first[0], first[1]), Values<T>::pack(first[2], first[3])};
         *reinterpret_cast<u32x2*>(at + a.pitch) =
             (u32x2){Values<T>::pack(second[0], second[1]), Values<T>::pack(second[2], second[3])};
+    }
+    if constexpr (KEEP == Keep::kFine) {
+        using F = Fine<T>;
+        uint16_t* at = a.gates + 2 * row * a.pitch + column;
+        *reinterpret_cast<u32x2*>(at) = (u32x2){F::upper(first[0], first[1]), F::upper(first[2], first[3])};
+        *reinterpret_cast<u32x2*>(at + a.pitch) = (u32x2){F::upper(second[0], second[1]), F::upper(second[2], second[3])};
+        char* lower = a.gates_lower + row * a.lower_pitch + F::kLowerBytes * (column / 8 * 8) + column % 8;
+        if constexpr (T == LSSO_HIP_BF16) {
+            *reinterpret_cast<uint32_t*>(lower) = F::lower(first, second);
+        } else {
+            *reinterpret_cast<uint32_t*>(lower) = F::third(first);
+            *reinterpret_cast<uint32_t*>(lower + 8) = F::third(second);
+        }
     }
 }
 
@@ -594,7 +713,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_product_kernel(FeedForward
 // ----------------------------------------------------------------- dg and du
 // dh goes through the exchange in FP32, 32 rows x 32 columns at a time: in its
 // rows the factors are read and dg, du written as whole pieces.
-template <int T, int MB, int NB>
+template <int T, int MB, int NB, bool FINE>
 __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mine, int lane, int64_t p0, int64_t q0,
                                               const f32x16 (&acc)[NB][MB]) {
     using Exchange = RowExchange<128>;
@@ -609,6 +728,7 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
         for (int n = 0; n < NB; ++n) {
             const int64_t column = q0 + 32 * n + 8 * (lane % kLanes);
             u32x4 raw[kSteps][2];
+            typename Fine<T>::Lower lower[FINE ? kSteps : 1];
             bool kept[kSteps];
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
@@ -617,6 +737,9 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
                     const uint16_t* at = a.gates + 2 * row * a.pitch + column;
                     raw[i][0] = load16_unaligned(at);
                     raw[i][1] = load16_unaligned(at + a.pitch);
+                    if constexpr (FINE) {
+                        lower[i].load(a.gates_lower + row * a.lower_pitch + Fine<T>::kLowerBytes * column);
+                    }
                     kept[i] = a.row_mask == nullptr || a.row_mask[row] != 0;
                 }
             }
@@ -636,8 +759,12 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
                 if (row < a.rows && column < a.pitch) {
                     float dg[8];
                     float du[8];
-                    Values<T>::unpack8(raw[i][0], dg);
-                    Values<T>::unpack8(raw[i][1], du);
+                    if constexpr (FINE) {
+                        lower[i].join(raw[i][0], raw[i][1], dg, du);
+                    } else {
+                        Values<T>::unpack8(raw[i][0], dg);
+                        Values<T>::unpack8(raw[i][1], du);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float dh = e < 4 ? low[e & 3] : high[e & 3];
@@ -657,7 +784,7 @@ __device__ __forceinline__ void grad_epilogue(const FeedForwardArgs& a, char* mi
 template <int T, int MB, int NB, int WP, int WQ>
 using GradShape = RowsShape<T, MB, NB, WP, WQ, RowExchange<128>::kSize>;
 
-template <int T, int MB, int NB, int WP, int WQ>
+template <int T, int MB, int NB, int WP, int WQ, bool FINE>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void grad_kernel(FeedForwardArgs a) {
     using S = GradShape<T, MB, NB, WP, WQ>;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
@@ -673,9 +800,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grad_kernel(FeedForwardArgs a
         lds, walk.left, a.stages, [&](char* to, int j) { stream.issue(to, j); },
         [&](int n) { return S::wave_q(wave) + 32 * n; },
         [&](const f32x16 (&acc)[NB][MB]) {
-            grad_epilogue<T, MB, NB>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
-                                     static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
-                                     static_cast<int64_t>(walk.q) * S::BQ + S::wave_q(wave), acc);
+            grad_epilogue<T, MB, NB, FINE>(a, lds + S::kRingBytes + S::kWaveBytes * wave, lane,
+                                           static_cast<int64_t>(walk.p) * S::BP + S::wave_p(wave),
+                                           static_cast<int64_t>(walk.q) * S::BQ + S::wave_q(wave), acc);
             walk.next();
         });
 }
@@ -885,7 +1012,7 @@ dim3 tile_grid(int tiles, int slots, int splits = 1) {
     return dim3(static_cast<unsigned>(8 * (per_xcd < slots ? per_xcd : slots)), static_cast<unsigned>(splits));
 }
 
-template <int T, int MB, int NB, int WP, int WQ, bool KEEP>
+template <int T, int MB, int NB, int WP, int WQ, Keep KEEP>
 hipError_t launch_gate(FeedForwardArgs a, hipStream_t stream) {
     using S = GateShape<T, MB, NB, WP, WQ>;
     a.stages = static_cast<int>((a.in_pitch + kRowsStageK - 1) / kRowsStageK);
@@ -895,8 +1022,8 @@ hipError_t launch_gate(FeedForwardArgs a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int T, bool KEEP>
-hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
+template <int T, Keep KEEP>
+hipError_t launch_tiles_gate(const FeedForwardArgs& a, hipStream_t stream) {
     switch (choose_edge(a.rows, 2 * a.pitch, 128, 2 * kCus)) {
         case Edge::kLarge: return launch_gate<T, 2, 4, 4, 2, KEEP>(a, stream);
         case Edge::kMiddle: return launch_gate<T, 2, 2, 2, 2, KEEP>(a, stream);
@@ -904,7 +1031,7 @@ hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
     }
 }
 
-template <int T, bool KEEP>
+template <int T, Keep KEEP>
 hipError_t launch_few_gate(const FeedForwardArgs& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((a.pitch + 15) / 16));
     if (a.rows <= 16) {
@@ -915,12 +1042,17 @@ hipError_t launch_few_gate(const FeedForwardArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int T, Keep KEEP>
+hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
+    return a.rows <= kFewRows ? launch_few_gate<T, KEEP>(a, stream) : launch_tiles_gate<T, KEEP>(a, stream);
+}
+
 template <int T>
 hipError_t launch_gate(const FeedForwardArgs& a, hipStream_t stream) {
-    if (a.rows <= kFewRows) {
-        return a.gates != nullptr ? launch_few_gate<T, true>(a, stream) : launch_few_gate<T, false>(a, stream);
+    if (a.gates == nullptr) {
+        return launch_gate<T, Keep::kNothing>(a, stream);
     }
-    return a.gates != nullptr ? launch_gate<T, true>(a, stream) : launch_gate<T, false>(a, stream);
+    return a.gates_lower != nullptr ? launch_gate<T, Keep::kFine>(a, stream) : launch_gate<T, Keep::kRounded>(a, stream);
 }
 
 template <int T, int MB, int NB, int WP, int WQ>
@@ -978,7 +1110,11 @@ hipError_t launch_grad(FeedForwardArgs a, hipStream_t stream) {
     a.stages = static_cast<int>((a.out_pitch + kRowsStageK - 1) / kRowsStageK);
     a.q_tiles = static_cast<int>((a.pitch + S::BQ - 1) / S::BQ);
     a.tiles = a.q_tiles * static_cast<int>((a.rows + S::BP - 1) / S::BP);
-    grad_kernel<T, MB, NB, WP, WQ><<<tile_grid(a.tiles, S::kSlots), S::kThreads, 0, stream>>>(a);
+    if (a.gates_lower != nullptr) {
+        grad_kernel<T, MB, NB, WP, WQ, true><<<tile_grid(a.tiles, S::kSlots), S::kThreads, 0, stream>>>(a);
+    } else {
+        grad_kernel<T, MB, NB, WP, WQ, false><<<tile_grid(a.tiles, S::kSlots), S::kThreads, 0, stream>>>(a);
+    }
     return hipGetLastError();
 }
 

@@ -361,7 +361,9 @@ struct FeedForwardArgs {
     const uint8_t* row_mask;    // [rows] or nullptr
     uint16_t* h;                // [rows, pitch]
     uint16_t* h_low;            // what rounding h left, of up to kFewRows rows
-    uint16_t* gates;            // [rows, 2, pitch]: u act'(g), act(g); or nullptr
+    uint16_t* gates;            // [rows, 2, pitch]: u act'(g), act(g), or their upper 16 bits; or nullptr
+    char* gates_lower;          // [rows, lower_pitch]: the other bits of fine factors; or nullptr
+    int64_t lower_pitch;
     const uint16_t* dy;         // [rows, out_pitch], row stride dy_stride
     int64_t dy_stride;
     uint16_t* grads;            // [rows, 2, pitch]: dg, du

@@ -417,7 +417,7 @@ __device__ __forceinline__ void run_rows_tiles(char* lds, int tiles, int stages,
     stage_barrier<0>();
 }
 
-// A wave's exchange of 32 rows of BYTES (64 or 128) through its own part of LDS,
+// A wave's exchange of 32 rows of BYTES (32, 64 or 128) through its own part of LDS,
 // from a lane per row to BYTES / 16 consecutive lanes per row: stored from the
 // accumulators' layout, an instruction covers 32 bytes of each of 32 rows, and
 // partly written lines cost the memory side twice (131,072 x 688 x 3 stores at
@@ -430,9 +430,11 @@ struct RowExchange {
     static constexpr int kRows = 64 / kLanes;        // per access
     static constexpr int kSteps = 32 / kRows;
     __device__ static __forceinline__ int swizzle(int row) {
-        return BYTES == 128 ? (row & 7) ^ ((row >> 3) & 1) : ((row >> 1) & 3) ^ ((row >> 3) & 1);
+        return BYTES == 128  ? (row & 7) ^ ((row >> 3) & 1)
+               : BYTES == 64 ? ((row >> 1) & 3) ^ ((row >> 3) & 1)
+                             : ((row >> 2) & 1) ^ ((row >> 3) & 1);
     }
-    // V: 8 or 16 bytes at `byte` of row lane % 32.
+    // V: 4, 8 or 16 bytes at `byte` of row lane % 32.
     template <typename V>
     __device__ static __forceinline__ void put(char* lds, int lane, int byte, const V& value) {
         const int r = lane & 31;

@@ -234,6 +234,24 @@ def test_workspaces_hold_every_size() -> None:
                 assert size.value >= 4 * rows * hidden
 
 
+def test_kept_factors_on_the_cpu() -> None:
+    library = hip.open_library()
+    gates, product = ctypes.c_size_t(), ctypes.c_size_t()
+    for rows, hidden, pitch, wide in ((4, 25, 32, 32), (3, 32, 32, 32), (7, 33, 40, 64), (1, 801, 808, 832)):
+        for code, dtype in ((1, torch.float16), (2, torch.bfloat16)):
+            for fine in (0, 1):
+                shape = block.FeedForwardShape(rows, 16, hidden, 16, 16, code, code, 1, fine)
+                assert library.lsso_hip_feed_forward_kept(
+                    ctypes.byref(shape), ctypes.byref(gates), ctypes.byref(product)) == 0
+                # 16-bit values: two factors, and a byte or two more of both per column, by 32 columns
+                assert gates.value == rows * (2 * pitch + fine * wide // code)
+                assert product.value == rows * pitch
+                assert block._feed_forward_kept(rows, hidden, dtype, bool(fine)) == (gates.value, pitch)
+    for fine in (-1, 2, 24):
+        shape = block.FeedForwardShape(4, 16, 24, 16, 16, 2, 2, 1, fine)
+        assert library.lsso_hip_feed_forward_kept(ctypes.byref(shape), ctypes.byref(gates), ctypes.byref(product)) < 0
+
+
 def test_workspaces_hold_every_buffer() -> None:
     """The sum of all that a call keeps beside each other: copies of operands with
     odd rows or of float32, h (its second part of few rows), dg and du, both
@@ -299,6 +317,74 @@ def test_float32_weights(native, widths, dtype) -> None:
                                              (20000, 64, 2112, 64), (40000, 72, 520, 264), (66000, 32, 64, 264)])
 def test_large_tiles_and_row_ranges(native, rows, k, hidden, n) -> None:
     _check(native, rows, k, hidden, n, torch.bfloat16, "gelu")
+
+
+def _step(native, x, weights, dy, kind, fine, mask=None):
+    leaves = [v.detach().requires_grad_() for v in (x, *weights)]
+    y = native.gated_feed_forward(*leaves, activation=kind, row_mask=mask, fine_factors=fine)
+    return dict(zip(("y", "x", "gate", "up", "down"), (y.detach(), *torch.autograd.grad(y, leaves, dy))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows,k,hidden,n", [(1, 64, 136, 48), (17, 33, 65, 31), (32, 96, 1000, 24), (33, 64, 136, 48),
+                                             (70, 7, 9, 3), (200, 300, 801, 300), (4104, 128, 264, 128),
+                                             (8000, 72, 2048, 520), (12000, 64, 264, 64)])
+def test_rounded_factors(native, rows, k, hidden, n, dtype) -> None:
+    """The same value and, to the roundings of the factors, gradients."""
+
+    x, weights, dy = _inputs(rows, k, hidden, n, dtype, dtype)
+    mask = torch.rand(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) < 0.8
+    got = _step(native, x, weights, dy, "gelu", False, mask)
+    _verify(got, _expected(x, weights, dy, "gelu", dtype, dtype, mask))
+    wide = _step(native, x, weights, dy, "gelu", True, mask)
+    assert torch.equal(got["y"], wide["y"]) and torch.equal(got["down"], wide["down"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("kind", ("silu", "gelu"))
+@pytest.mark.parametrize("rows,hidden", [(16, 40), (32, 33), (48, 136), (130, 801), (4100, 264), (9000, 520)])
+def test_fine_factors(native, dtype, kind, rows, hidden) -> None:
+    """dg and du of single products: x has at most one 1 in a row or a column, so
+    that dWu is act(g) dh of that row.  Then the factor's rounding (half a step of 12
+    bits, 2^-12, for bfloat16 and of 16, 2^-16, for float16), dg's or du's and the
+    output's are all that there is, beside act's and act''s own |g| 2^-22 and (1 + |g|)
+    2^-21.  The second rounding of a value of the type changes nothing."""
+
+    size = min(rows, 520)
+    generator = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.zeros(rows, size, device="cuda", dtype=dtype)
+    chosen = torch.randperm(rows, device="cuda", generator=generator)[:size]
+    x[chosen, torch.arange(size, device="cuda")] = 1
+    gate, up = (torch.randn(hidden, size, device="cuda", generator=generator).to(dtype) for _ in range(2))
+    down = torch.randn(1, hidden, device="cuda", generator=generator).to(dtype)
+    dy = torch.ones(rows, 1, device="cuda", dtype=dtype)
+    got = _step(native, x, (gate, up, down), dy, kind, True)
+    g, u, dh = gate.double(), up.double(), down.double().t()
+    act, slope = _act(g, kind)
+    e, f = torch.finfo(dtype).eps / 2, 2.0**-16 if dtype == torch.float16 else 2.0**-12
+    tiny = 2.0**-25 if dtype == torch.float16 else 2.0**-134
+    for name, value, error in (("up", act * dh, g.abs() * 2.0**-22 * dh.abs()),
+                               ("gate", u * slope * dh, (1 + g.abs()) * 2.0**-21 * (u * dh).abs())):
+        bound = (e + f) * value.abs() + error + tiny
+        assert ((got[name].double() - value).abs() <= 1.02 * bound).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", (16, 48))
+def test_factors_past_the_range_of_float16(native, rows) -> None:
+    """u act'(g) of 95,000 times 0.74: kept of 24 bits, with FP32's range."""
+
+    x = torch.eye(16, device="cuda").half().repeat(rows // 16, 1) * 200
+    gate, up = (torch.eye(16, device="cuda") * value for value in (0.0025, 475.0))
+    down, dy = torch.eye(16, device="cuda"), torch.full((rows, 16), 2.0**-10, device="cuda").half()
+    got = _step(native, x, [w.half() for w in (gate, up, down)], dy, "silu", True)
+    g, u = 200 * gate.half().double(), 95000.0
+    value = _act(g, "silu")[1] * u * 2.0**-10 * 200 * (rows // 16)
+    found = torch.diagonal(got["gate"]).double()
+    assert ((found - torch.diagonal(value)).abs() <= 2.0**-9 * torch.diagonal(value)).all()
+    assert not torch.isfinite(_step(native, x, [w.half() for w in (gate, up, down)], dy, "silu", False)["gate"]).all()
 
 
 @pytest.mark.gpu
