@@ -12,8 +12,8 @@
 //
 // Bound: HBM.  Forward 3, backward 2 streams of the tensor.  A thread takes one
 // block's 8 elements per step, 16 bytes of each 16-bit operand.  262,144 x 256 BF16:
-// forward 73 us (5.5 TB/s), backward 44 us (6.1 TB/s), a large copy's rate; the
-// generator's 20 products of 32 x 32 bits per thread hide under the loads.
+// forward 73 us (5.5 TB/s), backward 44 us (6.1 TB/s), where a large copy reaches 6.6;
+// the generator's 20 products of 32 x 32 bits per thread hide under the loads.
 
 #include "lsso_device.h"
 #include "lsso_internal.h"

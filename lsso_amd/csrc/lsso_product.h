@@ -10,8 +10,9 @@
 // passing registers (buffer_load ... lds, 16 bytes per lane), and a step's
 // fragments are read under the MFMAs of the step before.  LDS is written
 // linearly by the loads (lane i at 16 i), so bank conflicts are avoided by which
-// piece of memory a lane asks for (the swizzles below; the conflict counter reads
-// zero).  Rows past an operand's end, k past K and rows that a mask excludes are
+// piece of memory a lane asks for (the swizzles below: no conflict cycles in the
+// columns' kernel, 0.3 to 2% in the rows', 3 to 6% where the epilogue exchanges
+// most).  Rows past an operand's end, k past K and rows that a mask excludes are
 // loads past the buffer's end, which bring zeros and touch no memory.
 #pragma once
 
