@@ -105,7 +105,7 @@ def _without_tangents(*values: torch.Tensor | None) -> None:
         return
     for value in values:
         if value is not None and forward_ad.unpack_dual(value).tangent is not None:
-            raise NotImplementedError("the native operators have no forward-mode derivatives")
+            raise NotImplementedError("the native path has no forward-mode derivatives")
 
 
 def _mask_pointer(row_mask: torch.Tensor | None, shape: tuple, device: torch.device):

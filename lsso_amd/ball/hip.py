@@ -610,6 +610,7 @@ def forward_inference(
 ) -> torch.Tensor:
     """Inference-only native mixer (csrc/ball/binding.cpp:16-42)."""
 
+    block._without_tangents(projected, core_base_raw, core_drive_weight, eta_raw)
     if torch.is_grad_enabled() and _any_requires_grad(
         projected, core_base_raw, core_drive_weight, eta_raw, centered_positions, valid_counts
     ):
@@ -633,6 +634,7 @@ def forward_train(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Tape-producing native mixer (csrc/ball/binding.cpp:44-70)."""
 
+    block._without_tangents(projected, core_base_raw, core_drive_weight, eta_raw)
     if torch.is_grad_enabled() and _any_requires_grad(
         projected, core_base_raw, core_drive_weight, eta_raw, centered_positions, valid_counts
     ):
@@ -773,6 +775,7 @@ def fast_mix(
     if valid_counts is not None and valid_counts.requires_grad:
         raise ValueError("the LSSO HIP fast path does not support gradients for valid_counts")
     require_available()
+    block._without_tangents(projected, core_base_raw, core_drive_weight, eta_raw)
     if not torch.is_grad_enabled() or not _any_requires_grad(
         projected, core_base_raw, core_drive_weight, eta_raw
     ):
@@ -819,6 +822,7 @@ def mix_project(
     orchestration of reference model.py:389-405 in one pass).
     """
 
+    block._without_tangents(projected, core_base_raw, core_drive_weight, eta_raw, out_weight, out_bias)
     if torch.is_grad_enabled() and _any_requires_grad(
         projected, core_base_raw, core_drive_weight, eta_raw, centered_positions, valid_counts,
         out_weight, out_bias,
@@ -943,6 +947,7 @@ def layer_forward(
     per-kernel timing on the launch stream.
     """
 
+    block._without_tangents(x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw, out_weight, out_bias)
     if torch.is_grad_enabled() and _any_requires_grad(
         x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw, centered_positions,
         valid_counts, out_weight, out_bias,
@@ -1211,6 +1216,7 @@ def project_mix(
         if value is not None and value.requires_grad:
             raise ValueError(f"the LSSO HIP fast path does not support gradients for {name}")
     require_available()
+    block._without_tangents(x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw)
     if torch.is_grad_enabled() and _any_requires_grad(
         x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw
     ):
@@ -1366,6 +1372,7 @@ def layer_train(
         if value is not None and value.requires_grad:
             raise ValueError(f"the LSSO HIP fast path does not support gradients for {name}")
     require_available()
+    block._without_tangents(x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw, out_weight, out_bias)
     if torch.is_grad_enabled() and _any_requires_grad(
         x, in_weight, in_bias, core_base_raw, core_drive_weight, eta_raw, out_weight, out_bias
     ):
@@ -1624,6 +1631,7 @@ def linear(
     Differentiable (first order) when autograd needs it.
     """
 
+    block._without_tangents(value, weight, bias)
     if torch.is_grad_enabled() and _any_requires_grad(value, weight, bias):
         return _Linear.apply(value, weight, bias, output_dtype, row_mask)
     return _linear_forward(value, weight, bias, output_dtype, row_mask)

@@ -25,6 +25,8 @@ from threading import Lock
 
 import torch
 
+from .block import _without_tangents
+
 NAMESPACE = "lsso_equilibrium"
 
 # The reference's schemas, verbatim (csrc/ball/binding.cpp:80-95).
@@ -104,6 +106,7 @@ def _guarded(name: str, message: str):
             projected, core_base_raw, core_drive_weight, eta_raw, centered_positions, valid_counts
         ):
             raise RuntimeError(message)
+        _without_tangents(projected, core_base_raw, core_drive_weight, eta_raw)
         operator = getattr(getattr(torch.ops, NAMESPACE), name).default
         return operator.redispatch(
             keyset & torch._C._after_autograd_keyset, projected, core_base_raw, core_drive_weight,

@@ -101,6 +101,39 @@ def test_forward_mode_derivatives_are_refused(monkeypatch) -> None:
             hip.dropout_add(x, None, 0.1, 1)
 
 
+def test_the_mixer_refuses_forward_mode_derivatives(monkeypatch) -> None:
+    monkeypatch.setattr(hip, "require_available", lambda: None)
+    x, weight, mixed = torch.randn(1, 4, 8), torch.randn(8, 8), torch.zeros(1, 4, 24)
+    base, drive, eta = torch.zeros(1, 16, 16), torch.zeros(1, 8, 16), torch.zeros(1)
+    core = (base, drive, eta)
+    with torch.no_grad(), forward_ad.dual_level():
+        rows = forward_ad.make_dual(x, torch.ones_like(x))
+        dual = forward_ad.make_dual(eta, torch.ones_like(eta))
+        for call in (lambda: hip.linear(rows, weight, None, torch.bfloat16),
+                     lambda: hip.linear(x, weight, dual, torch.bfloat16),
+                     lambda: hip.fast_mix(mixed, base, drive, dual),
+                     lambda: hip.forward_inference(mixed, base, drive, dual),
+                     lambda: hip.forward_train(mixed, base, drive, dual),
+                     lambda: hip.project_mix(rows, weight, None, *core),
+                     lambda: hip.mix_project(mixed, base, drive, dual, None, None, weight, None, torch.bfloat16),
+                     lambda: hip.layer_forward(rows, weight, None, *core, None, None, weight, None),
+                     lambda: hip.layer_train(rows, weight, None, *core, weight, None)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+def test_a_layer_refuses_forward_mode_derivatives(native) -> None:
+    layer = LSSO(LSSOConfig(dim=64, num_heads=2, rank=16)).cuda()
+    for dim, length in ((64, 33), (64, 1)):
+        x = torch.randn(1, length, dim, device="cuda").bfloat16()
+        expected = layer(x, implementation="hip")
+        with forward_ad.dual_level():
+            assert torch.equal(layer(x, implementation="hip"), expected)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                layer(forward_ad.make_dual(x, torch.ones_like(x)), implementation="hip")
+
+
 @pytest.mark.gpu
 def test_forward_mode_leaves_plain_calls_alone(native) -> None:
     x = torch.randn(5, 8, device="cuda")
