@@ -985,11 +985,11 @@ __global__ __launch_bounds__(256) void pack_kernel(FeedForwardPack a) {
 //   and 18.3, 800 and 200 23.6 and 18.5;
 //   middle and large, the same y: 480 and 120 tiles (one and one) 39.9 and 47.6, 516 and
 //   129 (two and one) 56.3 and 50.8, 1,020 and 255 69.7 and 60.5, 1,032 and 258 (three
-//   and two) 82.0 and 93.0, 1,536 and 384 102 and 100, 1,548 and 387 (four and two) 133 and
-//   130, 3,072 and 768 (six and three) 224 and 187; the gate of K = 768: 512 and 128 18.1
-//   and 22.4, 544 and 136 23.8 and 22.6, 1,056 and 264 36.2 and 42.8, 1,568 and 392 53.7 and
-//   44.3.  (The gate of K = 256, whose epilogue is most of it, keeps 12.4 against 15.3
-//   on middle tiles up to 224 large ones, and loses 16.4 to 15.1 from 240 on.)
+//   and two) 82.0 and 93.0, 1,536 and 384 102 and 100, 1,548 and 387 (four and two) 133
+//   and 130, 6,144 and 1,536 (twelve and six) 436 and 366; the gate of K = 768: 512 and
+//   128 18.1 and 22.4, 544 and 136 23.8 and 22.6, 1,056 and 264 36.2 and 42.8, 1,568 and
+//   392 53.7 and 44.3.  (The gate of K = 256, whose epilogue is most of it, keeps 12.4
+//   against 15.3 on middle tiles up to 224 large ones, and loses 16.4 to 15.1 from 240.)
 enum class Edge { kLarge, kMiddle, kSmall };
 
 int64_t tiles_of(int64_t p, int64_t q, int64_t bp, int64_t bq) { return ((p + bp - 1) / bp) * ((q + bq - 1) / bq); }
