@@ -642,6 +642,147 @@ int lsso_hip_feed_forward_backward(const lsso_hip_feed_forward_shape* shape, con
                                    void* grad_x, void* grad_gate, void* grad_up, void* grad_down,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* Rotary positions. */
+#define LSSO_HIP_ROTARY_INTERLEAVED 1 /* pairs (2j, 2j + 1) */
+#define LSSO_HIP_ROTARY_HALF 2        /* pairs (j, j + rotary_features / 2) */
+
+/* A tensor [batch, length, heads, features] with unit feature stride and these
+ * strides in elements, and its output, contiguous.  x and y may be the same
+ * only if x is contiguous. */
+typedef struct lsso_hip_rotary_tensor {
+    const void* x;
+    void* y;
+    int64_t heads;
+    int64_t batch_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} lsso_hip_rotary_tensor;
+
+/* The pairs (x, x') among the first rotary_features of each head, turned:
+ * amplitude * (x cos a - x' sin a, x sin a + x' cos a), a = position *
+ * frequencies[j], in `layout` order; the other features are copied.  inverse:
+ * turned by -a, which is the gradient.  tensors: one or two (`count`), of one
+ * batch, length, features and dtype (LSSO_HIP_F16 / BF16 / F32).  frequencies:
+ * device float64 [rotary_features / 2], radians a position; angles are taken in
+ * 64 bits.  position_ids: as in lsso_hip_center_positions.  Up to 4,096
+ * features and heads. */
+int lsso_hip_rotary(const lsso_hip_rotary_tensor* tensors, int count, int dtype, int64_t batch,
+                    int64_t length, int64_t features, int64_t rotary_features, int layout,
+                    const double* frequencies, float amplitude, int inverse,
+                    const void* position_ids, int position_type, int64_t position_batch_stride,
+                    int64_t position_token_stride, void* stream);
+
+/* Group norm with an activation, channels last.  x: contiguous [samples, length,
+ * channels] of dtype (LSSO_HIP_F16 / BF16 / F32); groups divides channels;
+ * activation: 0 (none), LSSO_HIP_SILU or LSSO_HIP_GELU; parameter_type: of weight
+ * and bias, dtype or LSSO_HIP_F32. */
+typedef struct lsso_hip_group_norm_shape {
+    int64_t samples;
+    int64_t length;
+    int64_t channels;
+    int64_t groups;
+    int dtype;
+    int parameter_type;
+    int activation;
+    float eps;
+} lsso_hip_group_norm_shape;
+
+/* FP32 values that a forward keeps for its backward (0: it keeps none), and
+ * device scratch bytes of the forward and of the backward. */
+int lsso_hip_group_norm_sizes(const lsso_hip_group_norm_shape* shape, size_t* kept_floats,
+                              size_t* forward_bytes, size_t* backward_bytes);
+
+/* y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and variance over
+ * the tokens and channels of each group of a sample (the variance over their
+ * number).  weight, bias: [channels] or NULL (ones, zeros).  row_mask: optional
+ * device uint8 [samples, length]; rows whose byte is 0 count nowhere, whatever
+ * they hold, and are written as zeros.  statistics: lsso_hip_group_norm_sizes'
+ * kept_floats (NULL for none).  y: contiguous.  workspace: 256-byte aligned. */
+int lsso_hip_group_norm(const lsso_hip_group_norm_shape* shape, const void* x, const void* weight,
+                        const void* bias, const uint8_t* row_mask, float* statistics, void* y,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* First-order gradients of lsso_hip_group_norm for contiguous grad_y of dtype.
+ * grad_x: contiguous, of dtype; grad_weight, grad_bias: [channels] of
+ * parameter_type; each may be NULL.  FP32 sums in an order that depends on the
+ * sizes alone: deterministic. */
+int lsso_hip_group_norm_backward(const lsso_hip_group_norm_shape* shape, const void* grad_y,
+                                 const void* x, const void* weight, const void* bias,
+                                 const uint8_t* row_mask, const float* statistics, void* grad_x,
+                                 void* grad_weight, void* grad_bias, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* Strides in elements of a tensor [batch, length, heads, features] with unit
+ * feature stride. */
+typedef struct lsso_hip_head_strides {
+    int64_t batch;
+    int64_t token;
+    int64_t head;
+} lsso_hip_head_strides;
+
+/* Linear attention with a decay for each head:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t (x) v_t,   y_t = scale q_t S_t.
+ * q: [batch, length, heads, features]; k: [batch, length, kv_heads, features];
+ * v: [batch, length, kv_heads, value_features]; head h reads key and value head
+ * h / (heads / kv_heads).  dtype: LSSO_HIP_F16 or LSSO_HIP_BF16.  Up to 128
+ * features and value features. */
+typedef struct lsso_hip_linear_attention_shape {
+    int64_t batch;
+    int64_t length;
+    int64_t heads;
+    int64_t kv_heads;
+    int64_t features;
+    int64_t value_features;
+    int dtype;
+    float scale;
+    lsso_hip_head_strides q;
+    lsso_hip_head_strides k;
+    lsso_hip_head_strides v;
+} lsso_hip_linear_attention_shape;
+
+/* Device scratch bytes of lsso_hip_linear_attention, and (backward not 0) of
+ * lsso_hip_linear_attention_backward. */
+int lsso_hip_linear_attention_workspace_bytes(const lsso_hip_linear_attention_shape* shape,
+                                              int backward, size_t* bytes);
+
+/* The forward over whole sequences.  log_decay: float32 [heads], at most 0 (-inf: S
+ * is forgotten at once).  row_mask: optional device uint8 [batch, length]; tokens
+ * whose byte is 0 leave S as it is, whatever they hold, and their y is zero.
+ * initial_state: float32 [batch, heads, features, value_features] contiguous or
+ * NULL (zeros).  y: contiguous [batch, length, heads, value_features] of dtype.
+ * final_state: as initial_state, S after the last token, or NULL.
+ * S is FP32; products take 16-bit operands and accumulate in FP32, with P, S and
+ * the decayed v in two 16-bit parts each.  workspace: 256-byte aligned. */
+int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, const void* q,
+                              const void* k, const void* v, const float* log_decay,
+                              const uint8_t* row_mask, const float* initial_state, void* y,
+                              float* final_state, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* First-order gradients for grad_y [batch, length, heads, value_features] of dtype
+ * (strides grad_strides) and grad_final_state (float32 contiguous, or NULL: zeros).
+ * grad_q, grad_k, grad_v: contiguous, of dtype; grad_initial_state: float32
+ * contiguous; each may be NULL.  log_decay has no gradient.  Tokens that row_mask
+ * excludes have zero gradients and reach none.  Deterministic. */
+int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* shape,
+                                       const void* grad_y, const lsso_hip_head_strides* grad_strides,
+                                       const float* grad_final_state, const void* q, const void* k,
+                                       const void* v, const float* log_decay,
+                                       const uint8_t* row_mask, const float* initial_state,
+                                       void* grad_q, void* grad_k, void* grad_v,
+                                       float* grad_initial_state, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* One token of every sequence (shape->length is 1, token strides are unused): state
+ * [batch, heads, features, value_features] float32, contiguous but for its batch
+ * stride, becomes S of that token in place; y: contiguous [batch, heads,
+ * value_features].  row_mask: optional device uint8 [batch]; sequences whose byte is
+ * 0 keep their state, and their y is zero.  FP32 throughout. */
+int lsso_hip_linear_attention_step(const lsso_hip_linear_attention_shape* shape, const void* q,
+                                   const void* k, const void* v, const float* log_decay,
+                                   const uint8_t* row_mask, float* state,
+                                   int64_t state_batch_stride, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

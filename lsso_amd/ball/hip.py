@@ -20,8 +20,9 @@ from threading import Lock
 
 import torch
 
-from . import block, ops
+from . import block, causal, ops
 from .block import dropout_add, embedding, gated_feed_forward
+from .causal import group_norm, linear_attention, linear_attention_step, rotary
 from .reference import rotary_inverse_frequency
 
 _LOAD_LOCK = Lock()
@@ -71,6 +72,7 @@ _SYMBOLS = (
     "lsso_hip_linear_weight_grad_workspace_bytes",
     "lsso_hip_linear_weight_grad",
     *block.SYMBOLS,
+    *causal.SYMBOLS,
 )
 
 
@@ -194,6 +196,7 @@ def _declare(library: ctypes.CDLL) -> None:
     #    positions, mode, counts, tape, out_weight, grads (x, in_weight, in_bias, base, drive, eta, out_weight,
     #    out_bias), workspace, workspace_bytes, stream
     block.declare(library)
+    causal.declare(library)
 
 
 def default_library_path() -> Path:
@@ -1646,14 +1649,18 @@ __all__ = [
     "forward_inference",
     "forward_train",
     "gated_feed_forward",
+    "group_norm",
     "is_available",
     "layer_forward",
     "layer_train",
     "layer_supported",
     "linear",
+    "linear_attention",
+    "linear_attention_step",
     "load",
     "mix_project",
     "mix_project_supported",
     "project_mix",
     "require_available",
+    "rotary",
 ]

@@ -38,6 +38,10 @@ SOURCES = (
     "lsso_dropout.hip",
     "lsso_embedding.hip",
     "lsso_feed_forward.hip",
+    "lsso_causal_capi.hip",
+    "lsso_rotary.hip",
+    "lsso_group_norm.hip",
+    "lsso_linear_attention.hip",
 )
 PROBE_SOURCE = "lsso_probe.hip"
 PROBE_LIBRARY_NAME = f"liblsso_probe_{OFFLOAD_ARCH}.so"

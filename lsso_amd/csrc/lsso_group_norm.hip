@@ -1,0 +1,841 @@
+// Group norm with an activation, channels last:
+//   y = act(z),  z = w_c xhat + b_c,  xhat = (x - mean) rstd,
+// mean and rstd = 1 / sqrt(var + eps) over the n = tokens x channels of a group
+// of one sample.  With dz = dy act'(z) and dn = w_c dz,
+//   dx = rstd (dn - (sum of dn + xhat sum of dn xhat) / n),
+//   dw_c = sum of dz xhat,  db_c = sum of dz.
+// Rows that the mask excludes count nowhere and come out as zeros.
+//
+// Bound: HBM.  Two forms:
+//
+// Every token a sample of its own (heads of a token, or a layer norm): a group's
+// channels are read once, by a team of lanes that keeps them in registers, sums
+// them over its lanes, and writes y.  Teams of neighbouring groups sit next to
+// each other, so that a wave reads whole lines.  Each lane stays with its
+// channels while its workgroup walks over the rows, which leaves dw and db in
+// its registers to the end.
+//
+// Longer samples: a channels-last row holds all groups, and a group's share of it
+// may be 16 bytes, so a workgroup takes whole rows of a range of tokens and each
+// thread keeps to a few channels.  One launch leaves mean and squared deviations
+// of each channel of each range, one joins them to the groups' statistics, one
+// applies them (x is read again, from the last-level cache where it fits).  The
+// backward does the same with its two sums.
+//
+// Variances come from deviations: of four rows at a time from their own mean,
+// joined to what is known so far by the rule for two parts (Chan, Golub and
+// LeVeque, 1979).  Sums of squares lose a variance that is small beside the
+// mean's square, and a fixed pivot is worth as little as its outliers let it.
+
+#include "lsso_activation.h"
+#include "lsso_device.h"
+#include "lsso_internal.h"
+#include "lsso_values.h"
+
+#include "lsso_hip.h"
+
+namespace lsso_hip {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlockRows = 4;        // rows of a thread in flight
+constexpr int kTeamMost = 4;         // most pieces of a lane
+constexpr int64_t kMostGrid = 1 << 20;
+
+// act(z) and act'(z).  FP32 outputs show more than the fast forms hold (1e-5 of
+// the sigmoid's and the distribution function's own value).
+template <int T, bool SLOPE>
+__device__ __forceinline__ void act(int kind, float z, float& value, float& slope) {
+    if (kind == 0) {
+        value = z;
+        slope = 1.0f;
+    } else if constexpr (T != LSSO_HIP_F32) {
+        activation<SLOPE>(kind, z, value, slope);
+    } else if (kind == LSSO_HIP_SILU) {
+        const float s = 1.0f / (1.0f + expf(-z));
+        value = z * s;
+        slope = SLOPE ? s + value * (1.0f - s) : 0.0f;
+    } else {
+        const float phi = normcdff(z);
+        value = z * phi;
+        slope = SLOPE ? phi + 0.3989422804f * z * expf(-0.5f * z * z) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ float parameter(const void* values, int type, int c, float absent) {
+    if (values == nullptr) {
+        return absent;
+    }
+    switch (type) {
+        case LSSO_HIP_F16: return f16_bits_to_float(static_cast<const uint16_t*>(values)[c]);
+        case LSSO_HIP_BF16: return bf16_bits_to_float(static_cast<const uint16_t*>(values)[c]);
+        default: return static_cast<const float*>(values)[c];
+    }
+}
+
+__device__ __forceinline__ void store_parameter(void* values, int type, int c, float v) {
+    switch (type) {
+        case LSSO_HIP_F16: static_cast<uint16_t*>(values)[c] = to_f16_bits(v); break;
+        case LSSO_HIP_BF16: static_cast<uint16_t*>(values)[c] = to_bf16_bits(v); break;
+        default: static_cast<float*>(values)[c] = v; break;
+    }
+}
+
+// Sum over the team's lanes, a power of two of neighbours, in all of them.
+__device__ __forceinline__ float team_sum(float v, int lanes) {
+    for (int offset = 1; offset < lanes; offset *= 2) {
+        v += __shfl_xor(v, offset);
+    }
+    return v;
+}
+
+// Teams of a workgroup: `at_once` rows of `across` groups.
+struct Teams {
+    int lane;       // of the team
+    int group;
+    int row;
+    int at_once;
+    int across;
+    bool active;
+    __device__ __forceinline__ Teams(const GroupNormArgs& a) {
+        const int teams = kThreads / a.team;
+        across = 1;
+        while (across < a.groups && across < teams) {
+            across *= 2;
+        }
+        at_once = teams / across;
+        const int team = static_cast<int>(threadIdx.x) / a.team;
+        lane = static_cast<int>(threadIdx.x) % a.team;
+        group = static_cast<int>(blockIdx.y) * across + team % across;
+        row = team / across;
+        active = group < a.groups;
+    }
+};
+
+// T: type; V: channels of a piece; K: pieces of a lane; BACKWARD: dx and the
+// partials of dw and db instead of y.
+template <int T, int V, int K, bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
+    using Element = typename Values<T>::Element;
+    const Teams t(a);
+    const int size = a.channels / a.groups;
+    const int pieces = size / V;
+    const float share = 1.0f / static_cast<float>(size);
+    const int channel0 = (t.active ? t.group : 0) * size;
+    float w[K][V];
+    float b[K][V];
+    float grad_w[BACKWARD ? K : 1][V];
+    float grad_b[BACKWARD ? K : 1][V];
+    bool mine[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int piece = t.lane + a.team * k;
+        mine[k] = t.active && piece < pieces;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            w[k][i] = mine[k] ? parameter(a.weight, a.parameter_type, channel0 + piece * V + i, 1.0f) : 0.0f;
+            b[k][i] = mine[k] ? parameter(a.bias, a.parameter_type, channel0 + piece * V + i, 0.0f) : 0.0f;
+            if constexpr (BACKWARD) {
+                grad_w[k][i] = 0.0f;
+                grad_b[k][i] = 0.0f;
+            }
+        }
+    }
+    const int64_t step = static_cast<int64_t>(gridDim.x) * t.at_once;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * t.at_once; row0 < a.samples; row0 += step) {
+        const int64_t row = row0 + t.row;
+        const bool inside = row < a.samples;
+        const bool kept = inside && (a.row_mask == nullptr || a.row_mask[row] != 0);
+        const int64_t at = (inside ? row : 0) * a.channels + channel0;
+        float x[K][V];
+        float dy[BACKWARD ? K : 1][V];
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int piece = t.lane + a.team * k;
+            if (mine[k] && kept) {
+                load_values<T, V>(static_cast<const Element*>(a.x) + at + piece * V, x[k]);
+                if constexpr (BACKWARD) {
+                    load_values<T, V>(static_cast<const Element*>(a.dy) + at + piece * V, dy[k]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[k][i] = 0.0f;
+                    if constexpr (BACKWARD) {
+                        dy[k][i] = 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sum += x[k][i];
+            }
+        }
+        const float mean = team_sum(sum, a.team) * share;
+        float squares = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                x[k][i] = mine[k] ? x[k][i] - mean : 0.0f;
+                squares += x[k][i] * x[k][i];
+            }
+        }
+        const float rstd = 1.0f / sqrtf(team_sum(squares, a.team) * share + a.eps);
+        if constexpr (!BACKWARD) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float y[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float slope;
+                    act<T, false>(a.activation, x[k][i] * rstd * w[k][i] + b[k][i], y[i], slope);
+                    y[i] = kept ? y[i] : 0.0f;
+                }
+                if (mine[k] && inside) {
+                    store_values<T, V>(static_cast<Element*>(a.y) + at + (t.lane + a.team * k) * V, y);
+                }
+            }
+        } else {
+            float first = 0.0f;
+            float second = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[k][i] *= rstd;
+                    float value;
+                    float slope;
+                    act<T, true>(a.activation, x[k][i] * w[k][i] + b[k][i], value, slope);
+                    // A row that is left out has no part in any sum.
+                    const float dz = kept ? dy[k][i] * slope : 0.0f;
+                    const float normal = kept ? x[k][i] : 0.0f;
+                    grad_b[k][i] += dz;
+                    grad_w[k][i] += dz * normal;
+                    dy[k][i] = dz * w[k][i];
+                    first += dy[k][i];
+                    second += dy[k][i] * normal;
+                }
+            }
+            first = team_sum(first, a.team) * share;
+            second = team_sum(second, a.team) * share;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float dx[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dx[i] = kept ? rstd * (dy[k][i] - (first + x[k][i] * second)) : 0.0f;
+                }
+                if (a.dx != nullptr && mine[k] && inside) {
+                    store_values<T, V>(static_cast<Element*>(a.dx) + at + (t.lane + a.team * k) * V, dx);
+                }
+            }
+        }
+    }
+    if constexpr (BACKWARD) {
+        // The rows' teams of a group, one after the other: partials [blocks][dw, db][channels].
+        __shared__ float shared[kThreads][K * V + 1];
+        float* out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * a.channels;
+        const int stride = t.across * a.team;   // threads of one row
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    shared[threadIdx.x][k * V + i] = part == 0 ? grad_w[k][i] : grad_b[k][i];
+                }
+            }
+            __syncthreads();
+            if (t.row == 0) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float total = 0.0f;
+                        for (int r = 0; r < t.at_once; ++r) {
+                            total += shared[threadIdx.x + r * stride][k * V + i];
+                        }
+                        if (mine[k]) {
+                            out[part * a.channels + channel0 + (t.lane + a.team * k) * V + i] = total;
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+// The part of a workgroup of the kernels over splits: a thread keeps to one
+// piece of V channels and takes every at_once-th row of the split.
+template <int V>
+struct Columns {
+    int wide;        // pieces of the workgroup's channels
+    int at_once;
+    int channel;
+    int row;
+    bool active;
+    __device__ __forceinline__ Columns(const GroupNormArgs& a) {
+        const int pieces = a.channels / V;
+        const int first = static_cast<int>(blockIdx.y) * kThreads;
+        wide = pieces - first < kThreads ? pieces - first : kThreads;
+        at_once = kThreads / wide;
+        row = static_cast<int>(threadIdx.x) / wide;
+        channel = (first + static_cast<int>(threadIdx.x) % wide) * V;
+        active = row < at_once;
+    }
+};
+
+// Floats of a split's partials: two of each channel and the rows that count.
+__host__ __device__ inline int64_t partial_pitch(int channels) { return 2 * static_cast<int64_t>(channels) + 1; }
+
+// Rows at, at + step, ... (kBlockRows of them) of a thread: loads, and which count.
+template <int T, int V>
+__device__ __forceinline__ void load_rows(const void* from, const GroupNormArgs& a, int64_t sample, int64_t at, int step,
+                                          int64_t end, int channel, float (&v)[kBlockRows][V],
+                                          bool (&kept)[kBlockRows]) {
+    using Element = typename Values<T>::Element;
+#pragma unroll
+    for (int r = 0; r < kBlockRows; ++r) {
+        const int64_t row = at + static_cast<int64_t>(r) * step;
+        kept[r] = row < end && (a.row_mask == nullptr || a.row_mask[sample * a.length + row] != 0);
+        if (kept[r]) {
+            load_values<T, V>(static_cast<const Element*>(from) + (sample * a.length + row) * a.channels + channel,
+                              v[r]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[r][i] = 0.0f;
+            }
+        }
+    }
+}
+
+// Mean and squared deviations of each channel over a split's rows.
+template <int T, int V>
+__global__ __launch_bounds__(kThreads) void norm_statistics_kernel(GroupNormArgs a) {
+    __shared__ float shared[kThreads][2 * V + 1];
+    __shared__ float rows[kThreads];
+    const Columns<V> c(a);
+    const int64_t items = a.samples * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t sample = item / a.splits;
+        const int64_t begin = (item - sample * a.splits) * a.split_rows;
+        const int64_t end = begin + a.split_rows < a.length ? begin + a.split_rows : a.length;
+        float count = 0.0f;
+        float mean[V];
+        float squares[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mean[i] = 0.0f;
+            squares[i] = 0.0f;
+        }
+        if (c.active) {
+            for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
+                float v[kBlockRows][V];
+                bool kept[kBlockRows];
+                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
+                float some = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kBlockRows; ++r) {
+                    some += kept[r] ? 1.0f : 0.0f;
+                }
+                if (some > 0.0f) {
+                    const float share = 1.0f / some;
+                    const float all = count + some;
+                    const float weight = some / all;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < kBlockRows; ++r) {
+                            sum += v[r][i];
+                        }
+                        const float middle = sum * share;
+                        float deviations = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < kBlockRows; ++r) {
+                            const float d = kept[r] ? v[r][i] - middle : 0.0f;
+                            deviations += d * d;
+                        }
+                        const float apart = middle - mean[i];
+                        squares[i] += deviations + apart * apart * (count * weight);
+                        mean[i] += apart * weight;
+                    }
+                    count = all;
+                }
+            }
+        }
+        __syncthreads();   // the last item's readers are done
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            shared[threadIdx.x][i] = mean[i];
+            shared[threadIdx.x][V + i] = squares[i];
+        }
+        rows[threadIdx.x] = count;
+        __syncthreads();
+        float* out = a.partials + item * partial_pitch(a.channels);
+        for (int j = threadIdx.x; j < c.wide * V; j += kThreads) {
+            const int thread = j / V;
+            const int i = j - thread * V;
+            float n = 0.0f;
+            float m = 0.0f;
+            float s = 0.0f;
+            for (int r = 0; r < c.at_once; ++r) {
+                const float some = rows[thread + r * c.wide];
+                if (some > 0.0f) {
+                    const float weight = some / (n + some);
+                    const float apart = shared[thread + r * c.wide][i] - m;
+                    s += shared[thread + r * c.wide][V + i] + apart * apart * (n * weight);
+                    m += apart * weight;
+                    n += some;
+                }
+            }
+            const int channel = (static_cast<int>(blockIdx.y) * kThreads) * V + j;
+            out[channel] = m;
+            out[a.channels + channel] = s;
+            if (channel == 0) {
+                out[2 * a.channels] = n;
+            }
+        }
+    }
+}
+
+// Sum over the workgroup, in every thread.
+__device__ __forceinline__ float block_sum(float v, float* scratch) {
+    v = team_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        scratch[threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+        total += scratch[i];
+    }
+    return total;
+}
+
+// A group's statistics from its splits.
+__global__ __launch_bounds__(kThreads) void norm_join_kernel(GroupNormArgs a) {
+    __shared__ float scratch[kThreads / 64];
+    const int size = a.channels / a.groups;
+    const int64_t pitch = partial_pitch(a.channels);
+    const int64_t items = a.samples * a.groups;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t sample = item / a.groups;
+        const int channel0 = static_cast<int>(item - sample * a.groups) * size;
+        const float* part = a.partials + sample * a.splits * pitch;
+        const int64_t values = a.splits * size;
+        float n = 0.0f;
+        float sum = 0.0f;
+        for (int64_t j = threadIdx.x; j < values; j += kThreads) {
+            const int64_t split = j / size;
+            const float some = part[split * pitch + 2 * a.channels];
+            n += some;
+            sum += some * part[split * pitch + channel0 + (j - split * size)];
+        }
+        n = block_sum(n, scratch);
+        sum = block_sum(sum, scratch);
+        const float mean = n > 0.0f ? sum / n : 0.0f;
+        float squares = 0.0f;
+        for (int64_t j = threadIdx.x; j < values; j += kThreads) {
+            const int64_t split = j / size;
+            const float* at = part + split * pitch + channel0 + (j - split * size);
+            const float some = part[split * pitch + 2 * a.channels];
+            const float apart = some > 0.0f ? at[0] - mean : 0.0f;
+            squares += some > 0.0f ? at[a.channels] + some * apart * apart : 0.0f;
+        }
+        squares = block_sum(squares, scratch);
+        if (threadIdx.x == 0) {
+            a.statistics[2 * item] = mean;
+            a.statistics[2 * item + 1] = n > 0.0f ? 1.0f / sqrtf(squares / n + a.eps) : 0.0f;
+        }
+    }
+}
+
+// A thread's channels: w, b, and the statistics of their groups.
+template <int V>
+struct ChannelValues {
+    float w[V];
+    float b[V];
+    float mean[V];
+    float rstd[V];
+    __device__ __forceinline__ void parameters(const GroupNormArgs& a, int channel) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            w[i] = parameter(a.weight, a.parameter_type, channel + i, 1.0f);
+            b[i] = parameter(a.bias, a.parameter_type, channel + i, 0.0f);
+        }
+    }
+    __device__ __forceinline__ void of_sample(const GroupNormArgs& a, int64_t sample, int channel) {
+        const int size = a.channels / a.groups;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int64_t at = 2 * (sample * a.groups + (channel + i) / size);
+            mean[i] = a.statistics[at];
+            rstd[i] = a.statistics[at + 1];
+        }
+    }
+};
+
+template <int T, int V>
+__global__ __launch_bounds__(kThreads) void norm_apply_kernel(GroupNormArgs a) {
+    using Element = typename Values<T>::Element;
+    const Columns<V> c(a);
+    if (!c.active) {
+        return;   // no barrier follows
+    }
+    ChannelValues<V> channel;
+    channel.parameters(a, c.channel);
+    const int64_t items = a.samples * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t sample = item / a.splits;
+        const int64_t begin = (item - sample * a.splits) * a.split_rows;
+        const int64_t end = begin + a.split_rows < a.length ? begin + a.split_rows : a.length;
+        channel.of_sample(a, sample, c.channel);
+        for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
+            float v[kBlockRows][V];
+            bool kept[kBlockRows];
+            load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
+#pragma unroll
+            for (int r = 0; r < kBlockRows; ++r) {
+                const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
+                if (row < end) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float slope;
+                        float y;
+                        act<T, false>(a.activation,
+                                      (v[r][i] - channel.mean[i]) * channel.rstd[i] * channel.w[i] + channel.b[i], y,
+                                      slope);
+                        v[r][i] = kept[r] ? y : 0.0f;
+                    }
+                    store_values<T, V>(
+                        static_cast<Element*>(a.y) + (sample * a.length + row) * a.channels + c.channel, v[r]);
+                }
+            }
+        }
+    }
+}
+
+// DX: dx, from the groups' sums; else the sums of dz xhat and dz of each channel
+// over a split's rows.
+template <int T, int V, bool DX>
+__global__ __launch_bounds__(kThreads) void norm_grad_kernel(GroupNormArgs a) {
+    using Element = typename Values<T>::Element;
+    __shared__ float shared[DX ? 1 : kThreads][2 * V + 1];
+    __shared__ float rows[DX ? 1 : kThreads];
+    const Columns<V> c(a);
+    const int size = a.channels / a.groups;
+    ChannelValues<V> channel;
+    if (c.active) {
+        channel.parameters(a, c.channel);
+    }
+    const int64_t items = a.samples * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t sample = item / a.splits;
+        const int64_t begin = (item - sample * a.splits) * a.split_rows;
+        const int64_t end = begin + a.split_rows < a.length ? begin + a.split_rows : a.length;
+        float first[V];    // DX: the group's mean of dn, else this channel's sum of dz
+        float second[V];   // the same with xhat
+        float count = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            first[i] = 0.0f;
+            second[i] = 0.0f;
+        }
+        if (c.active) {
+            channel.of_sample(a, sample, c.channel);
+            if constexpr (DX) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int64_t at = 2 * (sample * a.groups + (c.channel + i) / size);
+                    first[i] = a.sums[at];
+                    second[i] = a.sums[at + 1];
+                }
+            }
+            for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
+                float v[kBlockRows][V];
+                float dy[kBlockRows][V];
+                bool kept[kBlockRows];
+                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
+                load_rows<T, V>(a.dy, a, sample, at, c.at_once, end, c.channel, dy, kept);
+#pragma unroll
+                for (int r = 0; r < kBlockRows; ++r) {
+                    const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
+                    count += kept[r] ? 1.0f : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float normal = kept[r] ? (v[r][i] - channel.mean[i]) * channel.rstd[i] : 0.0f;
+                        float value;
+                        float slope;
+                        act<T, true>(a.activation, normal * channel.w[i] + channel.b[i], value, slope);
+                        const float dz = kept[r] ? dy[r][i] * slope : 0.0f;
+                        if constexpr (DX) {
+                            v[r][i] = kept[r] ? channel.rstd[i] * (dz * channel.w[i] - (first[i] + normal * second[i]))
+                                              : 0.0f;
+                        } else {
+                            first[i] += dz;
+                            second[i] += dz * normal;
+                        }
+                    }
+                    if constexpr (DX) {
+                        if (row < end) {
+                            store_values<T, V>(
+                                static_cast<Element*>(a.dx) + (sample * a.length + row) * a.channels + c.channel,
+                                v[r]);
+                        }
+                    }
+                }
+            }
+        }
+        if constexpr (!DX) {
+            __syncthreads();   // the last item's readers are done
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                shared[threadIdx.x][i] = second[i];
+                shared[threadIdx.x][V + i] = first[i];
+            }
+            rows[threadIdx.x] = count;
+            __syncthreads();
+            float* out = a.partials + item * partial_pitch(a.channels);
+            for (int j = threadIdx.x; j < 2 * c.wide * V; j += kThreads) {
+                const int part = j >= c.wide * V ? 1 : 0;
+                const int thread = (j - part * c.wide * V) / V;
+                const int i = (j - part * c.wide * V) - thread * V;
+                float total = 0.0f;
+                for (int r = 0; r < c.at_once; ++r) {
+                    total += shared[thread + r * c.wide][part * V + i];
+                }
+                out[part * a.channels + static_cast<int>(blockIdx.y) * kThreads * V + thread * V + i] = total;
+            }
+            if (blockIdx.y == 0 && threadIdx.x == 0) {
+                float total = 0.0f;
+                for (int r = 0; r < c.at_once; ++r) {
+                    total += rows[r * c.wide];
+                }
+                out[2 * a.channels] = total;
+            }
+        }
+    }
+}
+
+// The groups' means of dn and dn xhat from the channels' sums of every split.
+__global__ __launch_bounds__(kThreads) void norm_grad_join_kernel(GroupNormArgs a) {
+    __shared__ float scratch[kThreads / 64];
+    const int size = a.channels / a.groups;
+    const int64_t pitch = partial_pitch(a.channels);
+    const int64_t items = a.samples * a.groups;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t sample = item / a.groups;
+        const int channel0 = static_cast<int>(item - sample * a.groups) * size;
+        const float* part = a.partials + sample * a.splits * pitch;
+        float n = 0.0f;
+        float first = 0.0f;
+        float second = 0.0f;
+        for (int64_t j = threadIdx.x; j < a.splits * size; j += kThreads) {
+            const int64_t split = j / size;
+            const int c = channel0 + static_cast<int>(j - split * size);
+            const float w = parameter(a.weight, a.parameter_type, c, 1.0f);
+            n += part[split * pitch + 2 * a.channels];
+            second += w * part[split * pitch + c];
+            first += w * part[split * pitch + a.channels + c];
+        }
+        n = block_sum(n, scratch);
+        first = block_sum(first, scratch);
+        second = block_sum(second, scratch);
+        if (threadIdx.x == 0) {
+            a.sums[2 * item] = n > 0.0f ? first / n : 0.0f;
+            a.sums[2 * item + 1] = n > 0.0f ? second / n : 0.0f;
+        }
+    }
+}
+
+// dw and db: column sums of `rows` partials, 16 of a column's rows at a time.
+constexpr int kSumColumns = 16;
+__global__ __launch_bounds__(kThreads) void norm_columns_kernel(GroupNormArgs a, int64_t rows, int64_t pitch) {
+    __shared__ float shared[kThreads / kSumColumns][kSumColumns + 1];
+    const int in = static_cast<int>(threadIdx.x) % kSumColumns;
+    const int at = static_cast<int>(threadIdx.x) / kSumColumns;
+    const int column = static_cast<int>(blockIdx.x) * kSumColumns + in;
+    float total = 0.0f;
+    if (column < 2 * a.channels) {
+#pragma unroll 8
+        for (int64_t r = at; r < rows; r += kThreads / kSumColumns) {
+            total += a.partials[r * pitch + column];
+        }
+    }
+    shared[at][in] = total;
+    __syncthreads();
+    if (at == 0 && column < 2 * a.channels) {
+        total = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kThreads / kSumColumns; ++r) {
+            total += shared[r][in];
+        }
+        void* out = column < a.channels ? a.grad_weight : a.grad_bias;
+        if (out != nullptr) {
+            store_parameter(out, a.parameter_type, column < a.channels ? column : column - a.channels, total);
+        }
+    }
+}
+
+template <int T, int V, int K>
+void launch_team_pieces(const GroupNormArgs& a, bool backward, hipStream_t stream) {
+    int across = 1;
+    while (across < a.groups && across < kThreads / a.team) {
+        across *= 2;
+    }
+    const dim3 grid(static_cast<unsigned>(a.blocks), static_cast<unsigned>((a.groups + across - 1) / across));
+    if (backward) {
+        team_norm_kernel<T, V, K, true><<<grid, kThreads, 0, stream>>>(a);
+    } else {
+        team_norm_kernel<T, V, K, false><<<grid, kThreads, 0, stream>>>(a);
+    }
+}
+
+template <int T, int V>
+void launch_team(const GroupNormArgs& a, bool backward, hipStream_t stream) {
+    switch (a.team_pieces) {
+        case 1: launch_team_pieces<T, V, 1>(a, backward, stream); break;
+        case 2: launch_team_pieces<T, V, 2>(a, backward, stream); break;
+        case 3: launch_team_pieces<T, V, 3>(a, backward, stream); break;
+        default: launch_team_pieces<T, V, 4>(a, backward, stream); break;
+    }
+}
+
+unsigned capped(int64_t blocks) { return static_cast<unsigned>(blocks < kMostGrid ? blocks : kMostGrid); }
+
+template <int T, int V>
+void launch_forward(const GroupNormArgs& a, hipStream_t stream) {
+    if (a.team != 0) {
+        launch_team<T, V>(a, false, stream);
+        return;
+    }
+    if (a.samples * a.splits == 0) {
+        return;
+    }
+    const dim3 grid(capped(a.samples * a.splits),
+                    static_cast<unsigned>((a.channels / V + kThreads - 1) / kThreads));
+    norm_statistics_kernel<T, V><<<grid, kThreads, 0, stream>>>(a);
+    norm_join_kernel<<<capped(a.samples * a.groups), kThreads, 0, stream>>>(a);
+    norm_apply_kernel<T, V><<<grid, kThreads, 0, stream>>>(a);
+}
+
+template <int T, int V>
+void launch_backward(const GroupNormArgs& a, hipStream_t stream) {
+    const unsigned columns = static_cast<unsigned>((2 * a.channels + kSumColumns - 1) / kSumColumns);
+    const bool parameters = a.grad_weight != nullptr || a.grad_bias != nullptr;
+    if (a.team != 0) {
+        launch_team<T, V>(a, true, stream);
+        if (parameters) {
+            norm_columns_kernel<<<columns, kThreads, 0, stream>>>(a, a.blocks, 2 * static_cast<int64_t>(a.channels));
+        }
+        return;
+    }
+    const bool rows = a.samples * a.splits > 0;
+    const dim3 grid(capped(a.samples * a.splits),
+                    static_cast<unsigned>((a.channels / V + kThreads - 1) / kThreads));
+    if (rows) {
+        norm_grad_kernel<T, V, false><<<grid, kThreads, 0, stream>>>(a);
+    }
+    if (parameters) {   // without rows they are zeros
+        norm_columns_kernel<<<columns, kThreads, 0, stream>>>(a, a.samples * a.splits, partial_pitch(a.channels));
+    }
+    if (rows && a.dx != nullptr) {
+        norm_grad_join_kernel<<<capped(a.samples * a.groups), kThreads, 0, stream>>>(a);
+        norm_grad_kernel<T, V, true><<<grid, kThreads, 0, stream>>>(a);
+    }
+}
+
+template <int T>
+void launch_vector(const GroupNormArgs& a, bool backward, hipStream_t stream) {
+    const auto run = [&](auto forward_form, auto backward_form) {
+        if (backward) {
+            backward_form(a, stream);
+        } else {
+            forward_form(a, stream);
+        }
+    };
+    switch (a.vector) {
+        case 8: run(launch_forward<T, 8>, launch_backward<T, 8>); break;
+        case 4: run(launch_forward<T, 4>, launch_backward<T, 4>); break;
+        case 2: run(launch_forward<T, 2>, launch_backward<T, 2>); break;
+        default: run(launch_forward<T, 1>, launch_backward<T, 1>); break;
+    }
+}
+
+hipError_t launch(const GroupNormArgs& a, int dtype, bool backward, hipStream_t stream) {
+    switch (dtype) {
+        case LSSO_HIP_F16: launch_vector<LSSO_HIP_F16>(a, backward, stream); break;
+        case LSSO_HIP_BF16: launch_vector<LSSO_HIP_BF16>(a, backward, stream); break;
+        default: launch_vector<LSSO_HIP_F32>(a, backward, stream); break;
+    }
+    return hipGetLastError();
+}
+
+int widest(int n) { return n % 8 == 0 ? 8 : (n % 4 == 0 ? 4 : (n % 2 == 0 ? 2 : 1)); }
+
+}  // namespace
+
+void plan_group_norm(GroupNormArgs* a, bool backward, size_t* partial_bytes) {
+    const int size = a->channels / a->groups;
+    a->team = 0;
+    a->vector = widest(size);
+    const int pieces = size / a->vector;
+    if (a->length == 1 && pieces <= 64 * kTeamMost) {
+        // The lanes and pieces that leave the fewest registers empty; of equals the
+        // most lanes, which hold fewer registers each.
+        int best = 1 << 30;
+        for (int k = 1; k <= kTeamMost; ++k) {
+            int lanes = 1;
+            while (lanes * k < pieces) {
+                lanes *= 2;
+            }
+            if (lanes <= 64 && lanes * k < best) {
+                best = lanes * k;
+                a->team = lanes;
+                a->team_pieces = k;
+            }
+        }
+        int across = 1;
+        while (across < a->groups && across < kThreads / a->team) {
+            across *= 2;
+        }
+        const int64_t at_once = kThreads / a->team / across;
+        const int64_t rows = (a->samples + at_once - 1) / at_once;
+        // Eight workgroups to a compute unit forward; half of it backward, whose
+        // partials are read again.
+        const int64_t most = backward ? 1024 : 2048;
+        a->blocks = rows < most ? (rows > 0 ? rows : 1) : most;
+        *partial_bytes = backward ? sizeof(float) * 2 * static_cast<size_t>(a->channels) * static_cast<size_t>(a->blocks) : 0;
+        return;
+    }
+    a->vector = widest(a->channels);
+    const int64_t across = (a->channels / a->vector + kThreads - 1) / kThreads;
+    const int64_t wide = a->channels / a->vector < kThreads ? a->channels / a->vector : kThreads;
+    const int64_t block = kBlockRows * (kThreads / wide);   // rows of a workgroup in flight
+    // About eight workgroups to a compute unit, each with a whole block of rows.
+    const int64_t items = a->samples * across;
+    const int64_t wanted = items > 0 && items < 2048 ? 2048 / items : 1;
+    const int64_t rows = (a->length + wanted - 1) / wanted;
+    a->split_rows = rows > 0 ? (rows + block - 1) / block * block : block;
+    a->splits = (a->length + a->split_rows - 1) / a->split_rows;
+    *partial_bytes = sizeof(float) * static_cast<size_t>(partial_pitch(a->channels)) * static_cast<size_t>(a->samples) *
+                     static_cast<size_t>(a->splits);
+}
+
+hipError_t launch_group_norm(const GroupNormArgs& a, int dtype, hipStream_t stream) {
+    return launch(a, dtype, false, stream);
+}
+
+hipError_t launch_group_norm_backward(const GroupNormArgs& a, int dtype, hipStream_t stream) {
+    return launch(a, dtype, true, stream);
+}
+
+}  // namespace lsso_hip

@@ -465,6 +465,145 @@ hipError_t launch_feed_forward_weights(const FeedForwardWeights& a, hipStream_t 
 hipError_t launch_feed_forward_join(const FeedForwardJoin& a, int outputs, hipStream_t stream);
 hipError_t launch_feed_forward_pack(const FeedForwardPack& a, int type, hipStream_t stream);
 
+// Rotary positions (lsso_rotary.hip).
+struct RotaryTensor {
+    const void* x;              // [batch, length, heads, features], unit feature stride
+    void* y;                    // contiguous
+    int64_t batch_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    int heads;
+    uint32_t head_magic;        // set by the launcher
+};
+
+struct RotaryArgs {
+    RotaryTensor tensors[2];
+    int count;
+    int64_t batch;
+    int64_t length;
+    int features;
+    int half;                   // pairs
+    const double* frequencies;  // [half] radians a position
+    float amplitude;
+    float sign;                 // -1: turned back
+    const void* positions;      // or nullptr: 0 .. length - 1
+    int position_type;
+    int64_t position_batch_stride;
+    int64_t position_token_stride;
+    int tile;                   // tokens, set by the launcher, as what follows
+    uint32_t half_magic;
+    int lanes_shift;            // log2 of the lanes of a row
+};
+
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, int layout, hipStream_t stream);
+
+// Group norm with an activation (lsso_group_norm.hip).
+struct GroupNormArgs {
+    const void* x;              // [samples, length, channels] contiguous
+    int64_t samples;
+    int64_t length;
+    int channels;
+    int groups;
+    const void* weight;         // [channels] of parameter_type, or nullptr: ones
+    const void* bias;           // [channels], or nullptr: zeros
+    int parameter_type;
+    float eps;
+    int activation;             // 0, LSSO_HIP_SILU or LSSO_HIP_GELU
+    const uint8_t* row_mask;    // [samples, length] or nullptr
+    void* y;                    // contiguous
+    float* statistics;          // [samples, groups, 2]: mean, 1 / sqrt(var + eps)
+    const void* dy;             // of the backward, as what follows
+    void* dx;                   // or nullptr
+    void* grad_weight;          // [channels] of parameter_type, or nullptr
+    void* grad_bias;
+    float* partials;            // workspace
+    float* sums;                // [samples, groups, 2]: mean of dn, mean of dn xhat
+    int64_t splits;             // set by plan_group_norm: workgroups along the tokens of a sample
+    int64_t split_rows;
+    int team;                   // tokens are samples: lanes of a group; 0: the kernels over splits
+    int team_pieces;            // pieces of a lane
+    int vector;                 // channels of a piece
+    int64_t blocks;             // of the team kernel's grid
+};
+
+// The plan and the bytes of partials, sums and (`keep` false) statistics.
+void plan_group_norm(GroupNormArgs* a, bool backward, size_t* partial_bytes);
+hipError_t launch_group_norm(const GroupNormArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_group_norm_backward(const GroupNormArgs& a, int dtype, hipStream_t stream);
+
+// Linear attention with a decay for each head (lsso_linear_attention.hip):
+//   out_t = sum over s <= t of decay^(tokens from s to t) (a_t . b_s) c_s.
+// A walk towards the front is the same with the last token's addresses and
+// negative token strides.
+struct WalkTensor {
+    const void* data;
+    int64_t batch;              // strides in elements
+    int64_t token;
+    int64_t head;
+    int heads_per;              // heads of the walk that read one head of this tensor
+};
+
+struct WalkArgs {
+    WalkTensor a;               // [batch, length, heads, features]
+    WalkTensor b;
+    WalkTensor c;               // [batch, length, heads, out_features]
+    WalkTensor out;             // [batch, length, heads, out_features]; no data: the last state alone
+    int wide_out;               // FP32, else of the inputs' type
+    int64_t batch;
+    int64_t length;
+    int heads;
+    int features;
+    int out_features;
+    const float* log_decay;     // [heads]
+    const uint8_t* mask;        // or nullptr
+    int64_t mask_batch;
+    int64_t mask_token;
+    float scale_within;         // of a_t . b_s
+    float scale_across;         // of a_t . state
+    float scale_update;         // of b_s (x) c_s
+    int shift;                  // the first state counts from the first token, not from before it
+    const float* first;         // [batch, heads, features, out_features] by these strides, or nullptr: zeros
+    int64_t first_row;
+    int64_t first_column;
+    float* last;                // the state after the last token, contiguous, or nullptr
+    float* states;              // [batch, heads, segments, features, out_features]: updates, then first states
+    int* counts;                // [batch, segments] tokens that count; unused with one segment
+    int64_t segment_chunks;     // set by plan_walk
+    int64_t segments;
+};
+
+constexpr int kWalkFeatures = 128;   // most features of a head
+void plan_walk(WalkArgs* a);
+hipError_t launch_walk(const WalkArgs& a, int dtype, hipStream_t stream);
+
+// out[r, g, :] = sum over its `shared` heads of partial[r, g * shared + i, :].
+struct HeadSumArgs {
+    const float* partial;       // [rows, kv_heads * shared, features] contiguous
+    void* out;                  // [rows, kv_heads, features] contiguous
+    int64_t rows;
+    int kv_heads;
+    int shared;
+    int features;
+};
+hipError_t launch_head_sum(const HeadSumArgs& a, int dtype, hipStream_t stream);
+
+struct AttentionStepArgs {
+    WalkTensor q;               // token strides unused
+    WalkTensor k;
+    WalkTensor v;
+    void* y;                    // [batch, heads, value_features] contiguous
+    int64_t batch;
+    int heads;
+    int features;
+    int value_features;
+    const float* log_decay;
+    const uint8_t* mask;        // [batch] or nullptr
+    float scale;
+    float* state;               // [batch, heads, features, value_features], batch stride state_batch
+    int64_t state_batch;
+};
+hipError_t launch_attention_step(const AttentionStepArgs& a, int dtype, hipStream_t stream);
+
 // Sets the calling thread's error message (lsso_hip_last_error) and returns code.
 int report(int code, const char* message) noexcept;
 int report_hip(hipError_t error, const char* where) noexcept;

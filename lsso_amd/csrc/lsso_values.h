@@ -79,4 +79,32 @@ struct Values<LSSO_HIP_F16> {
     }
 };
 
+// V (1, 2, 4 or 8) elements in one access (two of 8 FP32 elements).
+template <int T, int V>
+__device__ __forceinline__ void load_values(const typename Values<T>::Element* at, float (&v)[V]) {
+    if constexpr (V == 8) {
+        Values<T>::load8(at, v);
+    } else {
+        typename Values<T>::Element raw[V];
+        __builtin_memcpy(raw, at, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = Values<T>::load(raw + i);
+        }
+    }
+}
+template <int T, int V>
+__device__ __forceinline__ void store_values(typename Values<T>::Element* at, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        Values<T>::store8(at, v);
+    } else {
+        typename Values<T>::Element raw[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            Values<T>::store(raw + i, v[i]);
+        }
+        __builtin_memcpy(at, raw, sizeof(raw));
+    }
+}
+
 }  // namespace lsso_hip
