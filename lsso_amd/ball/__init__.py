@@ -1,5 +1,17 @@
 from .config import CoreMode, LSSOConfig
-from .layers import GatedFeedForward, ResidualDropout, TokenEmbedding
+from .layers import CausalMixer, GatedFeedForward, GroupNorm, ResidualDropout, TokenEmbedding
 from .model import LSSO
+from .reference import rotary_amplitude, rotary_frequencies
 
-__all__ = ["CoreMode", "GatedFeedForward", "LSSO", "LSSOConfig", "ResidualDropout", "TokenEmbedding"]
+__all__ = [
+    "CausalMixer",
+    "CoreMode",
+    "GatedFeedForward",
+    "GroupNorm",
+    "LSSO",
+    "LSSOConfig",
+    "ResidualDropout",
+    "TokenEmbedding",
+    "rotary_amplitude",
+    "rotary_frequencies",
+]

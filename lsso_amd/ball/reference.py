@@ -344,6 +344,205 @@ def dropout_add(
     return y.to(dtype=x.dtype)
 
 
+def rotary_frequencies(
+    rotary_features: int,
+    *,
+    base: float = _RANK_PHASE_BASE,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    original_length: int | None = None,
+    few_turns: float = 1.0,
+    many_turns: float = 32.0,
+) -> torch.Tensor:
+    """Radians a position of each pair of rotary positions, float64: base^(-2j / R).
+
+    For contexts ``factor`` times as long as a model was trained on, ``scaling``:
+    "linear" divides every frequency by the factor; "base" raises the base to
+    base * factor^(R / (R - 2)), which leaves the first pair and divides the last;
+    "turns" divides the pairs that make up to ``few_turns`` turns over
+    ``original_length`` positions, leaves those of ``many_turns`` and more, and goes
+    from one to the other in proportion to the turns."""
+
+    if not isinstance(rotary_features, int) or isinstance(rotary_features, bool):
+        raise TypeError(f"rotary_features must be an integer, got {type(rotary_features).__name__}")
+    if rotary_features < 2 or rotary_features % 2:
+        raise ValueError(f"rotary_features must be positive and even, got {rotary_features}")
+    if not base > 0.0 or not math.isfinite(base) or not factor > 0.0 or not math.isfinite(factor):
+        raise ValueError(f"base and factor must be positive, got {base} and {factor}")
+    half = rotary_features // 2
+    if scaling == "base":
+        if half == 1:
+            raise ValueError("scaling 'base' takes at least two pairs")
+        base = base * factor ** (half / (half - 1))
+    frequencies = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    if scaling == "linear":
+        return frequencies / factor
+    if scaling == "turns":
+        if original_length is None or original_length <= 0 or not few_turns < many_turns:
+            raise ValueError("scaling 'turns' takes a positive original_length and few_turns below many_turns")
+        turns = frequencies * (original_length / (2.0 * math.pi))
+        kept = ((turns - few_turns) / (many_turns - few_turns)).clamp(0.0, 1.0)
+        return frequencies * (kept + (1.0 - kept) / factor)
+    if scaling not in (None, "base"):
+        raise ValueError(f"scaling must be None, 'linear', 'base' or 'turns', got {scaling!r}")
+    return frequencies
+
+
+def rotary_amplitude(factor: float) -> float:
+    """What the turned features are multiplied by under scaling "turns": 1 + 0.1 ln factor."""
+
+    return 1.0 if factor <= 1.0 else 1.0 + 0.1 * math.log(factor)
+
+
+def rotary(
+    query: torch.Tensor,
+    key: torch.Tensor | None,
+    position_ids: torch.Tensor | None,
+    frequencies: torch.Tensor,
+    *,
+    layout: str = "interleaved",
+    amplitude: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The pairs of the first 2 * len(frequencies) features of [B, N, H, D] turned by
+    position * frequency, angles in FP64."""
+
+    if layout not in ("interleaved", "half"):
+        raise ValueError(f"layout must be 'interleaved' or 'half', got {layout!r}")
+    if position_ids is None:
+        position_ids = torch.arange(query.shape[1], device=query.device)
+    angles = position_ids.to(torch.float64)[..., None, None] * frequencies.to(torch.float64)
+    turned = 2 * frequencies.shape[0]
+
+    def turn(x: torch.Tensor) -> torch.Tensor:
+        calc_dtype = _calculation_dtype(x)
+        cos, sin = ((amplitude * value).to(calc_dtype) for value in (angles.cos(), angles.sin()))
+        value = x[..., :turned].to(calc_dtype)
+        if layout == "half":
+            first, second = value.chunk(2, dim=-1)
+            value = torch.cat((first * cos - second * sin, first * sin + second * cos), dim=-1)
+        else:
+            first, second = value[..., 0::2], value[..., 1::2]
+            value = torch.stack((first * cos - second * sin, first * sin + second * cos), dim=-1).flatten(-2)
+        return torch.cat((value.to(x.dtype), x[..., turned:]), dim=-1)
+
+    return turn(query), None if key is None else turn(key)
+
+
+def group_norm(
+    x: torch.Tensor,
+    groups: int,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    *,
+    eps: float = 1e-5,
+    activation: str | None = None,
+    row_mask: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """act((x - mean) / sqrt(var + eps) * weight + bias) of [B, ..., C], statistics over
+    the tokens that ``row_mask`` leaves and the channels of each group, in FP32 (FP64
+    for FP64 x), one cast; zeros for the others, which reach no gradient."""
+
+    calc_dtype = _calculation_dtype(x)
+    value = x.to(calc_dtype).reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+    kept = None if row_mask is None else row_mask.reshape(x.shape[0], -1, 1, 1)
+    if kept is not None:
+        value = torch.where(kept, value, torch.zeros_like(value))
+    tokens = value.shape[1] if kept is None else kept.sum(1, keepdim=True).clamp_min(1)
+    size = tokens * value.shape[3]
+    centred = value - value.sum((1, 3), keepdim=True) / size
+    if kept is not None:
+        centred = torch.where(kept, centred, torch.zeros_like(centred))
+    normal = (centred * torch.rsqrt(centred.square().sum((1, 3), keepdim=True) / size + eps)).reshape(x.shape)
+    if weight is not None:
+        normal = normal * weight.to(calc_dtype)
+    if bias is not None:
+        normal = normal + bias.to(calc_dtype)
+    act = {None: lambda z: z, "silu": functional.silu, "gelu": functional.gelu}[activation]
+    y = act(normal)
+    if row_mask is not None:
+        y = torch.where(row_mask[..., None], y, torch.zeros_like(y))
+    return y.to(x.dtype)
+
+
+_ATTENTION_CHUNK = 64
+
+
+def linear_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    log_decay: torch.Tensor,
+    *,
+    scale: float | None = None,
+    row_mask: torch.Tensor | None = None,
+    initial_state: torch.Tensor | None = None,
+    return_state: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """S_t = exp(log_decay) S_{t-1} + k_t (x) v_t, y_t = scale q_t S_t, by chunks in FP32
+    (FP64 for FP64 query).  Tokens that ``row_mask`` excludes leave S as it is; their y
+    is zero."""
+
+    batch, length, heads, features = query.shape
+    calc_dtype = _calculation_dtype(query)
+    scale = features**-0.5 if scale is None else scale
+    shared = heads // key.shape[2]
+    kept = torch.ones(batch, length, dtype=torch.bool, device=query.device) if row_mask is None else row_mask
+
+    def heads_first(x: torch.Tensor, repeat: int = 1) -> torch.Tensor:
+        x = x.to(calc_dtype)
+        x = torch.where(kept[..., None, None], x, torch.zeros_like(x))
+        return x.transpose(1, 2).repeat_interleave(repeat, dim=1)
+
+    q, k, v = heads_first(query), heads_first(key, shared), heads_first(value, shared)
+    # -inf forgets at once: 0 * -inf is kept out of the exponents.
+    rate = log_decay.to(calc_dtype).clamp_min(-1e30).view(1, heads, 1)
+    state = torch.zeros(batch, heads, features, v.shape[-1], dtype=calc_dtype, device=query.device)
+    if initial_state is not None:
+        state = initial_state.to(calc_dtype)
+    outputs = []
+    for begin in range(0, length, _ATTENTION_CHUNK):
+        some = slice(begin, begin + _ATTENTION_CHUNK)
+        rank = kept[:, some].cumsum(1).to(calc_dtype)[:, None, :]   # [B, 1, C]
+        total = rank[..., -1:]
+        apart = rank[..., :, None] - rank[..., None, :]
+        below = torch.ones(apart.shape[-2:], dtype=torch.bool, device=query.device).tril()
+        weights = torch.where(below, torch.exp(rate[..., None] * apart.clamp_min(0)), torch.zeros_like(apart))
+        scores = q[:, :, some] @ k[:, :, some].mT * weights
+        across = torch.exp(rate * rank)[..., None] * (q[:, :, some] @ state)
+        outputs.append(scores @ v[:, :, some] + across)
+        decayed = v[:, :, some] * torch.exp(rate * (total - rank))[..., None]
+        state = torch.exp(rate * total)[..., None] * state + k[:, :, some].mT @ decayed
+    y = torch.cat(outputs, dim=2) if outputs else v[:, :, :0]
+    y = (scale * y).transpose(1, 2)
+    y = torch.where(kept[..., None, None], y, torch.zeros_like(y)).to(query.dtype).contiguous()
+    return (y, state) if return_state else y
+
+
+def linear_attention_step(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    log_decay: torch.Tensor,
+    state: torch.Tensor,
+    *,
+    scale: float | None = None,
+    row_mask: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """One token of linear_attention; ``state`` is updated in place."""
+
+    calc_dtype = state.dtype
+    scale = query.shape[-1] ** -0.5 if scale is None else scale
+    shared = query.shape[1] // key.shape[1]
+    k, v = (x.to(calc_dtype).repeat_interleave(shared, dim=1) for x in (key, value))
+    new = torch.exp(log_decay.to(calc_dtype))[:, None, None] * state + k[..., :, None] * v[..., None, :]
+    y = scale * (query.to(calc_dtype)[..., None, :] @ new)[..., 0, :]
+    if row_mask is not None:
+        new = torch.where(row_mask[:, None, None, None], new, state)
+        y = torch.where(row_mask[:, None, None], y, torch.zeros_like(y))
+    state.copy_(new)
+    return y.to(query.dtype)
+
+
 __all__ = [
     "accretive_equilibrium_mix",
     "accretive_generator",
@@ -353,8 +552,14 @@ __all__ = [
     "dropout_keep",
     "embedding",
     "gated_feed_forward",
+    "group_norm",
     "linear",
+    "linear_attention",
+    "linear_attention_step",
     "qr_soft_frame",
     "rank_rotary",
+    "rotary",
+    "rotary_amplitude",
+    "rotary_frequencies",
     "rotary_inverse_frequency",
 ]
