@@ -740,27 +740,30 @@ typedef struct lsso_hip_linear_attention_shape {
     lsso_hip_head_strides v;
 } lsso_hip_linear_attention_shape;
 
-/* Device scratch bytes of lsso_hip_linear_attention, and (backward not 0) of
- * lsso_hip_linear_attention_backward. */
-int lsso_hip_linear_attention_workspace_bytes(const lsso_hip_linear_attention_shape* shape,
-                                              int backward, size_t* bytes);
+/* FP32 values that a forward can keep for its backward (0: none, the sequences are
+ * walked in one piece), and device scratch bytes of the forward and of the backward. */
+int lsso_hip_linear_attention_sizes(const lsso_hip_linear_attention_shape* shape,
+                                    size_t* kept_floats, size_t* forward_bytes,
+                                    size_t* backward_bytes);
 
 /* The forward over whole sequences.  log_decay: float32 [heads], at most 0 (-inf: S
  * is forgotten at once).  row_mask: optional device uint8 [batch, length]; tokens
  * whose byte is 0 leave S as it is, whatever they hold, and their y is zero.
  * initial_state: float32 [batch, heads, features, value_features] contiguous or
- * NULL (zeros).  y: contiguous [batch, length, heads, value_features] of dtype.
+ * NULL (zeros).  kept: lsso_hip_linear_attention_sizes' kept_floats, for the backward,
+ * or NULL.  y: contiguous [batch, length, heads, value_features] of dtype.
  * final_state: as initial_state, S after the last token, or NULL.
  * S is FP32; products take 16-bit operands and accumulate in FP32, with P, S and
  * the decayed v in two 16-bit parts each.  workspace: 256-byte aligned. */
 int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, const void* q,
                               const void* k, const void* v, const float* log_decay,
-                              const uint8_t* row_mask, const float* initial_state, void* y,
-                              float* final_state, void* workspace, size_t workspace_bytes,
-                              void* stream);
+                              const uint8_t* row_mask, const float* initial_state, float* kept,
+                              void* y, float* final_state, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* First-order gradients for grad_y [batch, length, heads, value_features] of dtype
  * (strides grad_strides) and grad_final_state (float32 contiguous, or NULL: zeros).
+ * kept: what the forward of the same shape kept, or NULL (it is made again).
  * grad_q, grad_k, grad_v: contiguous, of dtype; grad_initial_state: float32
  * contiguous; each may be NULL.  log_decay has no gradient.  Tokens that row_mask
  * excludes have zero gradients and reach none.  Deterministic. */
@@ -769,7 +772,7 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
                                        const float* grad_final_state, const void* q, const void* k,
                                        const void* v, const float* log_decay,
                                        const uint8_t* row_mask, const float* initial_state,
-                                       void* grad_q, void* grad_k, void* grad_v,
+                                       const float* kept, void* grad_q, void* grad_k, void* grad_v,
                                        float* grad_initial_state, void* workspace,
                                        size_t workspace_bytes, void* stream);
 

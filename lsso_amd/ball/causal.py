@@ -26,7 +26,7 @@ SYMBOLS = (
     "lsso_hip_group_norm_sizes",
     "lsso_hip_group_norm",
     "lsso_hip_group_norm_backward",
-    "lsso_hip_linear_attention_workspace_bytes",
+    "lsso_hip_linear_attention_sizes",
     "lsso_hip_linear_attention",
     "lsso_hip_linear_attention_backward",
     "lsso_hip_linear_attention_step",
@@ -101,13 +101,13 @@ def declare(library: ctypes.CDLL) -> None:
         # shape, x, weight, bias, mask, statistics, y, workspace, bytes, stream
         ("lsso_hip_group_norm_backward", [norm_p, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, size, vp]),
         # shape, grad_y, x, weight, bias, mask, statistics, grads (x, weight, bias), workspace, bytes, stream
-        ("lsso_hip_linear_attention_workspace_bytes", [attention_p, i32, size_p]),
-        ("lsso_hip_linear_attention", [attention_p, vp, vp, vp, vp, vp, vp, vp, vp, vp, size, vp]),
-        # shape, q, k, v, log_decay, mask, initial state, y, final state, workspace, bytes, stream
+        ("lsso_hip_linear_attention_sizes", [attention_p, size_p, size_p, size_p]),
+        ("lsso_hip_linear_attention", [attention_p, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, size, vp]),
+        # shape, q, k, v, log_decay, mask, initial state, kept, y, final state, workspace, bytes, stream
         ("lsso_hip_linear_attention_backward", [attention_p, vp, ctypes.POINTER(HeadStrides), vp, vp, vp, vp, vp, vp,
-                                                vp, vp, vp, vp, vp, vp, size, vp]),
-        # shape, grad_y, strides, grad of the final state, q, k, v, log_decay, mask, initial state, grads (q, k, v,
-        # initial state), workspace, bytes, stream
+                                                vp, vp, vp, vp, vp, vp, vp, size, vp]),
+        # shape, grad_y, strides, grad of the final state, q, k, v, log_decay, mask, initial state, kept, grads (q, k,
+        # v, initial state), workspace, bytes, stream
         ("lsso_hip_linear_attention_step", [attention_p, vp, vp, vp, vp, vp, vp, i64, vp, vp]),
         # shape, q, k, v, log_decay, mask, state, batch stride, y, stream
     ):
@@ -385,16 +385,16 @@ def group_norm(
 
 # ----------------------------------------------------------- linear attention
 @lru_cache(maxsize=1024)
-def _attention_plan(fields: tuple, strides: tuple, backward: int):
-    """(the native shape, its workspace's bytes): they depend on these numbers alone."""
+def _attention_plan(fields: tuple, strides: tuple):
+    """(the native shape, kept floats, forward and backward bytes): they depend on
+    these numbers alone."""
 
     hip = _hip()
     library = hip._library()
     native = LinearAttentionShape(*fields, *(HeadStrides(*s) for s in strides))
-    size = ctypes.c_size_t()
-    hip._check(library.lsso_hip_linear_attention_workspace_bytes(
-        ctypes.byref(native), backward, ctypes.byref(size)), library)
-    return ctypes.byref(native), size.value
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    hip._check(library.lsso_hip_linear_attention_sizes(ctypes.byref(native), *map(ctypes.byref, sizes)), library)
+    return ctypes.byref(native), *(size.value for size in sizes)
 
 
 def _attention_fields(query, key, value, scale):
@@ -402,15 +402,18 @@ def _attention_fields(query, key, value, scale):
     return batch, length, heads, key.shape[2], features, value.shape[3], _HALF_CODES[query.dtype], scale
 
 
-def _attention_launch(query, key, value, log_decay, scale, row_mask, initial_state, return_state):
+def _attention_launch(query, key, value, log_decay, scale, row_mask, initial_state, return_state, keep):
+    """(y, the last state or None, and with ``keep`` what the backward reads or None)."""
+
     hip = _hip()
     library = hip._library()
     device = query.device
     query, key, value = _unit(query), _unit(key), _unit(value)
     mask, mask_ptr = _mask_pointer(row_mask, query.shape[:2], device)
-    native, size = _attention_plan(
-        _attention_fields(query, key, value, scale), tuple(t.stride()[:3] for t in (query, key, value)), 0
+    native, kept, size, _ = _attention_plan(
+        _attention_fields(query, key, value, scale), tuple(t.stride()[:3] for t in (query, key, value))
     )
+    states = torch.empty(kept, dtype=torch.float32, device=device) if keep and kept else None
     state = initial_state if initial_state is None else initial_state.contiguous()
     batch, length, heads, features = query.shape
     y = torch.empty((batch, length, heads, value.shape[3]), dtype=query.dtype, device=device)
@@ -421,21 +424,23 @@ def _attention_launch(query, key, value, log_decay, scale, row_mask, initial_sta
     status = hip._launch(
         library.lsso_hip_linear_attention, device,
         native, query.data_ptr(), key.data_ptr(), value.data_ptr(), log_decay.data_ptr(), mask_ptr, _pointer(state),
-        y.data_ptr(), _pointer(last), _pointer(workspace), size,
+        _pointer(states), y.data_ptr(), _pointer(last), _pointer(workspace), size,
     )
     hip._check(status, library)
-    return y, last
+    return y, last, states
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, initial_state, log_decay, scale, row_mask, return_state):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(query, key, value, initial_state, log_decay, row_mask)
+        y, last, states = _attention_launch(
+            query, key, value, log_decay, scale, row_mask, initial_state, return_state, ctx.needs_input_grad[0]
+        )
+        saved = (query, key, value, initial_state, log_decay, row_mask, states)
+        ctx.save_for_backward(*saved)
         ctx.scale = scale
-        ctx.like = [None if v is None else (v.dtype, tuple(v.shape))
-                    for v in (query, key, value, initial_state, log_decay, row_mask)]
-        y, last = _attention_launch(query, key, value, log_decay, scale, row_mask, initial_state, return_state)
+        ctx.like = [None if v is None else (v.dtype, tuple(v.shape)) for v in saved]
         return (y, last) if return_state else y
 
     @staticmethod
@@ -447,7 +452,7 @@ class _LinearAttention(torch.autograd.Function):
         if (grad_y is None and grad_last is None) or not any(needs):
             return (None,) * 8
         device = (grad_last if grad_y is None else grad_y).device
-        names = ("query", "key", "value", "initial_state", "log_decay", "row_mask")
+        names = ("query", "key", "value", "initial_state", "log_decay", "row_mask", "states")
         saved = list(ctx.saved_tensors)
         for i, (name, like) in enumerate(zip(names, ctx.like)):
             if saved[i] is None:
@@ -455,7 +460,7 @@ class _LinearAttention(torch.autograd.Function):
             if saved[i].device != device or saved[i].dtype != like[0] or tuple(saved[i].shape) != like[1]:
                 _saved(saved[i], name, *like, device)
             saved[i] = _unit(saved[i]) if i < 3 else saved[i].contiguous()
-        query, key, value, initial_state, log_decay, row_mask = saved
+        query, key, value, initial_state, log_decay, row_mask, states = saved
         batch, length, heads, _features = query.shape
         if grad_y is None:
             grad_y = torch.zeros((1, 1, 1, value.shape[3]), dtype=query.dtype, device=device)
@@ -466,15 +471,15 @@ class _LinearAttention(torch.autograd.Function):
             torch.empty(like[1], dtype=like[0], device=device) if need else None
             for need, like in zip(needs, ctx.like)
         ]
-        native, size = _attention_plan(
-            _attention_fields(query, key, value, ctx.scale), tuple(t.stride()[:3] for t in (query, key, value)), 1
+        native, _, _, size = _attention_plan(
+            _attention_fields(query, key, value, ctx.scale), tuple(t.stride()[:3] for t in (query, key, value))
         )
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         status = hip._launch(
             library.lsso_hip_linear_attention_backward, device,
             native, grad_y.data_ptr(), ctypes.byref(HeadStrides(*grad_y.stride()[:3])), _pointer(grad_last),
             query.data_ptr(), key.data_ptr(), value.data_ptr(), log_decay.data_ptr(), _pointer(row_mask),
-            _pointer(initial_state), *(_pointer(grad) for grad in grads), _pointer(workspace), size,
+            _pointer(initial_state), _pointer(states), *(_pointer(grad) for grad in grads), _pointer(workspace), size,
         )
         hip._check(status, library)
         return (*grads, None, None, None, None)
@@ -559,7 +564,9 @@ def linear_attention(
         or (initial_state is not None and initial_state.requires_grad)
     ):
         return _LinearAttention.apply(query, key, value, initial_state, log_decay, scale, row_mask, return_state)
-    y, last = _attention_launch(query, key, value, log_decay, scale, row_mask, initial_state, return_state)
+    y, last, _ = _attention_launch(
+        query, key, value, log_decay, scale, row_mask, initial_state, return_state, False
+    )
     return (y, last) if return_state else y
 
 
@@ -598,9 +605,9 @@ def linear_attention_step(
     device = query.device
     query, key, value, log_decay = _unit(query), _unit(key), _unit(value), log_decay.contiguous()
     mask, mask_ptr = _mask_pointer(row_mask, (batch,), device)
-    native, _ = _attention_plan(
+    native, *_ = _attention_plan(
         (batch, 1, heads, key.shape[1], features, out, _HALF_CODES[query.dtype], scale),
-        tuple((t.stride(0), 0, t.stride(1)) for t in (query, key, value)), 0,
+        tuple((t.stride(0), 0, t.stride(1)) for t in (query, key, value)),
     )
     y = torch.empty((batch, heads, out), dtype=query.dtype, device=device)
     status = hip._launch(

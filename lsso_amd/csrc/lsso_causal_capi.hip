@@ -158,27 +158,27 @@ lsso_hip::WalkArgs walk_args(const lsso_hip_linear_attention_shape& s, const flo
     return w;
 }
 
-// Bytes of a walk's states and counts.
-size_t walk_bytes(const lsso_hip_linear_attention_shape& s, lsso_hip::WalkArgs* w, size_t* counts) {
-    lsso_hip::plan_walk(w);
-    if (w->segments == 1) {
-        return 0;
-    }
-    *counts = round256(sizeof(float) * static_cast<size_t>(s.batch * s.heads * w->segments) *
-                       static_cast<size_t>(s.features * s.value_features));
-    return *counts + round256(sizeof(int) * static_cast<size_t>(s.batch * w->segments));
-}
-
 struct AttentionLayout {
     size_t counts = 0;
-    size_t partial = 0;   // FP32 gradients of every head, where heads share one
+    size_t states = 0;
+    size_t partial = 0;       // FP32 gradients of every head, where heads share one
+    size_t kept_floats = 0;   // of states
     size_t bytes = 0;
 };
 
+// The workspace of a walk: updates, counts and states (which a training forward
+// keeps for its backward instead).
 AttentionLayout attention_layout(const lsso_hip_linear_attention_shape& s, bool backward) {
     AttentionLayout l;
     lsso_hip::WalkArgs w = walk_args(s, nullptr, nullptr);
-    l.bytes = walk_bytes(s, &w, &l.counts);
+    lsso_hip::plan_walk(&w);
+    if (w.segments > 1) {
+        const size_t state = static_cast<size_t>(s.batch * s.heads) * static_cast<size_t>(s.features * s.value_features);
+        l.counts = round256(sizeof(float) * state * static_cast<size_t>(w.pieces));
+        l.states = l.counts + round256(sizeof(int) * static_cast<size_t>(s.batch * w.pieces));
+        l.kept_floats = state * static_cast<size_t>(w.segments);
+        l.bytes = l.states + round256(sizeof(float) * l.kept_floats);
+    }
     if (backward && s.kv_heads < s.heads) {
         const int64_t widest = s.features > s.value_features ? s.features : s.value_features;
         l.partial = l.bytes;
@@ -359,22 +359,25 @@ int lsso_hip_group_norm_backward(const lsso_hip_group_norm_shape* shape, const v
     return error == hipSuccess ? LSSO_HIP_OK : report_hip(error, "group norm gradient launch");
 }
 
-int lsso_hip_linear_attention_workspace_bytes(const lsso_hip_linear_attention_shape* shape, int backward,
-                                              size_t* bytes) {
+int lsso_hip_linear_attention_sizes(const lsso_hip_linear_attention_shape* shape, size_t* kept_floats,
+                                    size_t* forward_bytes, size_t* backward_bytes) {
     const int status = check_linear_attention(shape);
     if (status != LSSO_HIP_OK) {
         return status;
     }
-    if (bytes == nullptr) {
-        return report(LSSO_HIP_EINVAL, "bytes must not be NULL");
+    if (kept_floats == nullptr || forward_bytes == nullptr || backward_bytes == nullptr) {
+        return report(LSSO_HIP_EINVAL, "kept_floats and the bytes must not be NULL");
     }
-    *bytes = attention_layout(*shape, backward != 0).bytes;
+    const AttentionLayout l = attention_layout(*shape, false);
+    *kept_floats = l.kept_floats;
+    *forward_bytes = l.bytes;
+    *backward_bytes = attention_layout(*shape, true).bytes;
     return LSSO_HIP_OK;
 }
 
 int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, const void* q, const void* k,
                               const void* v, const float* log_decay, const uint8_t* row_mask,
-                              const float* initial_state, void* y, float* final_state, void* workspace,
+                              const float* initial_state, float* kept, void* y, float* final_state, void* workspace,
                               size_t workspace_bytes, void* stream) {
     const int status = check_linear_attention(shape);
     if (status != LSSO_HIP_OK) {
@@ -388,13 +391,14 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
                          !aligned(k, 2) || !aligned(v, 2) || !aligned(y, 2))) {
         return report(LSSO_HIP_EINVAL, "q, k, v and y must not be NULL and be aligned to their type");
     }
-    if (log_decay == nullptr || !aligned(log_decay, 4) || !aligned(initial_state, 4) || !aligned(final_state, 4)) {
+    if (log_decay == nullptr || !aligned(log_decay, 4) || !aligned(initial_state, 4) || !aligned(final_state, 4) ||
+        !aligned(kept, 4)) {
         return report(LSSO_HIP_EINVAL, "log_decay must not be NULL, it and the states be aligned to float32");
     }
     const AttentionLayout l = attention_layout(s, false);
     if (bad_workspace(workspace, workspace_bytes, l.bytes)) {
         return report(LSSO_HIP_EINVAL,
-                      "workspace must be 256-byte aligned and of lsso_hip_linear_attention_workspace_bytes()");
+                      "workspace must be 256-byte aligned and of lsso_hip_linear_attention_sizes()");
     }
     char* ws = static_cast<char*>(workspace);
     lsso_hip::WalkArgs w = walk_args(s, log_decay, row_mask);
@@ -411,8 +415,12 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
     w.first_row = s.value_features;
     w.first_column = 1;
     w.last = final_state;
-    w.states = reinterpret_cast<float*>(ws);
+    w.fine = final_state != nullptr ? 1 : 0;
+    w.updates = reinterpret_cast<float*>(ws);
     w.counts = reinterpret_cast<int*>(ws + l.counts);
+    w.states = kept != nullptr ? kept : reinterpret_cast<float*>(ws + l.states);
+    w.states_row = s.value_features;
+    w.states_column = 1;
     lsso_hip::plan_walk(&w);
     const hipError_t error = lsso_hip::launch_walk(w, s.dtype, static_cast<hipStream_t>(stream));
     return error == hipSuccess ? LSSO_HIP_OK : report_hip(error, "linear attention launch");
@@ -421,7 +429,8 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
 int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* shape, const void* grad_y,
                                        const lsso_hip_head_strides* grad_strides, const float* grad_final_state,
                                        const void* q, const void* k, const void* v, const float* log_decay,
-                                       const uint8_t* row_mask, const float* initial_state, void* grad_q, void* grad_k,
+                                       const uint8_t* row_mask, const float* initial_state, const float* kept,
+                                       void* grad_q, void* grad_k,
                                        void* grad_v, float* grad_initial_state, void* workspace,
                                        size_t workspace_bytes, void* stream) {
     const int status = check_linear_attention(shape);
@@ -440,13 +449,13 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         return report(LSSO_HIP_EINVAL, "q, k, v and grad_y must not be NULL and be aligned to their type");
     }
     if (log_decay == nullptr || !aligned(log_decay, 4) || !aligned(initial_state, 4) || !aligned(grad_final_state, 4) ||
-        !aligned(grad_initial_state, 4) || !aligned(grad_q, 2) || !aligned(grad_k, 2) || !aligned(grad_v, 2)) {
+        !aligned(grad_initial_state, 4) || !aligned(kept, 4) || !aligned(grad_q, 2) || !aligned(grad_k, 2) || !aligned(grad_v, 2)) {
         return report(LSSO_HIP_EINVAL, "log_decay must not be NULL, it, the states and the gradients be aligned");
     }
     const AttentionLayout l = attention_layout(s, true);
     if (bad_workspace(workspace, workspace_bytes, l.bytes)) {
         return report(LSSO_HIP_EINVAL,
-                      "workspace must be 256-byte aligned and of lsso_hip_linear_attention_workspace_bytes()");
+                      "workspace must be 256-byte aligned and of lsso_hip_linear_attention_sizes()");
     }
     char* ws = static_cast<char*>(workspace);
     const auto queue = static_cast<hipStream_t>(stream);
@@ -464,8 +473,11 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         w.features = static_cast<int>(features);
         w.out_features = static_cast<int>(out_features);
         w.scale_within = s.scale;
-        w.states = reinterpret_cast<float*>(ws);
+        w.updates = reinterpret_cast<float*>(ws);
         w.counts = reinterpret_cast<int*>(ws + l.counts);
+        w.states = reinterpret_cast<float*>(ws + l.states);
+        w.states_row = out_features;
+        w.states_column = 1;
         lsso_hip::plan_walk(&w);
         return w;
     };
@@ -478,9 +490,17 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         w.first = initial_state;   // S transposed
         w.first_row = 1;
         w.first_column = s.value_features;
+        if (kept != nullptr) {   // the forward's, read transposed
+            w.reuse = 1;
+            w.states = const_cast<float*>(kept);
+            w.states_row = 1;
+            w.states_column = s.value_features;
+        }
         error = lsso_hip::launch_walk(w, s.dtype, queue);
     }
-    // To the front: S's gradient, from that of the last state on.
+    // To the front: S's gradient, from that of the last state on.  dk's states are
+    // dv's, transposed.
+    bool walked = false;
     const auto back = [&](const lsso_hip::WalkTensor& a, const lsso_hip::WalkTensor& b, const lsso_hip::WalkTensor& c,
                           int64_t features, int64_t out_features, void* grad, bool transposed, float* first_state) {
         const bool summed = shared > 1 && grad != nullptr;
@@ -500,6 +520,13 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         w.first_row = transposed ? 1 : out_features;
         w.first_column = transposed ? features : 1;
         w.last = first_state;
+        w.fine = first_state != nullptr ? 1 : 0;
+        if (walked) {
+            w.reuse = 1;
+            w.states_row = 1;
+            w.states_column = features;
+        }
+        walked = true;
         error = lsso_hip::launch_walk(w, s.dtype, queue);
         if (error == hipSuccess && summed && s.length > 0) {
             lsso_hip::HeadSumArgs sum{};

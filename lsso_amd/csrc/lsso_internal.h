@@ -566,10 +566,17 @@ struct WalkArgs {
     int64_t first_row;
     int64_t first_column;
     float* last;                // the state after the last token, contiguous, or nullptr
-    float* states;              // [batch, heads, segments, features, out_features]: updates, then first states
-    int* counts;                // [batch, segments] tokens that count; unused with one segment
-    int64_t segment_chunks;     // set by plan_walk
+    int fine;                   // the last state is asked for: BF16 updates in three parts
+    float* updates;             // [batch, heads, pieces, features, out_features]: what each piece adds to the state
+    int* counts;                // [batch, pieces] tokens that count
+    float* states;              // [batch, heads, segments, features, out_features]: before each segment's first token
+    int64_t states_row;         // their strides
+    int64_t states_column;
+    int reuse;                  // states are there already
+    int64_t segment_chunks;     // set by plan_walk: whole pieces
     int64_t segments;
+    int64_t piece_chunks;
+    int64_t pieces;             // of all segments but the last; 0 with one segment
 };
 
 constexpr int kWalkFeatures = 128;   // most features of a head

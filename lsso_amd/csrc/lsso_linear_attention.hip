@@ -79,43 +79,67 @@ __device__ __forceinline__ u32x4 join(const u32x2& low, const u32x2& high) {
 }
 
 // A chunk of one tensor on its way to LDS: 64 rows of `features` 16-bit values,
-// in 16-byte pieces, zeros past the features.
+// in 16-byte pieces.  WHOLE: whole pieces, and 64 rows within a buffer's 2^31
+// bytes, so that a piece's address is the chunk's and a lane's own offset; rows
+// and pieces that do not exist are zeros or, within the buffer, another row's.
 template <int WIDTH, int THREADS, bool WHOLE>
 struct ChunkLoads {
     static constexpr int kPieces = WIDTH / 8;                       // of a row
     static constexpr int kEach = kChunk * kPieces / THREADS;        // of a thread
     static_assert(kChunk * kPieces % THREADS == 0, "whole rounds");
     u32x4 raw[kEach];
+    const uint16_t* data;
+    int64_t stride;
+    int features;
+    uint32_t step;      // bytes between rows
+    uint32_t offset;    // of this thread's first piece in a whole chunk
 
     __device__ __forceinline__ static int row(int i) { return (static_cast<int>(threadIdx.x) + i * THREADS) / kPieces; }
     __device__ __forceinline__ static int column(int i) {
         return 8 * ((static_cast<int>(threadIdx.x) + i * THREADS) % kPieces);
     }
-    // rows: how many of the chunk exist; those past it read the last one.
-    __device__ __forceinline__ void issue(const uint16_t* from, int64_t stride, int rows, int features, int column0) {
+    __device__ __forceinline__ ChunkLoads(const uint16_t* data_, int64_t stride_, int features_)
+        : data(data_), stride(stride_), features(features_) {
+        static_assert(THREADS % kPieces == 0, "a thread's pieces are of one column");
+        step = static_cast<uint32_t>(2 * (stride < 0 ? -stride : stride));
+        offset = static_cast<uint32_t>(stride < 0 ? kChunk - 1 - row(0) : row(0)) * step + 2 * column(0);
+    }
+    // The `rows` rows from `token` on.
+    __device__ __forceinline__ void issue(int64_t token, int rows) {
+        if constexpr (WHOLE) {
+            const bool turned = stride < 0;
+            const BufferRsrc buffer =
+                make_buffer(data + (turned ? token + rows - 1 : token) * stride,
+                            static_cast<int64_t>(rows - 1) * step + 2 * features);
+            // Past the last row offsets wrap round, and out of the buffer.
+            const uint32_t at = offset - (turned ? static_cast<uint32_t>(kChunk - rows) * step : 0u);
+            const uint32_t round = (turned ? 0u - step : step) * (THREADS / kPieces);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int r = row(i) < rows ? row(i) : rows - 1;
-            const uint16_t* at = from + r * stride;
-            const int k = column0 + column(i);
-            if constexpr (WHOLE) {
-                raw[i] = load16_unaligned(at + (k < features ? k : 0));
-            } else if (features >= 8) {
-                raw[i] = load16_unaligned(at + piece_start<8>(k, features));
-            } else {
-                raw[i] = load_short_piece(at, k, features);
+            for (int i = 0; i < kEach; ++i) {
+                raw[i] = buffer_load16(buffer, at + i * round);
+            }
+        } else {
+            const uint16_t* from = data + token * stride;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint16_t* at = from + (row(i) < rows ? row(i) : rows - 1) * stride;
+                if (features >= 8) {
+                    raw[i] = load16_unaligned(at + piece_start<8>(column(i), features));
+                } else {
+                    raw[i] = load_short_piece(at, column(i), features);
+                }
             }
         }
     }
-    __device__ __forceinline__ u32x4 piece(int i, uint64_t kept, int features, int column0) const {
-        const int k = column0 + column(i);
+    // With zeros past the features, and for rows that do not count.
+    __device__ __forceinline__ u32x4 piece(int i, uint64_t kept) const {
         u32x4 v = raw[i];
         if constexpr (!WHOLE) {
             if (features >= 8) {
-                v = align_piece16(v, k, features);
+                v = align_piece16(v, column(i), features);
             }
         }
-        const bool in = k < features && ((kept >> row(i)) & 1) != 0;
+        const bool in = column(i) < features && ((kept >> row(i)) & 1) != 0;
         return in ? v : (u32x4){0u, 0u, 0u, 0u};
     }
 };
@@ -129,31 +153,43 @@ __device__ __forceinline__ u32x4 read_columns(const uint16_t* at, int pitch) {
     return (u32x4){low[0], low[1], high[0], high[1]};
 }
 
+__device__ __forceinline__ void buffer_store8(u32x2 value, BufferRsrc buffer, uint32_t offset) {
+    typedef __attribute__((ext_vector_type(2))) unsigned int Pair;
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Pair, value), buffer, offset, 0, 0);
+}
+
 __device__ __forceinline__ int64_t offset_of(const WalkTensor& t, int64_t batch, int head) {
     return batch * t.batch + (head / t.heads_per) * t.head;
 }
 
 // T: type; KT: 32-feature steps of a and b; NW: waves; WE: 16-column blocks of c
-// and S in a wave; WHOLE: rows are whole 16-byte pieces; STATES: the segment's
-// state alone.
-template <int T, int KT, int NW, int WE, bool WHOLE, bool STATES>
-__global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
+// and S in a wave; WHOLE: rows are whole 16-byte pieces; PARTS: of the decayed c;
+// STATES: the state alone that a piece of the sequence adds to.  Three waves of a
+// SIMD where the registers of a form allow it.
+template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE, bool STATES>
+__global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2) void walk_kernel(WalkArgs a) {
     constexpr int kThreads = 64 * NW;
     constexpr int kFeatures = 32 * KT;
     constexpr int kColumns = 16 * NW * WE;
     constexpr int kPitch = kFeatures + 8;        // rows 16 bytes apart modulo the banks
     constexpr int kColumnPitch = kColumns + 8;
-    constexpr int kParts = T == LSSO_HIP_BF16 ? 3 : 2;   // of the decayed c
+    constexpr int kPart = kTiles * 2 * 64 * 8;   // values of one part of P
     __shared__ __attribute__((aligned(16))) uint16_t lds_a[STATES ? 8 : kChunk * kPitch];
     __shared__ __attribute__((aligned(16))) uint16_t lds_b[kChunk * kPitch];
     __shared__ __attribute__((aligned(16))) uint16_t lds_c[kChunk * kColumnPitch];
     // P in operand order: [part][tile of t][32 s][lane][8 s].
-    __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : 2 * kTiles * 2 * 64 * 8];
-    __shared__ __attribute__((aligned(16))) float rank[kChunk];   // kept tokens of the chunk up to each
+    __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : 2 * kPart];
+    // Of each token of the chunk: the kept ones up to it; l to the power of the kept
+    // ones behind it, times scale_update; of those from it to the end of its 16; of
+    // those up to it, times scale_across.
+    __shared__ __attribute__((aligned(16))) float rank[kChunk];
+    __shared__ __attribute__((aligned(16))) float to_end[kChunk];
+    __shared__ __attribute__((aligned(16))) float to_tile[kChunk];
+    __shared__ __attribute__((aligned(16))) float from_start[kChunk];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
-    const int wave = tid >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int in = lane & 15;
     const int group = lane >> 4;
 
@@ -164,155 +200,196 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
     block /= blocks_across;
     const int head = static_cast<int>(block % a.heads);
     block /= a.heads;
-    const int64_t segments = STATES ? a.segments - 1 : a.segments;   // the last one's state is the walk's own
-    const int64_t segment = block % segments;
-    const int64_t batch = block / segments;
+    const int64_t parts = STATES ? a.pieces : a.segments;
+    const int64_t part = block % parts;
+    const int64_t batch = block / parts;
+    const int64_t system = batch * a.heads + head;
+    const int64_t size = static_cast<int64_t>(a.features) * a.out_features;
 
     const uint16_t* from_a = static_cast<const uint16_t*>(a.a.data) + offset_of(a.a, batch, head);
     const uint16_t* from_b = static_cast<const uint16_t*>(a.b.data) + offset_of(a.b, batch, head);
     const uint16_t* from_c = static_cast<const uint16_t*>(a.c.data) + offset_of(a.c, batch, head);
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + batch * a.mask_batch;
     const float rate = decay_rate(a.log_decay[head]);
-    const int64_t slot = (batch * a.heads + head) * static_cast<int64_t>(a.features) * a.out_features;
 
     const int64_t chunks = (a.length + kChunk - 1) / kChunk;
-    const int64_t begin = segment * a.segment_chunks;
-    const int64_t end = begin + a.segment_chunks < chunks ? begin + a.segment_chunks : chunks;
+    const int64_t step = STATES ? a.piece_chunks : a.segment_chunks;
+    const int64_t begin = part * step;
+    const int64_t end = begin + step < chunks ? begin + step : chunks;
 
-    // S: rows 16 dt + 4 group + r, column column0 + 16 (wave WE + we) + in.
-    f32x4 state[2 * KT][WE];
-#pragma unroll
-    for (int dt = 0; dt < 2 * KT; ++dt) {
-#pragma unroll
-        for (int we = 0; we < WE; ++we) {
-            state[dt][we] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        }
-    }
-    const auto state_row = [&](int dt, int r) { return 16 * dt + 4 * group + r; };
-    const auto state_column = [&](int we) { return column0 + 16 * (wave * WE + we) + in; };
-    // 1 as long as the exponents of the first state are one less than those of the tokens.
-    int pending = 0;
-    if constexpr (!STATES) {
-        const float* first = nullptr;
-        int64_t row_stride = a.out_features;
-        int64_t column_stride = 1;
-        if (a.segments > 1) {
-            first = a.states + ((batch * a.heads + head) * a.segments + segment) *
-                                   (static_cast<int64_t>(a.features) * a.out_features);
-        } else if (a.first != nullptr) {
-            first = a.first + slot;
-            row_stride = a.first_row;
-            column_stride = a.first_column;
-        }
-        if (first != nullptr) {
-#pragma unroll
-            for (int dt = 0; dt < 2 * KT; ++dt) {
-#pragma unroll
-                for (int we = 0; we < WE; ++we) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = state_row(dt, r);
-                        const int e = state_column(we);
-                        if (d < a.features && e < a.out_features) {
-                            state[dt][we][r] = first[d * row_stride + e * column_stride];
-                        }
-                    }
-                }
-            }
-        }
-        pending = a.shift;
-        for (int64_t i = 0; i < segment && pending != 0; ++i) {
-            pending = a.counts[batch * a.segments + i] == 0 ? 1 : 0;
-        }
-    }
-    int64_t counted = 0;
-
-    ChunkLoads<kFeatures, kThreads, WHOLE> loads_a;
-    ChunkLoads<kFeatures, kThreads, WHOLE> loads_b;
-    ChunkLoads<kColumns, kThreads, WHOLE> loads_c;
+    ChunkLoads<kFeatures, kThreads, WHOLE> loads_a(from_a, a.a.token, a.features);
+    ChunkLoads<kFeatures, kThreads, WHOLE> loads_b(from_b, a.b.token, a.features);
+    ChunkLoads<kColumns, kThreads, WHOLE> loads_c(from_c + column0, a.c.token, a.out_features - column0);
     uint8_t kept_byte = 0;
     const auto issue = [&](int64_t chunk) {
         const int64_t token = chunk * kChunk;
         const int rows = static_cast<int>(a.length - token < kChunk ? a.length - token : kChunk);
         if constexpr (!STATES) {
-            loads_a.issue(from_a + token * a.a.token, a.a.token, rows, a.features, 0);
+            loads_a.issue(token, rows);
         }
-        loads_b.issue(from_b + token * a.b.token, a.b.token, rows, a.features, 0);
-        loads_c.issue(from_c + token * a.c.token, a.c.token, rows, a.out_features, column0);
+        loads_b.issue(token, rows);
+        loads_c.issue(token, rows);
         kept_byte = lane >= rows ? 0 : (mask == nullptr ? 1 : mask[(token + lane) * a.mask_token]);
     };
     if (begin < end) {
         issue(begin);
     }
+
+    // S: rows 16 dt + 4 group + r, column column0 + 16 (wave WE + we) + in.
+    f32x4 state[2 * KT][WE];
+    const auto state_row = [](int lane_, int dt, int r) { return 16 * dt + 4 * (lane_ >> 4) + r; };
+    const auto state_column = [&](int lane_, int we) { return column0 + 16 * (wave * WE + we) + (lane_ & 15); };
+    const float* first = nullptr;
+    int64_t row_stride = a.out_features;
+    int64_t column_stride = 1;
+    // 1 as long as the exponents of the first state are one less than those of the tokens.
+    int pending = 0;
+    if constexpr (!STATES) {
+        if (a.segments > 1) {
+            first = a.states + (system * a.segments + part) * size;
+            row_stride = a.states_row;
+            column_stride = a.states_column;
+        } else if (a.first != nullptr) {
+            first = a.first + system * size;
+            row_stride = a.first_row;
+            column_stride = a.first_column;
+        }
+        pending = a.shift;
+        for (int64_t i = 0; i < part * (a.segment_chunks / a.piece_chunks) && pending != 0; ++i) {
+            pending = a.counts[batch * a.pieces + i] == 0 ? 1 : 0;
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < 2 * KT; ++dt) {
+#pragma unroll
+        for (int we = 0; we < WE; ++we) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = state_row(lane, dt, r);
+                const int e = state_column(lane, we);
+                float v = 0.0f;
+                if (!STATES && first != nullptr) {   // uniform
+                    const bool in_state = d < a.features && e < a.out_features;
+                    v = first[in_state ? d * row_stride + e * column_stride : 0];
+                    v = in_state ? v : 0.0f;
+                }
+                state[dt][we][r] = v;
+            }
+        }
+    }
+    if constexpr (!STATES) {
+        // Of a short tile the other half of its 32 s: zeros, and never written again.
+#pragma unroll
+        for (int i = 0; i < kTiles; i += 2) {
+            if (wave == i % NW) {
+                uint16_t* to = lds_p + ((i * 2 + i / 2) * 64 + lane) * 8 + 4;
+                *reinterpret_cast<u32x2*>(to) = (u32x2){0u, 0u};
+                *reinterpret_cast<u32x2*>(to + kPart) = (u32x2){0u, 0u};
+            }
+        }
+    }
+    const bool exact = a.features == kFeatures && column0 + kColumns <= a.out_features;
+    int64_t counted = 0;
+
     for (int64_t chunk = begin; chunk < end; ++chunk) {
         const uint64_t kept = __ballot(kept_byte != 0);
         const int total = __popcll(kept);
-        if (tid < kChunk) {
-            rank[tid] = static_cast<float>(__popcll(kept & (~uint64_t{0} >> (63 - tid))));
-        }
-        if constexpr (!STATES) {
-#pragma unroll
-            for (int i = 0; i < loads_a.kEach; ++i) {
-                // Within 32 features the order 8 g + 4 h + r of feature 16 h + 4 g
-                // + r, which is the order of S's rows in a lane group's registers.
-                const u32x4 v = loads_a.piece(i, kept, a.features, 0);
-                const int column = loads_a.column(i);
-                uint16_t* to = lds_a + loads_a.row(i) * kPitch + (column & ~31) + 2 * (column & 8) + ((column & 16) >> 2);
-                *reinterpret_cast<u32x2*>(to) = (u32x2){v[0], v[1]};
-                *reinterpret_cast<u32x2*>(to + 8) = (u32x2){v[2], v[3]};
+        const int less = total > 0 ? pending : 0;
+        const bool full = exact && total == kChunk;
+        {
+            const int count = __popcll(kept & (~uint64_t{0} >> (63 - lane)));
+            if (wave == 0) {
+                rank[lane] = static_cast<float>(count);
+                from_start[lane] = a.scale_across * __builtin_amdgcn_exp2f(rate * static_cast<float>(count - less));
+            }
+            if (wave == NW - 1) {
+                const int tile_end = __popcll(kept & (~uint64_t{0} >> (63 - (lane | 15))));
+                to_end[lane] = a.scale_update * __builtin_amdgcn_exp2f(rate * static_cast<float>(total - count));
+                to_tile[lane] = a.scale_within * __builtin_amdgcn_exp2f(rate * static_cast<float>(tile_end - count));
             }
         }
+        const auto stage = [&](bool whole) {
+            if constexpr (!STATES) {
 #pragma unroll
-        for (int i = 0; i < loads_b.kEach; ++i) {
-            *reinterpret_cast<u32x4*>(lds_b + loads_b.row(i) * kPitch + loads_b.column(i)) =
-                loads_b.piece(i, kept, a.features, 0);
-        }
+                for (int i = 0; i < loads_a.kEach; ++i) {
+                    // Within 32 features the order 8 g + 4 h + r of feature 16 h + 4 g
+                    // + r, which is the order of S's rows in a lane group's registers.
+                    const u32x4 v = whole ? loads_a.raw[i] : loads_a.piece(i, kept);
+                    const int column = loads_a.column(i);
+                    uint16_t* to =
+                        lds_a + loads_a.row(i) * kPitch + (column & ~31) + 2 * (column & 8) + ((column & 16) >> 2);
+                    *reinterpret_cast<u32x2*>(to) = (u32x2){v[0], v[1]};
+                    *reinterpret_cast<u32x2*>(to + 8) = (u32x2){v[2], v[3]};
+                }
+            }
 #pragma unroll
-        for (int i = 0; i < loads_c.kEach; ++i) {
-            *reinterpret_cast<u32x4*>(lds_c + loads_c.row(i) * kColumnPitch + loads_c.column(i)) =
-                loads_c.piece(i, kept, a.out_features, column0);
+            for (int i = 0; i < loads_b.kEach; ++i) {
+                *reinterpret_cast<u32x4*>(lds_b + loads_b.row(i) * kPitch + loads_b.column(i)) =
+                    whole ? loads_b.raw[i] : loads_b.piece(i, kept);
+            }
+#pragma unroll
+            for (int i = 0; i < loads_c.kEach; ++i) {
+                *reinterpret_cast<u32x4*>(lds_c + loads_c.row(i) * kColumnPitch + loads_c.column(i)) =
+                    whole ? loads_c.raw[i] : loads_c.piece(i, kept);
+            }
+        };
+        if (WHOLE && full) {
+            stage(true);
+        } else {
+            stage(false);
         }
         __syncthreads();
         if (chunk + 1 < end) {
             issue(chunk + 1);
         }
-        const int less = total > 0 ? pending : 0;
         f32x4 out[kTiles][WE];
         if constexpr (!STATES) {
-            // P, a tile of 16 t in a wave: lane column t, rows s.
-#pragma unroll
-            for (int round = 0; round < kTiles / NW; ++round) {
-                // Two tiles of a wave: one short, one long.
-                const int tile = round % 2 == 0 ? wave : kTiles - 1 - wave;
-                u32x4 query[KT];
+            // P: its tiles of 16 s by 16 t, lane column t, rows s; those below the
+            // diagonal and then those on it dealt to the waves.
+            const auto product = [&](int tile, int s) {
+                f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    query[k] = *reinterpret_cast<const u32x4*>(lds_a + (16 * tile + in) * kPitch + 32 * k + 8 * group);
+                    const u32x4 query =
+                        *reinterpret_cast<const u32x4*>(lds_a + (16 * tile + in) * kPitch + 32 * k + 8 * group);
+                    const uint16_t* row = lds_b + (16 * s + in) * kPitch + 32 * k + 4 * group;
+                    score = mfma_small<T>(
+                        join(*reinterpret_cast<const u32x2*>(row), *reinterpret_cast<const u32x2*>(row + 16)), query,
+                        score);
                 }
+                return score;
+            };
+            const auto put = [&](int tile, int s, const f32x4& score) {
+                u32x2 halves[2];
+                split<T>(score, halves);
+                uint16_t* to = lds_p + ((tile * 2 + (s >> 1)) * 64 + lane) * 8 + 4 * (s & 1);
+                *reinterpret_cast<u32x2*>(to) = halves[0];
+                *reinterpret_cast<u32x2*>(to + kPart) = halves[1];
+            };
+            constexpr int kBelow = kTiles * (kTiles - 1) / 2;
+#pragma unroll
+            for (int round = (kBelow - 1) / NW; round >= 0; --round) {
+                const int index = round * NW + wave;   // 0: (1, 0); 1, 2: (2, s); 3 .. 5: (3, s)
+                if (index < kBelow) {
+                    const int tile = index >= 3 ? 3 : (index >= 1 ? 2 : 1);
+                    const int s = index - tile * (tile - 1) / 2;
+                    // l^(t - s) by the end of the tile of s, between the two: neither factor is above 1.
+                    const float after =
+                        __builtin_amdgcn_exp2f(rate * (rank[16 * tile + in] - rank[16 * s + 15]));
+                    put(tile, s, product(tile, s) * *reinterpret_cast<const f32x4*>(to_tile + 16 * s + 4 * group) * after);
+                }
+            }
+#pragma unroll
+            for (int tile = wave; tile < kTiles; tile += NW) {
+                f32x4 score = product(tile, tile);
                 const float rank_t = rank[16 * tile + in];
-                for (int s = 0; s <= (tile | 1); ++s) {
-                    f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (s <= tile) {
+                const f32x4 rank_s = *reinterpret_cast<const f32x4*>(rank + 16 * tile + 4 * group);
 #pragma unroll
-                        for (int k = 0; k < KT; ++k) {
-                            const uint16_t* row = lds_b + (16 * s + in) * kPitch + 32 * k + 4 * group;
-                            const u32x2 low = *reinterpret_cast<const u32x2*>(row);
-                            const u32x2 high = *reinterpret_cast<const u32x2*>(row + 16);
-                            score = mfma_small<T>((u32x4){low[0], low[1], high[0], high[1]}, query[k], score);
-                        }
-                        const f32x4 rank_s = *reinterpret_cast<const f32x4*>(rank + 16 * s + 4 * group);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float weight = a.scale_within * __builtin_amdgcn_exp2f(rate * (rank_t - rank_s[r]));
-                            score[r] = s < tile || 4 * group + r <= in ? score[r] * weight : 0.0f;
-                        }
-                    }
-                    u32x2 part[2];
-                    split<T>(score, part);
-                    uint16_t* to = lds_p + (((tile * 2) + (s >> 1)) * 64 + lane) * 8 + 4 * (s & 1);
-                    *reinterpret_cast<u32x2*>(to) = part[0];
-                    *reinterpret_cast<u32x2*>(to + kTiles * 2 * 64 * 8) = part[1];
+                for (int r = 0; r < 4; ++r) {
+                    const float weight = a.scale_within * __builtin_amdgcn_exp2f(rate * (rank_t - rank_s[r]));
+                    score[r] = 4 * group + r <= in ? score[r] * weight : 0.0f;
                 }
+                put(tile, tile, score);
             }
             // a S, before the chunk's own tokens reach S.
             float factor = 1.0f;
@@ -352,12 +429,12 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
                 u32x4 low[WE];
 #pragma unroll
                 for (int we = 0; we < WE; ++we) {
-                    u32x2 first[2];
-                    u32x2 second[2];
-                    split<T>(state[2 * k][we] * factor, first);
-                    split<T>(state[2 * k + 1][we] * factor, second);
-                    high[we] = join(first[0], second[0]);
-                    low[we] = join(first[1], second[1]);
+                    u32x2 upper[2];
+                    u32x2 lower[2];
+                    split<T>(state[2 * k][we] * factor, upper);
+                    split<T>(state[2 * k + 1][we] * factor, lower);
+                    high[we] = join(upper[0], lower[0]);
+                    low[we] = join(upper[1], lower[1]);
                 }
 #pragma unroll
                 for (int tile = 0; tile < kTiles; ++tile) {
@@ -372,14 +449,12 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
             }
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
-                const float weight = a.scale_across * unfactor *
-                                     __builtin_amdgcn_exp2f(rate * (rank[16 * tile + in] - static_cast<float>(less)));
+                const float weight = unfactor * from_start[16 * tile + in];
 #pragma unroll
                 for (int we = 0; we < WE; ++we) {
                     out[tile][we] *= weight;
                 }
             }
-            __syncthreads();   // P is whole
         }
         const float decay = __builtin_amdgcn_exp2f(rate * static_cast<float>(total - less));
 #pragma unroll
@@ -391,50 +466,26 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
         }
         pending -= less;
         counted += total;
+        u32x4 value[2][WE];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {   // 32 tokens s
-            u32x4 value[WE];
             const uint16_t* transposed =
                 lds_c + (32 * j + 4 * group + (in >> 2)) * kColumnPitch + 16 * wave * WE + 4 * (in & 3);
+            const f32x4 weight0 = *reinterpret_cast<const f32x4*>(to_end + 32 * j + 4 * group);
+            const f32x4 weight1 = *reinterpret_cast<const f32x4*>(to_end + 32 * j + 16 + 4 * group);
+            u32x4 decayed[WE][PARTS];
 #pragma unroll
             for (int we = 0; we < WE; ++we) {
-                value[we] = read_columns(transposed + 16 * we, kColumnPitch);
-            }
-            if constexpr (!STATES) {
-#pragma unroll
-                for (int tile = 2 * j; tile < kTiles; ++tile) {
-                    const uint16_t* from = lds_p + ((tile * 2 + j) * 64 + lane) * 8;
-                    const u32x4 high = *reinterpret_cast<const u32x4*>(from);
-                    const u32x4 low = *reinterpret_cast<const u32x4*>(from + kTiles * 2 * 64 * 8);
-#pragma unroll
-                    for (int we = 0; we < WE; ++we) {
-                        out[tile][we] = mfma_small<T>(value[we], high, out[tile][we]);
-                        out[tile][we] = mfma_small<T>(value[we], low, out[tile][we]);
-                    }
-                }
-            }
-            float weight[8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f32x4 rank_s = *reinterpret_cast<const f32x4*>(rank + 32 * j + 16 * h + 4 * group);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    weight[4 * h + r] =
-                        a.scale_update * __builtin_amdgcn_exp2f(rate * (static_cast<float>(total) - rank_s[r]));
-                }
-            }
-            u32x4 parts[WE][kParts];
-#pragma unroll
-            for (int we = 0; we < WE; ++we) {
+                value[j][we] = read_columns(transposed + 16 * we, kColumnPitch);
                 float v[8];
-                Values<T>::unpack8(value[we], v);
-                u32x2 first[kParts];
-                u32x2 second[kParts];
-                split<T>((f32x4){v[0] * weight[0], v[1] * weight[1], v[2] * weight[2], v[3] * weight[3]}, first);
-                split<T>((f32x4){v[4] * weight[4], v[5] * weight[5], v[6] * weight[6], v[7] * weight[7]}, second);
+                Values<T>::unpack8(value[j][we], v);
+                u32x2 upper[PARTS];
+                u32x2 lower[PARTS];
+                split<T>((f32x4){v[0], v[1], v[2], v[3]} * weight0, upper);
+                split<T>((f32x4){v[4], v[5], v[6], v[7]} * weight1, lower);
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    parts[we][p] = join(first[p], second[p]);
+                for (int p = 0; p < PARTS; ++p) {
+                    decayed[we][p] = join(upper[p], lower[p]);
                 }
             }
             const uint16_t* keys = lds_b + (32 * j + 4 * group + (in >> 2)) * kPitch + 4 * (in & 3);
@@ -442,45 +493,75 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
             for (int dt = 0; dt < 2 * KT; ++dt) {
                 const u32x4 key = read_columns(keys + 16 * dt, kPitch);
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
+                for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
                     for (int we = 0; we < WE; ++we) {
-                        state[dt][we] = mfma_small<T>(key, parts[we][p], state[dt][we]);
+                        state[dt][we] = mfma_small<T>(key, decayed[we][p], state[dt][we]);
                     }
                 }
             }
         }
+        // P is whole, and nobody reads the chunk any more: the next one may be staged.
+        __syncthreads();
         if constexpr (!STATES) {
 #pragma unroll
-            for (int tile = 0; tile < kTiles; ++tile) {
-                const int64_t token = chunk * kChunk + 16 * tile + in;
-                if (token >= a.length || a.out.data == nullptr) {
-                    continue;
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int tile = 2 * j; tile < kTiles; ++tile) {
+                    const uint16_t* from = lds_p + ((tile * 2 + j) * 64 + lane) * 8;
+                    const u32x4 high = *reinterpret_cast<const u32x4*>(from);
+                    const u32x4 low = *reinterpret_cast<const u32x4*>(from + kPart);
+#pragma unroll
+                    for (int we = 0; we < WE; ++we) {
+                        out[tile][we] = mfma_small<T>(value[j][we], high, out[tile][we]);
+                        out[tile][we] = mfma_small<T>(value[j][we], low, out[tile][we]);
+                    }
                 }
-                const bool keep = ((kept >> (16 * tile + in)) & 1) != 0;
-                const int64_t row = offset_of(a.out, batch, head) + token * a.out.token;
+            }
+            if (a.out.data != nullptr) {
+                const int64_t token = chunk * kChunk;
+                if (WHOLE && full && a.wide_out == 0) {
+                    const bool turned = a.out.token < 0;
+                    const uint32_t step = static_cast<uint32_t>(2 * (turned ? -a.out.token : a.out.token));
+                    const BufferRsrc buffer = make_buffer(
+                        static_cast<const uint16_t*>(a.out.data) + offset_of(a.out, batch, head) + column0 +
+                            (turned ? token + kChunk - 1 : token) * a.out.token,
+                        static_cast<int64_t>(kChunk - 1) * step + 2 * kColumns);
+                    const uint32_t at =
+                        static_cast<uint32_t>(turned ? kChunk - 1 - in : in) * step + 2 * (16 * wave * WE + 4 * group);
 #pragma unroll
-                for (int we = 0; we < WE; ++we) {
-                    const int e = column0 + 16 * (wave * WE + we) + 4 * group;
-                    const f32x4 v = keep ? out[tile][we] : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-                    if (a.wide_out != 0) {
-                        float* to = static_cast<float*>(const_cast<void*>(a.out.data)) + row + e;
+                    for (int tile = 0; tile < kTiles; ++tile) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (e + r < a.out_features) {
-                                to[r] = v[r];
-                            }
+                        for (int we = 0; we < WE; ++we) {
+                            const f32x4 v = out[tile][we];
+                            buffer_store8((u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])}, buffer,
+                                          at + 16 * tile * (turned ? 0u - step : step) + 32 * we);
                         }
-                    } else {
-                        uint16_t* to = static_cast<uint16_t*>(const_cast<void*>(a.out.data)) + row + e;
-                        if (e + 4 <= a.out_features) {
-                            const u32x2 packed = {Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])};
-                            __builtin_memcpy(to, &packed, sizeof(packed));
-                        } else {
+                    }
+                } else {
+                    const int own = opaque_int(lane);   // nothing of this path is held across the loop
+                    const int t = own & 15;
+                    const int e0 = column0 + 16 * wave * WE + 4 * (own >> 4);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                if (e + r < a.out_features) {
-                                    Values<T>::store(to + r, v[r]);
+                    for (int tile = 0; tile < kTiles; ++tile) {
+                        if (token + 16 * tile + t < a.length) {
+                            const bool keep = ((kept >> (16 * tile + t)) & 1) != 0;
+#pragma unroll
+                            for (int we = 0; we < WE; ++we) {
+                                const int e = e0 + 16 * we;
+                                const int64_t at = offset_of(a.out, batch, head) +
+                                                   (token + 16 * tile + t) * a.out.token + e;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const float v = keep ? out[tile][we][r] : 0.0f;
+                                    if (e + r < a.out_features) {
+                                        if (a.wide_out != 0) {
+                                            static_cast<float*>(const_cast<void*>(a.out.data))[at + r] = v;
+                                        } else {
+                                            Values<T>::store(
+                                                static_cast<uint16_t*>(const_cast<void*>(a.out.data)) + at + r, v);
+                                        }
+                                    }
                                 }
                             }
                         }
@@ -488,32 +569,31 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
                 }
             }
         }
-        __syncthreads();   // the chunk's readers are done
     }
 
     float* to = nullptr;
     float multiplier = 1.0f;
     if constexpr (STATES) {
-        to = a.states + ((batch * a.heads + head) * a.segments + segment) *
-                            (static_cast<int64_t>(a.features) * a.out_features);
+        to = a.updates + (system * a.pieces + part) * size;
         if (head == 0 && column0 == 0 && tid == 0) {
-            a.counts[batch * a.segments + segment] = static_cast<int>(counted);
+            a.counts[batch * a.pieces + part] = static_cast<int>(counted);
         }
-    } else if (a.last != nullptr && segment == a.segments - 1) {
-        to = a.last + slot;
+    } else if (a.last != nullptr && part == a.segments - 1) {
+        to = a.last + system * size;
         // The walk's own exponents are one less than those of a state before its
         // last token, which a walk to the front ends with.
         multiplier = a.shift != 0 && pending == 0 ? __builtin_amdgcn_exp2f(rate) : 1.0f;
     }
     if (to != nullptr) {
+        const int own = opaque_int(lane);
 #pragma unroll
         for (int dt = 0; dt < 2 * KT; ++dt) {
 #pragma unroll
             for (int we = 0; we < WE; ++we) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int d = state_row(dt, r);
-                    const int e = state_column(we);
+                    const int d = state_row(own, dt, r);
+                    const int e = state_column(own, we);
                     if (d < a.features && e < a.out_features) {
                         to[d * a.out_features + e] = state[dt][we][r] * multiplier;
                     }
@@ -523,8 +603,9 @@ __global__ __launch_bounds__(64 * NW) void walk_kernel(WalkArgs a) {
     }
 }
 
-// states: each segment's update becomes the state before its first token.
+// The state before the first token of each segment, from what the pieces add.
 constexpr int kCarryThreads = 256;
+constexpr int kCarryAhead = 8;   // pieces in flight
 __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
     const int size = a.features * a.out_features;
     const int blocks = (size + kCarryThreads - 1) / kCarryThreads;
@@ -542,44 +623,73 @@ __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
         state = a.first[system * size + d * a.first_row + (i - d * a.out_features) * a.first_column];
     }
     int pending = a.shift;
-    float* at = a.states + system * a.segments * size + i;
-    float update = at[0];
-    for (int64_t s = 0; s < a.segments; ++s) {
-        const float next = s + 2 < a.segments ? at[(s + 1) * size] : 0.0f;   // in flight behind the store
-        at[s * size] = state;
-        if (s + 1 < a.segments) {
-            const int count = a.counts[batch * a.segments + s];
-            const int less = count > 0 ? pending : 0;
-            pending -= less;
-            state = state * __builtin_amdgcn_exp2f(rate * static_cast<float>(count - less)) + update;
+    const int each = static_cast<int>(a.segment_chunks / a.piece_chunks);
+    int left = 0;   // pieces of the segment
+    const float* from = a.updates + system * a.pieces * size + i;
+    const int* counts = a.counts + batch * a.pieces;
+    float* to = a.states + system * a.segments * size + i;
+    for (int64_t s0 = 0; s0 < a.pieces; s0 += kCarryAhead) {
+        float update[kCarryAhead];
+        int count[kCarryAhead];
+#pragma unroll
+        for (int j = 0; j < kCarryAhead; ++j) {
+            const int64_t s = s0 + j < a.pieces ? s0 + j : a.pieces - 1;
+            update[j] = from[s * size];
+            count[j] = counts[s];
         }
-        update = next;
+#pragma unroll
+        for (int j = 0; j < kCarryAhead; ++j) {
+            const int64_t s = s0 + j;
+            if (s < a.pieces) {
+                if (left == 0) {
+                    *to = state;
+                    to += size;
+                    left = each;
+                }
+                --left;
+                const int less = count[j] > 0 ? pending : 0;
+                pending -= less;
+                state = state * __builtin_amdgcn_exp2f(rate * static_cast<float>(count[j] - less)) + update[j];
+            }
+        }
     }
+    *to = state;   // of the last segment
+}
+
+template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE>
+void launch_parts(const WalkArgs& a, hipStream_t stream) {
+    constexpr int kColumns = 16 * NW * WE;
+    const int64_t across = (a.out_features + kColumns - 1) / kColumns;
+    const int64_t systems = a.batch * a.heads;
+    if (a.segments > 1 && a.reuse == 0) {
+        walk_kernel<T, KT, NW, WE, PARTS, WHOLE, true>
+            <<<static_cast<unsigned>(systems * a.pieces * across), 64 * NW, 0, stream>>>(a);
+        const int64_t blocks = (a.features * a.out_features + kCarryThreads - 1) / kCarryThreads;
+        carry_kernel<<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
+    }
+    walk_kernel<T, KT, NW, WE, PARTS, WHOLE, false>
+        <<<static_cast<unsigned>(systems * a.segments * across), 64 * NW, 0, stream>>>(a);
 }
 
 template <int T, int KT, int NW, int WE, bool WHOLE>
 void launch_form(const WalkArgs& a, hipStream_t stream) {
-    constexpr int kColumns = 16 * NW * WE;
-    const int64_t across = (a.out_features + kColumns - 1) / kColumns;
-    const int64_t systems = a.batch * a.heads;
-    if (a.segments > 1) {
-        walk_kernel<T, KT, NW, WE, WHOLE, true>
-            <<<static_cast<unsigned>(systems * (a.segments - 1) * across), 64 * NW, 0, stream>>>(a);
-        const int64_t blocks = (a.features * a.out_features + kCarryThreads - 1) / kCarryThreads;
-        carry_kernel<<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
+    // FP16 states are right to 2^-22 with two parts; of BF16 only one that is given
+    // back shows what two leave.
+    if (T == LSSO_HIP_BF16 && a.fine != 0) {
+        launch_parts<T, KT, NW, WE, T == LSSO_HIP_BF16 ? 3 : 2, WHOLE>(a, stream);
+    } else {
+        launch_parts<T, KT, NW, WE, 2, WHOLE>(a, stream);
     }
-    walk_kernel<T, KT, NW, WE, WHOLE, false>
-        <<<static_cast<unsigned>(systems * a.segments * across), 64 * NW, 0, stream>>>(a);
 }
 
 template <int T, int KT, bool WHOLE>
 void launch_columns(const WalkArgs& a, hipStream_t stream) {
     if (a.out_features <= 32) {
         launch_form<T, KT, 2, 1, WHOLE>(a, stream);
-    } else if (a.out_features <= 64) {
+    } else if (KT == 4 || a.out_features <= 64) {   // two column blocks a wave do not fit beside 128 rows of S
         launch_form<T, KT, 4, 1, WHOLE>(a, stream);
     } else {
-        launch_form<T, KT, 4, 2, WHOLE>(a, stream);
+        launch_form<T, KT, 4, KT == 4 ? 1 : 2, WHOLE>(a, stream);
     }
 }
 
@@ -707,20 +817,26 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(AttentionS
 void plan_walk(WalkArgs* a) {
     const int64_t chunks = (a->length + kChunk - 1) / kChunk;
     const int64_t systems = a->batch * a->heads;
-    // Segments until every compute unit has two workgroups, but none shorter than
-    // four chunks: a segment costs its state's write and two reads, and a second
-    // read of b and c.
-    int64_t segments = systems > 0 ? (512 + systems - 1) / systems : 1;
-    const int64_t most = (chunks + 3) / 4;
-    segments = segments < most ? segments : most;
-    segments = segments > 1 ? segments : 1;
-    a->segment_chunks = (chunks + segments - 1) / segments;
-    a->segment_chunks = a->segment_chunks > 0 ? a->segment_chunks : 1;
+    // Segments until every compute unit has three workgroups, but none shorter than
+    // two chunks; pieces of them until there are four.
+    const auto parts = [&](int64_t wanted, int64_t whole, int64_t least) {   // of `whole` chunks
+        int64_t count = systems > 0 ? (wanted + systems - 1) / systems : 1;
+        const int64_t most = (whole + least - 1) / least;
+        count = count < most ? count : most;
+        return count > 1 ? count : int64_t{1};
+    };
+    const int64_t segments = parts(768, chunks, 2);
+    int64_t segment_chunks = chunks > 0 ? (chunks + segments - 1) / segments : 1;
+    const int64_t pieces = segments > 1 ? parts((1024 + segments - 2) / (segments - 1), segment_chunks, 2) : 1;
+    a->piece_chunks = (segment_chunks + pieces - 1) / pieces;
+    a->segment_chunks = a->piece_chunks * pieces;
     a->segments = chunks > 0 ? (chunks + a->segment_chunks - 1) / a->segment_chunks : 1;
+    a->pieces = (a->segments - 1) * pieces;
 }
 
 hipError_t launch_walk(const WalkArgs& a, int dtype, hipStream_t stream) {
-    const bool whole = a.features % 8 == 0 && a.out_features % 8 == 0;
+    const auto near = [](const WalkTensor& t) { return t.token < (1 << 23) && t.token > -(1 << 23); };
+    const bool whole = a.features % 8 == 0 && a.out_features % 8 == 0 && near(a.a) && near(a.b) && near(a.c);
     if (dtype == LSSO_HIP_F16) {
         whole ? launch_features<LSSO_HIP_F16, true>(a, stream) : launch_features<LSSO_HIP_F16, false>(a, stream);
     } else {

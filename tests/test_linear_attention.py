@@ -119,37 +119,38 @@ def _shape(**changes):
 
 def test_refusals_on_the_cpu() -> None:
     library = hip.open_library()
-    size = ctypes.c_size_t()
+    kept, forward_size, backward_size = (ctypes.c_size_t() for _ in range(3))
+    pointers = [ctypes.byref(size) for size in (kept, forward_size, backward_size)]
 
-    def bytes_of(backward=0, out=ctypes.byref(size), **changes):
-        return library.lsso_hip_linear_attention_workspace_bytes(ctypes.byref(_shape(**changes)), backward, out)
+    def sizes(out=pointers[0], **changes):
+        return library.lsso_hip_linear_attention_sizes(ctypes.byref(_shape(**changes)), out, *pointers[1:])
 
     def forward(q=16, k=16, v=16, log_decay=16, state=None, y=16, last=None, workspace=None, count=0, **changes):
         return library.lsso_hip_linear_attention(
-            ctypes.byref(_shape(**changes)), q, k, v, log_decay, None, state, y, last, workspace, count, None)
+            ctypes.byref(_shape(**changes)), q, k, v, log_decay, None, state, None, y, last, workspace, count, None)
 
     def backward(grad=16, strides=causal.HeadStrides(96, 32, 8), last=None, q=16, log_decay=16, grad_q=16, grad_s=None,
                  workspace=None, count=0, **changes):
         return library.lsso_hip_linear_attention_backward(
             ctypes.byref(_shape(**changes)), grad, None if strides is None else ctypes.byref(strides), last, q, 16, 16,
-            log_decay, None, None, grad_q, None, None, grad_s, workspace, count, None)
+            log_decay, None, None, None, grad_q, None, None, grad_s, workspace, count, None)
 
     def step(q=16, state=16, stride=256, y=16, log_decay=16, **changes):
         return library.lsso_hip_linear_attention_step(
             ctypes.byref(_shape(**{"length": 1, **changes})), q, 16, 16, log_decay, None, state, stride, y, None)
 
-    assert bytes_of() == 0
-    # Shared heads: FP32 gradients of each, and past four chunks the segments' states.
-    assert bytes_of(1) == 0 and size.value == 2 * 3 * 4 * 8 * 4
-    assert bytes_of(length=1000, kv_heads=4) == 0 and size.value >= 2 * 4 * 4 * 64 * 4
+    # Shared heads: FP32 gradients of each, and past two chunks the segments' states.
+    assert sizes() == 0 and kept.value == 0 and forward_size.value == 0 and backward_size.value == 2 * 3 * 4 * 8 * 4
+    assert sizes(length=1000, kv_heads=4) == 0 and kept.value >= 2 * 2 * 4 * 64
+    assert forward_size.value >= 4 * kept.value and backward_size.value >= 4 * kept.value
     for wrong in ({"batch": -1}, {"length": -1}, {"heads": 0}, {"kv_heads": 3}, {"features": 0}, {"features": 129},
                   {"value_features": 129}, {"dtype": 3}, {"scale": math.inf}, {"scale": math.nan}, {"stride": 1},
                   {"batch": 2**22}, {"heads": 8192, "kv_heads": 1}, {"length": 2**31}):
-        assert bytes_of(**wrong) < 0, wrong
+        assert sizes(**wrong) < 0, wrong
         assert forward(**wrong) < 0 and step(**{**wrong, "length": wrong.get("length", 1)}) < 0, wrong
         assert library.lsso_hip_last_error()
-    assert bytes_of(out=None) < 0
-    assert library.lsso_hip_linear_attention_workspace_bytes(None, 0, ctypes.byref(size)) < 0
+    assert sizes(out=None) < 0
+    assert library.lsso_hip_linear_attention_sizes(None, *pointers) < 0
     assert forward(batch=0) == 0 and forward(length=0) == 0 and backward(batch=0) == 0 and step(batch=0) == 0
     for wrong in ({"q": None}, {"k": 17}, {"v": None}, {"y": None}, {"log_decay": None}, {"log_decay": 18},
                   {"state": 18}, {"last": 18}, {"length": 1000}, {"length": 1000, "workspace": 255, "count": 1 << 30},
