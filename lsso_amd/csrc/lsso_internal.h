@@ -573,9 +573,10 @@ struct WalkArgs {
     int64_t states_row;         // their strides
     int64_t states_column;
     int reuse;                  // states are there already
-    int64_t segment_chunks;     // set by plan_walk: whole pieces
+    int64_t segment_chunks;     // set by plan_walk
     int64_t segments;
     int64_t piece_chunks;
+    int64_t segment_pieces;     // of a segment, the last of them shorter
     int64_t pieces;             // of all segments but the last; 0 with one segment
 };
 

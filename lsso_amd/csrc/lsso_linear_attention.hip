@@ -46,6 +46,9 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kTiles = kChunk / 16;
+constexpr int kPairs = 6;   // tiles of t by pairs of tiles of s, on and below the diagonal
+// Where in P the pair of tiles with tile s is, of tile t >= s.
+__device__ __forceinline__ constexpr int pair_of(int t, int s) { return t + (t == 3 ? 1 : 0) + (s >> 1); }
 constexpr double kLog2e = 1.4426950408889634;
 
 // log2 of the decay; a head that forgets at once (-inf) keeps l^0 = 1.
@@ -153,6 +156,12 @@ __device__ __forceinline__ u32x4 read_columns(const uint16_t* at, int pitch) {
     return (u32x4){low[0], low[1], high[0], high[1]};
 }
 
+// xcd_local_block in 32 bits.
+__device__ __forceinline__ uint32_t xcd_local_block32(uint32_t physical, uint32_t blocks) {
+    const uint32_t per_xcd = blocks / 8;
+    return physical >= per_xcd * 8 ? physical : (physical % 8) * per_xcd + physical / 8;
+}
+
 __device__ __forceinline__ void buffer_store8(u32x2 value, BufferRsrc buffer, uint32_t offset) {
     typedef __attribute__((ext_vector_type(2))) unsigned int Pair;
     __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Pair, value), buffer, offset, 0, 0);
@@ -160,6 +169,20 @@ __device__ __forceinline__ void buffer_store8(u32x2 value, BufferRsrc buffer, ui
 
 __device__ __forceinline__ int64_t offset_of(const WalkTensor& t, int64_t batch, int head) {
     return batch * t.batch + (head / t.heads_per) * t.head;
+}
+
+// The largest value of a wave's lanes, all of them not negative, as bits.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x121, 0xf, 0xf, true));   // row_ror:1 of 16 lanes
+    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x122, 0xf, 0xf, true));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xf, 0xf, true));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xf, 0xf, true));
+    const uint32_t r0 = __builtin_amdgcn_readlane(static_cast<int>(v), 0);
+    const uint32_t r1 = __builtin_amdgcn_readlane(static_cast<int>(v), 16);
+    const uint32_t r2 = __builtin_amdgcn_readlane(static_cast<int>(v), 32);
+    const uint32_t r3 = __builtin_amdgcn_readlane(static_cast<int>(v), 48);
+    return larger(larger(r0, r1), larger(r2, r3));
 }
 
 // T: type; KT: 32-feature steps of a and b; NW: waves; WE: 16-column blocks of c
@@ -173,11 +196,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     constexpr int kColumns = 16 * NW * WE;
     constexpr int kPitch = kFeatures + 8;        // rows 16 bytes apart modulo the banks
     constexpr int kColumnPitch = kColumns + 8;
-    constexpr int kPart = kTiles * 2 * 64 * 8;   // values of one part of P
+    constexpr int kPart = kPairs * 64 * 8;       // values of one part of P
     __shared__ __attribute__((aligned(16))) uint16_t lds_a[STATES ? 8 : kChunk * kPitch];
     __shared__ __attribute__((aligned(16))) uint16_t lds_b[kChunk * kPitch];
     __shared__ __attribute__((aligned(16))) uint16_t lds_c[kChunk * kColumnPitch];
-    // P in operand order: [part][tile of t][32 s][lane][8 s].
+    // P in operand order: [part][pair][lane][8 s].
     __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : 2 * kPart];
     // Of each token of the chunk: the kept ones up to it; l to the power of the kept
     // ones behind it, times scale_update; of those from it to the end of its 16; of
@@ -194,17 +217,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     const int group = lane >> 4;
 
     // Heads of a token next to each other, on one XCD: they share lines.
-    const int blocks_across = (a.out_features + kColumns - 1) / kColumns;
-    int64_t block = xcd_local_block(blockIdx.x, gridDim.x);
-    const int column0 = static_cast<int>(block % blocks_across) * kColumns;
-    block /= blocks_across;
-    const int head = static_cast<int>(block % a.heads);
-    block /= a.heads;
-    const int64_t parts = STATES ? a.pieces : a.segments;
-    const int64_t part = block % parts;
-    const int64_t batch = block / parts;
-    const int64_t system = batch * a.heads + head;
-    const int64_t size = static_cast<int64_t>(a.features) * a.out_features;
+    // (In 32 bits: a division of 64 takes longer than a chunk's products.)
+    const uint32_t blocks_across = static_cast<uint32_t>((a.out_features + kColumns - 1) / kColumns);
+    const uint32_t parts = static_cast<uint32_t>(STATES ? a.pieces : a.segments);
+    const uint32_t index = static_cast<uint32_t>(xcd_local_block32(blockIdx.x, gridDim.x));
+    const uint32_t row_of_blocks = index / blocks_across;
+    const int column0 = static_cast<int>(index - row_of_blocks * blocks_across) * kColumns;
+    const uint32_t row_of_heads = row_of_blocks / static_cast<uint32_t>(a.heads);
+    const int head = static_cast<int>(row_of_blocks - row_of_heads * static_cast<uint32_t>(a.heads));
+    const uint32_t batch = row_of_heads / parts;
+    const uint32_t part = row_of_heads - batch * parts;
+    const int64_t system = static_cast<int64_t>(batch) * a.heads + head;
+    const int size = a.features * a.out_features;
 
     const uint16_t* from_a = static_cast<const uint16_t*>(a.a.data) + offset_of(a.a, batch, head);
     const uint16_t* from_b = static_cast<const uint16_t*>(a.b.data) + offset_of(a.b, batch, head);
@@ -213,17 +237,25 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     const float rate = decay_rate(a.log_decay[head]);
 
     const int64_t chunks = (a.length + kChunk - 1) / kChunk;
-    const int64_t step = STATES ? a.piece_chunks : a.segment_chunks;
-    const int64_t begin = part * step;
-    const int64_t end = begin + step < chunks ? begin + step : chunks;
+    const uint32_t segment = STATES ? part / static_cast<uint32_t>(a.segment_pieces) : part;
+    const int64_t piece = STATES ? part - segment * static_cast<uint32_t>(a.segment_pieces) : 0;
+    const int64_t begin = segment * a.segment_chunks + piece * a.piece_chunks;
+    const int64_t behind = STATES && piece * a.piece_chunks + a.piece_chunks < a.segment_chunks
+                               ? begin + a.piece_chunks
+                               : (segment + 1) * a.segment_chunks;
+    const int64_t end = behind < chunks ? behind : chunks;
 
     ChunkLoads<kFeatures, kThreads, WHOLE> loads_a(from_a, a.a.token, a.features);
     ChunkLoads<kFeatures, kThreads, WHOLE> loads_b(from_b, a.b.token, a.features);
     ChunkLoads<kColumns, kThreads, WHOLE> loads_c(from_c + column0, a.c.token, a.out_features - column0);
     uint8_t kept_byte = 0;
+    const auto rows_of = [&](int64_t chunk) {
+        const int64_t left = a.length - chunk * kChunk;
+        return static_cast<int>(left < kChunk ? left : kChunk);
+    };
     const auto issue = [&](int64_t chunk) {
         const int64_t token = chunk * kChunk;
-        const int rows = static_cast<int>(a.length - token < kChunk ? a.length - token : kChunk);
+        const int rows = rows_of(chunk);
         if constexpr (!STATES) {
             loads_a.issue(token, rows);
         }
@@ -240,22 +272,22 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     const auto state_row = [](int lane_, int dt, int r) { return 16 * dt + 4 * (lane_ >> 4) + r; };
     const auto state_column = [&](int lane_, int we) { return column0 + 16 * (wave * WE + we) + (lane_ & 15); };
     const float* first = nullptr;
-    int64_t row_stride = a.out_features;
-    int64_t column_stride = 1;
+    int row_stride = a.out_features;
+    int column_stride = 1;
     // 1 as long as the exponents of the first state are one less than those of the tokens.
     int pending = 0;
     if constexpr (!STATES) {
         if (a.segments > 1) {
             first = a.states + (system * a.segments + part) * size;
-            row_stride = a.states_row;
-            column_stride = a.states_column;
+            row_stride = static_cast<int>(a.states_row);
+            column_stride = static_cast<int>(a.states_column);
         } else if (a.first != nullptr) {
             first = a.first + system * size;
-            row_stride = a.first_row;
-            column_stride = a.first_column;
+            row_stride = static_cast<int>(a.first_row);
+            column_stride = static_cast<int>(a.first_column);
         }
         pending = a.shift;
-        for (int64_t i = 0; i < part * (a.segment_chunks / a.piece_chunks) && pending != 0; ++i) {
+        for (int64_t i = 0; i < part * a.segment_pieces && pending != 0; ++i) {
             pending = a.counts[batch * a.pieces + i] == 0 ? 1 : 0;
         }
     }
@@ -282,7 +314,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
 #pragma unroll
         for (int i = 0; i < kTiles; i += 2) {
             if (wave == i % NW) {
-                uint16_t* to = lds_p + ((i * 2 + i / 2) * 64 + lane) * 8 + 4;
+                uint16_t* to = lds_p + (pair_of(i, i) * 64 + lane) * 8 + 4;
                 *reinterpret_cast<u32x2*>(to) = (u32x2){0u, 0u};
                 *reinterpret_cast<u32x2*>(to + kPart) = (u32x2){0u, 0u};
             }
@@ -290,6 +322,72 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     }
     const bool exact = a.features == kFeatures && column0 + kColumns <= a.out_features;
     int64_t counted = 0;
+
+    const auto write = [&](int64_t chunk, uint64_t keep, f32x4 (&out)[kTiles][WE]) {
+        const int64_t token = chunk * kChunk;
+        const int rows = rows_of(chunk);
+        if (keep != ~uint64_t{0}) {   // uniform
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+#pragma unroll
+                for (int we = 0; we < WE; ++we) {
+                    out[tile][we] =
+                        ((keep >> (16 * tile + in)) & 1) != 0 ? out[tile][we] : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
+        }
+        if constexpr (WHOLE) {
+            const int bytes = a.wide_out != 0 ? 4 : 2;
+            const bool turned = a.out.token < 0;
+            const uint32_t row = static_cast<uint32_t>(bytes * (turned ? -a.out.token : a.out.token));
+            const char* data = static_cast<const char*>(a.out.data) +
+                               bytes * (offset_of(a.out, batch, head) + column0 +
+                                        (turned ? token + rows - 1 : token) * a.out.token);
+            const int columns = a.out_features - column0;
+            const BufferRsrc buffer = make_buffer(data, static_cast<int64_t>(rows - 1) * row + bytes * columns);
+            const int e = 16 * wave * WE + 4 * group;
+            // Rows past the last wrap round, and out of the buffer; so does what is past the features.
+            const uint32_t at = static_cast<uint32_t>(turned ? rows - 1 - in : in) * row + bytes * e;
+            const uint32_t round = 16 * (turned ? 0u - row : row);
+#pragma unroll
+            for (int we = 0; we < WE; ++we) {
+                const bool some = e + 16 * we < columns;
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) {
+                    const f32x4 v = out[tile][we];
+                    const uint32_t to = some ? at + tile * round + 16 * bytes * we : kOutOfRange;
+                    if (a.wide_out != 0) {
+                        buffer_store16(__builtin_bit_cast(u32x4, v), buffer, to);
+                    } else {
+                        buffer_store8((u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])}, buffer, to);
+                    }
+                }
+            }
+        } else {
+            const int own = opaque_int(lane);   // nothing of this path is held across the loop
+            const int e0 = column0 + 16 * wave * WE + 4 * (own >> 4);
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                const int t = 16 * tile + (own & 15);
+                const int64_t at = offset_of(a.out, batch, head) + (token + t) * a.out.token + e0;
+#pragma unroll
+                for (int we = 0; we < WE; ++we) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int c = 16 * we + r;
+                        if (t < rows && e0 + c < a.out_features) {
+                            if (a.wide_out != 0) {
+                                static_cast<float*>(const_cast<void*>(a.out.data))[at + c] = out[tile][we][r];
+                            } else {
+                                Values<T>::store(static_cast<uint16_t*>(const_cast<void*>(a.out.data)) + at + c,
+                                                 out[tile][we][r]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    };
 
     for (int64_t chunk = begin; chunk < end; ++chunk) {
         const uint64_t kept = __ballot(kept_byte != 0);
@@ -362,7 +460,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
             const auto put = [&](int tile, int s, const f32x4& score) {
                 u32x2 halves[2];
                 split<T>(score, halves);
-                uint16_t* to = lds_p + ((tile * 2 + (s >> 1)) * 64 + lane) * 8 + 4 * (s & 1);
+                uint16_t* to = lds_p + (pair_of(tile, s) * 64 + lane) * 8 + 4 * (s & 1);
                 *reinterpret_cast<u32x2*>(to) = halves[0];
                 *reinterpret_cast<u32x2*>(to + kPart) = halves[1];
             };
@@ -395,22 +493,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
             float factor = 1.0f;
             float unfactor = 1.0f;
             if constexpr (T == LSSO_HIP_F16) {
-                float most = 0.0f;
+                uint32_t most = 0;
 #pragma unroll
                 for (int dt = 0; dt < 2 * KT; ++dt) {
 #pragma unroll
                     for (int we = 0; we < WE; ++we) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            most = fmaxf(most, fabsf(state[dt][we][r]));
+                            const uint32_t bits = __float_as_uint(state[dt][we][r]) & 0x7fffffffu;
+                            most = bits > most ? bits : most;
                         }
                     }
                 }
-#pragma unroll
-                for (int offset = 1; offset < 64; offset *= 2) {
-                    most = fmaxf(most, __shfl_xor(most, offset));
-                }
-                const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+                const int exponent = static_cast<int>(wave_max(most) >> 23) - 127;
                 if (exponent > -100 && exponent < 128) {   // neither next to nothing nor infinite
                     factor = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
                     unfactor = __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
@@ -508,7 +603,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int tile = 2 * j; tile < kTiles; ++tile) {
-                    const uint16_t* from = lds_p + ((tile * 2 + j) * 64 + lane) * 8;
+                    const uint16_t* from = lds_p + (pair_of(tile, 2 * j) * 64 + lane) * 8;
                     const u32x4 high = *reinterpret_cast<const u32x4*>(from);
                     const u32x4 low = *reinterpret_cast<const u32x4*>(from + kPart);
 #pragma unroll
@@ -519,54 +614,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
                 }
             }
             if (a.out.data != nullptr) {
-                const int64_t token = chunk * kChunk;
-                if (WHOLE && full && a.wide_out == 0) {
-                    const bool turned = a.out.token < 0;
-                    const uint32_t step = static_cast<uint32_t>(2 * (turned ? -a.out.token : a.out.token));
-                    const BufferRsrc buffer = make_buffer(
-                        static_cast<const uint16_t*>(a.out.data) + offset_of(a.out, batch, head) + column0 +
-                            (turned ? token + kChunk - 1 : token) * a.out.token,
-                        static_cast<int64_t>(kChunk - 1) * step + 2 * kColumns);
-                    const uint32_t at =
-                        static_cast<uint32_t>(turned ? kChunk - 1 - in : in) * step + 2 * (16 * wave * WE + 4 * group);
-#pragma unroll
-                    for (int tile = 0; tile < kTiles; ++tile) {
-#pragma unroll
-                        for (int we = 0; we < WE; ++we) {
-                            const f32x4 v = out[tile][we];
-                            buffer_store8((u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])}, buffer,
-                                          at + 16 * tile * (turned ? 0u - step : step) + 32 * we);
-                        }
-                    }
-                } else {
-                    const int own = opaque_int(lane);   // nothing of this path is held across the loop
-                    const int t = own & 15;
-                    const int e0 = column0 + 16 * wave * WE + 4 * (own >> 4);
-#pragma unroll
-                    for (int tile = 0; tile < kTiles; ++tile) {
-                        if (token + 16 * tile + t < a.length) {
-                            const bool keep = ((kept >> (16 * tile + t)) & 1) != 0;
-#pragma unroll
-                            for (int we = 0; we < WE; ++we) {
-                                const int e = e0 + 16 * we;
-                                const int64_t at = offset_of(a.out, batch, head) +
-                                                   (token + 16 * tile + t) * a.out.token + e;
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const float v = keep ? out[tile][we][r] : 0.0f;
-                                    if (e + r < a.out_features) {
-                                        if (a.wide_out != 0) {
-                                            static_cast<float*>(const_cast<void*>(a.out.data))[at + r] = v;
-                                        } else {
-                                            Values<T>::store(
-                                                static_cast<uint16_t*>(const_cast<void*>(a.out.data)) + at + r, v);
-                                        }
-                                    }
-                                }
-                            }
-                        }
-                    }
-                }
+                write(chunk, kept, out);
             }
         }
     }
@@ -605,7 +653,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
 
 // The state before the first token of each segment, from what the pieces add.
 constexpr int kCarryThreads = 256;
-constexpr int kCarryAhead = 8;   // pieces in flight
+constexpr int kCarryAhead = 16;   // pieces in flight
 __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
     const int size = a.features * a.out_features;
     const int blocks = (size + kCarryThreads - 1) / kCarryThreads;
@@ -623,33 +671,34 @@ __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
         state = a.first[system * size + d * a.first_row + (i - d * a.out_features) * a.first_column];
     }
     int pending = a.shift;
-    const int each = static_cast<int>(a.segment_chunks / a.piece_chunks);
+    const int each = static_cast<int>(a.segment_pieces);
     int left = 0;   // pieces of the segment
     const float* from = a.updates + system * a.pieces * size + i;
     const int* counts = a.counts + batch * a.pieces;
     float* to = a.states + system * a.segments * size + i;
-    for (int64_t s0 = 0; s0 < a.pieces; s0 += kCarryAhead) {
+    const int pieces = static_cast<int>(a.pieces);
+    for (int s0 = 0; s0 < pieces; s0 += kCarryAhead) {
+        const int some = pieces - s0 < kCarryAhead ? pieces - s0 : kCarryAhead;
         float update[kCarryAhead];
-        int count[kCarryAhead];
 #pragma unroll
         for (int j = 0; j < kCarryAhead; ++j) {
-            const int64_t s = s0 + j < a.pieces ? s0 + j : a.pieces - 1;
-            update[j] = from[s * size];
-            count[j] = counts[s];
+            if (j < some) {   // uniform
+                update[j] = from[static_cast<int64_t>(s0 + j) * size];
+            }
         }
 #pragma unroll
         for (int j = 0; j < kCarryAhead; ++j) {
-            const int64_t s = s0 + j;
-            if (s < a.pieces) {
+            if (j < some) {
                 if (left == 0) {
                     *to = state;
                     to += size;
                     left = each;
                 }
                 --left;
-                const int less = count[j] > 0 ? pending : 0;
+                const int count = counts[s0 + j];
+                const int less = count > 0 ? pending : 0;
                 pending -= less;
-                state = state * __builtin_amdgcn_exp2f(rate * static_cast<float>(count[j] - less)) + update[j];
+                state = state * __builtin_amdgcn_exp2f(rate * static_cast<float>(count - less)) + update[j];
             }
         }
     }
@@ -817,21 +866,23 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(AttentionS
 void plan_walk(WalkArgs* a) {
     const int64_t chunks = (a->length + kChunk - 1) / kChunk;
     const int64_t systems = a->batch * a->heads;
-    // Segments until every compute unit has three workgroups, but none shorter than
-    // two chunks; pieces of them until there are four.
+    // Segments until every compute unit has as many workgroups as it holds (three, of
+    // more than 64 features two), but none shorter than two chunks; pieces of them
+    // until there are four.
+    const int64_t held = a->features > 64 || a->out_features > 64 ? 512 : 768;
     const auto parts = [&](int64_t wanted, int64_t whole, int64_t least) {   // of `whole` chunks
         int64_t count = systems > 0 ? (wanted + systems - 1) / systems : 1;
         const int64_t most = (whole + least - 1) / least;
         count = count < most ? count : most;
         return count > 1 ? count : int64_t{1};
     };
-    const int64_t segments = parts(768, chunks, 2);
-    int64_t segment_chunks = chunks > 0 ? (chunks + segments - 1) / segments : 1;
-    const int64_t pieces = segments > 1 ? parts((1024 + segments - 2) / (segments - 1), segment_chunks, 2) : 1;
-    a->piece_chunks = (segment_chunks + pieces - 1) / pieces;
-    a->segment_chunks = a->piece_chunks * pieces;
+    const int64_t segments = parts(held, chunks, 2);
+    a->segment_chunks = chunks > 0 ? (chunks + segments - 1) / segments : 1;
     a->segments = chunks > 0 ? (chunks + a->segment_chunks - 1) / a->segment_chunks : 1;
-    a->pieces = (a->segments - 1) * pieces;
+    a->segment_pieces = a->segments > 1 ? parts((1024 + a->segments - 2) / (a->segments - 1), a->segment_chunks, 2) : 1;
+    a->piece_chunks = (a->segment_chunks + a->segment_pieces - 1) / a->segment_pieces;
+    a->segment_pieces = (a->segment_chunks + a->piece_chunks - 1) / a->piece_chunks;
+    a->pieces = (a->segments - 1) * a->segment_pieces;
 }
 
 hipError_t launch_walk(const WalkArgs& a, int dtype, hipStream_t stream) {
