@@ -651,58 +651,71 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     }
 }
 
-// The state before the first token of each segment, from what the pieces add.
+// The state before the first token of each segment, from what the pieces add; V
+// elements of it to a thread, AHEAD pieces in flight.
 constexpr int kCarryThreads = 256;
-constexpr int kCarryAhead = 16;   // pieces in flight
+template <int V, int AHEAD>
 __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
     const int size = a.features * a.out_features;
-    const int blocks = (size + kCarryThreads - 1) / kCarryThreads;
-    const int64_t system = blockIdx.x / blocks;   // batch, head
-    const int i = static_cast<int>(blockIdx.x - system * blocks) * kCarryThreads + static_cast<int>(threadIdx.x);
-    if (i >= size) {
-        return;
-    }
-    const int64_t batch = system / a.heads;
-    const int head = static_cast<int>(system - batch * a.heads);
-    const float rate = decay_rate(a.log_decay[head]);
-    float state = 0.0f;
-    if (a.first != nullptr) {
-        const int d = i / a.out_features;
-        state = a.first[system * size + d * a.first_row + (i - d * a.out_features) * a.first_column];
+    const uint32_t blocks = static_cast<uint32_t>((size + V * kCarryThreads - 1) / (V * kCarryThreads));
+    const uint32_t system = blockIdx.x / blocks;   // batch, head
+    const int i = static_cast<int>((blockIdx.x - system * blocks) * kCarryThreads + threadIdx.x) * V;
+    const uint32_t batch = system / static_cast<uint32_t>(a.heads);
+    const float rate = decay_rate(a.log_decay[system - batch * static_cast<uint32_t>(a.heads)]);
+    const bool mine = i < size;
+    float state[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        state[v] = 0.0f;
+        if (a.first != nullptr && mine) {
+            const int d = (i + v) / a.out_features;
+            state[v] = a.first[static_cast<int64_t>(system) * size + d * a.first_row +
+                               (i + v - d * a.out_features) * a.first_column];
+        }
     }
     int pending = a.shift;
     const int each = static_cast<int>(a.segment_pieces);
     int left = 0;   // pieces of the segment
-    const float* from = a.updates + system * a.pieces * size + i;
+    const float* from = a.updates + system * a.pieces * size + (mine ? i : 0);
     const int* counts = a.counts + batch * a.pieces;
     float* to = a.states + system * a.segments * size + i;
     const int pieces = static_cast<int>(a.pieces);
-    for (int s0 = 0; s0 < pieces; s0 += kCarryAhead) {
-        const int some = pieces - s0 < kCarryAhead ? pieces - s0 : kCarryAhead;
-        float update[kCarryAhead];
+    const int lane = static_cast<int>(threadIdx.x) & (AHEAD - 1);
+    const auto store = [&]() {
+        if (mine) {
+            store_values<LSSO_HIP_F32, V>(to, state);
+        }
+        to += size;
+    };
+    for (int s0 = 0; s0 < pieces; s0 += AHEAD) {
+        const int some = pieces - s0 < AHEAD ? pieces - s0 : AHEAD;
+        // One load of all the counts: a scalar load of each would be waited for.
+        const int these = counts[s0 + (lane < some ? lane : 0)];
+        float update[AHEAD][V];
 #pragma unroll
-        for (int j = 0; j < kCarryAhead; ++j) {
-            if (j < some) {   // uniform
-                update[j] = from[static_cast<int64_t>(s0 + j) * size];
-            }
+        for (int j = 0; j < AHEAD; ++j) {   // the last one again where there are fewer
+            load_values<LSSO_HIP_F32, V>(from + static_cast<int64_t>(s0 + (j < some ? j : some - 1)) * size, update[j]);
         }
 #pragma unroll
-        for (int j = 0; j < kCarryAhead; ++j) {
-            if (j < some) {
+        for (int j = 0; j < AHEAD; ++j) {
+            if (j < some) {   // uniform
                 if (left == 0) {
-                    *to = state;
-                    to += size;
+                    store();
                     left = each;
                 }
                 --left;
-                const int count = counts[s0 + j];
+                const int count = __builtin_amdgcn_readlane(these, j);
                 const int less = count > 0 ? pending : 0;
                 pending -= less;
-                state = state * __builtin_amdgcn_exp2f(rate * static_cast<float>(count - less)) + update[j];
+                const float decay = __builtin_amdgcn_exp2f(rate * static_cast<float>(count - less));
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    state[v] = state[v] * decay + update[j][v];
+                }
             }
         }
     }
-    *to = state;   // of the last segment
+    store();   // of the last segment
 }
 
 template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE>
@@ -713,8 +726,17 @@ void launch_parts(const WalkArgs& a, hipStream_t stream) {
     if (a.segments > 1 && a.reuse == 0) {
         walk_kernel<T, KT, NW, WE, PARTS, WHOLE, true>
             <<<static_cast<unsigned>(systems * a.pieces * across), 64 * NW, 0, stream>>>(a);
-        const int64_t blocks = (a.features * a.out_features + kCarryThreads - 1) / kCarryThreads;
-        carry_kernel<<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
+        // Four elements to a thread where that leaves a workgroup to each compute unit.
+        const int64_t elements = a.features * a.out_features;
+        const int64_t blocks = (elements + 4 * kCarryThreads - 1) / (4 * kCarryThreads);
+        if (elements % 4 != 0 || systems * blocks < 256) {
+            carry_kernel<1, 32><<<static_cast<unsigned>(systems * ((elements + kCarryThreads - 1) / kCarryThreads)),
+                                  kCarryThreads, 0, stream>>>(a);
+        } else if (a.pieces > 4) {
+            carry_kernel<4, 16><<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
+        } else {
+            carry_kernel<4, 4><<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
+        }
     }
     walk_kernel<T, KT, NW, WE, PARTS, WHOLE, false>
         <<<static_cast<unsigned>(systems * a.segments * across), 64 * NW, 0, stream>>>(a);
@@ -879,7 +901,7 @@ void plan_walk(WalkArgs* a) {
     const int64_t segments = parts(held, chunks, 2);
     a->segment_chunks = chunks > 0 ? (chunks + segments - 1) / segments : 1;
     a->segments = chunks > 0 ? (chunks + a->segment_chunks - 1) / a->segment_chunks : 1;
-    a->segment_pieces = a->segments > 1 ? parts((1024 + a->segments - 2) / (a->segments - 1), a->segment_chunks, 2) : 1;
+    a->segment_pieces = a->segments > 1 ? parts(1024 / (a->segments - 1) / systems * systems, a->segment_chunks, 2) : 1;
     a->piece_chunks = (a->segment_chunks + a->segment_pieces - 1) / a->segment_pieces;
     a->segment_pieces = (a->segment_chunks + a->piece_chunks - 1) / a->piece_chunks;
     a->pieces = (a->segments - 1) * a->segment_pieces;
