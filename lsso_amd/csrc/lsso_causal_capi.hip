@@ -234,7 +234,7 @@ int lsso_hip_rotary(const lsso_hip_rotary_tensor* tensors, int count, int dtype,
         if (batch * length > 0 && (t.x == nullptr || t.y == nullptr || !aligned(t.x, bytes) || !aligned(t.y, bytes))) {
             return report(LSSO_HIP_EINVAL, "x and y must not be NULL and be aligned to their type");
         }
-        a.tensors[i] = {t.x, t.y, t.batch_stride, t.token_stride, t.head_stride, static_cast<int>(t.heads), 0};
+        a.tensors[i] = {t.x, t.y, t.batch_stride, t.token_stride, t.head_stride, static_cast<int>(t.heads)};
     }
     if (batch * length == 0) {
         return LSSO_HIP_OK;

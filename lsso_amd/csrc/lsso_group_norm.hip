@@ -43,16 +43,16 @@ constexpr int kBlockRows = 4;        // rows of a thread in flight
 constexpr int kTeamMost = 4;         // most pieces of a lane
 constexpr int64_t kMostGrid = 1 << 20;
 
-// act(z) and act'(z).  FP32 outputs show more than the fast forms hold (1e-5 of
-// the sigmoid's and the distribution function's own value).
-template <int T, bool SLOPE>
-__device__ __forceinline__ void act(int kind, float z, float& value, float& slope) {
-    if (kind == 0) {
+// act(z) and act'(z) of one kind.  FP32 outputs show more than the fast forms hold
+// (1e-5 of the sigmoid's and the distribution function's own value).
+template <int T, int KIND, bool SLOPE>
+__device__ __forceinline__ void act(float z, float& value, float& slope) {
+    if constexpr (KIND == 0) {
         value = z;
         slope = 1.0f;
     } else if constexpr (T != LSSO_HIP_F32) {
-        activation<SLOPE>(kind, z, value, slope);
-    } else if (kind == LSSO_HIP_SILU) {
+        activation<SLOPE>(KIND, z, value, slope);
+    } else if constexpr (KIND == LSSO_HIP_SILU) {
         const float s = 1.0f / (1.0f + expf(-z));
         value = z * s;
         slope = SLOPE ? s + value * (1.0f - s) : 0.0f;
@@ -60,6 +60,22 @@ __device__ __forceinline__ void act(int kind, float z, float& value, float& slop
         const float phi = normcdff(z);
         value = z * phi;
         slope = SLOPE ? phi + 0.3989422804f * z * expf(-0.5f * z * z) : 0.0f;
+    }
+}
+
+template <int KIND>
+struct Kind {
+    static constexpr int value = KIND;
+};
+// f of the activation's kind: one branch for all of a row's elements.
+template <typename F>
+__device__ __forceinline__ void by_kind(int kind, F f) {
+    if (kind == 0) {
+        f(Kind<0>{});
+    } else if (kind == LSSO_HIP_SILU) {
+        f(Kind<LSSO_HIP_SILU>{});
+    } else {
+        f(Kind<LSSO_HIP_GELU>{});
     }
 }
 
@@ -82,10 +98,31 @@ __device__ __forceinline__ void store_parameter(void* values, int type, int c, f
     }
 }
 
-// Sum over the team's lanes, a power of two of neighbours, in all of them.
+// Sum over the team's lanes, a power of two of neighbours, in all of them: up to 16
+// by moves within a row of lanes, which wait for no LDS.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v) {
+    return __builtin_bit_cast(float,
+                              __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float team_sum(float v, int lanes) {
-    for (int offset = 1; offset < lanes; offset *= 2) {
-        v += __shfl_xor(v, offset);
+    if (lanes > 1) {
+        v += moved<0xb1>(v);    // quad_perm 1, 0, 3, 2
+    }
+    if (lanes > 2) {
+        v += moved<0x4e>(v);    // quad_perm 2, 3, 0, 1
+    }
+    if (lanes > 4) {
+        v += moved<0x141>(v);   // row_half_mirror: of the other four lanes, which hold one value
+    }
+    if (lanes > 8) {
+        v += moved<0x140>(v);   // row_mirror: of the other eight
+    }
+    if (lanes > 16) {
+        v += __shfl_xor(v, 16);
+    }
+    if (lanes > 32) {
+        v += __shfl_xor(v, 32);
     }
     return v;
 }
@@ -142,94 +179,120 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
             }
         }
     }
+    // Rows of a team in flight: as many as hold 32 values of x.
+    constexpr int kFlight = K * V <= 8 ? (BACKWARD ? 2 : 4) : (K * V <= 16 ? 2 : 1);
     const int64_t step = static_cast<int64_t>(gridDim.x) * t.at_once;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * t.at_once; row0 < a.samples; row0 += step) {
-        const int64_t row = row0 + t.row;
-        const bool inside = row < a.samples;
-        const bool kept = inside && (a.row_mask == nullptr || a.row_mask[row] != 0);
-        const int64_t at = (inside ? row : 0) * a.channels + channel0;
-        float x[K][V];
-        float dy[BACKWARD ? K : 1][V];
-        float sum = 0.0f;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * t.at_once; row0 < a.samples; row0 += kFlight * step) {
+        bool inside[kFlight];
+        bool kept[kFlight];
+        int64_t at[kFlight];
+        Raw<T, V> raw_x[kFlight][K];
+        Raw<T, V> raw_dy[kFlight][BACKWARD ? K : 1];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int piece = t.lane + a.team * k;
-            if (mine[k] && kept) {
-                load_values<T, V>(static_cast<const Element*>(a.x) + at + piece * V, x[k]);
-                if constexpr (BACKWARD) {
-                    load_values<T, V>(static_cast<const Element*>(a.dy) + at + piece * V, dy[k]);
+        for (int f = 0; f < kFlight; ++f) {
+            const int64_t row = row0 + t.row + f * step;
+            inside[f] = row < a.samples;
+            kept[f] = inside[f] && (a.row_mask == nullptr || a.row_mask[row] != 0);
+            at[f] = (inside[f] ? row : 0) * a.channels + channel0;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int piece = t.lane + a.team * k;
+                raw_x[f][k].clear();
+                if (mine[k] && kept[f]) {
+                    raw_x[f][k].load(static_cast<const Element*>(a.x) + at[f] + piece * V);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[k][i] = 0.0f;
-                    if constexpr (BACKWARD) {
-                        dy[k][i] = 0.0f;
+                if constexpr (BACKWARD) {
+                    raw_dy[f][k].clear();
+                    if (mine[k] && kept[f]) {
+                        raw_dy[f][k].load(static_cast<const Element*>(a.dy) + at[f] + piece * V);
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sum += x[k][i];
-            }
         }
-        const float mean = team_sum(sum, a.team) * share;
-        float squares = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[k][i] = mine[k] ? x[k][i] - mean : 0.0f;
-                squares += x[k][i] * x[k][i];
-            }
-        }
-        const float rstd = 1.0f / sqrtf(team_sum(squares, a.team) * share + a.eps);
-        if constexpr (!BACKWARD) {
+        for (int f = 0; f < kFlight; ++f) {
+            float x[K][V];
+            float dy[BACKWARD ? K : 1][V];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                float y[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float slope;
-                    act<T, false>(a.activation, x[k][i] * rstd * w[k][i] + b[k][i], y[i], slope);
-                    y[i] = kept ? y[i] : 0.0f;
-                }
-                if (mine[k] && inside) {
-                    store_values<T, V>(static_cast<Element*>(a.y) + at + (t.lane + a.team * k) * V, y);
+                raw_x[f][k].values(x[k]);
+                if constexpr (BACKWARD) {
+                    raw_dy[f][k].values(dy[k]);
                 }
             }
-        } else {
-            float first = 0.0f;
-            float second = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    x[k][i] *= rstd;
-                    float value;
-                    float slope;
-                    act<T, true>(a.activation, x[k][i] * w[k][i] + b[k][i], value, slope);
-                    // A row that is left out has no part in any sum.
-                    const float dz = kept ? dy[k][i] * slope : 0.0f;
-                    const float normal = kept ? x[k][i] : 0.0f;
-                    grad_b[k][i] += dz;
-                    grad_w[k][i] += dz * normal;
-                    dy[k][i] = dz * w[k][i];
-                    first += dy[k][i];
-                    second += dy[k][i] * normal;
+                    sum += x[k][i];
                 }
             }
-            first = team_sum(first, a.team) * share;
-            second = team_sum(second, a.team) * share;
+            const float mean = team_sum(sum, a.team) * share;
+            float squares = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                float dx[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    dx[i] = kept ? rstd * (dy[k][i] - (first + x[k][i] * second)) : 0.0f;
+                    x[k][i] = mine[k] ? x[k][i] - mean : 0.0f;
+                    squares += x[k][i] * x[k][i];
                 }
-                if (a.dx != nullptr && mine[k] && inside) {
-                    store_values<T, V>(static_cast<Element*>(a.dx) + at + (t.lane + a.team * k) * V, dx);
+            }
+            const float rstd = 1.0f / sqrtf(team_sum(squares, a.team) * share + a.eps);
+            if constexpr (!BACKWARD) {
+                by_kind(a.activation, [&](auto kind) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            float y;
+                            float slope;
+                            act<T, decltype(kind)::value, false>(x[k][i] * rstd * w[k][i] + b[k][i], y, slope);
+                            x[k][i] = kept[f] ? y : 0.0f;
+                        }
+                    }
+                });
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (mine[k] && inside[f]) {
+                        store_values<T, V>(static_cast<Element*>(a.y) + at[f] + (t.lane + a.team * k) * V, x[k]);
+                    }
+                }
+            } else {
+                float first = 0.0f;
+                float second = 0.0f;
+                by_kind(a.activation, [&](auto kind) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            x[k][i] *= rstd;
+                            float value;
+                            float slope;
+                            act<T, decltype(kind)::value, true>(x[k][i] * w[k][i] + b[k][i], value, slope);
+                            // A row that is left out has no part in any sum.
+                            const float dz = kept[f] ? dy[k][i] * slope : 0.0f;
+                            const float normal = kept[f] ? x[k][i] : 0.0f;
+                            grad_b[k][i] += dz;
+                            grad_w[k][i] += dz * normal;
+                            dy[k][i] = dz * w[k][i];
+                            first += dy[k][i];
+                            second += dy[k][i] * normal;
+                        }
+                    }
+                });
+                first = team_sum(first, a.team) * share;
+                second = team_sum(second, a.team) * share;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    float dx[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        dx[i] = kept[f] ? rstd * (dy[k][i] - (first + x[k][i] * second)) : 0.0f;
+                    }
+                    if (a.dx != nullptr && mine[k] && inside[f]) {
+                        store_values<T, V>(static_cast<Element*>(a.dx) + at[f] + (t.lane + a.team * k) * V, dx);
+                    }
                 }
             }
         }
@@ -295,21 +358,16 @@ __host__ __device__ inline int64_t partial_pitch(int channels) { return 2 * stat
 // Rows at, at + step, ... (kBlockRows of them) of a thread: loads, and which count.
 template <int T, int V>
 __device__ __forceinline__ void load_rows(const void* from, const GroupNormArgs& a, int64_t sample, int64_t at, int step,
-                                          int64_t end, int channel, float (&v)[kBlockRows][V],
+                                          int64_t end, int channel, Raw<T, V> (&v)[kBlockRows],
                                           bool (&kept)[kBlockRows]) {
     using Element = typename Values<T>::Element;
 #pragma unroll
     for (int r = 0; r < kBlockRows; ++r) {
         const int64_t row = at + static_cast<int64_t>(r) * step;
         kept[r] = row < end && (a.row_mask == nullptr || a.row_mask[sample * a.length + row] != 0);
+        v[r].clear();
         if (kept[r]) {
-            load_values<T, V>(static_cast<const Element*>(from) + (sample * a.length + row) * a.channels + channel,
-                              v[r]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                v[r][i] = 0.0f;
-            }
+            v[r].load(static_cast<const Element*>(from) + (sample * a.length + row) * a.channels + channel);
         }
     }
 }
@@ -335,10 +393,15 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(GroupNormArgs
         }
         if (c.active) {
             for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
-                float v[kBlockRows][V];
+                Raw<T, V> raw[kBlockRows];
                 bool kept[kBlockRows];
-                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
+                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, raw, kept);
+                float v[kBlockRows][V];
                 float some = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kBlockRows; ++r) {
+                    raw[r].values(v[r]);
+                }
 #pragma unroll
                 for (int r = 0; r < kBlockRows; ++r) {
                     some += kept[r] ? 1.0f : 0.0f;
@@ -466,20 +529,42 @@ struct ChannelValues {
     float mean[V];
     float rstd[V];
     __device__ __forceinline__ void parameters(const GroupNormArgs& a, int channel) {
+        if (a.parameter_type == LSSO_HIP_F32 && a.weight != nullptr && a.bias != nullptr) {   // uniform
+            load_values<LSSO_HIP_F32, V>(static_cast<const float*>(a.weight) + channel, w);
+            load_values<LSSO_HIP_F32, V>(static_cast<const float*>(a.bias) + channel, b);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             w[i] = parameter(a.weight, a.parameter_type, channel + i, 1.0f);
             b[i] = parameter(a.bias, a.parameter_type, channel + i, 0.0f);
         }
     }
-    __device__ __forceinline__ void of_sample(const GroupNormArgs& a, int64_t sample, int channel) {
-        const int size = a.channels / a.groups;
+    // Two values of each group, to the channels of each.
+    __device__ __forceinline__ static void spread(const GroupNormArgs& a, const float* from, int64_t sample, int channel,
+                                                  float (&first)[V], float (&second)[V]) {
+        const uint32_t size = static_cast<uint32_t>(a.channels) / static_cast<uint32_t>(a.groups);
+        const float* groups = from + 2 * sample * a.groups;
+        if (size % V == 0) {   // uniform: the channels are of one group
+            const uint32_t group = static_cast<uint32_t>(channel) / size;
+            const float one = groups[2 * group];
+            const float two = groups[2 * group + 1];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                first[i] = one;
+                second[i] = two;
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int64_t at = 2 * (sample * a.groups + (channel + i) / size);
-            mean[i] = a.statistics[at];
-            rstd[i] = a.statistics[at + 1];
+            const uint32_t group = static_cast<uint32_t>(channel + i) / size;
+            first[i] = groups[2 * group];
+            second[i] = groups[2 * group + 1];
         }
+    }
+    __device__ __forceinline__ void of_sample(const GroupNormArgs& a, int64_t sample, int channel) {
+        spread(a, a.statistics, sample, channel, mean, rstd);
     }
 };
 
@@ -499,24 +584,27 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(GroupNormArgs a) {
         const int64_t end = begin + a.split_rows < a.length ? begin + a.split_rows : a.length;
         channel.of_sample(a, sample, c.channel);
         for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
-            float v[kBlockRows][V];
+            Raw<T, V> raw[kBlockRows];
             bool kept[kBlockRows];
-            load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
+            load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, raw, kept);
 #pragma unroll
             for (int r = 0; r < kBlockRows; ++r) {
-                const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
-                if (row < end) {
+                float v[V];
+                raw[r].values(v);
+                by_kind(a.activation, [&](auto kind) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         float slope;
                         float y;
-                        act<T, false>(a.activation,
-                                      (v[r][i] - channel.mean[i]) * channel.rstd[i] * channel.w[i] + channel.b[i], y,
-                                      slope);
-                        v[r][i] = kept[r] ? y : 0.0f;
+                        act<T, decltype(kind)::value, false>(
+                            (v[i] - channel.mean[i]) * channel.rstd[i] * channel.w[i] + channel.b[i], y, slope);
+                        v[i] = kept[r] ? y : 0.0f;
                     }
+                });
+                const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
+                if (row < end) {
                     store_values<T, V>(
-                        static_cast<Element*>(a.y) + (sample * a.length + row) * a.channels + c.channel, v[r]);
+                        static_cast<Element*>(a.y) + (sample * a.length + row) * a.channels + c.channel, v);
                 }
             }
         }
@@ -531,7 +619,6 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(GroupNormArgs a) {
     __shared__ float shared[DX ? 1 : kThreads][2 * V + 1];
     __shared__ float rows[DX ? 1 : kThreads];
     const Columns<V> c(a);
-    const int size = a.channels / a.groups;
     ChannelValues<V> channel;
     if (c.active) {
         channel.parameters(a, c.channel);
@@ -552,43 +639,43 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(GroupNormArgs a) {
         if (c.active) {
             channel.of_sample(a, sample, c.channel);
             if constexpr (DX) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int64_t at = 2 * (sample * a.groups + (c.channel + i) / size);
-                    first[i] = a.sums[at];
-                    second[i] = a.sums[at + 1];
-                }
+                ChannelValues<V>::spread(a, a.sums, sample, c.channel, first, second);
             }
             for (int64_t at = begin + c.row; at < end; at += kBlockRows * c.at_once) {
-                float v[kBlockRows][V];
-                float dy[kBlockRows][V];
+                Raw<T, V> raw_x[kBlockRows];
+                Raw<T, V> raw_dy[kBlockRows];
                 bool kept[kBlockRows];
-                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, v, kept);
-                load_rows<T, V>(a.dy, a, sample, at, c.at_once, end, c.channel, dy, kept);
+                load_rows<T, V>(a.x, a, sample, at, c.at_once, end, c.channel, raw_x, kept);
+                load_rows<T, V>(a.dy, a, sample, at, c.at_once, end, c.channel, raw_dy, kept);
 #pragma unroll
                 for (int r = 0; r < kBlockRows; ++r) {
-                    const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
                     count += kept[r] ? 1.0f : 0.0f;
+                    float x[V];
+                    float dy[V];
+                    raw_x[r].values(x);
+                    raw_dy[r].values(dy);
+                    by_kind(a.activation, [&](auto kind) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float normal = kept[r] ? (v[r][i] - channel.mean[i]) * channel.rstd[i] : 0.0f;
-                        float value;
-                        float slope;
-                        act<T, true>(a.activation, normal * channel.w[i] + channel.b[i], value, slope);
-                        const float dz = kept[r] ? dy[r][i] * slope : 0.0f;
-                        if constexpr (DX) {
-                            v[r][i] = kept[r] ? channel.rstd[i] * (dz * channel.w[i] - (first[i] + normal * second[i]))
-                                              : 0.0f;
-                        } else {
-                            first[i] += dz;
-                            second[i] += dz * normal;
+                        for (int i = 0; i < V; ++i) {
+                            const float normal = kept[r] ? (x[i] - channel.mean[i]) * channel.rstd[i] : 0.0f;
+                            float value;
+                            float slope;
+                            act<T, decltype(kind)::value, true>(normal * channel.w[i] + channel.b[i], value, slope);
+                            const float dz = kept[r] ? dy[i] * slope : 0.0f;
+                            if constexpr (DX) {
+                                x[i] = kept[r] ? channel.rstd[i] * (dz * channel.w[i] - (first[i] + normal * second[i]))
+                                               : 0.0f;
+                            } else {
+                                first[i] += dz;
+                                second[i] += dz * normal;
+                            }
                         }
-                    }
+                    });
                     if constexpr (DX) {
+                        const int64_t row = at + static_cast<int64_t>(r) * c.at_once;
                         if (row < end) {
                             store_values<T, V>(
-                                static_cast<Element*>(a.dx) + (sample * a.length + row) * a.channels + c.channel,
-                                v[r]);
+                                static_cast<Element*>(a.dx) + (sample * a.length + row) * a.channels + c.channel, x);
                         }
                     }
                 }
@@ -820,9 +907,9 @@ void plan_group_norm(GroupNormArgs* a, bool backward, size_t* partial_bytes) {
     const int64_t across = (a->channels / a->vector + kThreads - 1) / kThreads;
     const int64_t wide = a->channels / a->vector < kThreads ? a->channels / a->vector : kThreads;
     const int64_t block = kBlockRows * (kThreads / wide);   // rows of a workgroup in flight
-    // About eight workgroups to a compute unit, each with a whole block of rows.
+    // About four workgroups to a compute unit, each with whole blocks of rows.
     const int64_t items = a->samples * across;
-    const int64_t wanted = items > 0 && items < 2048 ? 2048 / items : 1;
+    const int64_t wanted = items > 0 && items < 1024 ? 1024 / items : 1;
     const int64_t rows = (a->length + wanted - 1) / wanted;
     a->split_rows = rows > 0 ? (rows + block - 1) / block * block : block;
     a->splits = (a->length + a->split_rows - 1) / a->split_rows;

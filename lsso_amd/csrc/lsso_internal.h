@@ -473,7 +473,6 @@ struct RotaryTensor {
     int64_t token_stride;
     int64_t head_stride;
     int heads;
-    uint32_t head_magic;        // set by the launcher
 };
 
 struct RotaryArgs {
@@ -490,9 +489,7 @@ struct RotaryArgs {
     int position_type;
     int64_t position_batch_stride;
     int64_t position_token_stride;
-    int tile;                   // tokens, set by the launcher, as what follows
-    uint32_t half_magic;
-    int lanes_shift;            // log2 of the lanes of a row
+    int heads_each;             // heads of a workgroup, set by the launcher
 };
 
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, int layout, hipStream_t stream);

@@ -7,11 +7,14 @@
 //
 // Angles are products in 64 bits, brought into one turn before they are rounded
 // to 32: a position of a million times a frequency of 1 has no correct digit
-// left of its cosine in 32 bits.  That costs a few FP64 operations and a sine
-// and cosine for each token and pair, so a workgroup makes them once for a tile
-// of tokens, keeps them in LDS, and turns all heads of both tensors with them.
+// left of its cosine in 32 bits.
 //
-// Bound: HBM, one read and one write of each tensor.
+// Bound: HBM, one read and one write of each tensor.  A thread takes the same few
+// features of every head of a token, so that each phase is made once, with the
+// first heads' loads already on their way, and nothing passes through LDS.  (The
+// phases of a tile of tokens made first, kept in LDS and read by all heads took 115
+// us instead of 95 at 64 x 4,096 tokens of 4 + 4 heads of 64 in BF16: the loads
+// waited for them and for two barriers.)
 
 #include "lsso_device.h"
 #include "lsso_internal.h"
@@ -24,15 +27,8 @@ namespace lsso_hip {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTable = 2048;      // phases of a tile: 16 KB of LDS
-constexpr int kMostTokens = 16;   // of a tile
-constexpr int kRows = 4;          // rows of a thread in flight
-constexpr int kMostTiles = 4096;  // of a grid; each workgroup takes every gridDim.x-th tile
-
-// i / d for i d < 2^32, by magic = ceil(2^32 / d).
-__device__ __forceinline__ uint32_t divide(uint32_t i, uint32_t magic) {
-    return magic == 0 ? i : __umulhi(i, magic);   // 0: d is 1
-}
+constexpr int kHeads = 4;   // of a thread in flight
+constexpr int64_t kMostGrid = 1 << 22;
 
 __device__ double position_at(const RotaryArgs& a, int64_t batch, int64_t token) {
     const int64_t at = batch * a.position_batch_stride + token * a.position_token_stride;
@@ -45,148 +41,139 @@ __device__ double position_at(const RotaryArgs& a, int64_t batch, int64_t token)
     }
 }
 
+// n / d of not negative numbers, in 32 bits where they fit (a division of 64 takes long).
+__device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
+    return n <= 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
+}
+
 // T: type; HALF: the partner of feature j is feature j + half, else pairs are
-// neighbours; V: features of an access, which divides what a lane turns at once
-// (half of the rotated part, or all of it).
+// neighbours; V: features of an access, which divides what is turned (half of the
+// rotated part, or all of it).
 template <int T, bool HALF, int V>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     using Element = typename Values<T>::Element;
-    __shared__ float2 table[kTable];
-    __shared__ double position[kMostTokens];
-    __shared__ int64_t base[2][kMostTokens];
-    const int tid = threadIdx.x;
+    constexpr int kPhases = HALF ? V : V / 2;
     const int half = a.half;
-    const int turned = HALF ? half / V : 2 * half / V;                       // units that turn
-    const int copied = (a.features - 2 * half + V - 1) / V;                  // units that are copied
-    const int units = turned + copied;
-    const int64_t tokens = a.batch * a.length;
-    const int64_t tiles = (tokens + a.tile - 1) / a.tile;
-    const int lanes = 1 << a.lanes_shift;
-    const int rows_at_once = kThreads >> a.lanes_shift;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t first = tile * a.tile;
-        const int count = static_cast<int>(tokens - first < a.tile ? tokens - first : a.tile);
-        __syncthreads();   // the last tile's readers are done
-        if (tid < count) {
-            const int64_t batch = (first + tid) / a.length;
-            const int64_t token = first + tid - batch * a.length;
-            position[tid] = position_at(a, batch, token);
-            for (int w = 0; w < a.count; ++w) {
-                base[w][tid] = batch * a.tensors[w].batch_stride + token * a.tensors[w].token_stride;
+    const int turned = HALF ? half / V : 2 * half / V;                             // units of a head that turn
+    const int units = turned + (a.features - 2 * half + V - 1) / V;                // and that are copied
+    const int64_t items = a.batch * a.length * units;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; item < items; item += step) {
+        const int64_t row = divide(item, units);
+        const int unit = static_cast<int>(item - row * units);
+        const int64_t batch = divide(row, a.length);
+        const int64_t token = row - batch * a.length;
+        const bool turns = unit < turned;
+        const int feature = unit * V + (HALF && !turns ? half : 0);
+        const bool whole = turns || feature + V <= a.features;
+        // The heads of both tensors in one row, of which this workgroup takes a part.
+        const int heads0 = a.tensors[0].heads;
+        const int heads = heads0 + (a.count > 1 ? a.tensors[1].heads : 0);
+        const int first = static_cast<int>(blockIdx.y) * a.heads_each;
+        const int last = first + a.heads_each < heads ? first + a.heads_each : heads;
+        const auto from = [&](int head) {
+            const RotaryTensor& t = a.tensors[head < heads0 ? 0 : 1];
+            return static_cast<const Element*>(t.x) + batch * t.batch_stride + token * t.token_stride +
+                   (head < heads0 ? head : head - heads0) * t.head_stride + feature;
+        };
+        const auto to = [&](int head) {
+            const RotaryTensor& t = a.tensors[head < heads0 ? 0 : 1];
+            return static_cast<Element*>(t.y) +
+                   (row * t.heads + (head < heads0 ? head : head - heads0)) * a.features + feature;
+        };
+        if (!whole) {
+            for (int head = first; head < last; ++head) {
+                for (int i = 0; feature + i < a.features; ++i) {
+                    to(head)[i] = from(head)[i];
+                }
+            }
+            continue;
+        }
+        Raw<T, V> raw[kHeads];
+        Raw<T, V> other[HALF ? kHeads : 1];
+        const auto load = [&](int head0) {
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) {
+                if (head0 + k < last) {
+                    const Element* at = from(head0 + k);
+                    raw[k].load(at);
+                    if constexpr (HALF) {
+                        if (turns) {
+                            other[k].load(at + half);
+                        }
+                    }
+                }
+            }
+        };
+        load(first);
+        float cosine[kPhases];
+        float sine[kPhases];
+        if (turns) {
+            const double position = position_at(a, batch, token);
+            const double* frequencies = a.frequencies + (HALF ? feature : feature / 2);
+#pragma unroll
+            for (int i = 0; i < kPhases; ++i) {
+                // In turns, so that the whole ones can be dropped.
+                const double angle = position * (frequencies[i] * 0.15915494309189535);
+                sincospif(2.0f * static_cast<float>(angle - rint(angle)), &sine[i], &cosine[i]);
+                cosine[i] *= a.amplitude;
+                sine[i] *= a.amplitude * a.sign;
             }
         }
-        __syncthreads();
-        for (int i = tid; i < count * half; i += kThreads) {
-            const int t = divide(i, a.half_magic);
-            // In turns, so that the whole ones can be dropped.
-            const double turns = position[t] * (a.frequencies[i - t * half] * 0.15915494309189535);
-            float sine;
-            float cosine;
-            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
-            table[i] = make_float2(a.amplitude * cosine, a.amplitude * a.sign * sine);
-        }
-        __syncthreads();
-        for (int w = 0; w < a.count; ++w) {
-            const RotaryTensor& tensor = a.tensors[w];
-            const Element* x = static_cast<const Element*>(tensor.x);
-            Element* y = static_cast<Element*>(tensor.y);
-            const int rows = count * tensor.heads;
-            for (int row0 = tid >> a.lanes_shift; row0 < rows; row0 += kRows * rows_at_once) {
-                for (int u = tid & (lanes - 1); u < units; u += lanes) {
-                    const bool turns = u < turned;
-                    const int feature = u * V + (HALF && !turns ? half : 0);
-                    const bool whole = turns || feature + V <= a.features;
-                    float v[kRows][V];
-                    float other[kRows][HALF ? V : 1];
+        for (int head0 = first; head0 < last; head0 += kHeads) {
+            if (head0 != first) {
+                load(head0);
+            }
 #pragma unroll
-                    for (int k = 0; k < kRows; ++k) {
-                        const int row = row0 + k * rows_at_once;
-                        if (row < rows) {
-                            const int t = divide(row, tensor.head_magic);
-                            const Element* at =
-                                x + base[w][t] + (row - t * tensor.heads) * tensor.head_stride + feature;
-                            if (whole) {
-                                load_values<T, V>(at, v[k]);
-                                if constexpr (HALF) {
-                                    if (turns) {
-                                        load_values<T, V>(at + half, other[k]);
-                                    }
-                                }
-                            } else {
+            for (int k = 0; k < kHeads; ++k) {
+                if (head0 + k >= last) {
+                    break;
+                }
+                Element* at = to(head0 + k);
+                float v[V];
+                raw[k].values(v);
+                if (!turns) {
+                    store_values<T, V>(at, v);
+                } else if constexpr (HALF) {
+                    float first_half[V];
+                    float second_half[V];
+                    other[k].values(second_half);
 #pragma unroll
-                                for (int i = 0; i < V; ++i) {
-                                    v[k][i] = feature + i < a.features ? Values<T>::load(at + i) : 0.0f;
-                                }
-                            }
-                        }
+                    for (int i = 0; i < V; ++i) {
+                        first_half[i] = v[i] * cosine[i] - second_half[i] * sine[i];
+                        second_half[i] = v[i] * sine[i] + second_half[i] * cosine[i];
                     }
+                    store_values<T, V>(at, first_half);
+                    store_values<T, V>(at + half, second_half);
+                } else {
+                    float both[V];
 #pragma unroll
-                    for (int k = 0; k < kRows; ++k) {
-                        const int row = row0 + k * rows_at_once;
-                        if (row >= rows) {
-                            continue;
-                        }
-                        const int t = divide(row, tensor.head_magic);
-                        Element* to = y + (first * tensor.heads + row) * a.features + feature;
-                        if (!turns) {
-                            if (whole) {
-                                store_values<T, V>(to, v[k]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < V; ++i) {
-                                    if (feature + i < a.features) {
-                                        Values<T>::store(to + i, v[k][i]);
-                                    }
-                                }
-                            }
-                        } else if constexpr (HALF) {
-                            const float2* phase = table + t * half + feature;
-                            float second[V];
-#pragma unroll
-                            for (int i = 0; i < V; ++i) {
-                                const float2 p = phase[i];
-                                const float value = v[k][i] * p.x - other[k][i] * p.y;
-                                second[i] = v[k][i] * p.y + other[k][i] * p.x;
-                                v[k][i] = value;
-                            }
-                            store_values<T, V>(to, v[k]);
-                            store_values<T, V>(to + half, second);
-                        } else {
-                            const float2* phase = table + t * half + feature / 2;
-#pragma unroll
-                            for (int i = 0; i < V; i += 2) {
-                                const float2 p = phase[i / 2];
-                                const float value = v[k][i] * p.x - v[k][i + 1] * p.y;
-                                v[k][i + 1] = v[k][i] * p.y + v[k][i + 1] * p.x;
-                                v[k][i] = value;
-                            }
-                            store_values<T, V>(to, v[k]);
-                        }
+                    for (int i = 0; i < V; i += 2) {
+                        both[i] = v[i] * cosine[i / 2] - v[i + 1] * sine[i / 2];
+                        both[i + 1] = v[i] * sine[i / 2] + v[i + 1] * cosine[i / 2];
                     }
+                    store_values<T, V>(at, both);
                 }
             }
         }
     }
 }
 
-uint32_t magic(uint32_t d) { return d == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d); }
-
 template <int T, bool HALF, int V>
 void launch(RotaryArgs a, hipStream_t stream) {
     const int units = (HALF ? a.half : 2 * a.half) / V + (a.features - 2 * a.half + V - 1) / V;
-    a.lanes_shift = 0;
-    while ((1 << a.lanes_shift) < units && (1 << a.lanes_shift) < kThreads) {
-        ++a.lanes_shift;
+    const int64_t items = a.batch * a.length * units;
+    const int64_t blocks = (items + kThreads - 1) / kThreads;
+    const int heads = a.tensors[0].heads + (a.count > 1 ? a.tensors[1].heads : 0);
+    // All heads to a thread, unless that leaves compute units without two workgroups:
+    // then fewer, whose phases are made more than once.
+    int parts = 1;
+    while (parts * kHeads < heads && blocks * parts < 512) {
+        ++parts;
     }
-    const int64_t tokens = a.batch * a.length;
-    // A tile as large as its phases fit, but no larger than leaves eight tiles
-    // to a compute unit.
-    int64_t tile = (tokens + 2047) / 2048;
-    const int64_t most = a.half > 0 ? kTable / a.half : kMostTokens;
-    tile = tile > most ? most : tile;
-    a.tile = static_cast<int>(tile > kMostTokens ? kMostTokens : tile);
-    const int64_t tiles = (tokens + a.tile - 1) / a.tile;
-    const unsigned grid = static_cast<unsigned>(tiles < kMostTiles ? tiles : kMostTiles);
+    a.heads_each = (heads + parts - 1) / parts;
+    parts = (heads + a.heads_each - 1) / a.heads_each;
+    const dim3 grid(static_cast<unsigned>(blocks < kMostGrid ? blocks : kMostGrid), static_cast<unsigned>(parts));
     rotary_kernel<T, HALF, V><<<grid, kThreads, 0, stream>>>(a);
 }
 
@@ -215,14 +202,9 @@ void launch_layout(const RotaryArgs& a, int layout, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_rotary(const RotaryArgs& args, int dtype, int layout, hipStream_t stream) {
-    RotaryArgs a = args;
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, int layout, hipStream_t stream) {
     if (a.batch * a.length == 0 || a.count == 0) {
         return hipSuccess;
-    }
-    a.half_magic = magic(static_cast<uint32_t>(a.half));
-    for (int w = 0; w < a.count; ++w) {
-        a.tensors[w].head_magic = magic(static_cast<uint32_t>(a.tensors[w].heads));
     }
     switch (dtype) {
         case LSSO_HIP_F16: launch_layout<LSSO_HIP_F16>(a, layout, stream); break;

@@ -79,31 +79,61 @@ struct Values<LSSO_HIP_F16> {
     }
 };
 
-// V (1, 2, 4 or 8) elements in one access (two of 8 FP32 elements).
+// V (1, 2, 4 or 8) elements in one access (two of 8 FP32 elements): as they are
+// loaded, so that what else there is to do need not wait for them, and through FP32.
 template <int T, int V>
-__device__ __forceinline__ void load_values(const typename Values<T>::Element* at, float (&v)[V]) {
-    if constexpr (V == 8) {
-        Values<T>::load8(at, v);
-    } else {
-        typename Values<T>::Element raw[V];
-        __builtin_memcpy(raw, at, sizeof(raw));
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            v[i] = Values<T>::load(raw + i);
+struct Raw {
+    static constexpr int kBytes = V * static_cast<int>(sizeof(typename Values<T>::Element));
+    static constexpr int kWords = (kBytes + 3) / 4;
+    uint32_t word[kWords];
+    __device__ __forceinline__ void load(const void* at) {
+        if constexpr (kBytes == 2) {
+            word[0] = *static_cast<const uint16_t*>(at);
+        } else {
+            __builtin_memcpy(word, at, kBytes);
         }
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            word[i] = 0;
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[V]) const {
+        if constexpr (T == LSSO_HIP_F32) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i] = __uint_as_float(word[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i] = i % 2 == 0 ? Values<T>::low(word[i / 2]) : Values<T>::high(word[i / 2]);
+            }
+        }
+    }
+};
+template <int T, int V>
+__device__ __forceinline__ void load_values(const typename Values<T>::Element* at, float (&v)[V]) {
+    Raw<T, V> raw;
+    raw.load(at);
+    raw.values(v);
 }
 template <int T, int V>
 __device__ __forceinline__ void store_values(typename Values<T>::Element* at, const float (&v)[V]) {
     if constexpr (V == 8) {
         Values<T>::store8(at, v);
+    } else if constexpr (V == 1) {
+        Values<T>::store(at, v[0]);
+    } else if constexpr (T == LSSO_HIP_F32) {
+        __builtin_memcpy(at, v, sizeof(v));
     } else {
-        typename Values<T>::Element raw[V];
+        uint32_t word[V / 2];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            Values<T>::store(raw + i, v[i]);
+        for (int i = 0; i < V / 2; ++i) {
+            word[i] = Values<T>::pack(v[2 * i], v[2 * i + 1]);
         }
-        __builtin_memcpy(at, raw, sizeof(raw));
+        __builtin_memcpy(at, word, sizeof(word));
     }
 }
 
