@@ -81,6 +81,40 @@ __device__ __forceinline__ u32x4 join(const u32x2& low, const u32x2& high) {
     return (u32x4){low[0], low[1], high[0], high[1]};
 }
 
+// Where the rows of a chunk are.  A walk goes on by one addition to a pointer: what
+// a chunk costs in scalar instructions, each wave pays.  Rows in the order of the
+// walk; `low` is the lowest address of a whole chunk.
+struct ChunkRows {
+    const char* low;
+    int64_t advance;      // bytes from chunk to chunk
+    int64_t stride;       // bytes from row to row
+    uint32_t step;        // its size
+    int records;          // bytes of a whole chunk
+
+    // data: of token 0; the chunk that begins with `token` first.
+    __device__ __forceinline__ ChunkRows(const void* data, int64_t token_stride, int bytes, int columns, int token)
+        : stride(token_stride * bytes) {
+        step = static_cast<uint32_t>(stride < 0 ? -stride : stride);
+        low = static_cast<const char*>(data) + (stride < 0 ? token + kChunk - 1 : token) * stride;
+        advance = kChunk * stride;
+        const int64_t all = static_cast<int64_t>(kChunk - 1) * step + bytes * columns;
+        records = all > 0x7fffffff ? 0x7fffffff : static_cast<int>(all);
+    }
+    __device__ __forceinline__ bool turned() const { return stride < 0; }
+    // The buffer of the first `rows` rows.  Rows past them are behind its end: in a
+    // turned chunk, whose last rows are its lowest, before its base, from where their
+    // offsets wrap round.
+    __device__ __forceinline__ BufferRsrc buffer(int rows) const {
+        const int missing = kChunk - rows;
+        return make_buffer(low - (turned() ? missing * stride : 0), records - static_cast<int>(missing * step));
+    }
+    // Offset of row 0's bytes `at` in that buffer.
+    __device__ __forceinline__ uint32_t offset(int row, int rows, uint32_t at) const {
+        return static_cast<uint32_t>(turned() ? rows - 1 - row : row) * step + at;
+    }
+    __device__ __forceinline__ uint32_t round(int count) const { return count * (turned() ? 0u - step : step); }
+};
+
 // A chunk of one tensor on its way to LDS: 64 rows of `features` 16-bit values,
 // in 16-byte pieces.  WHOLE: whole pieces, and 64 rows within a buffer's 2^31
 // bytes, so that a piece's address is the chunk's and a lane's own offset; rows
@@ -90,42 +124,32 @@ struct ChunkLoads {
     static constexpr int kPieces = WIDTH / 8;                       // of a row
     static constexpr int kEach = kChunk * kPieces / THREADS;        // of a thread
     static_assert(kChunk * kPieces % THREADS == 0, "whole rounds");
+    static_assert(THREADS % kPieces == 0, "a thread's pieces are of one column");
     u32x4 raw[kEach];
-    const uint16_t* data;
-    int64_t stride;
+    ChunkRows rows_at;
     int features;
-    uint32_t step;      // bytes between rows
-    uint32_t offset;    // of this thread's first piece in a whole chunk
 
     __device__ __forceinline__ static int row(int i) { return (static_cast<int>(threadIdx.x) + i * THREADS) / kPieces; }
     __device__ __forceinline__ static int column(int i) {
         return 8 * ((static_cast<int>(threadIdx.x) + i * THREADS) % kPieces);
     }
-    __device__ __forceinline__ ChunkLoads(const uint16_t* data_, int64_t stride_, int features_)
-        : data(data_), stride(stride_), features(features_) {
-        static_assert(THREADS % kPieces == 0, "a thread's pieces are of one column");
-        step = static_cast<uint32_t>(2 * (stride < 0 ? -stride : stride));
-        offset = static_cast<uint32_t>(stride < 0 ? kChunk - 1 - row(0) : row(0)) * step + 2 * column(0);
-    }
-    // The `rows` rows from `token` on.
-    __device__ __forceinline__ void issue(int64_t token, int rows) {
+    __device__ __forceinline__ ChunkLoads(const uint16_t* data, int64_t token_stride, int features_, int token)
+        : rows_at(data, token_stride, 2, features_, token), features(features_) {}
+    // The next chunk, of `rows` rows.
+    __device__ __forceinline__ void issue(int rows) {
         if constexpr (WHOLE) {
-            const bool turned = stride < 0;
-            const BufferRsrc buffer =
-                make_buffer(data + (turned ? token + rows - 1 : token) * stride,
-                            static_cast<int64_t>(rows - 1) * step + 2 * features);
-            // Past the last row offsets wrap round, and out of the buffer.
-            const uint32_t at = offset - (turned ? static_cast<uint32_t>(kChunk - rows) * step : 0u);
-            const uint32_t round = (turned ? 0u - step : step) * (THREADS / kPieces);
+            const BufferRsrc buffer = rows_at.buffer(rows);
+            const uint32_t at = rows_at.offset(row(0), rows, 2 * column(0));
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                raw[i] = buffer_load16(buffer, at + i * round);
+                raw[i] = buffer_load16(buffer, at + i * rows_at.round(THREADS / kPieces));
             }
         } else {
-            const uint16_t* from = data + token * stride;
+            const char* first = rows_at.low - (rows_at.turned() ? (kChunk - 1) * rows_at.stride : 0);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                const uint16_t* at = from + (row(i) < rows ? row(i) : rows - 1) * stride;
+                const uint16_t* at = reinterpret_cast<const uint16_t*>(
+                    first + (row(i) < rows ? row(i) : rows - 1) * rows_at.stride);
                 if (features >= 8) {
                     raw[i] = load16_unaligned(at + piece_start<8>(column(i), features));
                 } else {
@@ -133,6 +157,7 @@ struct ChunkLoads {
                 }
             }
         }
+        rows_at.low += rows_at.advance;
     }
     // With zeros past the features, and for rows that do not count.
     __device__ __forceinline__ u32x4 piece(int i, uint64_t kept) const {
@@ -236,32 +261,34 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + batch * a.mask_batch;
     const float rate = decay_rate(a.log_decay[head]);
 
-    const int64_t chunks = (a.length + kChunk - 1) / kChunk;
-    const uint32_t segment = STATES ? part / static_cast<uint32_t>(a.segment_pieces) : part;
-    const int64_t piece = STATES ? part - segment * static_cast<uint32_t>(a.segment_pieces) : 0;
-    const int64_t begin = segment * a.segment_chunks + piece * a.piece_chunks;
-    const int64_t behind = STATES && piece * a.piece_chunks + a.piece_chunks < a.segment_chunks
-                               ? begin + a.piece_chunks
-                               : (segment + 1) * a.segment_chunks;
-    const int64_t end = behind < chunks ? behind : chunks;
+    const int length = static_cast<int>(a.length);
+    const int chunks = (length + kChunk - 1) / kChunk;
+    const int segment_chunks = static_cast<int>(a.segment_chunks);
+    const int piece_chunks = static_cast<int>(a.piece_chunks);
+    const int segment = static_cast<int>(STATES ? part / static_cast<uint32_t>(a.segment_pieces) : part);
+    const int piece = STATES ? static_cast<int>(part) - segment * static_cast<int>(a.segment_pieces) : 0;
+    const int begin = segment * segment_chunks + piece * piece_chunks;
+    const int behind = STATES && (piece + 1) * piece_chunks < segment_chunks ? begin + piece_chunks
+                                                                             : (segment + 1) * segment_chunks;
+    const int end = behind < chunks ? behind : chunks;
 
-    ChunkLoads<kFeatures, kThreads, WHOLE> loads_a(from_a, a.a.token, a.features);
-    ChunkLoads<kFeatures, kThreads, WHOLE> loads_b(from_b, a.b.token, a.features);
-    ChunkLoads<kColumns, kThreads, WHOLE> loads_c(from_c + column0, a.c.token, a.out_features - column0);
+    ChunkLoads<kFeatures, kThreads, WHOLE> loads_a(from_a, a.a.token, a.features, begin * kChunk);
+    ChunkLoads<kFeatures, kThreads, WHOLE> loads_b(from_b, a.b.token, a.features, begin * kChunk);
+    ChunkLoads<kColumns, kThreads, WHOLE> loads_c(from_c + column0, a.c.token, a.out_features - column0,
+                                                  begin * kChunk);
     uint8_t kept_byte = 0;
-    const auto rows_of = [&](int64_t chunk) {
-        const int64_t left = a.length - chunk * kChunk;
-        return static_cast<int>(left < kChunk ? left : kChunk);
+    const auto rows_of = [&](int chunk) {
+        const int left = length - chunk * kChunk;
+        return left < kChunk ? left : kChunk;
     };
-    const auto issue = [&](int64_t chunk) {
-        const int64_t token = chunk * kChunk;
+    const auto issue = [&](int chunk) {
         const int rows = rows_of(chunk);
         if constexpr (!STATES) {
-            loads_a.issue(token, rows);
+            loads_a.issue(rows);
         }
-        loads_b.issue(token, rows);
-        loads_c.issue(token, rows);
-        kept_byte = lane >= rows ? 0 : (mask == nullptr ? 1 : mask[(token + lane) * a.mask_token]);
+        loads_b.issue(rows);
+        loads_c.issue(rows);
+        kept_byte = lane >= rows ? 0 : (mask == nullptr ? 1 : mask[(chunk * kChunk + lane) * a.mask_token]);
     };
     if (begin < end) {
         issue(begin);
@@ -321,10 +348,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
         }
     }
     const bool exact = a.features == kFeatures && column0 + kColumns <= a.out_features;
-    int64_t counted = 0;
+    int counted = 0;
 
-    const auto write = [&](int64_t chunk, uint64_t keep, f32x4 (&out)[kTiles][WE]) {
-        const int64_t token = chunk * kChunk;
+    const int out_bytes = a.wide_out != 0 ? 4 : 2;
+    ChunkRows rows_out(static_cast<const char*>(a.out.data) + out_bytes * (offset_of(a.out, batch, head) + column0),
+                       a.out.token, out_bytes, a.out_features - column0, begin * kChunk);
+    const auto write = [&](int chunk, uint64_t keep, f32x4 (&out)[kTiles][WE]) {
         const int rows = rows_of(chunk);
         if (keep != ~uint64_t{0}) {   // uniform
 #pragma unroll
@@ -337,25 +366,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
             }
         }
         if constexpr (WHOLE) {
-            const int bytes = a.wide_out != 0 ? 4 : 2;
-            const bool turned = a.out.token < 0;
-            const uint32_t row = static_cast<uint32_t>(bytes * (turned ? -a.out.token : a.out.token));
-            const char* data = static_cast<const char*>(a.out.data) +
-                               bytes * (offset_of(a.out, batch, head) + column0 +
-                                        (turned ? token + rows - 1 : token) * a.out.token);
-            const int columns = a.out_features - column0;
-            const BufferRsrc buffer = make_buffer(data, static_cast<int64_t>(rows - 1) * row + bytes * columns);
+            const BufferRsrc buffer = rows_out.buffer(rows);
             const int e = 16 * wave * WE + 4 * group;
-            // Rows past the last wrap round, and out of the buffer; so does what is past the features.
-            const uint32_t at = static_cast<uint32_t>(turned ? rows - 1 - in : in) * row + bytes * e;
-            const uint32_t round = 16 * (turned ? 0u - row : row);
+            const uint32_t at = rows_out.offset(in, rows, out_bytes * e);
 #pragma unroll
             for (int we = 0; we < WE; ++we) {
-                const bool some = e + 16 * we < columns;
+                const bool some = e + 16 * we < a.out_features - column0;
 #pragma unroll
                 for (int tile = 0; tile < kTiles; ++tile) {
                     const f32x4 v = out[tile][we];
-                    const uint32_t to = some ? at + tile * round + 16 * bytes * we : kOutOfRange;
+                    const uint32_t to = some ? at + tile * rows_out.round(16) + 16 * out_bytes * we : kOutOfRange;
                     if (a.wide_out != 0) {
                         buffer_store16(__builtin_bit_cast(u32x4, v), buffer, to);
                     } else {
@@ -363,13 +383,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
                     }
                 }
             }
+            rows_out.low += rows_out.advance;
         } else {
             const int own = opaque_int(lane);   // nothing of this path is held across the loop
             const int e0 = column0 + 16 * wave * WE + 4 * (own >> 4);
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
                 const int t = 16 * tile + (own & 15);
-                const int64_t at = offset_of(a.out, batch, head) + (token + t) * a.out.token + e0;
+                const int64_t at = offset_of(a.out, batch, head) + (chunk * kChunk + t) * a.out.token + e0;
 #pragma unroll
                 for (int we = 0; we < WE; ++we) {
 #pragma unroll
@@ -389,7 +410,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
         }
     };
 
-    for (int64_t chunk = begin; chunk < end; ++chunk) {
+    for (int chunk = begin; chunk < end; ++chunk) {
         const uint64_t kept = __ballot(kept_byte != 0);
         const int total = __popcll(kept);
         const int less = total > 0 ? pending : 0;
@@ -624,7 +645,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     if constexpr (STATES) {
         to = a.updates + (system * a.pieces + part) * size;
         if (head == 0 && column0 == 0 && tid == 0) {
-            a.counts[batch * a.pieces + part] = static_cast<int>(counted);
+            a.counts[batch * a.pieces + part] = counted;
         }
     } else if (a.last != nullptr && part == a.segments - 1) {
         to = a.last + system * size;
