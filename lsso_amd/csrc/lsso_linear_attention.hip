@@ -215,7 +215,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // STATES: the state alone that a piece of the sequence adds to.  Three waves of a
 // SIMD where the registers of a form allow it.
 template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE, bool STATES>
-__global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2) void walk_kernel(WalkArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (NW == 2 && KT == 4 ? 1 : 2)) void walk_kernel(WalkArgs a) {
     constexpr int kThreads = 64 * NW;
     constexpr int kFeatures = 32 * KT;
     constexpr int kColumns = 16 * NW * WE;
@@ -223,15 +223,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     constexpr int kColumnPitch = kColumns + 8;
     constexpr int kPart = kPairs * 64 * 8;       // values of one part of P
     __shared__ __attribute__((aligned(16))) uint16_t lds_a[STATES ? 8 : kChunk * kPitch];
-    __shared__ __attribute__((aligned(16))) uint16_t lds_b[kChunk * kPitch];
-    __shared__ __attribute__((aligned(16))) uint16_t lds_c[kChunk * kColumnPitch];
+    // The state alone leaves room for two chunks, and needs a barrier less for it.
+    constexpr int kBuffers = STATES ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) uint16_t lds_bs[kBuffers][kChunk * kPitch];
+    __shared__ __attribute__((aligned(16))) uint16_t lds_cs[kBuffers][kChunk * kColumnPitch];
     // P in operand order: [part][pair][lane][8 s].
     __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : 2 * kPart];
     // Of each token of the chunk: the kept ones up to it; l to the power of the kept
     // ones behind it, times scale_update; of those from it to the end of its 16; of
     // those up to it, times scale_across.
     __shared__ __attribute__((aligned(16))) float rank[kChunk];
-    __shared__ __attribute__((aligned(16))) float to_end[kChunk];
+    __shared__ __attribute__((aligned(16))) float to_ends[kBuffers][kChunk];
     __shared__ __attribute__((aligned(16))) float to_tile[kChunk];
     __shared__ __attribute__((aligned(16))) float from_start[kChunk];
 
@@ -411,6 +413,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
     };
 
     for (int chunk = begin; chunk < end; ++chunk) {
+        uint16_t* lds_b = lds_bs[STATES ? chunk & 1 : 0];
+        uint16_t* lds_c = lds_cs[STATES ? chunk & 1 : 0];
+        float* to_end = to_ends[STATES ? chunk & 1 : 0];
         const uint64_t kept = __ballot(kept_byte != 0);
         const int total = __popcll(kept);
         const int less = total > 0 ? pending : 0;
@@ -617,9 +622,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : 2
                 }
             }
         }
-        // P is whole, and nobody reads the chunk any more: the next one may be staged.
-        __syncthreads();
         if constexpr (!STATES) {
+            // P is whole, and nobody reads the chunk any more: the next one may be staged.
+            __syncthreads();
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -909,20 +914,20 @@ __global__ __launch_bounds__(kStepThreads) void attention_step_kernel(AttentionS
 void plan_walk(WalkArgs* a) {
     const int64_t chunks = (a->length + kChunk - 1) / kChunk;
     const int64_t systems = a->batch * a->heads;
-    // Segments until every compute unit has as many workgroups as it holds (three, of
-    // more than 64 features two), but none shorter than two chunks; pieces of them
-    // until there are four.
-    const int64_t held = a->features > 64 || a->out_features > 64 ? 512 : 768;
-    const auto parts = [&](int64_t wanted, int64_t whole, int64_t least) {   // of `whole` chunks
-        int64_t count = systems > 0 ? (wanted + systems - 1) / systems : 1;
-        const int64_t most = (whole + least - 1) / least;
-        count = count < most ? count : most;
-        return count > 1 ? count : int64_t{1};
+    // As many segments as the device holds at once (three workgroups to a compute unit,
+    // of more than 64 features two: a round more costs its whole time), but none
+    // shorter than two chunks; pieces of them until there are 1,024 workgroups.
+    const bool wide = a->features > 64 || a->out_features > 64;
+    const int64_t blocks = systems * (a->features > 64 && a->out_features > 64 ? 2 : 1);
+    const auto parts = [&](int64_t held, int64_t whole) {   // of `whole` chunks
+        const int64_t count = blocks > 0 ? held / blocks : 1;
+        const int64_t most = (whole + 1) / 2;
+        return count > most ? most : (count > 1 ? count : int64_t{1});
     };
-    const int64_t segments = parts(held, chunks, 2);
+    const int64_t segments = chunks > 0 ? parts(wide ? 512 : 768, chunks) : 1;
     a->segment_chunks = chunks > 0 ? (chunks + segments - 1) / segments : 1;
     a->segments = chunks > 0 ? (chunks + a->segment_chunks - 1) / a->segment_chunks : 1;
-    a->segment_pieces = a->segments > 1 ? parts(1024 / (a->segments - 1) / systems * systems, a->segment_chunks, 2) : 1;
+    a->segment_pieces = a->segments > 1 ? parts(1024 / (a->segments - 1), a->segment_chunks) : 1;
     a->piece_chunks = (a->segment_chunks + a->segment_pieces - 1) / a->segment_pieces;
     a->segment_pieces = (a->segment_chunks + a->piece_chunks - 1) / a->piece_chunks;
     a->pieces = (a->segments - 1) * a->segment_pieces;
