@@ -725,7 +725,7 @@ typedef struct lsso_hip_head_strides {
  * q: [batch, length, heads, features]; k: [batch, length, kv_heads, features];
  * v: [batch, length, kv_heads, value_features]; head h reads key and value head
  * h / (heads / kv_heads).  dtype: LSSO_HIP_F16 or LSSO_HIP_BF16.  Up to 128
- * features and value features. */
+ * features and value features, 4,096 heads and 2^22 sequences times heads. */
 typedef struct lsso_hip_linear_attention_shape {
     int64_t batch;
     int64_t length;

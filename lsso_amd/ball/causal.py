@@ -548,8 +548,9 @@ def linear_attention(
 
     S is FP32; products take 16-bit operands, each FP32 one in two parts, and
     accumulate in FP32: y and the gradients are off by one rounding of their type.
-    In float16 scale * (q . k) must stay below 65,504.  Differentiable (first order)
-    in query, key, value and initial_state, deterministically; log_decay is fixed."""
+    In float16 scale * (q . k), and scale * (grad_y . v) of the gradients, must stay
+    below 65,504.  Differentiable (first order) in query, key, value and
+    initial_state, deterministically; log_decay is fixed."""
 
     _hip().require_available()
     _without_tangents(query, key, value, log_decay, initial_state)

@@ -27,7 +27,7 @@ constexpr int64_t kMostRotary = 4096;
 constexpr int64_t kMostChannels = 1 << 20;
 constexpr int64_t kMostSamples = 1 << 30;
 constexpr int64_t kMostLength = 1 << 30;
-constexpr int64_t kMostBlocks = 1 << 23;            // a launch takes fewer than 2^32 threads
+constexpr int64_t kMostBlocks = 1 << 22;            // two workgroups of 256 threads to each: fewer than 2^32 threads
 
 bool strides_fit(int64_t batch, int64_t token, int64_t head) {
     return batch >= 0 && token >= 0 && head >= 0 && batch <= kMostTokens && token <= kMostTokens && head <= kMostTokens;
@@ -114,7 +114,7 @@ int check_linear_attention(const lsso_hip_linear_attention_shape* s) {
     if (s->heads > kMostHeads || s->length > kMostLength || s->batch > kMostBlocks ||
         s->batch * s->heads > kMostBlocks) {
         return report(LSSO_HIP_EUNSUPPORTED,
-                      "linear attention takes up to 2^30 tokens, 4,096 heads and 2^23 sequences times heads");
+                      "linear attention takes up to 2^30 tokens, 4,096 heads and 2^22 sequences times heads");
     }
     if (s->dtype != LSSO_HIP_F16 && s->dtype != LSSO_HIP_BF16) {
         return report(LSSO_HIP_EUNSUPPORTED, "linear attention takes float16 or bfloat16");
@@ -430,9 +430,8 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
                                        const lsso_hip_head_strides* grad_strides, const float* grad_final_state,
                                        const void* q, const void* k, const void* v, const float* log_decay,
                                        const uint8_t* row_mask, const float* initial_state, const float* kept,
-                                       void* grad_q, void* grad_k,
-                                       void* grad_v, float* grad_initial_state, void* workspace,
-                                       size_t workspace_bytes, void* stream) {
+                                       void* grad_q, void* grad_k, void* grad_v, float* grad_initial_state,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
     const int status = check_linear_attention(shape);
     if (status != LSSO_HIP_OK) {
         return status;
@@ -449,7 +448,8 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         return report(LSSO_HIP_EINVAL, "q, k, v and grad_y must not be NULL and be aligned to their type");
     }
     if (log_decay == nullptr || !aligned(log_decay, 4) || !aligned(initial_state, 4) || !aligned(grad_final_state, 4) ||
-        !aligned(grad_initial_state, 4) || !aligned(kept, 4) || !aligned(grad_q, 2) || !aligned(grad_k, 2) || !aligned(grad_v, 2)) {
+        !aligned(grad_initial_state, 4) || !aligned(kept, 4) || !aligned(grad_q, 2) || !aligned(grad_k, 2) ||
+        !aligned(grad_v, 2)) {
         return report(LSSO_HIP_EINVAL, "log_decay must not be NULL, it, the states and the gradients be aligned");
     }
     const AttentionLayout l = attention_layout(s, true);

@@ -145,7 +145,7 @@ def test_refusals_on_the_cpu() -> None:
     assert forward_size.value >= 4 * kept.value and backward_size.value >= 4 * kept.value
     for wrong in ({"batch": -1}, {"length": -1}, {"heads": 0}, {"kv_heads": 3}, {"features": 0}, {"features": 129},
                   {"value_features": 129}, {"dtype": 3}, {"scale": math.inf}, {"scale": math.nan}, {"stride": 1},
-                  {"batch": 2**22}, {"heads": 8192, "kv_heads": 1}, {"length": 2**31}):
+                  {"batch": 2**22}, {"batch": 2**23, "heads": 1, "kv_heads": 1}, {"heads": 8192, "kv_heads": 1}, {"length": 2**31}):
         assert sizes(**wrong) < 0, wrong
         assert forward(**wrong) < 0 and step(**{**wrong, "length": wrong.get("length", 1)}) < 0, wrong
         assert library.lsso_hip_last_error()
