@@ -523,7 +523,7 @@ struct GroupNormArgs {
     int64_t blocks;             // of the team kernel's grid
 };
 
-// The plan and the bytes of partials, sums and (`keep` false) statistics.
+// Sets the plan; partial_bytes: of `partials`.
 void plan_group_norm(GroupNormArgs* a, bool backward, size_t* partial_bytes);
 hipError_t launch_group_norm(const GroupNormArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_group_norm_backward(const GroupNormArgs& a, int dtype, hipStream_t stream);
