@@ -490,18 +490,17 @@ __global__ __launch_bounds__(kThreads) void norm_statistics_kernel(GroupNormArgs
         for (int j = threadIdx.x; j < c.wide * V; j += kThreads) {
             const int thread = j / V;
             const int i = j - thread * V;
-            float n = 0.0f;
-            float m = 0.0f;
+            // Two sums that wait for nobody: a merge of two at a time is a chain of divisions.
+            const float pivot = shared[thread][i];
+            float apart = 0.0f;
+            for (int r = 0; r < c.at_once; ++r) {
+                apart += rows[r * c.wide] * (shared[thread + r * c.wide][i] - pivot);
+            }
+            const float m = kept_rows > 0.0f ? pivot + apart / kept_rows : 0.0f;
             float s = 0.0f;
             for (int r = 0; r < c.at_once; ++r) {
-                const float some = rows[thread + r * c.wide];
-                if (some > 0.0f) {
-                    const float weight = some / (n + some);
-                    const float apart = shared[thread + r * c.wide][i] - m;
-                    s += shared[thread + r * c.wide][V + i] + apart * apart * (n * weight);
-                    m += apart * weight;
-                    n += some;
-                }
+                const float off = shared[thread + r * c.wide][i] - m;
+                s += shared[thread + r * c.wide][V + i] + rows[r * c.wide] * off * off;
             }
             if (layout.by_group) {
                 shared[thread][i] = m;
