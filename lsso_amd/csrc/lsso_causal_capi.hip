@@ -146,15 +146,21 @@ lsso_hip::WalkTensor turned(lsso_hip::WalkTensor t, int64_t length, int64_t byte
     return t;
 }
 
+// The forward's shape and the plan of every walk of it, made here alone: a workspace
+// laid out for one plan must not be written under another.  (The backward's walks
+// exchange features and value features; their states have as many values.)
 lsso_hip::WalkArgs walk_args(const lsso_hip_linear_attention_shape& s, const float* log_decay, const uint8_t* mask) {
     lsso_hip::WalkArgs w{};
     w.batch = s.batch;
     w.length = s.length;
     w.heads = static_cast<int>(s.heads);
+    w.features = static_cast<int>(s.features);
+    w.out_features = static_cast<int>(s.value_features);
     w.log_decay = log_decay;
     w.mask = mask;
     w.mask_batch = s.length;
     w.mask_token = 1;
+    lsso_hip::plan_walk(&w);
     return w;
 }
 
@@ -170,8 +176,7 @@ struct AttentionLayout {
 // keeps for its backward instead).
 AttentionLayout attention_layout(const lsso_hip_linear_attention_shape& s, bool backward) {
     AttentionLayout l;
-    lsso_hip::WalkArgs w = walk_args(s, nullptr, nullptr);
-    lsso_hip::plan_walk(&w);
+    const lsso_hip::WalkArgs w = walk_args(s, nullptr, nullptr);
     if (w.segments > 1) {
         const size_t state = static_cast<size_t>(s.batch * s.heads) * static_cast<size_t>(s.features * s.value_features);
         l.counts = round256(sizeof(float) * state * static_cast<size_t>(w.pieces));
@@ -406,8 +411,6 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
     w.b = tensor(k, s.k, s.heads / s.kv_heads);
     w.c = tensor(v, s.v, s.heads / s.kv_heads);
     w.out = tensor(y, dense(s.length, s.heads, s.value_features), 1);
-    w.features = static_cast<int>(s.features);
-    w.out_features = static_cast<int>(s.value_features);
     w.scale_within = s.scale;
     w.scale_across = s.scale;
     w.scale_update = 1.0f;
@@ -421,7 +424,6 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
     w.states = kept != nullptr ? kept : reinterpret_cast<float*>(ws + l.states);
     w.states_row = s.value_features;
     w.states_column = 1;
-    lsso_hip::plan_walk(&w);
     const hipError_t error = lsso_hip::launch_walk(w, s.dtype, static_cast<hipStream_t>(stream));
     return error == hipSuccess ? LSSO_HIP_OK : report_hip(error, "linear attention launch");
 }
@@ -478,7 +480,6 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         w.states = reinterpret_cast<float*>(ws + l.states);
         w.states_row = out_features;
         w.states_column = 1;
-        lsso_hip::plan_walk(&w);
         return w;
     };
     hipError_t error = hipSuccess;
