@@ -77,6 +77,15 @@ __device__ __forceinline__ int64_t xcd_local_block(int64_t physical, int64_t blo
     return (physical % 8) * per_xcd + physical / 8;
 }
 
+// n / d of numbers that are not negative, in 32 bits where both fit (a division of 64
+// takes long).
+__host__ __device__ constexpr int64_t quotient(int64_t n, int64_t d) {
+    return ((n | d) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
+}
+static_assert(quotient(3, (int64_t{1} << 32) + 3) == 0 && quotient(5, int64_t{1} << 32) == 0, "a long divisor");
+static_assert(quotient((int64_t{1} << 40) + 9, 4) == (int64_t{1} << 38) + 2, "a long dividend");
+static_assert(quotient(0xffffffff, 0xffffffff) == 1 && quotient(7, 2) == 3, "both of 32 bits");
+
 // Raw buffer access.  An access past a buffer's num_records bytes does not
 // touch memory: loads return zero and stores are dropped.  Tile loops use
 // this instead of branches around their edge accesses, so every memory

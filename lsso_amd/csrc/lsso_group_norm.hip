@@ -356,11 +356,6 @@ struct Columns {
     }
 };
 
-// n / d of not negative numbers, in 32 bits where they fit (a division of 64 takes long).
-__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
-    return n <= 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
-}
-
 // A split's partials: the rows that count, two values of each group (by_group: a
 // workgroup has all channels) or of each channel, and in the backward two of each
 // channel in front of them.

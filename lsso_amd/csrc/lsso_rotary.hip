@@ -41,11 +41,6 @@ __device__ double position_at(const RotaryArgs& a, int64_t batch, int64_t token)
     }
 }
 
-// n / d of not negative numbers, in 32 bits where they fit (a division of 64 takes long).
-__device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
-    return n <= 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
-}
-
 // T: type; HALF: the partner of feature j is feature j + half, else pairs are
 // neighbours; V: features of an access, which divides what is turned (half of the
 // rotated part, or all of it).
@@ -59,9 +54,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     const int64_t items = a.batch * a.length * units;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; item < items; item += step) {
-        const int64_t row = divide(item, units);
+        const int64_t row = quotient(item, units);
         const int unit = static_cast<int>(item - row * units);
-        const int64_t batch = divide(row, a.length);
+        const int64_t batch = quotient(row, a.length);
         const int64_t token = row - batch * a.length;
         const bool turns = unit < turned;
         const int feature = unit * V + (HALF && !turns ? half : 0);
