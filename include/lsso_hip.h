@@ -753,8 +753,9 @@ int lsso_hip_linear_attention_sizes(const lsso_hip_linear_attention_shape* shape
  * NULL (zeros).  kept: lsso_hip_linear_attention_sizes' kept_floats, for the backward,
  * or NULL.  y: contiguous [batch, length, heads, value_features] of dtype.
  * final_state: as initial_state, S after the last token, or NULL.
- * S is FP32; products take 16-bit operands and accumulate in FP32, with P, S and
- * the decayed v in two 16-bit parts each.  workspace: 256-byte aligned. */
+ * S is FP32; products take 16-bit operands and accumulate in FP32, with P, S and the
+ * decayed v in three parts of BF16 (24 bits) or two of FP16 (22).  workspace:
+ * 256-byte aligned. */
 int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, const void* q,
                               const void* k, const void* v, const float* log_decay,
                               const uint8_t* row_mask, const float* initial_state, float* kept,

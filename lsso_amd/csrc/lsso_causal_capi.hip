@@ -418,7 +418,6 @@ int lsso_hip_linear_attention(const lsso_hip_linear_attention_shape* shape, cons
     w.first_row = s.value_features;
     w.first_column = 1;
     w.last = final_state;
-    w.fine = final_state != nullptr ? 1 : 0;
     w.updates = reinterpret_cast<float*>(ws);
     w.counts = reinterpret_cast<int*>(ws + l.counts);
     w.states = kept != nullptr ? kept : reinterpret_cast<float*>(ws + l.states);
@@ -521,7 +520,6 @@ int lsso_hip_linear_attention_backward(const lsso_hip_linear_attention_shape* sh
         w.first_row = transposed ? 1 : out_features;
         w.first_column = transposed ? features : 1;
         w.last = first_state;
-        w.fine = first_state != nullptr ? 1 : 0;
         if (walked) {
             w.reuse = 1;
             w.states_row = 1;

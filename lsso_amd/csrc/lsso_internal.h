@@ -563,7 +563,6 @@ struct WalkArgs {
     int64_t first_row;
     int64_t first_column;
     float* last;                // the state after the last token, contiguous, or nullptr
-    int fine;                   // the last state is asked for: BF16 updates in three parts
     float* updates;             // [batch, heads, pieces, features, out_features]: what each piece adds to the state
     int* counts;                // [batch, pieces] tokens that count
     float* states;              // [batch, heads, segments, features, out_features]: before each segment's first token

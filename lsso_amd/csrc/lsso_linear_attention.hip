@@ -27,13 +27,14 @@
 // starts with the third.
 //
 // What is rounded: the MFMAs take 16-bit operands, and P, S and l^(n-s) c are
-// FP32 values.  P and S go in as two 16-bit parts, the second what rounding left
-// of the first, so that outputs are off by one rounding of their own; one part
-// would leave sqrt(2) to sqrt(3).  l^(n-s) c, which makes the FP32 state, goes in
-// as two parts of FP16, and of BF16 as three if the state is returned (two leave it
-// 2.4e-6 off).  FP16: S is scaled by a power of two that brings its largest value in
-// a wave to 2^14 before it is split (the state of many tokens passes 65,504); P must
-// stay below 65,504.
+// FP32 values.  Each goes in as parts, every next one what is left of those before
+// it: three of BF16, which hold it whole, or two of FP16 (22 bits), so that S is an
+// FP32 state and outputs are rounded once.  (Two rounded parts of BF16 left S 2.4e-6
+// off, and of y and the gradients enough last bits for 1.1e-4 of their norm.  They
+// took 74 us a walk at 64 x 2,048 tokens of 4 heads of 64, three truncated ones 84,
+// three rounded ones 86.)  FP16: S is scaled
+// by a power of two that brings its largest value in a wave to 2^14 before it is
+// split (the state of many tokens passes 65,504); P must stay below 65,504.
 //
 // Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
 // 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
@@ -67,21 +68,39 @@ __device__ __forceinline__ float decay_rate(float log_decay) {
     return rate < -1.0e30f ? -1.0e30f : rate;
 }
 
-// Four FP32 values as PARTS 16-bit ones each: rounded, then what that left.  Of
-// a value that rounds to infinity the second part is held finite: the opposite
-// infinity or a NaN would make a NaN of the product.
-template <int T, int PARTS>
-__device__ __forceinline__ void split(f32x4 v, u32x2 (&part)[PARTS]) {
-    constexpr float kMost = T == LSSO_HIP_F16 ? 64.0f : 1.0e38f;   // past any rounding error
+// Parts that an FP32 value goes into the matrix instructions in.
+template <int T>
+constexpr int kParts = T == LSSO_HIP_BF16 ? 3 : 2;
+
+// Four FP32 values as 16-bit parts each.  BF16: upper bits, three times, which hold
+// all 24 (rounded parts take a third more instructions); FP16: rounded, then what that
+// left.  Of a value that is or rounds to infinity the second part is held finite: the
+// opposite infinity or a NaN would make a NaN of the product.
+template <int T>
+__device__ __forceinline__ void split(f32x4 v, u32x2 (&part)[kParts<T>]) {
+    constexpr float kMost = T == LSSO_HIP_F16 ? 64.0f : 1.0e38f;   // past any remainder
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-        part[p] = (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])};
-        if (p + 1 < PARTS) {
-            const f32x4 rounded = {Values<T>::low(part[p][0]), Values<T>::high(part[p][0]),
-                                   Values<T>::low(part[p][1]), Values<T>::high(part[p][1])};
+    for (int p = 0; p < kParts<T>; ++p) {
+        f32x4 taken;
+        if constexpr (T == LSSO_HIP_BF16) {
+            uint32_t bits[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[i] = __builtin_amdgcn_fmed3f(v[i] - rounded[i], -kMost, kMost);
+                bits[i] = __float_as_uint(v[i]);
+                taken[i] = __uint_as_float(bits[i] & 0xffff0000u);
+            }
+            part[p] = (u32x2){__builtin_amdgcn_perm(bits[1], bits[0], 0x07060302u),
+                              __builtin_amdgcn_perm(bits[3], bits[2], 0x07060302u)};
+        } else {
+            part[p] = (u32x2){Values<T>::pack(v[0], v[1]), Values<T>::pack(v[2], v[3])};
+            taken = (f32x4){Values<T>::low(part[p][0]), Values<T>::high(part[p][0]), Values<T>::low(part[p][1]),
+                            Values<T>::high(part[p][1])};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] -= taken[i];
+            if (p == 0) {
+                v[i] = __builtin_amdgcn_fmed3f(v[i], -kMost, kMost);
             }
         }
     }
@@ -221,16 +240,17 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 }
 
 // T: type; KT: 32-feature steps of a and b; NW: waves; WE: 16-column blocks of c
-// and S in a wave; WHOLE: rows are whole 16-byte pieces; PARTS: of the decayed c;
-// STATES: the state alone that a piece of the sequence adds to.  Three waves of a
-// SIMD where the registers of a form allow it.
-template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE, bool STATES>
+// and S in a wave; WHOLE: rows are whole 16-byte pieces; STATES: the state alone
+// that a piece of the sequence adds to.  Three waves of a SIMD where the registers
+// of a form allow it.
+template <int T, int KT, int NW, int WE, bool WHOLE, bool STATES>
 __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (NW == 2 && KT == 4 ? 1 : 2)) void walk_kernel(WalkArgs a) {
     constexpr int kThreads = 64 * NW;
     constexpr int kFeatures = 32 * KT;
     constexpr int kColumns = 16 * NW * WE;
     constexpr int kPitch = kFeatures + 8;        // rows 16 bytes apart modulo the banks
     constexpr int kColumnPitch = kColumns + 8;
+    constexpr int PARTS = kParts<T>;
     constexpr int kPart = kPairs * 64 * 8;       // values of one part of P
     __shared__ __attribute__((aligned(16))) uint16_t lds_a[STATES ? 8 : kChunk * kPitch];
     // The state alone leaves room for two chunks, and needs a barrier less for it.
@@ -238,7 +258,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
     __shared__ __attribute__((aligned(16))) uint16_t lds_bs[kBuffers][kChunk * kPitch];
     __shared__ __attribute__((aligned(16))) uint16_t lds_cs[kBuffers][kChunk * kColumnPitch];
     // P in operand order: [part][pair][lane][8 s].
-    __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : 2 * kPart];
+    __shared__ __attribute__((aligned(16))) uint16_t lds_p[STATES ? 8 : PARTS * kPart];
     // Of each token of the chunk: the kept ones up to it; l to the power of the kept
     // ones behind it, times scale_update; of those from it to the end of its 16; of
     // those up to it, times scale_across.
@@ -372,8 +392,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
         for (int i = 0; i < kTiles; i += 2) {
             if (wave == i % NW) {
                 uint16_t* to = lds_p + (pair_of(i, i) * 64 + lane) * 8 + 4;
-                *reinterpret_cast<u32x2*>(to) = (u32x2){0u, 0u};
-                *reinterpret_cast<u32x2*>(to + kPart) = (u32x2){0u, 0u};
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    *reinterpret_cast<u32x2*>(to + p * kPart) = (u32x2){0u, 0u};
+                }
             }
         }
     }
@@ -512,11 +534,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                 return score;
             };
             const auto put = [&](int tile, int s, const f32x4& score) {
-                u32x2 halves[2];
-                split<T>(score, halves);
+                u32x2 parts_of[PARTS];
+                split<T>(score, parts_of);
                 uint16_t* to = lds_p + (pair_of(tile, s) * 64 + lane) * 8 + 4 * (s & 1);
-                *reinterpret_cast<u32x2*>(to) = halves[0];
-                *reinterpret_cast<u32x2*>(to + kPart) = halves[1];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    *reinterpret_cast<u32x2*>(to + p * kPart) = parts_of[p];
+                }
             };
             constexpr int kBelow = kTiles * (kTiles - 1) / 2;
 #pragma unroll
@@ -574,16 +598,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
             }
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
-                u32x4 high[WE];
-                u32x4 low[WE];
+                u32x4 from_state[WE][PARTS];
 #pragma unroll
                 for (int we = 0; we < WE; ++we) {
-                    u32x2 upper[2];
-                    u32x2 lower[2];
+                    u32x2 upper[PARTS];
+                    u32x2 lower[PARTS];
                     split<T>(state[2 * k][we] * factor, upper);
                     split<T>(state[2 * k + 1][we] * factor, lower);
-                    high[we] = join(upper[0], lower[0]);
-                    low[we] = join(upper[1], lower[1]);
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        from_state[we][p] = join(upper[p], lower[p]);
+                    }
                 }
 #pragma unroll
                 for (int tile = 0; tile < kTiles; ++tile) {
@@ -591,8 +616,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                         *reinterpret_cast<const u32x4*>(lds_a + (16 * tile + in) * kPitch + 32 * k + 8 * group);
 #pragma unroll
                     for (int we = 0; we < WE; ++we) {
-                        out[tile][we] = mfma_small<T>(high[we], query, out[tile][we]);
-                        out[tile][we] = mfma_small<T>(low[we], query, out[tile][we]);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            out[tile][we] = mfma_small<T>(from_state[we][p], query, out[tile][we]);
+                        }
                     }
                 }
             }
@@ -658,12 +685,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
 #pragma unroll
                 for (int tile = 2 * j; tile < kTiles; ++tile) {
                     const uint16_t* from = lds_p + (pair_of(tile, 2 * j) * 64 + lane) * 8;
-                    const u32x4 high = *reinterpret_cast<const u32x4*>(from);
-                    const u32x4 low = *reinterpret_cast<const u32x4*>(from + kPart);
 #pragma unroll
-                    for (int we = 0; we < WE; ++we) {
-                        out[tile][we] = mfma_small<T>(value[j][we], high, out[tile][we]);
-                        out[tile][we] = mfma_small<T>(value[j][we], low, out[tile][we]);
+                    for (int p = 0; p < PARTS; ++p) {
+                        const u32x4 score = *reinterpret_cast<const u32x4*>(from + p * kPart);
+#pragma unroll
+                        for (int we = 0; we < WE; ++we) {
+                            out[tile][we] = mfma_small<T>(value[j][we], score, out[tile][we]);
+                        }
                     }
                 }
             }
@@ -772,13 +800,13 @@ __global__ __launch_bounds__(kCarryThreads) void carry_kernel(WalkArgs a) {
     store();   // of the last segment
 }
 
-template <int T, int KT, int NW, int WE, int PARTS, bool WHOLE>
-void launch_parts(const WalkArgs& a, hipStream_t stream) {
+template <int T, int KT, int NW, int WE, bool WHOLE>
+void launch_form(const WalkArgs& a, hipStream_t stream) {
     constexpr int kColumns = 16 * NW * WE;
     const int64_t across = (a.out_features + kColumns - 1) / kColumns;
     const int64_t systems = a.batch * a.heads;
     if (a.segments > 1 && a.reuse == 0) {
-        walk_kernel<T, KT, NW, WE, PARTS, WHOLE, true>
+        walk_kernel<T, KT, NW, WE, WHOLE, true>
             <<<static_cast<unsigned>(systems * a.pieces * across), 64 * NW, 0, stream>>>(a);
         // Four elements to a thread where that leaves a workgroup to each compute unit.
         const int64_t elements = a.features * a.out_features;
@@ -792,19 +820,8 @@ void launch_parts(const WalkArgs& a, hipStream_t stream) {
             carry_kernel<4, 4><<<static_cast<unsigned>(systems * blocks), kCarryThreads, 0, stream>>>(a);
         }
     }
-    walk_kernel<T, KT, NW, WE, PARTS, WHOLE, false>
+    walk_kernel<T, KT, NW, WE, WHOLE, false>
         <<<static_cast<unsigned>(systems * a.segments * across), 64 * NW, 0, stream>>>(a);
-}
-
-template <int T, int KT, int NW, int WE, bool WHOLE>
-void launch_form(const WalkArgs& a, hipStream_t stream) {
-    // FP16 states are right to 2^-22 with two parts; of BF16 only one that is given
-    // back shows what two leave.
-    if (T == LSSO_HIP_BF16 && a.fine != 0) {
-        launch_parts<T, KT, NW, WE, T == LSSO_HIP_BF16 ? 3 : 2, WHOLE>(a, stream);
-    } else {
-        launch_parts<T, KT, NW, WE, 2, WHOLE>(a, stream);
-    }
 }
 
 template <int T, int KT, bool WHOLE>

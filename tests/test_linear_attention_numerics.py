@@ -1,0 +1,57 @@
+"""What the factors of linear attention's products are held to: outputs of BF16 as
+those of FP32 factors, small and large values of FP16, and values that are not finite."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from lsso_amd.ball import reference as canonical
+from test_linear_attention import _inputs
+
+
+def _exact(inputs, log_decay, scale, dy, ds):
+    """(y, S, dq, dk, dv, dS_0) of the reference path in FP64 (itself tested against
+    the definition)."""
+
+    ends = [x.detach().double().requires_grad_() for x in inputs]
+    ys = canonical.linear_attention(*ends[:3], log_decay.double(), scale=scale, initial_state=ends[3], return_state=True)
+    return [x.detach() for x in (*ys, *torch.autograd.grad(ys, ends, (dy.double(), ds.double())))]
+
+
+def _native(native, inputs, log_decay, scale, dy, ds):
+    leaves = [x.detach().requires_grad_() for x in inputs]
+    ys = native.linear_attention(*leaves[:3], log_decay, scale=scale, initial_state=leaves[3], return_state=True)
+    return [x.detach() for x in (*ys, *torch.autograd.grad(ys, leaves, (dy, ds)))]
+
+
+def _tensors(size, dtype, seed=0):
+    q, k, v, log_decay, generator = _inputs(*size, dtype, seed)
+    state, ds = (torch.randn(size[0], size[2], size[4], size[5], generator=generator) for _ in range(2))
+    dy = torch.randn(size[0], size[1], size[2], size[5], generator=generator).to(dtype)
+    return [x.cuda() for x in (q, k, v, state)], log_decay.cuda(), dy.cuda(), ds.cuda()
+
+
+def _apart(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(2, 700, 4, 2, 64, 64), (1, 300, 2, 2, 128, 96), (3, 64, 2, 2, 32, 16)])
+def test_bfloat16_outputs_are_those_of_fp32_factors(native, size) -> None:
+    """FP32 sums of about 200 terms are off by sqrt(200) 2^-24 = 8e-7 of the result's
+    size.  That moves one in 6,000 values over a rounding border (8e-7 of steps of
+    2^-8 to 2^-7), by such a step: sqrt(1.6e-4) 5.5e-3 = 7e-5 of the norm.  States and
+    their gradients, which are FP32, are off by a few roundings in a row: 2^-21."""
+
+    inputs, log_decay, dy, ds = _tensors(size, torch.bfloat16)
+    scale = size[4] ** -0.5
+    for i, (a, e) in enumerate(zip(_native(native, inputs, log_decay, scale, dy, ds),
+                                   _exact(inputs, log_decay, scale, dy, ds))):
+        bound = 2.0**-21 if i in (1, 5) else 8e-5
+        assert _apart(a, e.to(a.dtype)) <= bound, i
+    # What is returned beside it changes no value.
+    assert torch.equal(native.linear_attention(*inputs[:3], log_decay),
+                       native.linear_attention(*inputs[:3], log_decay, return_state=True)[0])

@@ -105,3 +105,33 @@ def test_wide_segments(native, dtype, size, kind) -> None:
     small = 8.0 + scale * size[4]
     for a, e, m in zip(found, values, sizes):
         assert ((a.detach().double() - e.detach()).abs() <= _bound(e.detach(), m.detach(), dtype, small)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+def test_wide_segments_alone(native, dtype) -> None:
+    """Without gradients, and each gradient by itself: as in one call of all.  dk by
+    itself makes states of its own, where it reads those of dv, transposed: then both
+    are within their bound of the same value."""
+
+    size = (3, 900, 6, 6, 96, 80)
+    inputs, log_decay, mask, dy, _ = _leaves(size, dtype, "suffix", 8)
+    leaves = [x.clone().requires_grad_() for x in inputs]
+
+    def run(q, k, v, state):
+        return native.linear_attention(q, k, v, log_decay, row_mask=mask, initial_state=state, return_state=True)
+
+    y, last = run(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    alone, state = run(*inputs)
+    assert torch.equal(alone, y) and torch.equal(state, last)
+    sizes = [x.abs().requires_grad_() for x in inputs]
+    (most,) = torch.autograd.grad(run(*sizes)[0], sizes[1], dy.abs())
+    for i in range(4):
+        one = [x.clone().requires_grad_(j == i) for j, x in enumerate(inputs)]
+        (grad,) = torch.autograd.grad(run(*one)[0], one[i], dy)
+        if i != 1:
+            assert torch.equal(grad, grads[i])
+        else:
+            bound = 2 * _bound(grads[1].double(), most.double(), dtype, 8.0 + 96**0.5)
+            assert ((grad.double() - grads[1].double()).abs() <= bound).all()
