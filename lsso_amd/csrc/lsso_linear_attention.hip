@@ -32,9 +32,10 @@
 // FP32 state and outputs are rounded once.  (Two rounded parts of BF16 left S 2.4e-6
 // off, and of y and the gradients enough last bits for 1.1e-4 of their norm.  They
 // took 74 us a walk at 64 x 2,048 tokens of 4 heads of 64, three truncated ones 84,
-// three rounded ones 86.)  FP16: S is scaled
-// by a power of two that brings its largest value in a wave to 2^14 before it is
-// split (the state of many tokens passes 65,504); P must stay below 65,504.
+// three rounded ones 86.)  FP16:
+// powers of two bring the decayed c of each column (of a small gradient, its terms
+// are far below FP16's normal range) and S of each wave (of many tokens, it passes
+// 65,504) to 2^13 and more before they are split; P must stay below 65,504.
 //
 // Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
 // 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
@@ -200,6 +201,30 @@ struct ChunkLoads {
         return in ? v : (u32x4){0u, 0u, 0u, 0u};
     }
 };
+
+// The power of two that brings the largest of some values to 2^13 .. 2^14, where FP16
+// parts hold their 22 bits, and the way back; none of next to nothing, of an infinity
+// or a NaN.
+struct Power {
+    float to = 1.0f;
+    float back = 1.0f;
+    __device__ __forceinline__ explicit Power(float most) {
+        const int exponent = static_cast<int>((__float_as_uint(most) & 0x7fffffffu) >> 23) - 127;
+        if (exponent > -100 && exponent < 128) {
+            to = __uint_as_float(static_cast<uint32_t>(127 + 13 - exponent) << 23);
+            back = __uint_as_float(static_cast<uint32_t>(127 - 13 + exponent) << 23);
+        }
+    }
+};
+
+// The largest of lanes i, i + 16, i + 32 and i + 48, in all of them.
+__device__ __forceinline__ float column_max(float v) {
+    const uint32_t bits = __float_as_uint(v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    const uint32_t some = __float_as_uint(fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1])));
+    const auto halves = __builtin_amdgcn_permlane32_swap(some, some, false, false);
+    return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
 
 // 8 values of k (or s) for one lane: rows at `at` and 16 rows on, read
 // transposed; lane i of 16 receives column i.
@@ -642,38 +667,69 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
         }
         pending -= less;
         counted += total;
+        // l^(n-s) c of the lane's column e, in parts: 32 tokens at a time, or in FP16 all
+        // 64, brought to their range by a power of two of each column, which the sum is
+        // freed of before it meets S.
+        constexpr int kSpan = T == LSSO_HIP_F16 ? 2 : 1;   // of 32 tokens
         u32x4 value[2][WE];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {   // 32 tokens s
-            const uint16_t* transposed =
-                lds_c + (32 * j + 4 * group + (in >> 2)) * kColumnPitch + 16 * wave * WE + 4 * (in & 3);
-            const f32x4 weight0 = *reinterpret_cast<const f32x4*>(to_end + 32 * j + 4 * group);
-            const f32x4 weight1 = *reinterpret_cast<const f32x4*>(to_end + 32 * j + 16 + 4 * group);
-            u32x4 decayed[WE][PARTS];
+        for (int j0 = 0; j0 < 2; j0 += kSpan) {
+            u32x4 decayed[kSpan][WE][PARTS];
+            float back[WE];
 #pragma unroll
             for (int we = 0; we < WE; ++we) {
-                value[j][we] = read_columns(transposed + 16 * we, kColumnPitch);
-                float v[8];
-                Values<T>::unpack8(value[j][we], v);
-                u32x2 upper[PARTS];
-                u32x2 lower[PARTS];
-                split<T>((f32x4){v[0], v[1], v[2], v[3]} * weight0, upper);
-                split<T>((f32x4){v[4], v[5], v[6], v[7]} * weight1, lower);
+                f32x4 v[kSpan][2];
+                float most = 0.0f;
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    decayed[we][p] = join(upper[p], lower[p]);
+                for (int j = 0; j < kSpan; ++j) {
+                    const int s0 = 32 * (j0 + j) + 4 * group;
+                    value[j0 + j][we] = read_columns(
+                        lds_c + (s0 + (in >> 2)) * kColumnPitch + 16 * (wave * WE + we) + 4 * (in & 3), kColumnPitch);
+                    float c[8];
+                    Values<T>::unpack8(value[j0 + j][we], c);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        v[j][h] = (f32x4){c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3]} *
+                                  *reinterpret_cast<const f32x4*>(to_end + s0 + 16 * h);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            most = fmaxf(most, fabsf(v[j][h][i]));
+                        }
+                    }
+                }
+                const Power power(T == LSSO_HIP_F16 ? column_max(most) : 0.0f);
+                back[we] = power.back;
+#pragma unroll
+                for (int j = 0; j < kSpan; ++j) {
+                    u32x2 upper[PARTS];
+                    u32x2 lower[PARTS];
+                    split<T>(v[j][0] * power.to, upper);
+                    split<T>(v[j][1] * power.to, lower);
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        decayed[j][we][p] = join(upper[p], lower[p]);
+                    }
                 }
             }
-            const uint16_t* keys = lds_b + (32 * j + 4 * group + (in >> 2)) * kPitch + 4 * (in & 3);
 #pragma unroll
             for (int dt = 0; dt < 2 * KT; ++dt) {
-                const u32x4 key = read_columns(keys + 16 * dt, kPitch);
+                u32x4 key[kSpan];
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
+                for (int j = 0; j < kSpan; ++j) {
+                    const int s0 = 32 * (j0 + j) + 4 * group;
+                    key[j] = read_columns(lds_b + (s0 + (in >> 2)) * kPitch + 4 * (in & 3) + 16 * dt, kPitch);
+                }
 #pragma unroll
-                    for (int we = 0; we < WE; ++we) {
-                        state[dt][we] = mfma_small<T>(key, decayed[we][p], state[dt][we]);
+                for (int we = 0; we < WE; ++we) {
+                    f32x4 sum = T == LSSO_HIP_F16 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : state[dt][we];
+#pragma unroll
+                    for (int j = 0; j < kSpan; ++j) {
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            sum = mfma_small<T>(key[j], decayed[j][we][p], sum);
+                        }
                     }
+                    state[dt][we] = T == LSSO_HIP_F16 ? state[dt][we] + sum * back[we] : sum;
                 }
             }
         }

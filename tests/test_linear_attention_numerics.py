@@ -55,3 +55,33 @@ def test_bfloat16_outputs_are_those_of_fp32_factors(native, size) -> None:
     # What is returned beside it changes no value.
     assert torch.equal(native.linear_attention(*inputs[:3], log_decay),
                        native.linear_attention(*inputs[:3], log_decay, return_state=True)[0])
+
+
+def _rounded_once(a, e, m) -> bool:
+    """a is e but for one rounding to FP16 (half of 2^-24 below its normal range), the
+    parts' 22 bits, FP32 sums of 200 terms and an exponential's last bits: 2^-16 of the
+    terms' size m at worst."""
+
+    bound = 2.0**-11 * (1 + 2.0**-10) * e.abs() + 2.0**-25 + 2.0**-16 * m
+    return bool(((a.double() - e).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(2, 700, 4, 2, 64, 64), (1, 300, 2, 2, 128, 96), (2, 64, 2, 2, 32, 16), (1, 200, 2, 1, 33, 7)])
+@pytest.mark.parametrize("small", (1e-2, 1e-3, 1e-4, 1e-5))
+def test_small_float16_values_keep_their_bits_in_states(native, size, small) -> None:
+    """S of small v and its gradient of small dy, which are FP32: 22 bits of each term
+    and sqrt(200) roundings of the sums, 2^-20 of the norm.  dv and y of them: one
+    rounding."""
+
+    inputs, log_decay, dy, ds = _tensors(size, torch.float16)
+    scale = size[4] ** -0.5
+    inputs[2] = (inputs[2] * small).half()
+    inputs[3], ds, dy = inputs[3] * small, ds * small, (dy * small).half()
+    found = _native(native, inputs, log_decay, scale, dy, ds)
+    exact = _exact(inputs, log_decay, scale, dy, ds)
+    sizes = _exact([x.abs() for x in inputs], log_decay, scale, dy.abs(), ds.abs())
+    for i in (1, 5):
+        assert _apart(found[i], exact[i]) <= 2.0**-20
+    for i in (0, 4):
+        assert _rounded_once(found[i], exact[i], sizes[i])
