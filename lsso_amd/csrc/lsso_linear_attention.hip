@@ -33,9 +33,10 @@
 // off, and of y and the gradients enough last bits for 1.1e-4 of their norm.  They
 // took 74 us a walk at 64 x 2,048 tokens of 4 heads of 64, three truncated ones 84,
 // three rounded ones 86.)  FP16:
-// powers of two bring the decayed c of each column (of a small gradient, its terms
-// are far below FP16's normal range) and S of each wave (of many tokens, it passes
-// 65,504) to 2^13 and more before they are split; P must stay below 65,504.
+// values are brought to 2^13 and more by powers of two before they are split, and the
+// sums freed of them: the decayed c of each column and each row of P (of a small
+// gradient, their terms are far below FP16's normal range, and a product may pass
+// 65,504), and S of each wave (of many tokens, it passes 65,504 too).
 //
 // Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
 // 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
@@ -145,6 +146,27 @@ struct ChunkRows {
     __device__ __forceinline__ uint32_t round(int count) const { return count * (turned() ? 0u - step : step); }
 };
 
+// The larger of v and of another lane's: a move within a row of 16 lanes.
+template <int CONTROL>
+__device__ __forceinline__ uint32_t larger_of(uint32_t v) {
+    const uint32_t other = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CONTROL, 0xf, 0xf, true);
+    return v > other ? v : other;
+}
+
+// The largest value of a wave's lanes, all of them not negative, as bits.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    v = larger_of<0x121>(v);   // row_ror:1
+    v = larger_of<0x122>(v);
+    v = larger_of<0x124>(v);
+    v = larger_of<0x128>(v);
+    const uint32_t r0 = __builtin_amdgcn_readlane(static_cast<int>(v), 0);
+    const uint32_t r1 = __builtin_amdgcn_readlane(static_cast<int>(v), 16);
+    const uint32_t r2 = __builtin_amdgcn_readlane(static_cast<int>(v), 32);
+    const uint32_t r3 = __builtin_amdgcn_readlane(static_cast<int>(v), 48);
+    return larger(larger(r0, r1), larger(r2, r3));
+}
+
 // A chunk of one tensor on its way to LDS: 64 rows of `features` 16-bit values,
 // in 16-byte pieces.  WHOLE: whole pieces, and 64 rows within a buffer's 2^31
 // bytes, so that a piece's address is the chunk's and a lane's own offset; rows
@@ -200,22 +222,37 @@ struct ChunkLoads {
         const bool in = column(i) < features && ((kept >> row(i)) & 1) != 0;
         return in ? v : (u32x4){0u, 0u, 0u, 0u};
     }
-};
-
-// The power of two that brings the largest of some values to 2^13 .. 2^14, where FP16
-// parts hold their 22 bits, and the way back; none of next to nothing, of an infinity
-// or a NaN.
-struct Power {
-    float to = 1.0f;
-    float back = 1.0f;
-    __device__ __forceinline__ explicit Power(float most) {
-        const int exponent = static_cast<int>((__float_as_uint(most) & 0x7fffffffu) >> 23) - 127;
-        if (exponent > -100 && exponent < 128) {
-            to = __uint_as_float(static_cast<uint32_t>(127 + 13 - exponent) << 23);
-            back = __uint_as_float(static_cast<uint32_t>(127 - 13 + exponent) << 23);
+    // The largest bits without a sign of a row, in all lanes that have a piece of it.
+    __device__ __forceinline__ static uint32_t row_most(const u32x4& v) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 pair = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
         }
+        uint32_t most = pair[0] > pair[1] ? pair[0] : pair[1];
+        most = larger_of<0xb1>(most);        // quad_perm 1, 0, 3, 2
+        most = larger_of<0x4e>(most);        // quad_perm 2, 3, 0, 1
+        if constexpr (kPieces >= 8) {
+            most = larger_of<0x141>(most);   // row_half_mirror
+        }
+        if constexpr (kPieces >= 16) {
+            most = larger_of<0x140>(most);   // row_mirror
+        }
+        return most;
     }
 };
+
+// The exponent of the power of two that brings the largest of some values to 2^13 ..
+// 2^14, where FP16 parts hold their 22 bits; none of next to nothing, of an infinity
+// or a NaN.
+__device__ __forceinline__ int power_of(float most) {
+    const int exponent = static_cast<int>((__float_as_uint(most) & 0x7fffffffu) >> 23) - 127;
+    return exponent > -100 && exponent < 128 ? 13 - exponent : 0;
+}
+__device__ __forceinline__ float two_to(int exponent) {   // of -126 .. 127
+    return __uint_as_float(static_cast<uint32_t>(127 + exponent) << 23);
+}
 
 // The largest of lanes i, i + 16, i + 32 and i + 48, in all of them.
 __device__ __forceinline__ float column_max(float v) {
@@ -250,20 +287,6 @@ __device__ __forceinline__ int64_t offset_of(const WalkTensor& t, int64_t batch,
     return batch * t.batch + (head / t.heads_per) * t.head;
 }
 
-// The largest value of a wave's lanes, all of them not negative, as bits.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x121, 0xf, 0xf, true));   // row_ror:1 of 16 lanes
-    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x122, 0xf, 0xf, true));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xf, 0xf, true));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xf, 0xf, true));
-    const uint32_t r0 = __builtin_amdgcn_readlane(static_cast<int>(v), 0);
-    const uint32_t r1 = __builtin_amdgcn_readlane(static_cast<int>(v), 16);
-    const uint32_t r2 = __builtin_amdgcn_readlane(static_cast<int>(v), 32);
-    const uint32_t r3 = __builtin_amdgcn_readlane(static_cast<int>(v), 48);
-    return larger(larger(r0, r1), larger(r2, r3));
-}
-
 // T: type; KT: 32-feature steps of a and b; NW: waves; WE: 16-column blocks of c
 // and S in a wave; WHOLE: rows are whole 16-byte pieces; STATES: the state alone
 // that a piece of the sequence adds to.  Three waves of a SIMD where the registers
@@ -291,6 +314,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
     __shared__ __attribute__((aligned(16))) float to_ends[kBuffers][kChunk];
     __shared__ __attribute__((aligned(16))) float to_tile[kChunk];
     __shared__ __attribute__((aligned(16))) float from_start[kChunk];
+    // FP16: the largest bits of each row of a and of b.
+    constexpr bool kScaled = T == LSSO_HIP_F16 && !STATES;
+    __shared__ uint32_t most_a[kScaled ? kChunk : 1];
+    __shared__ uint32_t most_b[kScaled ? kChunk : 1];
+    __shared__ __attribute__((aligned(16))) float unscale[kScaled ? kColumns : 4];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -426,6 +454,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
     }
     const bool exact = a.features == kFeatures && column0 + kColumns <= a.out_features;
     int counted = 0;
+    // 2 to the power of it is past features * scale_within * l^(t-s).
+    const float widest = static_cast<float>(a.features) * fabsf(a.scale_within) *
+                         __builtin_amdgcn_exp2f(static_cast<float>(kChunk) * fmaxf(rate, 0.0f));
+    const int past_scale =
+        __builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(widest) >> 23)) - 126;
 
     const int out_bytes = a.wide_out != 0 ? 4 : 2;
     ChunkRows rows_out(static_cast<const char*>(a.out.data) + out_bytes * (offset_of(a.out, batch, head) + column0),
@@ -519,12 +552,24 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                         lds_a + loads_a.row(i) * kPitch + (column & ~31) + 2 * (column & 8) + ((column & 16) >> 2);
                     *reinterpret_cast<u32x2*>(to) = (u32x2){v[0], v[1]};
                     *reinterpret_cast<u32x2*>(to + 8) = (u32x2){v[2], v[3]};
+                    if constexpr (kScaled) {
+                        const uint32_t most = loads_a.row_most(v);
+                        if (column == 0) {
+                            most_a[loads_a.row(i)] = most;
+                        }
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < loads_b.kEach; ++i) {
-                *reinterpret_cast<u32x4*>(lds_b + loads_b.row(i) * kPitch + loads_b.column(i)) =
-                    whole ? loads_b.raw[i] : loads_b.piece(i, kept);
+                const u32x4 v = whole ? loads_b.raw[i] : loads_b.piece(i, kept);
+                *reinterpret_cast<u32x4*>(lds_b + loads_b.row(i) * kPitch + loads_b.column(i)) = v;
+                if constexpr (kScaled) {
+                    const uint32_t most = loads_b.row_most(v);
+                    if (loads_b.column(i) == 0) {
+                        most_b[loads_b.row(i)] = most;
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < loads_c.kEach; ++i) {
@@ -542,6 +587,41 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
             issue(chunk + 1);
         }
         f32x4 out[kTiles][WE];
+        // FP16: the exponent of the power of two of the row of P that the lane has of a
+        // tile.  |a_t . b_s| is below features * 2^(of a_t's largest + of the chunk's
+        // largest b + 2): P comes to 2^15 at most, and a value of 2^-17 of that bound
+        // still has its 22 bits.  (No power is above 2^60, so that what came before, which
+        // is multiplied by it too, stays finite.)
+        int most_key = 0;
+        if constexpr (kScaled) {
+            most_key = static_cast<int>(wave_max(most_b[lane]) >> 10);
+        }
+        const auto row_power = [&](int tile) {
+            int query = 0;
+            if constexpr (kScaled) {
+                query = static_cast<int>(most_a[16 * tile + in] >> 10);
+            }
+            const int past = (query > 1 ? query : 1) + (most_key > 1 ? most_key : 1) - 28 + past_scale;
+            const int power = 15 - past;
+            return power > 60 ? 60 : (power < -100 ? -100 : power);
+        };
+        // FP16: the exponent of the power of two for S.
+        int held[WE];
+#pragma unroll
+        for (int we = 0; we < WE; ++we) {
+            held[we] = 0;
+            if constexpr (T == LSSO_HIP_F16) {
+                float most = 0.0f;
+#pragma unroll
+                for (int dt = 0; dt < 2 * KT; ++dt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        most = fmaxf(most, fabsf(state[dt][we][r]));
+                    }
+                }
+                held[we] = power_of(__uint_as_float(wave_max(__float_as_uint(most))));
+            }
+        }
         if constexpr (!STATES) {
             // P: its tiles of 16 s by 16 t, lane column t, rows s; those below the
             // diagonal and then those on it dealt to the waves.
@@ -558,7 +638,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                 }
                 return score;
             };
-            const auto put = [&](int tile, int s, const f32x4& score) {
+            const auto put = [&](int tile, int s, f32x4 score) {
+                if constexpr (kScaled) {
+                    score *= ldexpf(1.0f, row_power(tile));
+                }
                 u32x2 parts_of[PARTS];
                 split<T>(score, parts_of);
                 uint16_t* to = lds_p + (pair_of(tile, s) * 64 + lane) * 8 + 4 * (s & 1);
@@ -592,26 +675,15 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                 }
                 put(tile, tile, score);
             }
-            // a S, before the chunk's own tokens reach S.
-            float factor = 1.0f;
-            float unfactor = 1.0f;
-            if constexpr (T == LSSO_HIP_F16) {
-                uint32_t most = 0;
+            // a S, before the chunk's own tokens reach S.  FP16: each column of S times a power
+            // of two, which y's rows e are freed of.
+            const int own = opaque_int(lane);   // no address of these is held across the loop
+            float factor[WE];
 #pragma unroll
-                for (int dt = 0; dt < 2 * KT; ++dt) {
-#pragma unroll
-                    for (int we = 0; we < WE; ++we) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t bits = __float_as_uint(state[dt][we][r]) & 0x7fffffffu;
-                            most = bits > most ? bits : most;
-                        }
-                    }
-                }
-                const int exponent = static_cast<int>(wave_max(most) >> 23) - 127;
-                if (exponent > -100 && exponent < 128) {   // neither next to nothing nor infinite
-                    factor = __uint_as_float(static_cast<uint32_t>(127 + 14 - exponent) << 23);
-                    unfactor = __uint_as_float(static_cast<uint32_t>(127 - 14 + exponent) << 23);
+            for (int we = 0; we < WE; ++we) {
+                factor[we] = two_to(held[we]);
+                if (kScaled && own < 16) {
+                    unscale[16 * (wave * WE + we) + own] = two_to(-held[we]);
                 }
             }
 #pragma unroll
@@ -628,8 +700,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                 for (int we = 0; we < WE; ++we) {
                     u32x2 upper[PARTS];
                     u32x2 lower[PARTS];
-                    split<T>(state[2 * k][we] * factor, upper);
-                    split<T>(state[2 * k + 1][we] * factor, lower);
+                    split<T>(state[2 * k][we] * factor[we], upper);
+                    split<T>(state[2 * k + 1][we] * factor[we], lower);
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
                         from_state[we][p] = join(upper[p], lower[p]);
@@ -648,88 +720,119 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                     }
                 }
             }
+            if constexpr (kScaled) {
+                wave_lds_order();   // unscale: this wave's own columns
+            }
 #pragma unroll
             for (int tile = 0; tile < kTiles; ++tile) {
-                const float weight = unfactor * from_start[16 * tile + in];
+                float weight = from_start[16 * tile + in];
+                if constexpr (kScaled) {
+                    weight = ldexpf(weight, row_power(tile));
+                }
 #pragma unroll
                 for (int we = 0; we < WE; ++we) {
                     out[tile][we] *= weight;
+                    if constexpr (kScaled) {
+                        out[tile][we] *= *reinterpret_cast<const f32x4*>(unscale + 16 * (wave * WE + we) + 4 * (own >> 4));
+                    }
                 }
-            }
-        }
-        const float decay = __builtin_amdgcn_exp2f(rate * static_cast<float>(total - less));
-#pragma unroll
-        for (int dt = 0; dt < 2 * KT; ++dt) {
-#pragma unroll
-            for (int we = 0; we < WE; ++we) {
-                state[dt][we] *= decay;
             }
         }
         pending -= less;
         counted += total;
-        // l^(n-s) c of the lane's column e, in parts: 32 tokens at a time, or in FP16 all
-        // 64, brought to their range by a power of two of each column, which the sum is
-        // freed of before it meets S.
-        constexpr int kSpan = T == LSSO_HIP_F16 ? 2 : 1;   // of 32 tokens
+        // The tiles' powers, a byte each: behind the barrier most_a is the next chunk's.
+        uint32_t powers = 0;
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                powers |= static_cast<uint32_t>(row_power(tile) & 0xff) << (8 * tile);
+            }
+        }
+        // c of the lane's column e, and S decayed.  FP16: a power of two brings l^(n-s) c of
+        // each column to its range; S is multiplied by it too, which must not pass 2^100,
+        // and freed of it at the end.
+        const float decay = __builtin_amdgcn_exp2f(rate * static_cast<float>(total - less));
         u32x4 value[2][WE];
+        float power[WE];
+        const auto weighted = [&](int j, int we, int h) {   // of 4 tokens
+            const u32x4& raw = value[j][we];
+            const f32x4 c = {Values<T>::low(raw[2 * h]), Values<T>::high(raw[2 * h]), Values<T>::low(raw[2 * h + 1]),
+                             Values<T>::high(raw[2 * h + 1])};
+            return c * *reinterpret_cast<const f32x4*>(to_end + 32 * j + 16 * h + 4 * group);
+        };
+        const auto read_value = [&](int j, int we) {
+            value[j][we] = read_columns(
+                lds_c + (32 * j + 4 * group + (in >> 2)) * kColumnPitch + 16 * (wave * WE + we) + 4 * (in & 3), kColumnPitch);
+        };
 #pragma unroll
-        for (int j0 = 0; j0 < 2; j0 += kSpan) {
-            u32x4 decayed[kSpan][WE][PARTS];
-            float back[WE];
-#pragma unroll
-            for (int we = 0; we < WE; ++we) {
-                f32x4 v[kSpan][2];
+        for (int we = 0; we < WE; ++we) {
+            power[we] = 1.0f;
+            if constexpr (T == LSSO_HIP_F16) {
                 float most = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kSpan; ++j) {
-                    const int s0 = 32 * (j0 + j) + 4 * group;
-                    value[j0 + j][we] = read_columns(
-                        lds_c + (s0 + (in >> 2)) * kColumnPitch + 16 * (wave * WE + we) + 4 * (in & 3), kColumnPitch);
-                    float c[8];
-                    Values<T>::unpack8(value[j0 + j][we], c);
+                for (int j = 0; j < 2; ++j) {
+                    read_value(j, we);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        v[j][h] = (f32x4){c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3]} *
-                                  *reinterpret_cast<const f32x4*>(to_end + s0 + 16 * h);
+                        const f32x4 v = weighted(j, we, h);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            most = fmaxf(most, fabsf(v[j][h][i]));
+                            most = fmaxf(most, fabsf(v[i]));
                         }
                     }
                 }
-                const Power power(T == LSSO_HIP_F16 ? column_max(most) : 0.0f);
-                back[we] = power.back;
+                const int room = held[we] + 87;   // to 2^100
+                const int wanted = power_of(column_max(most));
+                const int exponent = wanted < room ? wanted : room;
+                power[we] = two_to(exponent);
+                // The weighted values are made again: held, they cost 16 registers more.
 #pragma unroll
-                for (int j = 0; j < kSpan; ++j) {
-                    u32x2 upper[PARTS];
-                    u32x2 lower[PARTS];
-                    split<T>(v[j][0] * power.to, upper);
-                    split<T>(v[j][1] * power.to, lower);
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        decayed[j][we][p] = join(upper[p], lower[p]);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    asm volatile("" : "+v"(value[j][we]) : : "memory");
                 }
             }
 #pragma unroll
             for (int dt = 0; dt < 2 * KT; ++dt) {
-                u32x4 key[kSpan];
+                state[dt][we] *= decay * power[we];
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < kSpan; ++j) {
-                    const int s0 = 32 * (j0 + j) + 4 * group;
-                    key[j] = read_columns(lds_b + (s0 + (in >> 2)) * kPitch + 4 * (in & 3) + 16 * dt, kPitch);
+        for (int j = 0; j < 2; ++j) {   // 32 tokens s
+            u32x4 decayed[WE][PARTS];
+#pragma unroll
+            for (int we = 0; we < WE; ++we) {
+                if constexpr (T != LSSO_HIP_F16) {
+                    read_value(j, we);
                 }
+                u32x2 upper[PARTS];
+                u32x2 lower[PARTS];
+                split<T>(weighted(j, we, 0) * power[we], upper);
+                split<T>(weighted(j, we, 1) * power[we], lower);
 #pragma unroll
-                for (int we = 0; we < WE; ++we) {
-                    f32x4 sum = T == LSSO_HIP_F16 ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : state[dt][we];
+                for (int p = 0; p < PARTS; ++p) {
+                    decayed[we][p] = join(upper[p], lower[p]);
+                }
+            }
+            const uint16_t* keys = lds_b + (32 * j + 4 * group + (in >> 2)) * kPitch + 4 * (in & 3);
 #pragma unroll
-                    for (int j = 0; j < kSpan; ++j) {
+            for (int dt = 0; dt < 2 * KT; ++dt) {
+                const u32x4 key = read_columns(keys + 16 * dt, kPitch);
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            sum = mfma_small<T>(key[j], decayed[j][we][p], sum);
-                        }
+                for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                    for (int we = 0; we < WE; ++we) {
+                        state[dt][we] = mfma_small<T>(key, decayed[we][p], state[dt][we]);
                     }
-                    state[dt][we] = T == LSSO_HIP_F16 ? state[dt][we] + sum * back[we] : sum;
+                }
+            }
+        }
+        if constexpr (T == LSSO_HIP_F16) {
+#pragma unroll
+            for (int we = 0; we < WE; ++we) {
+                const float back = __uint_as_float((254u << 23) - __float_as_uint(power[we]));
+#pragma unroll
+                for (int dt = 0; dt < 2 * KT; ++dt) {
+                    state[dt][we] *= back;
                 }
             }
         }
@@ -748,6 +851,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                         for (int we = 0; we < WE; ++we) {
                             out[tile][we] = mfma_small<T>(value[j][we], score, out[tile][we]);
                         }
+                    }
+                }
+            }
+            if constexpr (kScaled) {
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) {
+                    const float back = ldexpf(1.0f, -static_cast<int8_t>(powers >> (8 * tile)));
+#pragma unroll
+                    for (int we = 0; we < WE; ++we) {
+                        out[tile][we] *= back;
                     }
                 }
             }

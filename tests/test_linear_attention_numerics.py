@@ -85,3 +85,62 @@ def test_small_float16_values_keep_their_bits_in_states(native, size, small) -> 
         assert _apart(found[i], exact[i]) <= 2.0**-20
     for i in (0, 4):
         assert _rounded_once(found[i], exact[i], sizes[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(2, 700, 4, 2, 64, 64), (1, 300, 2, 2, 128, 96), (2, 64, 2, 2, 32, 16), (1, 200, 2, 1, 33, 7)])
+@pytest.mark.parametrize("small", (1e-2, 1e-4, 1e-5))
+def test_small_float16_values_keep_their_bits_in_products(native, size, small) -> None:
+    """dq and dk of small dy, whose products with v are small, and y and dv of small k:
+    one rounding."""
+
+    for which in ("dy", "k"):
+        inputs, log_decay, dy, ds = _tensors(size, torch.float16)
+        scale = size[4] ** -0.5
+        if which == "dy":
+            dy, ds = (dy * small).half(), ds * small
+        else:
+            inputs[1], inputs[3] = (inputs[1] * small).half(), inputs[3] * small
+        found = _native(native, inputs, log_decay, scale, dy, ds)
+        exact = _exact(inputs, log_decay, scale, dy, ds)
+        sizes = _exact([x.abs() for x in inputs], log_decay, scale, dy.abs(), ds.abs())
+        for i in (0, 2, 3, 4):
+            assert _rounded_once(found[i], exact[i], sizes[i]), (which, i)
+
+
+@pytest.mark.gpu
+def test_rows_of_float16_of_different_sizes(native) -> None:
+    """A chunk's queries, and their gradients, from 2^-10 to 2^10: each row has a power of
+    its own."""
+
+    size = (1, 130, 2, 1, 64, 64)
+    inputs, log_decay, dy, ds = _tensors(size, torch.float16)
+    rows = (2.0 ** torch.linspace(-10.0, 10.0, 65, device="cuda").round()).repeat(2).view(1, 130, 1, 1)
+    inputs[0], dy = (inputs[0] * rows).half(), (dy / rows).half()
+    found = _native(native, inputs, log_decay, 0.125, dy, ds)
+    exact = _exact(inputs, log_decay, 0.125, dy, ds)
+    sizes = _exact([x.abs() for x in inputs], log_decay, 0.125, dy.abs(), ds.abs())
+    for i in (0, 2):   # rows of y and dq are each of one size; those of dk and dv are sums over all
+        assert _rounded_once(found[i], exact[i], sizes[i])
+    for i in (3, 4):
+        assert _rounded_once(found[i], exact[i], sizes[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", (1.0, 2.0**20, 2.0**-30))
+def test_float16_products_past_65504(native, scale) -> None:
+    """scale (q . k) of up to 10^12 and of 10^-9, brought back by v: FP32 values."""
+
+    size = (1, 150, 2, 2, 64, 32)
+    inputs, log_decay, dy, ds = _tensors(size, torch.float16)
+    inputs[0], inputs[1] = (inputs[0] * 100).half(), (inputs[1] * 100).half()
+    v = 1e-5 if scale == 1.0 else (2.0**-24 if scale > 1.0 else 100.0)
+    inputs[2], inputs[3], dy = (inputs[2] * v).half(), inputs[3] * v, dy * 0
+    found = _native(native, inputs, log_decay, scale, dy, ds)
+    exact = _exact(inputs, log_decay, scale, dy, ds)
+    sizes = _exact([x.abs() for x in inputs], log_decay, scale, dy.abs(), ds.abs())
+    past = exact[0].abs() > 65000.0
+    assert torch.isfinite(found[0][~past]).all()
+    inside = torch.where(past, 0.0, found[0].double()), torch.where(past, 0.0, exact[0])
+    assert _rounded_once(*inside, sizes[0])
+    assert _apart(found[1], exact[1]) <= 2.0**-20
