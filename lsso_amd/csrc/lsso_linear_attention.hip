@@ -36,7 +36,8 @@
 // values are brought to 2^13 and more by powers of two before they are split, and the
 // sums freed of them: the decayed c of each column and each row of P (of a small
 // gradient, their terms are far below FP16's normal range, and a product may pass
-// 65,504), and S of each wave (of many tokens, it passes 65,504 too).
+// 65,504), and each column of S (of many tokens, it passes 65,504 too, in one feature
+// of v and not in another).
 //
 // Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
 // 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
             const int power = 15 - past;
             return power > 60 ? 60 : (power < -100 ? -100 : power);
         };
-        // FP16: the exponent of the power of two for S.
+        // FP16: the exponent of the power of two for each column of S.
         int held[WE];
 #pragma unroll
         for (int we = 0; we < WE; ++we) {
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
                         most = fmaxf(most, fabsf(state[dt][we][r]));
                     }
                 }
-                held[we] = power_of(__uint_as_float(wave_max(__float_as_uint(most))));
+                held[we] = power_of(column_max(most));
             }
         }
         if constexpr (!STATES) {

@@ -144,3 +144,44 @@ def test_float16_products_past_65504(native, scale) -> None:
     inside = torch.where(past, 0.0, found[0].double()), torch.where(past, 0.0, exact[0])
     assert _rounded_once(*inside, sizes[0])
     assert _apart(found[1], exact[1]) <= 2.0**-20
+
+
+@pytest.mark.gpu
+def test_float16_columns_of_different_sizes(native) -> None:
+    """Value features from 2^-10 to 2^13, and states past 65,504 beside small ones: each
+    column of S has a power of its own."""
+
+    size = (2, 260, 2, 1, 64, 48)
+    inputs, log_decay, dy, ds = _tensors(size, torch.float16)
+    columns = 2.0 ** torch.linspace(-10.0, 13.0, 48, device="cuda").round()
+    order = torch.randperm(48, generator=torch.Generator().manual_seed(0)).cuda()
+    inputs[2], inputs[3] = (inputs[2] * columns[order]).half(), inputs[3] * columns[order] * 2.0**20
+    inputs[0] = (inputs[0] * 2.0**-10).half()
+    found = _native(native, inputs, log_decay, 0.125, dy, ds)
+    exact = _exact(inputs, log_decay, 0.125, dy, ds)
+    sizes = _exact([x.abs() for x in inputs], log_decay, 0.125, dy.abs(), ds.abs())
+    past = exact[0].abs() > 65000.0
+    inside = torch.where(past, 0.0, found[0].double()), torch.where(past, 0.0, exact[0])
+    assert _rounded_once(*inside, sizes[0])
+    for e in range(48):
+        assert _apart(found[1][..., e], exact[1][..., e]) <= 2.0**-20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_an_infinite_column_of_a_state_leaves_the_others(native, dtype) -> None:
+    """States of 10^6, one value feature of them infinite."""
+
+    inputs, log_decay, dy, ds = _tensors((1, 130, 2, 2, 32, 32), dtype)
+    inputs[0], inputs[3] = (inputs[0] * 2.0**-8).to(dtype), inputs[3] * 1e6
+    wild = [*inputs[:3], inputs[3].clone()]
+    wild[3][..., 5] = math.inf
+    y, last = native.linear_attention(*wild[:3], log_decay, scale=0.125, initial_state=wild[3], return_state=True)
+    expected, after = native.linear_attention(*inputs[:3], log_decay, scale=0.125, initial_state=inputs[3], return_state=True)
+    others = torch.arange(32, device="cuda") != 5
+    assert torch.equal(y[..., others], expected[..., others]) and torch.equal(last[..., others], after[..., others])
+    assert not torch.isfinite(y[..., 5]).any() and torch.isposinf(last[..., 5]).all()
+    exact = _exact(inputs, log_decay, 0.125, dy, ds)
+    sizes = _exact([x.abs() for x in inputs], log_decay, 0.125, dy.abs(), ds.abs())
+    if dtype == torch.float16:
+        assert _rounded_once(expected, exact[0], sizes[0])
