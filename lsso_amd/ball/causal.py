@@ -548,7 +548,8 @@ def linear_attention(
 
     S is FP32; products take 16-bit operands, FP32 ones as parts that hold them (24
     bits in BF16, 22 in FP16), and accumulate in FP32: y and the gradients are off by
-    one rounding of their type.  Differentiable (first order) in query, key, value and
+    one rounding of their type.  An infinity or a NaN reaches its token's y and those
+    behind it, and in a gradient those before it.  Differentiable (first order) in query, key, value and
     initial_state, deterministically; log_decay is fixed."""
 
     _hip().require_available()

@@ -39,6 +39,10 @@
 // 65,504), and each column of S (of many tokens, it passes 65,504 too, in one feature
 // of v and not in another).
 //
+// What is not finite stays causal: a zero of P above the diagonal times an infinite c
+// would be a NaN, so a chunk whose S shows one takes P c without it and makes its
+// column NaN from its token on.
+//
 // Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
 // 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
 // 17 of them for the first chunk's loads and the launch's end, where workgroups finish
@@ -262,6 +266,25 @@ __device__ __forceinline__ float column_max(float v) {
     const uint32_t some = __float_as_uint(fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1])));
     const auto halves = __builtin_amdgcn_permlane32_swap(some, some, false, false);
     return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// Zeros in place of the infinities and NaNs among read_columns' 8 values of the tokens
+// s0 .. s0 + 3 and s0 + 16 .. s0 + 19; how far the chunk's end is from the first of them.
+template <int T>
+__device__ __forceinline__ float drop_wild(u32x4& v, int s0) {
+    constexpr uint32_t kExponent = T == LSSO_HIP_F16 ? 0x7c00u : 0x7f80u;
+    float reach = 0.0f;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        const uint32_t exponent = kExponent << (16 * (i & 1));
+        if ((v[i / 2] & exponent) == exponent) {
+            v[i / 2] &= (i & 1) != 0 ? 0x0000ffffu : 0xffff0000u;
+            reach = static_cast<float>(kChunk - (s0 + 16 * (i >> 2) + (i & 3)));
+        }
+    }
+    return reach;
 }
 
 // 8 values of k (or s) for one lane: rows at `at` and 16 rows on, read
@@ -595,7 +618,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
         // is multiplied by it too, stays finite.)
         int most_key = 0;
         if constexpr (kScaled) {
-            most_key = static_cast<int>(wave_max(most_b[lane]) >> 10);
+            const uint32_t key = most_b[lane];   // P is no number, scaled or not, where b is none
+            most_key = static_cast<int>(wave_max(key < 0x7c00u ? key : 0u) >> 10);
         }
         const auto row_power = [&](int tile) {
             int query = 0;
@@ -840,6 +864,33 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
         if constexpr (!STATES) {
             // P is whole, and nobody reads the chunk any more: the next one may be staged.
             __syncthreads();
+            // A c that is not finite made S so.  P's zeros for earlier tokens must not meet
+            // it: from its token on the column is a NaN, and the product takes a zero.
+            bool broken = false;
+#pragma unroll
+            for (int we = 0; we < WE; ++we) {
+                broken = broken || !finite(state[0][we][0]);
+            }
+            if (__any(broken)) {
+                const int own = opaque_int(lane);   // nothing of this path is held across the loop
+#pragma unroll
+                for (int we = 0; we < WE; ++we) {
+                    float reach = 0.0f;   // from the first such token of the column to the chunk's end
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        reach = fmaxf(reach, drop_wild<T>(value[j][we], 32 * j + 4 * (own >> 4)));
+                    }
+                    reach = column_max(reach);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int clean = kChunk - static_cast<int>(__shfl(reach, 4 * (own >> 4) + r)) - (own & 15);
+#pragma unroll
+                        for (int tile = 0; tile < kTiles; ++tile) {
+                            out[tile][we][r] = 16 * tile < clean ? out[tile][we][r] : __builtin_nanf("");
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll

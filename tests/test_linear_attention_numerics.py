@@ -185,3 +185,56 @@ def test_an_infinite_column_of_a_state_leaves_the_others(native, dtype) -> None:
     sizes = _exact([x.abs() for x in inputs], log_decay, 0.125, dy.abs(), ds.abs())
     if dtype == torch.float16:
         assert _rounded_once(expected, exact[0], sizes[0])
+
+
+def _agree(a, b) -> bool:
+    """The same values: a chunk's power of two is that of its largest finite exponents,
+    which a zero in place of an infinity leaves."""
+
+    return torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("size", [(1, 200, 2, 1, 64, 64), (1, 700, 2, 2, 24, 40), (2, 130, 4, 4, 13, 9), (1, 150, 1, 1, 128, 128)])
+@pytest.mark.parametrize("wild", (math.inf, -math.inf, math.nan))
+@pytest.mark.parametrize("token", (70, 95, 127))
+def test_what_is_not_finite_reaches_no_earlier_token(native, dtype, size, wild, token) -> None:
+    """One value of v, q, k or dy: y of the tokens before it, gradients of those behind
+    it, and value features beside it, as with a zero in its place."""
+
+    inputs, log_decay, dy, ds = _tensors(size, dtype)
+    scale, feature = size[4] ** -0.5, 5
+    others = torch.arange(max(size[4:]), device="cuda") != feature
+    before, behind = slice(0, token), slice(token + 1, size[1])
+
+    def run(name, value):
+        tensors = {"q": inputs[0], "k": inputs[1], "v": inputs[2], "dy": dy}
+        tensors = {key: x.detach().clone() for key, x in tensors.items()}
+        tensors[name][0, token, 0, feature] = value
+        names = ("y", "s", "dq", "dk", "dv", "ds")
+        return dict(zip(names, _native(native, [tensors["q"], tensors["k"], tensors["v"], inputs[3]], log_decay, scale,
+                                       tensors["dy"], ds)))
+
+    found, plain = run("v", wild), run("v", 0.0)
+    assert torch.equal(found["y"][:, before], plain["y"][:, before])
+    assert torch.equal(found["y"][..., others[:size[5]]], plain["y"][..., others[:size[5]]])
+    assert not torch.isfinite(found["y"][0, token, 0, feature]) and not torch.isfinite(found["s"][0, 0, :, feature]).any()
+    assert _agree(found["dq"][:, before], plain["dq"][:, before])
+    assert torch.equal(found["dk"][:, behind], plain["dk"][:, behind])
+    found, plain = run("dy", wild), run("dy", 0.0)
+    assert torch.equal(found["y"], plain["y"]) and torch.equal(found["s"], plain["s"])
+    assert torch.equal(found["dv"][:, behind], plain["dv"][:, behind])
+    assert torch.equal(found["dv"][..., others[:size[5]]], plain["dv"][..., others[:size[5]]])
+    assert not torch.isfinite(found["dv"][0, token, 0, feature])
+    assert _agree(found["dk"][:, behind], plain["dk"][:, behind])
+    rows = torch.arange(size[1], device="cuda") != token
+    assert torch.equal(found["dq"][:, rows], plain["dq"][:, rows])
+    found, plain = run("k", wild), run("k", 0.0)
+    assert _agree(found["y"][:, before], plain["y"][:, before])
+    assert torch.equal(found["dq"][:, before], plain["dq"][:, before])
+    assert torch.equal(found["dv"][:, rows], plain["dv"][:, rows])
+    found, plain = run("q", wild), run("q", 0.0)
+    assert torch.equal(found["y"][:, rows], plain["y"][:, rows])
+    assert torch.equal(found["dk"][:, behind], plain["dk"][:, behind])
+    assert _agree(found["dv"][:, behind], plain["dv"][:, behind])
