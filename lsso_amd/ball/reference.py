@@ -467,6 +467,28 @@ def group_norm(
 _ATTENTION_CHUNK = 64
 
 
+def _within_chunks(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rate: torch.Tensor, rank: torch.Tensor
+) -> torch.Tensor:
+    """sum over s <= t of exp(rate (rank_t - rank_s)) (q_t . k_s) v_s within the chunks of
+    [B, H, chunks, tokens, features], tokens a power of two.  The second half of every
+    block against its first, from blocks of two on: no zero stands for a later token,
+    whose infinities it would turn to NaN."""
+
+    y = (q * k).sum(-1, keepdim=True) * v
+    half = 1
+    while half < q.shape[-2]:
+        first, second = (
+            [x.unflatten(dim, (-1, 2, half)).select(dim - 1, i) for x, dim in ((q, -2), (k, -2), (v, -2), (rank, -1))]
+            for i in (0, 1)
+        )
+        weights = torch.exp(rate[..., None, None, None] * (second[3][..., :, None] - first[3][..., None, :]))
+        part = (second[0] @ first[1].mT * weights) @ first[2]
+        y = y + torch.stack((torch.zeros_like(part), part), dim=-3).flatten(-4, -2)
+        half *= 2
+    return y
+
+
 def linear_attention(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -488,31 +510,33 @@ def linear_attention(
     shared = heads // key.shape[2]
     kept = torch.ones(batch, length, dtype=torch.bool, device=query.device) if row_mask is None else row_mask
 
+    tokens = min(_ATTENTION_CHUNK, 1 << max(0, length - 1).bit_length())
+    room = -length % tokens
+
     def heads_first(x: torch.Tensor, repeat: int = 1) -> torch.Tensor:
+        """[B, H, chunks, tokens, features]"""
+
         x = x.to(calc_dtype)
         x = torch.where(kept[..., None, None], x, torch.zeros_like(x))
-        return x.transpose(1, 2).repeat_interleave(repeat, dim=1)
+        x = functional.pad(x.transpose(1, 2), (0, 0, 0, room)).unflatten(2, (-1, tokens))
+        return x.repeat_interleave(repeat, dim=1)
 
     q, k, v = heads_first(query), heads_first(key, shared), heads_first(value, shared)
     # -inf forgets at once: 0 * -inf is kept out of the exponents.
     rate = log_decay.to(calc_dtype).clamp_min(-1e30).view(1, heads, 1)
+    rank = functional.pad(kept, (0, room)).unflatten(1, (-1, tokens)).cumsum(-1).to(calc_dtype)[:, None]
     state = torch.zeros(batch, heads, features, v.shape[-1], dtype=calc_dtype, device=query.device)
     if initial_state is not None:
         state = initial_state.to(calc_dtype)
     outputs = []
-    for begin in range(0, length, _ATTENTION_CHUNK):
-        some = slice(begin, begin + _ATTENTION_CHUNK)
-        rank = kept[:, some].cumsum(1).to(calc_dtype)[:, None, :]   # [B, 1, C]
-        total = rank[..., -1:]
-        apart = rank[..., :, None] - rank[..., None, :]
-        below = torch.ones(apart.shape[-2:], dtype=torch.bool, device=query.device).tril()
-        weights = torch.where(below, torch.exp(rate[..., None] * apart.clamp_min(0)), torch.zeros_like(apart))
-        scores = q[:, :, some] @ k[:, :, some].mT * weights
-        across = torch.exp(rate * rank)[..., None] * (q[:, :, some] @ state)
-        outputs.append(scores @ v[:, :, some] + across)
-        decayed = v[:, :, some] * torch.exp(rate * (total - rank))[..., None]
-        state = torch.exp(rate * total)[..., None] * state + k[:, :, some].mT @ decayed
-    y = torch.cat(outputs, dim=2) if outputs else v[:, :, :0]
+    for chunk in range(q.shape[2]):
+        here = rank[:, :, chunk]   # [B, 1, tokens]
+        total = here[..., -1:]
+        outputs.append(torch.exp(rate * here)[..., None] * (q[:, :, chunk] @ state))
+        decayed = v[:, :, chunk] * torch.exp(rate * (total - here))[..., None]
+        state = torch.exp(rate * total)[..., None] * state + k[:, :, chunk].mT @ decayed
+    y = v if not outputs else torch.stack(outputs, dim=2) + _within_chunks(q, k, v, rate, rank)
+    y = y.flatten(2, 3)[:, :, :length]
     y = (scale * y).transpose(1, 2)
     y = torch.where(kept[..., None, None], y, torch.zeros_like(y)).to(query.dtype).contiguous()
     return (y, state) if return_state else y
