@@ -162,7 +162,13 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
     const Teams t(a);
     const int size = a.channels / a.groups;
     const int pieces = size / V;
-    const float share = 1.0f / static_cast<float>(size);
+    // Of FP32 divided: the reciprocal's own rounding shows.
+    const float count = static_cast<float>(size);
+    const float share = 1.0f / count;
+    const auto mean_of = [&](float sum) {
+        sum = team_sum(sum, a.team);
+        return T == LSSO_HIP_F32 ? sum / count : sum * share;
+    };
     const int channel0 = (t.active ? t.group : 0) * size;
     float w[K][V];
     float b[K][V];
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
                     sum += x[k][i];
                 }
             }
-            const float mean = team_sum(sum, a.team) * share;
+            const float mean = mean_of(sum);
             float squares = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
                     squares += x[k][i] * x[k][i];
                 }
             }
-            const float rstd = 1.0f / sqrtf(team_sum(squares, a.team) * share + a.eps);
+            const float rstd = 1.0f / sqrtf(mean_of(squares) + a.eps);
             if constexpr (!BACKWARD) {
                 by_kind(a.activation, [&](auto kind) {
 #pragma unroll
@@ -285,8 +291,8 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
                         }
                     }
                 });
-                first = team_sum(first, a.team) * share;
-                second = team_sum(second, a.team) * share;
+                first = mean_of(first);
+                second = mean_of(second);
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     float dx[V];
