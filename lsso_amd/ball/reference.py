@@ -443,8 +443,9 @@ def group_norm(
     for FP64 x), one cast; zeros for the others, which reach no gradient."""
 
     calc_dtype = _calculation_dtype(x)
-    value = x.to(calc_dtype).reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
-    kept = None if row_mask is None else row_mask.reshape(x.shape[0], -1, 1, 1)
+    rows = (x.shape[0], math.prod(x.shape[1:-1]))
+    value = x.to(calc_dtype).reshape(*rows, groups, x.shape[-1] // groups)
+    kept = None if row_mask is None else row_mask.reshape(*rows, 1, 1)
     if kept is not None:
         value = torch.where(kept, value, torch.zeros_like(value))
     tokens = value.shape[1] if kept is None else kept.sum(1, keepdim=True).clamp_min(1)
