@@ -218,14 +218,10 @@ class CausalMixer(nn.Module):
         if not 1 <= frequencies.shape[0] <= self.head_dim // 2:
             raise ValueError(f"frequencies must be 1 to {self.head_dim // 2}, got {frequencies.shape[0]}")
         self.layout, self.amplitude = layout, float(amplitude)
-        # Of a moved module only the device changes: both lose what they are for
-        # in a type of fewer bits.
-        self._fixed = {
-            "frequencies": frequencies.detach().to(device="cpu", dtype=torch.float64),
-            "log_decay": self._decays(num_heads, shortest, longest),
-        }
-        for name, value in self._fixed.items():
-            self.register_buffer(name, value.clone(), persistent=False)
+        device = torch.empty(0).device   # where the layers below are made
+        frequencies = frequencies.detach().to(device=device, dtype=torch.float64, copy=True)
+        self.register_buffer("frequencies", frequencies, persistent=False)
+        self.register_buffer("log_decay", self._decays(num_heads, shortest, longest), persistent=False)
         self.w_in = nn.Linear(dim, (num_heads + 2 * kv_heads) * self.head_dim, bias=bias)
         self.norm = GroupNorm(num_heads, dim, activation=activation)
         self.w_o = nn.Linear(dim, dim, bias=bias)
@@ -236,9 +232,12 @@ class CausalMixer(nn.Module):
         return torch.log1p(-1.0 / (shortest * (longest / shortest) ** spread)).float()
 
     def _apply(self, *arguments, **keywords):
+        # Of a moved module only the device changes: both lose what they are for in a
+        # type of fewer bits.  What the program wrote into them goes with them.
+        fixed = {name: getattr(self, name) for name in ("frequencies", "log_decay")}
         result = super()._apply(*arguments, **keywords)
         device = self.w_o.weight.device
-        for name, value in self._fixed.items():
+        for name, value in fixed.items():
             setattr(self, name, value.to(device))
         return result
 
