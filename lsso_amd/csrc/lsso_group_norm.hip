@@ -9,8 +9,8 @@
 // Bound: HBM.  Two forms:
 //
 // Every token a sample of its own (heads of a token, or a layer norm): a group's
-// channels are read once, by a team of lanes that keeps them in registers, sums
-// them over its lanes, and writes y.  Teams of neighbouring groups sit next to
+// channels are read once, by a team of lanes (up to a wave, or the workgroup) that
+// keeps them in registers, sums them over its lanes, and writes y.  Teams of neighbouring groups sit next to
 // each other, so that a wave reads whole lines.  Each lane stays with its
 // channels while its workgroup walks over the rows, which leaves dw and db in
 // its registers to the end.
@@ -44,7 +44,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlockRows = 4;        // rows of a thread in flight
-constexpr int kTeamMost = 4;         // most pieces of a lane
+constexpr int kTeamMost = 4;         // most pieces of a lane of a wave's team
+constexpr int kLaneMost = 32;        // most values of a lane
 constexpr int64_t kMostGrid = 1 << 20;
 
 // act(z) and act'(z) of one kind.  FP32 outputs show more than the fast forms hold
@@ -165,8 +166,26 @@ __global__ __launch_bounds__(kThreads) void team_norm_kernel(GroupNormArgs a) {
     // Of FP32 divided: the reciprocal's own rounding shows.
     const float count = static_cast<float>(size);
     const float share = 1.0f / count;
+    // A team of the whole workgroup passes its waves' sums through LDS, in two places by
+    // turns: whoever writes one again has met all its readers at the other's barrier.
+    __shared__ float waves[2][kThreads / 64];
+    int turn = 0;
     const auto mean_of = [&](float sum) {
-        sum = team_sum(sum, a.team);
+        if (a.team <= 64) {   // uniform
+            sum = team_sum(sum, a.team);
+        } else {
+            sum = team_sum(sum, 64);
+            if ((threadIdx.x & 63) == 0) {
+                waves[turn][threadIdx.x >> 6] = sum;
+            }
+            __syncthreads();
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kThreads / 64; ++i) {
+                sum += waves[turn][i];
+            }
+            turn ^= 1;
+        }
         return T == LSSO_HIP_F32 ? sum / count : sum * share;
     };
     const int channel0 = (t.active ? t.group : 0) * size;
@@ -911,7 +930,23 @@ void launch_team(const GroupNormArgs& a, bool backward, hipStream_t stream) {
         case 1: launch_team_pieces<T, V, 1>(a, backward, stream); break;
         case 2: launch_team_pieces<T, V, 2>(a, backward, stream); break;
         case 3: launch_team_pieces<T, V, 3>(a, backward, stream); break;
-        default: launch_team_pieces<T, V, 4>(a, backward, stream); break;
+        case 4: launch_team_pieces<T, V, 4>(a, backward, stream); break;
+        default:   // of narrow pieces, up to the 32 values that four of 8 are
+            if constexpr (V <= 4) {
+                if (a.team_pieces == 8) {
+                    launch_team_pieces<T, V, 8>(a, backward, stream);
+                }
+            }
+            if constexpr (V <= 2) {
+                if (a.team_pieces == 16) {
+                    launch_team_pieces<T, V, 16>(a, backward, stream);
+                }
+            }
+            if constexpr (V == 1) {
+                if (a.team_pieces == 32) {
+                    launch_team_pieces<T, V, 32>(a, backward, stream);
+                }
+            }
     }
 }
 
@@ -998,9 +1033,16 @@ void plan_group_norm(GroupNormArgs* a, bool backward, size_t* partial_bytes) {
     a->team = 0;
     a->vector = widest(size);
     const int pieces = size / a->vector;
-    if (a->length == 1 && pieces <= 64 * kTeamMost) {
-        // The lanes and pieces that leave the fewest registers empty; of equals the
-        // most lanes, which hold fewer registers each.
+    if (a->length == 1 && size <= kThreads * kLaneMost) {
+        // The lanes of a wave and pieces that leave the fewest registers empty; of equals
+        // the most lanes, which hold fewer registers each.  Wider: the workgroup (65,536 x 4,096
+        // in FP16: 240 us forward and 606 trained; as samples of one row they left 2 GiB
+        // of partials and took 2,740 and 6,910).
+        a->team = kThreads;
+        a->team_pieces = (pieces + kThreads - 1) / kThreads;
+        if (a->team_pieces > 4) {
+            a->team_pieces = a->team_pieces <= 8 ? 8 : (a->team_pieces <= 16 ? 16 : 32);
+        }
         int best = 1 << 30;
         for (int k = 1; k <= kTeamMost; ++k) {
             int lanes = 1;

@@ -517,7 +517,7 @@ struct GroupNormArgs {
     float* sums;                // [samples, groups, 2]: mean of dn, mean of dn xhat
     int64_t splits;             // set by plan_group_norm: workgroups along the tokens of a sample
     int64_t split_rows;
-    int team;                   // tokens are samples: lanes of a group; 0: the kernels over splits
+    int team;                   // tokens are samples: lanes of a group, up to 64 or 256; 0: the kernels over splits
     int team_pieces;            // pieces of a lane
     int vector;                 // channels of a piece
     int64_t blocks;             // of the team kernel's grid
