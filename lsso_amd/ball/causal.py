@@ -344,7 +344,9 @@ def group_norm(
     they hold, give zeros and reach no gradient.  y: contiguous, of x's type.
 
     Statistics and sums are FP32, variances from deviations.  Differentiable (first
-    order) in x, weight and bias, deterministically."""
+    order) in x, weight and bias, deterministically.  Tokens by themselves of groups of
+    more than 8,192 channels go as samples of one row, with a workspace of two FP32
+    values for each of x."""
 
     _hip().require_available()
     _without_tangents(x, weight, bias)
@@ -548,9 +550,9 @@ def linear_attention(
 
     S is FP32; products take 16-bit operands, FP32 ones as parts that hold them (24
     bits in BF16, 22 in FP16), and accumulate in FP32: y and the gradients are off by
-    one rounding of their type.  An infinity or a NaN reaches its token's y and those
-    behind it, and in a gradient those before it.  Differentiable (first order) in query, key, value and
-    initial_state, deterministically; log_decay is fixed."""
+    one rounding of their type.  An infinity or a NaN reaches no y before its token.
+    Differentiable (first order) in query, key, value and initial_state,
+    deterministically; log_decay is fixed."""
 
     _hip().require_available()
     _without_tangents(query, key, value, log_decay, initial_state)

@@ -43,11 +43,11 @@
 // would be a NaN, so a chunk whose S shows one takes P c without it and makes its
 // column NaN from its token on.
 //
-// Bound: HBM and what a chunk's barriers leave open.  64 x 2,048 tokens of 4 heads of
-// 64 in BF16 (268 MB a walk, 41 us at the rate of a large copy): a walk takes 74 us,
-// 17 of them for the first chunk's loads and the launch's end, where workgroups finish
-// between 45 and 63 us; the rest runs at 5.6 TB/s.  Chunks are loaded one ahead.  On
-// the same case, slower: one barrier a chunk and LDS twice (82 us); eight waves that
+// Bound: what a chunk's barriers and its waves' own chains of products leave open.  64 x
+// 2,048 tokens of 4 heads of 64 in BF16 (268 MB a walk, 41 us at the rate of a large
+// copy): a walk takes 82 to 86 us; its waves issue 29% of their time and wait 52%, the
+// MFMAs are busy 20%.  Chunks are loaded one ahead.  On the same case with two parts of
+// P, S and c (74 us), slower: one barrier a chunk and LDS twice (82 us); eight waves that
 // share the rows of S (79 to 104); four workgroups to a compute unit, whose registers
 // spill (88).  Two chunks ahead changed nothing.
 
@@ -428,7 +428,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KT * WE <= 2 && WE == 1 ? 3 : (
         }
     }
     // Of a transposed state a lane's rows are neighbours in memory: four to a load (34
-    // us instead of 36 a walk at 2 x 4,096 tokens of 6 heads of 128 in FP16).  Four
+    // us instead of 36 a walk at 2 x 4,096 tokens of 6 heads of 128 in FP16, before its
+    // powers of two).  Four
     // columns to a load of the other order, exchanged among four lanes, were no faster.
     if (!STATES && first != nullptr && row_stride == 1 && a.features % 4 == 0) {   // uniform
 #pragma unroll
