@@ -528,7 +528,7 @@ def linear_attention(
     rank = functional.pad(kept, (0, room)).unflatten(1, (-1, tokens)).cumsum(-1).to(calc_dtype)[:, None]
     state = torch.zeros(batch, heads, features, v.shape[-1], dtype=calc_dtype, device=query.device)
     if initial_state is not None:
-        state = initial_state.to(calc_dtype)
+        state = initial_state.to(calc_dtype, copy=True)   # a step may follow, in place
     outputs = []
     for chunk in range(q.shape[2]):
         here = rank[:, :, chunk]   # [B, 1, tokens]

@@ -29,6 +29,19 @@ def _run(device, implementation, dtype):
         assert y.shape == shape and not any(grad.any() for grad in grads)
 
 
+def test_a_state_that_no_token_changes_is_a_copy() -> None:
+    """Steps change the state that a prompt returned in place, an empty one's too."""
+
+    mixer = CausalMixer(64, 4, kv_heads=2)
+    first = torch.randn(1, 4, 16, 16)
+    kept = first.clone()
+    with torch.no_grad():
+        _, state = mixer(torch.zeros(1, 0, 64), state=first, return_state=True)
+        assert torch.equal(state, first)
+        mixer.step(torch.randn(1, 64), state, torch.zeros(1, dtype=torch.int64))
+    assert torch.equal(first, kept) and not torch.equal(state, kept)
+
+
 def test_reference() -> None:
     _run("cpu", "reference", torch.float32)
 
